@@ -277,7 +277,7 @@ def _plain_pages(s):
     fits = there & (c + n <= mp * page)
     holes = (p >= (c // page)[:, None]) & (p < ((c + n + page - 1) // page)[:, None]) & (table < 0) & fits[:, None]
     need = holes.sum(1)
-    ok = fits & (starts[1:] <= s["slots"].numel()) & (need.cumsum(0) <= count)
+    ok = fits & (starts[1:] <= s["slots"].numel()) & ((need == 0) | (need.cumsum(0) <= count))
     take = holes & ok[:, None]
     k = (count - take.view(-1).cumsum(0)).clamp(min=0)
     table.copy_(torch.where(take, free[k].view(B, mp), table))
