@@ -21,6 +21,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
+_L = ctypes.c_long
 
 _SIGS = {
     "aila_hip_last_error": ([], ctypes.c_char_p),
@@ -41,6 +42,16 @@ _SIGS = {
     "aila_hip_gqa_prefill_cached_workspace_size": ([_I, _I, _I, _I, _I], _SZ),
     "aila_hip_gqa_prefill_cached_ws": ([_P, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _I, _I, _P], _I),
     "aila_hip_copy_to_cache": ([_P, _P, _I, _I, _I, _I, _I, _P], _I),
+    "aila_hip_kv_pages_reserve": ([_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P], _I),
+    "aila_hip_kv_pages_release": ([_P, _P, _P, _P, _I, _I, _I, _P], _I),
+    "aila_hip_kv_append_paged_fp8": ([_P, _P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P], _I),
+    "aila_hip_kv_read_paged_fp8": ([_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P], _I),
+    "aila_hip_gqa_decode_paged_fp8_workspace_size": ([_I, _I, _I, _I, _I], _SZ),
+    "aila_hip_gqa_decode_paged_fp8": ([_P, _L, _P, _P, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _I, _I, _P, _I, _I, _P,
+                                       _P], _I),
+    "aila_hip_gqa_prefill_paged_fp8_workspace_size": ([_I, _I, _I, _I, _I, _I], _SZ),
+    "aila_hip_gqa_prefill_paged_fp8": ([_P, _L, _P, _P, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _I, _I, _I, _P, _I, _I,
+                                        _P, _P, _P], _I),
     "aila_hip_deltanet_decode": ([_P, _P, _P, _P, _P, _P, _P, _P, _P,
                                   _I, _I, _I, _I, _I, _F, _F, _P], _I),
     "aila_hip_deltanet_prefill_workspace_size": ([_I, _I, _I, _I, _I], _SZ),
@@ -406,6 +417,233 @@ def copy_to_cache(new_kv, cache, start_pos: int, stream=None):
                                       _stream(stream))
     _check(rc, "aila_hip_copy_to_cache")
     return cache
+
+
+# ------------------------------------------------ 8-bit paged KV cache ----
+_SCALE_ROWS = 16   # rows of a page that share a scale
+
+
+def _same_device(stream, *tensors):
+    """The tensors' one device has to be the one whose stream the call runs on."""
+    import torch
+    for t in tensors:
+        if t is not None and t.get_device() != tensors[0].get_device():
+            raise ValueError(f"tensors on different devices: {tensors[0].device} and {t.device}")
+    dev = torch.cuda.current_device() if stream is None else stream.device_index
+    if tensors[0].get_device() != dev:
+        raise ValueError(f"tensors on {tensors[0].device}, but the call's stream is on cuda:{dev}: "
+                         "make it inside torch.cuda.device(...)")
+
+
+def _need_rows(t, tokens, heads, dim, name):
+    """[tokens, heads, dim] bf16 whose tokens may be strided (views of a fused
+    projection row); returns the token stride in elements."""
+    import torch
+    if t is None:
+        raise ValueError(f"{name} is required")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    if t.dtype != torch.bfloat16:
+        raise ValueError(f"{name}: dtype {t.dtype}, expected {torch.bfloat16}")
+    if tuple(t.shape) != (tokens, heads, dim):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {(tokens, heads, dim)}")
+    st = t.stride()
+    if st[2] != 1 or (heads > 1 and st[1] != dim):
+        raise ValueError(f"{name}: strides {st}, expected a token's [{heads}, {dim}] values to be contiguous")
+    step = st[0] if tokens > 1 else max(heads * dim, st[0])
+    if step < heads * dim or step % 8:
+        raise ValueError(f"{name}: token stride {step} must be a multiple of 8 and at least {heads * dim}")
+    if t.data_ptr() % 16:
+        raise ValueError(f"{name} must be 16-byte aligned")
+    return step
+
+
+def _need_pages(k_pages, v_pages, k_scale, v_scale):
+    """Checks the four arrays of an 8-bit paged cache; returns (num_pages, Hkv, page_size, D)."""
+    import torch
+    if k_pages is None or k_pages.dim() != 4:
+        raise ValueError("k_pages must be [num_pages, Hkv, page_size, D]")
+    P, Hkv, page_size, D = shape = tuple(k_pages.shape)
+    _need(k_pages, torch.float8_e4m3fn, shape, "k_pages")
+    _need(v_pages, torch.float8_e4m3fn, shape, "v_pages")
+    _need(k_scale, torch.float32, (P, Hkv, page_size // _SCALE_ROWS), "k_scale", align=4)
+    _need(v_scale, torch.float32, (P, Hkv, page_size // _SCALE_ROWS), "v_scale", align=4)
+    return shape
+
+
+def _new_out(make, stream):
+    """An output for work on `stream`, from that stream's memory."""
+    import torch
+    if stream is None:
+        return make()
+    with torch.cuda.stream(stream):
+        return make()
+
+
+def _workspace_bytes(workspace):
+    if workspace is None:
+        return 0
+    if not workspace.is_cuda or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous device tensor")
+    return workspace.numel() * workspace.element_size()
+
+
+def paged_fp8_cache(num_pages: int, Hkv: int, page_size: int, D: int, device=None):
+    """An empty 8-bit paged cache: (k_pages, v_pages, k_scale, v_scale)."""
+    import torch
+    if page_size <= 0 or page_size % _SCALE_ROWS:
+        raise ValueError(f"page_size {page_size} must be a positive multiple of {_SCALE_ROWS}")
+    dev = device if device is not None else torch.device("cuda", torch.cuda.current_device())
+    pages = [torch.zeros((num_pages, Hkv, page_size, D), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+             for _ in range(2)]
+    scales = [torch.ones((num_pages, Hkv, page_size // _SCALE_ROWS), dtype=torch.float32, device=dev) for _ in range(2)]
+    return (*pages, *scales)
+
+
+def kv_pages_reserve(cached_lens, new_lens, block_table, free_pages, free_count, page_size: int, slots,
+                     query_start=None, seq_lens=None, stream=None):
+    """Pages and slots for B requests' new tokens, on the device. cached_lens,
+    new_lens int32 [B]; block_table int32 [B, max_pages] (-1: no page yet);
+    free_pages int32 [num_pages], a stack whose entries [0, free_count[0]) are
+    free; slots int32 [max_tokens] (written whole). -> (query_start [B+1],
+    seq_lens [B], slots). seq_lens is 0 for requests that did not fit the
+    table, the batch or the free pages; their slots are -1."""
+    import torch
+    B, max_pages = block_table.shape
+    i32 = torch.int32
+    _need(cached_lens, i32, (B,), "cached_lens", align=4)
+    _need(new_lens, i32, (B,), "new_lens", align=4)
+    _need(block_table, i32, (B, max_pages), "block_table", align=4)
+    _need(free_pages, i32, (free_pages.numel(),), "free_pages", align=4)
+    _need(free_count, i32, (1,), "free_count", align=4)
+    _need(slots, i32, (slots.numel(),), "slots", align=4)
+    if query_start is None:
+        query_start = _new_out(lambda: torch.empty(B + 1, dtype=i32, device=block_table.device), stream)
+    if seq_lens is None:
+        seq_lens = _new_out(lambda: torch.empty(B, dtype=i32, device=block_table.device), stream)
+    _need(query_start, i32, (B + 1,), "query_start", align=4)
+    _need(seq_lens, i32, (B,), "seq_lens", align=4)
+    _same_device(stream, block_table, cached_lens, new_lens, free_pages, free_count, slots, query_start, seq_lens)
+    rc = lib().aila_hip_kv_pages_reserve(_ptr(cached_lens), _ptr(new_lens), _ptr(block_table), _ptr(free_pages),
+                                         _ptr(free_count), _ptr(query_start), _ptr(seq_lens), _ptr(slots), B, max_pages,
+                                         int(page_size), free_pages.numel(), slots.numel(), _stream(stream))
+    _check(rc, "aila_hip_kv_pages_reserve")
+    return query_start, seq_lens, slots
+
+
+def kv_pages_release(release, block_table, free_pages, free_count, stream=None):
+    """Push the pages of the rows with release[b] != 0 (int32 [B]) back onto the
+    free stack; their table entries become -1."""
+    import torch
+    B, max_pages = block_table.shape
+    _need(release, torch.int32, (B,), "release", align=4)
+    _need(block_table, torch.int32, (B, max_pages), "block_table", align=4)
+    _need(free_pages, torch.int32, (free_pages.numel(),), "free_pages", align=4)
+    _need(free_count, torch.int32, (1,), "free_count", align=4)
+    _same_device(stream, block_table, release, free_pages, free_count)
+    rc = lib().aila_hip_kv_pages_release(_ptr(release), _ptr(block_table), _ptr(free_pages), _ptr(free_count), B,
+                                         max_pages, free_pages.numel(), _stream(stream))
+    _check(rc, "aila_hip_kv_pages_release")
+
+
+def kv_append_paged_fp8(k_new, v_new, k_pages, v_pages, k_scale, v_scale, slots, stream=None):
+    """Quantise k_new/v_new [T, Hkv, D] bf16 into the rows `slots` (int32 [T],
+    -1: skip) of an 8-bit paged cache: k_pages/v_pages [num_pages, Hkv,
+    page_size, D] float8_e4m3fn, k_scale/v_scale [num_pages, Hkv,
+    page_size / 16] float32. The tokens may be strided (both alike)."""
+    import torch
+    P, Hkv, page_size, D = _need_pages(k_pages, v_pages, k_scale, v_scale)
+    T = slots.numel()
+    _need(slots, torch.int32, (T,), "slots", align=4)
+    step = _need_rows(k_new, T, Hkv, D, "k_new")
+    if _need_rows(v_new, T, Hkv, D, "v_new") != step and T > 1:
+        raise ValueError(f"k_new and v_new: token strides {step} and {v_new.stride(0)} differ")
+    _same_device(stream, k_pages, v_pages, k_scale, v_scale, k_new, v_new, slots)
+    rc = lib().aila_hip_kv_append_paged_fp8(_ptr(k_new), _ptr(v_new), step, _ptr(k_pages), _ptr(v_pages), _ptr(k_scale),
+                                            _ptr(v_scale), _ptr(slots), T, Hkv, D, page_size, P, _stream(stream))
+    _check(rc, "aila_hip_kv_append_paged_fp8")
+
+
+def kv_read_paged_fp8(k_pages, v_pages, k_scale, v_scale, slots, k_out=None, v_out=None, stream=None):
+    """Rows `slots` (int32 [T]; zeros for -1) of an 8-bit paged cache as the
+    values they stand for -> (k, v) [T, Hkv, D] bf16."""
+    import torch
+    P, Hkv, page_size, D = _need_pages(k_pages, v_pages, k_scale, v_scale)
+    T = slots.numel()
+    _need(slots, torch.int32, (T,), "slots", align=4)
+    if k_out is None:
+        k_out = _new_out(lambda: torch.empty((T, Hkv, D), dtype=torch.bfloat16, device=k_pages.device), stream)
+    if v_out is None:
+        v_out = _new_out(lambda: torch.empty((T, Hkv, D), dtype=torch.bfloat16, device=k_pages.device), stream)
+    _need(k_out, torch.bfloat16, (T, Hkv, D), "k_out")
+    _need(v_out, torch.bfloat16, (T, Hkv, D), "v_out")
+    _same_device(stream, k_pages, v_pages, k_scale, v_scale, slots, k_out, v_out)
+    rc = lib().aila_hip_kv_read_paged_fp8(_ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), _ptr(slots),
+                                          _ptr(k_out), _ptr(v_out), T, Hkv, D, page_size, P, _stream(stream))
+    _check(rc, "aila_hip_kv_read_paged_fp8")
+    return k_out, v_out
+
+
+def gqa_decode_paged_fp8_workspace_size(B: int, Hq: int, Hkv: int, D: int, max_len: int) -> int:
+    return int(lib().aila_hip_gqa_decode_paged_fp8_workspace_size(B, Hq, Hkv, D, max_len))
+
+
+def gqa_decode_paged_fp8(q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, max_len: int, out=None,
+                         workspace=None, stream=None):
+    """Decode over an 8-bit paged cache. q [B,Hq,D] bf16 (sequences may be
+    strided); the cache as kv_append_paged_fp8; block_table int32 [B,
+    max_pages]; seq_lens int32 [B] (taken as max_len where larger) -> out
+    [B,Hq,D]. workspace: uint8 device tensor (see
+    gqa_decode_paged_fp8_workspace_size), or None for one workgroup per
+    sequence and KV head."""
+    import torch
+    B, Hq, D = q.shape
+    P, Hkv, page_size, Dk = _need_pages(k_pages, v_pages, k_scale, v_scale)
+    max_pages = block_table.shape[1]
+    step = _need_rows(q, B, Hq, Dk, "q")
+    _need(block_table, torch.int32, (B, max_pages), "block_table", align=4)
+    _need(seq_lens, torch.int32, (B,), "seq_lens", align=4)
+    if out is None:
+        out = _new_out(lambda: torch.empty((B, Hq, D), dtype=q.dtype, device=q.device), stream)
+    _need(out, torch.bfloat16, (B, Hq, D), "out")
+    ws_bytes = _workspace_bytes(workspace)
+    _same_device(stream, q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, out, workspace)
+    rc = lib().aila_hip_gqa_decode_paged_fp8(_ptr(q), step, _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale),
+                                             _ptr(out), _ptr(workspace), ws_bytes, B, Hq, Hkv, D, page_size, P,
+                                             _ptr(block_table), max_pages, int(max_len), _ptr(seq_lens), _stream(stream))
+    _check(rc, "aila_hip_gqa_decode_paged_fp8")
+    return out
+
+
+def gqa_prefill_paged_fp8_workspace_size(T: int, B: int, Hq: int, Hkv: int, D: int, max_len: int) -> int:
+    return int(lib().aila_hip_gqa_prefill_paged_fp8_workspace_size(T, B, Hq, Hkv, D, max_len))
+
+
+def gqa_prefill_paged_fp8(q, k_pages, v_pages, k_scale, v_scale, block_table, query_start, seq_lens, max_len: int,
+                          out=None, workspace=None, stream=None):
+    """Causal attention of a ragged batch over an 8-bit paged cache that holds
+    the new rows already. q [T,Hq,D] bf16, request b's tokens at query_start[b]
+    .. query_start[b+1] (int32 [B+1]); seq_lens int32 [B] counts the rows after
+    them -> out [T,Hq,D] (rows from query_start[B] on are not touched)."""
+    import torch
+    T, Hq, D = q.shape
+    P, Hkv, page_size, Dk = _need_pages(k_pages, v_pages, k_scale, v_scale)
+    B, max_pages = block_table.shape
+    step = _need_rows(q, T, Hq, Dk, "q")
+    _need(block_table, torch.int32, (B, max_pages), "block_table", align=4)
+    _need(query_start, torch.int32, (B + 1,), "query_start", align=4)
+    _need(seq_lens, torch.int32, (B,), "seq_lens", align=4)
+    if out is None:
+        out = _new_out(lambda: torch.empty((T, Hq, D), dtype=q.dtype, device=q.device), stream)
+    _need(out, torch.bfloat16, (T, Hq, D), "out")
+    ws_bytes = _workspace_bytes(workspace)
+    _same_device(stream, q, k_pages, v_pages, k_scale, v_scale, block_table, query_start, seq_lens, out, workspace)
+    rc = lib().aila_hip_gqa_prefill_paged_fp8(_ptr(q), step, _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale),
+                                              _ptr(out), _ptr(workspace), ws_bytes, T, B, Hq, Hkv, D, page_size, P,
+                                              _ptr(block_table), max_pages, int(max_len), _ptr(query_start),
+                                              _ptr(seq_lens), _stream(stream))
+    _check(rc, "aila_hip_gqa_prefill_paged_fp8")
+    return out
 
 
 # ------------------------------------------------------------ DeltaNet ----

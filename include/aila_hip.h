@@ -280,6 +280,140 @@ int aila_hip_copy_to_cache(const void* new_kv, void* cache, int S,
                            int start_pos, int H, int D, int max_seq,
                            void* stream);
 
+/* ------------------------------------------- 8-bit paged KV cache --- */
+
+/* The paged cache of aila_hip_gqa_decode_paged held in 8 bits, with the tables
+ * that its pages are found by kept on the device. The reference has one bf16
+ * contiguous cache per sequence (src/memory/KVCache.hpp:9-45) and no
+ * counterpart to these.
+ *
+ *   k_pages, v_pages  [num_pages, Hkv, page_size, D] e4m3 (OCP: largest value
+ *                     448, no infinities), page_size a multiple of 16
+ *   k_scale, v_scale  [num_pages, Hkv, page_size / 16] fp32: the scale of a
+ *                     block of 16 rows of a page and head, a power of two. A
+ *                     stored value is code * scale, which is exact in bf16.
+ *   block_table       int[B, max_pages]: row r of request b is row r % page_size
+ *                     of page block_table[b * max_pages + r / page_size]; -1
+ *                     where there is no page.
+ *   slot              page * page_size + row in page (num_pages * page_size
+ *                     < 2^31). -1: no row.
+ * A serving step: reserve -> append -> decode or prefill, every layer with the
+ * same tables and slots and its own pages; release when a request ends. All
+ * lengths are read on the device, so the step can be captured in a HIP graph.
+ * Supported: D in {64, 128, 256}. */
+
+/* Pages and slots for the new tokens of B requests (B <= 2048).
+ *   cached_lens[b], new_lens[b]  rows that request b holds, and tokens it adds.
+ *                     Negative: the request is absent (0 tokens, length 0).
+ *   free_pages, free_count  stack of free pages: entries [0, *free_count) of
+ *                     int[num_pages] are free. Pages are taken from its top.
+ *   query_start[B+1]  out: request b's tokens are [query_start[b],
+ *                     query_start[b+1]) of the batch, the sum of new_lens before
+ *                     (requests that are not admitted keep their place;
+ *                     saturates at 2^31 - 1).
+ *   seq_lens[B]       out: cached_lens[b] + new_lens[b], or 0 if not admitted.
+ *                     May not be the array of cached_lens or new_lens.
+ *   slots[max_tokens] out: the slot of each token; -1 for tokens of requests
+ *                     that are not admitted and behind the last.
+ * The table entries that request b's new rows need (pages cached / page_size
+ * to the last) and that hold no page yet (< 0) each take one, in order of
+ * request and page; entries that hold one keep it, so a call repeated, or made
+ * after rejected tokens were taken back, takes no page twice. A request is
+ * admitted if its rows fit the table, its tokens fit max_tokens, and, where it
+ * needs pages, the free pages cover its need and that of every request before
+ * it whose rows fit. Requests that are not admitted leave table and stack
+ * alone. Calls on one stack must not overlap in time. */
+int aila_hip_kv_pages_reserve(const int* cached_lens, const int* new_lens,
+                              int* block_table, const int* free_pages,
+                              int* free_count, int* query_start, int* seq_lens,
+                              int* slots, int B, int max_pages, int page_size,
+                              int num_pages, int max_tokens, void* stream);
+
+/* Give back every page of the rows b of block_table with release[b] != 0: the
+ * entries >= 0 are pushed onto the stack in order of request and page and
+ * become -1 (releasing a row again gives nothing back). A page stands in one
+ * row only: pages are not counted. */
+int aila_hip_kv_pages_release(const int* release, int* block_table,
+                              int* free_pages, int* free_count, int B,
+                              int max_pages, int num_pages, void* stream);
+
+/* Quantise T tokens' K/V rows into the cache. k_new/v_new: token t's [Hkv, D]
+ * bf16 values at + t * new_stride elements (a multiple of 8), 16-byte aligned;
+ * slots int[T] (-1, or any slot outside the pool: the token is skipped).
+ * Tokens whose slots fall into one block of 16 rows must stand next to each
+ * other in row order, as aila_hip_kv_pages_reserve leaves them, and two runs of
+ * one call may not meet in a block. For such a run and each head, with a the
+ * largest finite |x|:
+ *   e = the smallest integer with a <= 448 * 2^e, within [-100, 119]; if rows
+ *       of the block stand before the run, not less than the block's exponent;
+ *   code = e4m3(x * 2^-e), to nearest even, NaN for NaN and infinities (which do
+ *       not count for a), saturated beyond 448 (at e = 119 only).
+ * If e exceeds the block's exponent, the rows before the run are requantised to
+ * it (exact but for underflow). Rows behind the run are left as they were and
+ * are not valid until written. */
+int aila_hip_kv_append_paged_fp8(const void* k_new, const void* v_new,
+                                 long new_stride, void* k_pages, void* v_pages,
+                                 float* k_scale, float* v_scale,
+                                 const int* slots, int T, int Hkv, int D,
+                                 int page_size, int num_pages, void* stream);
+
+/* Read rows back by slot, as the values they stand for: k_out/v_out [T, Hkv, D]
+ * bf16; zeros for slots outside the pool. (Handing a sequence to the bf16 entry
+ * points, export, inspection.) */
+int aila_hip_kv_read_paged_fp8(const void* k_pages, const void* v_pages,
+                               const float* k_scale, const float* v_scale,
+                               const int* slots, void* k_out, void* v_out,
+                               int T, int Hkv, int D, int page_size,
+                               int num_pages, void* stream);
+
+/* Single-token GQA decode over the 8-bit pages (the 8-bit form of
+ * aila_hip_gqa_decode_paged; ops::attention_decode, src/ops/AttentionOps.cpp:
+ * 499-643). q: sequence b's [Hq, D] bf16 at + b * q_stride elements (a multiple
+ * of 8); out [B, Hq, D] bf16. Sequence b attends rows [0, min(seq_lens[b],
+ * max_len)); none: 0. Rows whose table entry is outside [0, num_pages) are
+ * masked. Any integer Hq / Hkv (one workgroup serves up to 16 query heads of a
+ * KV head), B <= 4096. Softmax scale 1/sqrt(D).
+ * The work is shared evenly by the workgroups whatever the lengths are;
+ * workspace_size bytes let as many work as the device holds, a smaller
+ * workspace fewer, and NULL one per sequence and KV head (no split). */
+size_t aila_hip_gqa_decode_paged_fp8_workspace_size(int B, int Hq, int Hkv,
+                                                    int D, int max_len);
+int aila_hip_gqa_decode_paged_fp8(const void* q, long q_stride,
+                                  const void* k_pages, const void* v_pages,
+                                  const float* k_scale, const float* v_scale,
+                                  void* out, void* workspace,
+                                  size_t workspace_bytes, int B, int Hq,
+                                  int Hkv, int D, int page_size, int num_pages,
+                                  const int* block_table, int max_pages,
+                                  int max_len, const int* seq_lens,
+                                  void* stream);
+
+/* Causal GQA over the 8-bit pages for a ragged batch: prompts, turns over a
+ * cached prefix and single tokens side by side (ops::attention_prefill_cached,
+ * src/ops/AttentionOps.cpp:2308-2507, for B requests at once). The new tokens'
+ * rows are in the cache already (aila_hip_kv_append_paged_fp8).
+ *   q        token t's [Hq, D] bf16 at + t * q_stride elements; out [T, Hq, D]
+ *   query_start int[B+1], seq_lens int[B]: as aila_hip_kv_pages_reserve leaves
+ *            them. Token query_start[b] + i, of n = query_start[b+1] -
+ *            query_start[b], attends rows [0, L - n + i], L = min(seq_lens[b],
+ *            max_len); none: 0. Tokens from query_start[B] on are not touched.
+ * Other arguments as aila_hip_gqa_decode_paged_fp8. T is the number of rows of
+ * q and out; query_start must not decrease nor pass T (what passes it is not
+ * computed). */
+size_t aila_hip_gqa_prefill_paged_fp8_workspace_size(int T, int B, int Hq,
+                                                     int Hkv, int D,
+                                                     int max_len);
+int aila_hip_gqa_prefill_paged_fp8(const void* q, long q_stride,
+                                   const void* k_pages, const void* v_pages,
+                                   const float* k_scale, const float* v_scale,
+                                   void* out, void* workspace,
+                                   size_t workspace_bytes, int T, int B,
+                                   int Hq, int Hkv, int D, int page_size,
+                                   int num_pages, const int* block_table,
+                                   int max_pages, int max_len,
+                                   const int* query_start, const int* seq_lens,
+                                   void* stream);
+
 /* ----------------------------------------------------------- DeltaNet --- */
 
 /* One Gated DeltaNet decode step (the recurrence of
