@@ -81,7 +81,8 @@ __device__ __forceinline__ int share_begin(int w, int units, int groups) {
 }
 
 template <int D>
-__global__ __launch_bounds__(kThreads, 2) void gqa_decode_paged_fp8_kernel(PagedFp8 c, Fp8DecodeArgs a) {
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void gqa_decode_paged_fp8_kernel(PagedFp8 c, Fp8DecodeArgs a) {
+  constexpr int kDepth = 3;    // strips of a wave in registers
   extern __shared__ __attribute__((aligned(16))) unsigned char s_dyn[];
   float* s_acc = reinterpret_cast<float*>(s_dyn);             // [kWaves][tile][D]
   float* s_ml = s_acc + kWaves * a.tile * D;                  // [kWaves][tile][2]
@@ -147,27 +148,28 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_decode_paged_fp8_kernel(Paged
                                       blk_end);
       const int n1 = min(ns - n0, 32);
       auto load = [&](Strip<D>& s, int n) __attribute__((always_inline)) {
-        load_strip<D, true>(s, c, __builtin_amdgcn_readlane(mine.bid, 2 * n), __builtin_amdgcn_readlane(mine.bid, 2 * n + 1),
-                            m16, g4);
+        const bool in = n < n1;
+        const int ba = __builtin_amdgcn_readlane(mine.bid, 2 * n & 63), bb = __builtin_amdgcn_readlane(mine.bid, (2 * n + 1) & 63);
+        load_strip<D, true>(s, c, in ? ba : -1, in ? bb : -1, m16, g4);
       };
       auto step = [&](Strip<D>& s, int n) __attribute__((always_inline)) {
         const int ba = __builtin_amdgcn_readlane(mine.bid, 2 * n), bb = __builtin_amdgcn_readlane(mine.bid, 2 * n + 1);
         const float ka = readlane_f(mine.ks, 2 * n) * a.scale_log2, kb = readlane_f(mine.ks, 2 * n + 1) * a.scale_log2;
         const float va = readlane_f(mine.vs, 2 * n), vb = readlane_f(mine.vs, 2 * n + 1);
         const int row = row0 + (n0 + n) * kUnit;
-        if (row + 32 <= end && ba >= 0 && bb >= 0)
-          strip_step<D, false>(col, s, q, ka, kb, va, vb, row, end, true, true, g4);
-        else
-          strip_step<D, true>(col, s, q, ka, kb, va, vb, row, end, ba >= 0, bb >= 0, g4);
+        strip_step<D>(col, s, q, ka, kb, va, vb, row + 32 > end || (ba | bb) < 0, row, end, ba >= 0, bb >= 0, g4);
       };
-      Strip<D> s0, s1;
-      load(s0, 0);
-      for (int n = 0; n < n1; n += 2) {
-        if (n + 1 < n1) load(s1, n + 1);
-        step(s0, n);
-        if (n + 1 >= n1) break;
-        if (n + 2 < n1) load(s0, n + 2);
-        step(s1, n + 1);
+      Strip<D> s[kDepth];
+#pragma unroll
+      for (int i = 0; i < kDepth - 1; ++i) load(s[i], i);
+      for (int n = 0; n < n1; n += kDepth) {
+#pragma unroll
+        for (int i = 0; i < kDepth; ++i) {
+          if (n + i < n1) {
+            load(s[(i + kDepth - 1) % kDepth], n + i + kDepth - 1);
+            step(s[i], n + i);
+          }
+        }
       }
     }
 

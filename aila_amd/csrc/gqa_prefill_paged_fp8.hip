@@ -86,10 +86,8 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_prefill_paged_fp8_kernel(Page
       Strip<D> s;
       load_strip<D, false>(s, c, ba, bb, m16, g4);
       const int at = 32 * (n0 + i);
-      if (at + 32 <= full && r0 + 16 <= n * a.group && ba >= 0 && bb >= 0)
-        strip_step<D, false>(col, s, q, ka, kb, va, vb, at, lim, true, true, g4);
-      else
-        strip_step<D, true>(col, s, q, ka, kb, va, vb, at, lim, ba >= 0, bb >= 0, g4);
+      strip_step<D>(col, s, q, ka, kb, va, vb, at + 32 > full || r0 + 16 > n * a.group || (ba | bb) < 0, at, lim, ba >= 0,
+                    bb >= 0, g4);
     }
   }
   const float l = xrow4_sum(col.l);

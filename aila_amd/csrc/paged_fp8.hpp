@@ -96,33 +96,37 @@ struct Strip {
   uint32_t v[8][VW];
 };
 
+// Buffer loads, each block a buffer of its own: one that has no page (bid < 0)
+// has no bytes, and its loads return zeros without going to memory, so a
+// pipeline of strips needs no branch around its loads.
 template <int D, bool NT>
 __device__ __forceinline__ void load_strip(Strip<D>& s, const PagedFp8& c, int bid_a, int bid_b, int m16, int g4) {
+  constexpr int kAux = NT ? 2 : 0;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    const size_t base = static_cast<size_t>(max(x ? bid_b : bid_a, 0)) * (kScaleRows * D);
-    const uint8_t* kp = c.k_pages + base + m16 * D + 16 * g4;
+    const int bid = x ? bid_b : bid_a;
+    const size_t base = static_cast<size_t>(max(bid, 0)) * (kScaleRows * D);
+    const int bytes = bid >= 0 ? kScaleRows * D : 0;
+    const __amdgpu_buffer_rsrc_t kr =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(c.k_pages) + base, 0, bytes, kBufferRsrcWord3);
+    const __amdgpu_buffer_rsrc_t vr =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(c.v_pages) + base, 0, bytes, kBufferRsrcWord3);
 #pragma unroll
-    for (int kk = 0; kk < Strip<D>::KK; ++kk) {
-      const u32x4* p = reinterpret_cast<const u32x4*>(kp + 64 * kk);
-      s.k[x][kk] = NT ? __builtin_nontemporal_load(p) : *p;
-    }
-    const uint8_t* vp = c.v_pages + base + 4 * g4 * D + m16 * (D / 16);
+    for (int kk = 0; kk < Strip<D>::KK; ++kk)
+      s.k[x][kk] = __builtin_amdgcn_raw_buffer_load_b128(kr, m16 * D + 16 * g4 + 64 * kk, 0, kAux);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      const int at = (4 * g4 + j) * D + m16 * (D / 16);
       if constexpr (D == 256) {
-        const u32x4* p = reinterpret_cast<const u32x4*>(vp + j * D);
-        const u32x4 w = NT ? __builtin_nontemporal_load(p) : *p;
+        const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(vr, at, 0, kAux);
 #pragma unroll
         for (int i = 0; i < 4; ++i) s.v[4 * x + j][i] = w[i];
       } else if constexpr (D == 128) {
-        const u32x2* p = reinterpret_cast<const u32x2*>(vp + j * D);
-        const u32x2 w = NT ? __builtin_nontemporal_load(p) : *p;
+        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(vr, at, 0, kAux);
         s.v[4 * x + j][0] = w[0];
         s.v[4 * x + j][1] = w[1];
       } else {
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(vp + j * D);
-        s.v[4 * x + j][0] = NT ? __builtin_nontemporal_load(p) : *p;
+        s.v[4 * x + j][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, at, 0, kAux);
       }
     }
   }
@@ -160,7 +164,7 @@ __device__ __forceinline__ void v_tiles(const uint32_t (&v)[8], bf16x8_t (&t)[4]
   for (int i = 0; i < 4; ++i) t[i] = as_bf16x8(o[i]);
 }
 
-// One strip into a column's softmax. `row` is the strip's first row; with MASK
+// One strip into a column's softmax. `row` is the strip's first row; if masked,
 // a column attends rows < lim of the blocks that have a page (ok_a, ok_b).
 // ka, kb: the K scales times log2(e) / sqrt(D). The V scales go into P, where
 // they are exact. P goes in as the sum of two bf16 (16 bits): one would double the output's rounding error, and the
@@ -172,9 +176,52 @@ __device__ __forceinline__ void v_tiles(const uint32_t (&v)[8], bf16x8_t (&t)[4]
 // back there.
 constexpr float kLazyLog2 = 8.0f;
 
-template <int D, bool MASK>
+// The bytes of w that are NaN codes (0x7f, 0xff), as 0x80 each.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// Takes the NaN codes out of a masked strip's V and puts NaN into the outputs
+// of the columns that attend them.
+template <int D>
+__device__ __forceinline__ void mend_strip(Column<D>& c, Strip<D>& s, int row, int lim, bool ok_a, bool ok_b, int g4) {
+  uint32_t seen = 0;
+#pragma unroll
+  for (int w = 0; w < D / 64; ++w) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) seen |= nan_codes(s.v[j][w]);
+  }
+  if (__ballot(seen != 0) == 0) return;
+  u32x4 pa;   // 1 where the column attends the row
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int r = row + (e < 2 ? 0 : 16) + 4 * g4 + 2 * (e & 1);
+    const bool ok = e < 2 ? ok_a : ok_b;
+    pa[e] = (ok && r < lim ? 0x3f80u : 0u) | (ok && r + 1 < lim ? 0x3f800000u : 0u);
+  }
+#pragma unroll
+  for (int w = 0; w < D / 64; ++w) {
+    uint32_t one[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t n = nan_codes(s.v[j][w]) >> 7;
+      one[j] = n * 0x38u;      // the code of 1
+      s.v[j][w] &= ~(n * 0xffu);
+    }
+    bf16x8_t t[4];
+    v_tiles(one, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 n = mfma16x16x32(t[i], as_bf16x8(pa), f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+      for (int j = 0; j < 4; ++j)   // n[j] is 0 or at least 1
+        c.acc[4 * w + i][j] = __uint_as_float(__float_as_uint(c.acc[4 * w + i][j]) |
+                                              ((0u - min(__float_as_uint(n[j]), 1u)) & 0x7fc00000u));
+    }
+  }
+}
+
+template <int D>
 __device__ __forceinline__ void strip_step(Column<D>& c, Strip<D>& s, const bf16x8_t (&q)[D / 32], float ka, float kb,
-                                           float va, float vb, int row, int lim, bool ok_a, bool ok_b, int g4) {
+                                           float va, float vb, bool masked, int row, int lim, bool ok_a, bool ok_b, int g4) {
   f32x4 sa = {0.f, 0.f, 0.f, 0.f}, sb = sa;
 #pragma unroll
   for (int kk = 0; kk < D / 64; ++kk) {
@@ -187,17 +234,22 @@ __device__ __forceinline__ void strip_step(Column<D>& c, Strip<D>& s, const bf16
     sb = mfma16x16x32(hi, q[2 * kk + 1], sb);
   }
   float x[8];
-  float top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     x[j] = sa[j] * ka;
     x[4 + j] = sb[j] * kb;
-    if constexpr (MASK) {
+  }
+  if (masked) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
       if (!(ok_a && row + 4 * g4 + j < lim)) x[j] = -INFINITY;
       if (!(ok_b && row + 16 + 4 * g4 + j < lim)) x[4 + j] = -INFINITY;
     }
-    top = fmaxf(top, fmaxf(x[j], x[4 + j]));
+    mend_strip<D>(c, s, row, lim, ok_a, ok_b, g4);
   }
+  float top = x[0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
   top = xrow4_max(top);
   // The reference maximum moves only when a row exceeds it by 2^8: until then
   // P <= 2^8 and nothing is lost, and the accumulators need no rescaling.
@@ -222,47 +274,12 @@ __device__ __forceinline__ void strip_step(Column<D>& c, Strip<D>& s, const bf16
     ph[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
     pl[e] = pack_bf16x2(x[2 * e] - __uint_as_float(ph[e] << 16), x[2 * e + 1] - __uint_as_float(ph[e] & 0xffff0000u));
   }
-  uint32_t nan_seen = 0;
-  if constexpr (MASK) {
-#pragma unroll
-    for (int w = 0; w < D / 64; ++w) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) nan_seen |= ((s.v[j][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-    }
-  }
-  const bool mend = MASK && __ballot(nan_seen != 0) != 0;
-  u32x4 pa = {0u, 0u, 0u, 0u};   // 1 where the column attends the row
-  if (mend) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = row + (e < 2 ? 0 : 16) + 4 * g4 + 2 * (e & 1);
-      const bool ok = e < 2 ? ok_a : ok_b;
-      pa[e] = (ok && r < lim ? 0x3f80u : 0u) | (ok && r + 1 < lim ? 0x3f800000u : 0u);
-    }
-  }
 #pragma unroll
   for (int w = 0; w < D / 64; ++w) {
     uint32_t v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = s.v[j][w];
     bf16x8_t t[4];
-    if (mend) {
-      uint32_t one[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t n = (((v[j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-        one[j] = n * 0x38u;      // the code of 1
-        v[j] &= ~(n * 0xffu);
-      }
-      v_tiles(one, t);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 n = mfma16x16x32(t[i], as_bf16x8(pa), f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n[j] > 0.f) c.acc[4 * w + i][j] = __uint_as_float(0x7fc00000u);
-      }
-    }
     v_tiles(v, t);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
