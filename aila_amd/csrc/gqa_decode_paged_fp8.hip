@@ -26,7 +26,6 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kUnit = 32 * kWaves;     // rows of a unit
 constexpr int kMaxTile = 16;           // query heads of a workgroup
 constexpr int kMaxSequences = 4096;    // their unit counts live in LDS
-constexpr int kMaxGroups = 512;        // workgroups of a split
 constexpr int kRecTail = 4;
 
 struct Fp8DecodeArgs {
@@ -295,10 +294,12 @@ int launch(const PagedFp8& c, const Fp8DecodeArgs& a, int groups, hipStream_t st
   return check_launch("gqa_decode_paged_fp8");
 }
 
-// Workgroups a split may use: one a unit, as many as the device holds at most.
-long split_groups(int B, int heads, int max_len) {
+// Workgroups a split may use: one a unit, and as many as the 256 CUs hold at
+// most (the kernel's registers: 1, 2 or 3 a CU), so that all run at once.
+long split_groups(int B, int heads, int max_len, int D) {
   const long units = std::max(1L, (static_cast<long>(max_len) + kUnit - 1) / kUnit);
-  return std::min<long>(kMaxGroups, static_cast<long>(B) * heads * units);
+  const long resident = 256 * (D == 256 ? 1 : D == 128 ? 2 : 3);
+  return std::min<long>(resident, static_cast<long>(B) * heads * units);
 }
 
 }  // namespace
@@ -309,7 +310,7 @@ extern "C" size_t aila_hip_gqa_decode_paged_fp8_workspace_size(int B, int Hq, in
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || max_len < 0) return 0;
   int tile, chunks;
   head_tiles(Hq / Hkv, &tile, &chunks);
-  return split_groups(B, Hkv * chunks, max_len) * record_bytes(tile, D);
+  return split_groups(B, Hkv * chunks, max_len, D) * record_bytes(tile, D);
 }
 
 extern "C" int aila_hip_gqa_decode_paged_fp8(const void* q, long q_stride, const void* k_pages, const void* v_pages,
@@ -353,7 +354,7 @@ extern "C" int aila_hip_gqa_decode_paged_fp8(const void* q, long q_stride, const
     if (workspace_bytes < 2 * rec)
       return set_error(AILA_HIP_EWORKSPACE, "gqa_decode_paged_fp8: workspace %zu bytes holds < 2 workgroups' records (%zu bytes each)",
                        workspace_bytes, rec);
-    groups = std::min<long>(split_groups(B, heads, max_len), static_cast<long>(workspace_bytes / rec));
+    groups = std::min<long>(split_groups(B, heads, max_len, D), static_cast<long>(workspace_bytes / rec));
     a.part = static_cast<float*>(workspace);
   }
   const hipStream_t st = static_cast<hipStream_t>(stream);
