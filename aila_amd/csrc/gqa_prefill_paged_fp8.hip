@@ -39,7 +39,7 @@ constexpr int kRows = 32 * kGroupWaves;    // query rows of a tile
 constexpr int kMaxSequences = 4096;
 constexpr int kCus = 256;
 constexpr int kNoKey = 0x7fffffff;
-constexpr int kAhead = 4;      // LDS operand reads in flight ahead of their MFMAs
+
 
 struct Fp8PrefillArgs {
   const bf16* q;
@@ -82,6 +82,7 @@ struct Cfg {
   static constexpr int RAW = BN * D;              // bytes of a tile as codes
   static constexpr int DMA = RAW / (1024 * kGroupWaves);   // DMA instructions a wave and tile
   static constexpr int KI = BN * CH / kGroup;     // 16-code pieces of K a thread converts
+  static constexpr int AHEAD = D == 256 ? 2 : 4;  // LDS operand reads in flight ahead of their MFMAs
   static constexpr int GROUP_LDS = 2 * OPS + 4 * RAW;
   static constexpr int LDS = 2 * GROUP_LDS;
   static_assert(LDS >= kGroupWaves * DT * 16 * 64 * 4, "the groups' outputs meet in LDS");
@@ -100,6 +101,14 @@ __device__ __forceinline__ float half_max(float x) {
 __device__ __forceinline__ float half_sum(float x) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// x, as a value the compiler cannot follow: what is made of it inside a loop is
+// made there again, a few instructions, and not kept in registers (or spilled)
+// over all loops around it.
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 // Head dim of row m of output part dt (the order in which V's bytes pair up).
@@ -354,12 +363,13 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
       const int tile = tile_of(j);
       unsigned char* dst = (isv ? v_raw : k_raw) + (j & 1) * C::RAW;
       const uint8_t* pages = isv ? c.v_pages : c.k_pages;
+      const int ln = here(lane);
 #pragma unroll
       for (int i = 0; i < C::DMA; ++i) {
         const int piece = i * kGroupWaves + wave;               // KiB of the tile
         const int bid = bid_of(tile, piece * 1024 / (kScaleRows * D));
         const u32x4 rsrc = buffer_rsrc(pages + static_cast<size_t>(max(bid, 0)) * (kScaleRows * D), bid >= 0 ? kScaleRows * D : 0);
-        const int idx = piece * 64 + lane;
+        const int idx = piece * 64 + ln;
         const int r = idx / C::CH, p = idx % C::CH;
         const int off = (r % kScaleRows) * D + (isv ? p : p ^ piece_swizzle<D>(r)) * 16;
         dma16_to_lds(rsrc, off, dst + piece * 1024);
@@ -372,14 +382,17 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
       return __shfl(isv ? (next ? rb.vs : ra.vs) : (next ? rb.ks : ra.ks), ref_lane(tile, blk));
     };
     auto convert_k = [&](int j) __attribute__((always_inline)) {
-      const unsigned char* raw = k_raw + (j & 1) * C::RAW;
-      const int r = t % C::BN;
+      const int th = here(t);
+      const int r = th % C::BN, s0 = th / C::BN;
+      constexpr int kStep = kGroup / C::BN;
       const float sc = scale_of(false, tile_of(j), r / kScaleRows);
+      unsigned char* dst0 = k_ops + (((r / 32) * C::STEPS + s0) * 64 + (r & 31)) * 16;
+      const unsigned char* raw0 = k_raw + (j & 1) * C::RAW + r * D;
 #pragma unroll
       for (int i = 0; i < C::KI; ++i) {
-        const int s = (t + kGroup * i) / C::BN;                  // piece: MFMA step s
-        const u32x4 w = ld16(raw + r * D + ((s ^ piece_swizzle<D>(r)) << 4));
-        unsigned char* dst = k_ops + (((r / 32) * C::STEPS + s) * 64 + (r & 31)) * 16;
+        const int s = s0 + kStep * i;                            // piece: MFMA step s
+        const u32x4 w = ld16(raw0 + ((s ^ piece_swizzle<D>(r)) << 4));
+        unsigned char* dst = dst0 + kStep * i * 1024;
         *reinterpret_cast<u32x4*>(dst) = u32x4{fp8x2_to_bf16x2<false>(w[0], sc), fp8x2_to_bf16x2<true>(w[0], sc),
                                                fp8x2_to_bf16x2<false>(w[1], sc), fp8x2_to_bf16x2<true>(w[1], sc)};
         *reinterpret_cast<u32x4*>(dst + 512) = u32x4{fp8x2_to_bf16x2<false>(w[2], sc), fp8x2_to_bf16x2<true>(w[2], sc),
@@ -396,9 +409,10 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
       return ragged || (tile + 1) * C::BN > full || held_blocks(tile) != kAllBlocks;
     };
     auto convert_v = [&](int j) __attribute__((always_inline)) {
-      if (D == 64 && t >= 128) return;
+      if (D == 64 && wave >= 2) return;
       const unsigned char* raw = v_raw + (j & 1) * C::RAW;
-      const int o = t / (D / 4), dq = t % (D / 4);               // 8 keys x 4 dims
+      const int th = here(t);
+      const int o = th / (D / 4), dq = th % (D / 4);             // 8 keys x 4 dims
       const int st = o >> 1, h8 = o & 1;                         // 16-key step of the tile, half
       const int key = 16 * st + 4 * h8;
       const float sc = scale_of(true, tile_of(j), st);
@@ -456,17 +470,17 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
     for (int d = 0; d < C::DT; ++d) o[d] = f32x16{};
     float m = -INFINITY, l = 0.f;
 
-    // Operands are read kAhead ahead of the products that take them; the schedule
+    // Operands are read AHEAD ahead of the products that take them; the schedule
     // barriers keep it so (left alone, the compiler reads them all first, and
     // spills).
     auto pv = [&]() __attribute__((always_inline)) {
       constexpr int N = 2 * C::KT * C::DT;
       bf16x8_t v[N];
 #pragma unroll
-      for (int i = 0; i < kAhead && i < N; ++i) v[i] = as_bf16x8(ld16(v_ops + (i * 64 + lane) * 16));
+      for (int i = 0; i < C::AHEAD && i < N; ++i) v[i] = as_bf16x8(ld16(v_ops + (i * 64 + lane) * 16));
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (i + kAhead < N) v[i + kAhead] = as_bf16x8(ld16(v_ops + ((i + kAhead) * 64 + lane) * 16));
+        if (i + C::AHEAD < N) v[i + C::AHEAD] = as_bf16x8(ld16(v_ops + ((i + C::AHEAD) * 64 + lane) * 16));
         const int s = i / C::DT, d = i % C::DT;
         o[d] = mfma32(v[i], as_bf16x8(p[s >> 1][s & 1]), o[d]);
         __builtin_amdgcn_sched_barrier(0);
@@ -481,10 +495,10 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
 #pragma unroll
       for (int x = 0; x < C::KT; ++x) sc[x] = f32x16{};
 #pragma unroll
-      for (int i = 0; i < kAhead && i < N; ++i) k[i] = load(i);
+      for (int i = 0; i < C::AHEAD && i < N; ++i) k[i] = load(i);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (i + kAhead < N) k[i + kAhead] = load(i + kAhead);
+        if (i + C::AHEAD < N) k[i + C::AHEAD] = load(i + C::AHEAD);
         sc[i % C::KT] = mfma32(k[i], q[i / C::KT], sc[i % C::KT]);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -572,6 +586,12 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
     __syncthreads();
 
     // ---- the groups' states meet ---------------------------------------------
+    {
+    const int lane = here(threadIdx.x & 63), l32 = lane & 31, hf = lane >> 5;
+    const int row = it.r0 + wave * 32 + l32;
+    const bool there = row < rows;
+    const int tok = there ? row / a.group : 0;
+    const int h = kvh * a.group + row % a.group;
     l = half_sum(l);
     float* s_o = reinterpret_cast<float*>(s_dyn);                                    // [wave][part][quad][lane] f32x4
     if (grp == 1) {
@@ -641,6 +661,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
           }
         }
       }
+    }
     }
     __syncthreads();   // LDS is the next item's
   }
