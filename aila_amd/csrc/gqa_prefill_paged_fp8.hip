@@ -83,6 +83,9 @@ struct Cfg {
   static constexpr int DMA = RAW / (1024 * kGroupWaves);   // DMA instructions a wave and tile
   static constexpr int KI = BN * CH / kGroup;     // 16-code pieces of K a thread converts
   static constexpr int AHEAD = D == 256 ? 2 : 4;  // LDS operand reads in flight ahead of their MFMAs
+  static constexpr int SEG = D == 256 ? 768 : 2048;   // blocks of a segment of keys, looked up at once
+  static constexpr int QL = D == 256 ? 5 : 0;     // MFMA steps whose query operand is kept in LDS: the registers do not hold it
+  static constexpr bool LOAD_FIRST = D != 256;    // a vector phase reads its codes before its softmax
   static constexpr int GROUP_LDS = 2 * OPS + 4 * RAW;
   static constexpr int LDS = 2 * GROUP_LDS;
   static_assert(LDS >= kGroupWaves * DT * 16 * 64 * 4, "the groups' outputs meet in LDS");
@@ -110,6 +113,8 @@ __device__ __forceinline__ int here(int x) {
   asm volatile("" : "+v"(x));
   return x;
 }
+
+__device__ __forceinline__ void pin(u32x4& x) { asm volatile("" : "+v"(x)); }
 
 // Head dim of row m of output part dt (the order in which V's bytes pair up).
 template <int D>
@@ -307,6 +312,10 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
   extern __shared__ __attribute__((aligned(1024))) unsigned char s_dyn[];
   __shared__ int s_nan[D];      // first masked-tile key whose V holds NaN in this dim
   __shared__ float s_ml[kRows][2];
+  // Blocks of the segment of keys being walked: index in the pool (-1: none), scales.
+  __shared__ __attribute__((aligned(16))) int s_bid[C::SEG];
+  __shared__ float s_ks[C::SEG], s_vs[C::SEG];
+  __shared__ __attribute__((aligned(16))) unsigned char s_q[(C::QL ? kGroupWaves * C::QL : 1) * 1024];
   const int grp = __builtin_amdgcn_readfirstlane(threadIdx.x / kGroup);
   const int t = threadIdx.x % kGroup, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -316,6 +325,20 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
   unsigned char* v_ops = mine + C::OPS;
   unsigned char* k_raw = mine + 2 * C::OPS;            // two tiles
   unsigned char* v_raw = k_raw + 2 * C::RAW;           // two tiles
+  // This thread's places, in bytes: of its codes in a page (K: pieces exchanged;
+  // V: lane * 16), of the codes it converts, and of the operands it makes.
+  constexpr int kKib = kScaleRows * D / 1024;          // KiB of a block
+  const unsigned uh = threadIdx.x % kGroup, ul = threadIdx.x & 63;
+  const unsigned kr = (64 / C::CH) * (wave % kKib) + ul / C::CH;     // row in its block
+  const int k_off = (ul / C::CH) * D + ((ul % C::CH) ^ piece_swizzle<D>(kr)) * 16;
+  const unsigned cr = uh % C::BN, cs = uh / C::BN;     // K: row of the tile, first piece
+  const int k_from = cr * D + ((cs ^ piece_swizzle<D>(cr)) << 4);
+  const int k_to = ((cr / 32 * C::STEPS + cs) * 64 + cr % 32) * 16;
+  const unsigned oc = uh / (D / 4), dq = uh % (D / 4);  // V: octet of keys, quad of dims
+  const int v_from = (16 * (oc >> 1) + 4 * (oc & 1)) * D + 4 * dq;
+  int v_dt, v_row;
+  out_slot<D>(dq, 0, &v_dt, &v_row);
+  const int v_to = (((oc >> 1) * C::DT + v_dt) * 64 + (oc & 1) * 32 + v_row) * 16;
   const int kvh = static_cast<int>(blockIdx.x) % c.Hkv, wl = static_cast<int>(blockIdx.x) / c.Hkv;
 
   for (int round = 0;; ++round) {
@@ -327,263 +350,287 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
     const int row = it.r0 + wave * 32 + l32;          // this lane's query row
     const bool there = row < rows;
     const int tok = there ? row / a.group : 0;
-    const int h = kvh * a.group + row % a.group;
     const int lim = there ? max(it.len - it.n + tok + 1, 0) : 0;    // keys it attends
-    const int full = max(it.len - it.n + it.r0 / a.group + 1, 0);   // keys that all rows attend
-    const int end = max(it.len - it.n + min(it.n - 1, (it.r0 + kRows - 1) / a.group) + 1, 0);
-    const bool ragged = it.r0 + kRows > rows;
-    const int blk_end = (end + kScaleRows - 1) / kScaleRows;
-    const int count = (it.t1 - it.t0 + 1) / 2;         // tiles of a group, the last of group 1 perhaps none
-    auto tile_of = [&](int j) __attribute__((always_inline)) { return it.t0 + 2 * j + grp; };
-
-    if (threadIdx.x < D) s_nan[threadIdx.x] = kNoKey;
-
-    // Blocks of 1024 keys at a time, lane i the i-th: the current ones and the next.
-    constexpr int kTilesPerRef = 1024 / C::BN;
-    int ref_at = tile_of(0) / kTilesPerRef;
-    auto fetch = [&](int at) __attribute__((always_inline)) { return block_ref(c, it.b, kvh, at * 64 + lane, blk_end); };
-    BlockRef ra = fetch(ref_at), rb = fetch(ref_at + 1);
-    auto advance = [&](int tile) __attribute__((always_inline)) {
-      if (tile / kTilesPerRef > ref_at) {
-        ++ref_at;
-        ra = rb;
-        rb = fetch(ref_at + 1);
-      }
-    };
-    // block `i` (0 .. NB-1) of a tile
-    auto ref_lane = [&](int tile, int i) __attribute__((always_inline)) { return (tile * C::NB + i) & 63; };
-    auto bid_of = [&](int tile, int i) __attribute__((always_inline)) {
-      const int x = tile / kTilesPerRef > ref_at ? rb.bid : ra.bid;
-      const int bid = __builtin_amdgcn_readlane(x, ref_lane(tile, i));
-      return tile < it.t1 ? bid : -1;
-    };
-
-    // ---- DMA of a tile's codes -------------------------------------------
-    auto dma = [&](bool isv, int j) __attribute__((always_inline)) {
-      const int tile = tile_of(j);
-      unsigned char* dst = (isv ? v_raw : k_raw) + (j & 1) * C::RAW;
-      const uint8_t* pages = isv ? c.v_pages : c.k_pages;
-      const int ln = here(lane);
-#pragma unroll
-      for (int i = 0; i < C::DMA; ++i) {
-        const int piece = i * kGroupWaves + wave;               // KiB of the tile
-        const int bid = bid_of(tile, piece * 1024 / (kScaleRows * D));
-        const u32x4 rsrc = buffer_rsrc(pages + static_cast<size_t>(max(bid, 0)) * (kScaleRows * D), bid >= 0 ? kScaleRows * D : 0);
-        const int idx = piece * 64 + ln;
-        const int r = idx / C::CH, p = idx % C::CH;
-        const int off = (r % kScaleRows) * D + (isv ? p : p ^ piece_swizzle<D>(r)) * 16;
-        dma16_to_lds(rsrc, off, dst + piece * 1024);
-      }
-    };
-
-    // ---- codes -> operands ------------------------------------------------
-    auto scale_of = [&](bool isv, int tile, int blk) __attribute__((always_inline)) {
-      const bool next = tile / kTilesPerRef > ref_at;
-      return __shfl(isv ? (next ? rb.vs : ra.vs) : (next ? rb.ks : ra.ks), ref_lane(tile, blk));
-    };
-    auto convert_k = [&](int j) __attribute__((always_inline)) {
-      const int th = here(t);
-      const int r = th % C::BN, s0 = th / C::BN;
-      constexpr int kStep = kGroup / C::BN;
-      const float sc = scale_of(false, tile_of(j), r / kScaleRows);
-      unsigned char* dst0 = k_ops + (((r / 32) * C::STEPS + s0) * 64 + (r & 31)) * 16;
-      const unsigned char* raw0 = k_raw + (j & 1) * C::RAW + r * D;
-#pragma unroll
-      for (int i = 0; i < C::KI; ++i) {
-        const int s = s0 + kStep * i;                            // piece: MFMA step s
-        const u32x4 w = ld16(raw0 + ((s ^ piece_swizzle<D>(r)) << 4));
-        unsigned char* dst = dst0 + kStep * i * 1024;
-        *reinterpret_cast<u32x4*>(dst) = u32x4{fp8x2_to_bf16x2<false>(w[0], sc), fp8x2_to_bf16x2<true>(w[0], sc),
-                                               fp8x2_to_bf16x2<false>(w[1], sc), fp8x2_to_bf16x2<true>(w[1], sc)};
-        *reinterpret_cast<u32x4*>(dst + 512) = u32x4{fp8x2_to_bf16x2<false>(w[2], sc), fp8x2_to_bf16x2<true>(w[2], sc),
-                                                     fp8x2_to_bf16x2<false>(w[3], sc), fp8x2_to_bf16x2<true>(w[3], sc)};
-      }
-    };
-    // bit i: block i of the tile has a page and is this run's
-    constexpr unsigned kAllBlocks = (1u << C::NB) - 1;
-    auto held_blocks = [&](int tile) __attribute__((always_inline)) {
-      const int x = tile / kTilesPerRef > ref_at ? rb.bid : ra.bid;
-      return tile < it.t1 ? static_cast<unsigned>(__ballot(x >= 0) >> ref_lane(tile, 0)) & kAllBlocks : 0u;
-    };
-    auto is_masked = [&](int tile) __attribute__((always_inline)) {
-      return ragged || (tile + 1) * C::BN > full || held_blocks(tile) != kAllBlocks;
-    };
-    auto convert_v = [&](int j) __attribute__((always_inline)) {
-      if (D == 64 && wave >= 2) return;
-      const unsigned char* raw = v_raw + (j & 1) * C::RAW;
-      const int th = here(t);
-      const int o = th / (D / 4), dq = th % (D / 4);             // 8 keys x 4 dims
-      const int st = o >> 1, h8 = o & 1;                         // 16-key step of the tile, half
-      const int key = 16 * st + 4 * h8;
-      const float sc = scale_of(true, tile_of(j), st);
-      uint32_t v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        v[e] = *reinterpret_cast<const uint32_t*>(raw + (key + (e & 3) + 8 * (e >> 2)) * D + 4 * dq);
-      if (is_masked(tile_of(j))) {
-        if (!(held_blocks(tile_of(j)) >> st & 1)) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = 0u;
-        }
-        // 0 times NaN is NaN: a masked row must not carry one into the product.
-        // NaN codes are taken out and remembered by dim; the epilogue puts NaN
-        // into the rows that attend the first.
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          uint32_t n = nan_codes(v[e]);
-          if (n) {
-            v[e] &= ~((n >> 7) * 0xffu);
-            for (; n; n &= n - 1)
-              atomicMin(&s_nan[4 * dq + (__builtin_ctz(n) >> 3)], tile_of(j) * C::BN + key + (e & 3) + 8 * (e >> 2));
-          }
-        }
-      }
-      u32x4 w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t lo = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], 0x05010400u);
-        const uint32_t hi = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], 0x07030602u);
-        w[0][e] = fp8x2_to_bf16x2<false>(lo, sc);
-        w[1][e] = fp8x2_to_bf16x2<true>(lo, sc);
-        w[2][e] = fp8x2_to_bf16x2<false>(hi, sc);
-        w[3][e] = fp8x2_to_bf16x2<true>(hi, sc);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        int dt, m;
-        out_slot<D>(dq, i, &dt, &m);
-        *reinterpret_cast<u32x4*>(v_ops + ((st * C::DT + dt) * 64 + h8 * 32 + m) * 16) = w[i];
-      }
-    };
+    // tiles from this one on hold keys that not all rows attend (rows past the
+    // request's are computed, whatever they give, and not stored)
+    const int mask_from = max(it.len - it.n + it.r0 / a.group + 1, 0) / C::BN;
+    const int blk_end = (tile_end(a, it) + kScaleRows - 1) / kScaleRows;
 
     // ---- state ---------------------------------------------------------------
-    bf16x8_t q[C::STEPS];
+    bf16x8_t q[C::STEPS - C::QL];
+    {
+      const bf16* src = a.q + static_cast<size_t>(it.q0 + tok) * a.q_stride + static_cast<size_t>(kvh * a.group + row % a.group) * D + 8 * hf;
 #pragma unroll
-    for (int s = 0; s < C::STEPS; ++s) {
-      u32x4 w = {0u, 0u, 0u, 0u};
-      if (there) w = ld16(a.q + static_cast<size_t>(it.q0 + tok) * a.q_stride + static_cast<size_t>(h) * D + 16 * s + 8 * hf);
-      q[s] = as_bf16x8(w);
+      for (int s = 0; s < C::STEPS; ++s) {
+        u32x4 w = {0u, 0u, 0u, 0u};
+        if (there) w = ld16(src + 16 * s);
+        if (s >= C::QL) q[s - C::QL] = as_bf16x8(w);
+        else if (grp == 0) *reinterpret_cast<u32x4*>(s_q + ((wave * C::QL + s) * 64 + lane) * 16) = w;   // read behind barriers
+      }
     }
     f32x16 o[C::DT], sc[C::KT];
     u32x4 p[C::KT][2];
 #pragma unroll
     for (int d = 0; d < C::DT; ++d) o[d] = f32x16{};
     float m = -INFINITY, l = 0.f;
+    if (threadIdx.x < D) s_nan[threadIdx.x] = kNoKey;
 
-    // Operands are read AHEAD ahead of the products that take them; the schedule
-    // barriers keep it so (left alone, the compiler reads them all first, and
-    // spills).
-    auto pv = [&]() __attribute__((always_inline)) {
-      constexpr int N = 2 * C::KT * C::DT;
-      bf16x8_t v[N];
-#pragma unroll
-      for (int i = 0; i < C::AHEAD && i < N; ++i) v[i] = as_bf16x8(ld16(v_ops + (i * 64 + lane) * 16));
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (i + C::AHEAD < N) v[i + C::AHEAD] = as_bf16x8(ld16(v_ops + ((i + C::AHEAD) * 64 + lane) * 16));
-        const int s = i / C::DT, d = i % C::DT;
-        o[d] = mfma32(v[i], as_bf16x8(p[s >> 1][s & 1]), o[d]);
-        __builtin_amdgcn_sched_barrier(0);
+    for (int s0 = it.t0; s0 < it.t1; s0 += C::SEG / C::NB - 8) {
+      const int s1 = min(it.t1, s0 + C::SEG / C::NB - 8);
+      const int count = (s1 - s0 + 1) / 2;         // tiles of a group, the last of group 1 perhaps none
+      // group 1 walks the odd tiles of the segment; block 0 of tile j
+      auto first_block = [&](int j) __attribute__((always_inline)) { return (2 * j + grp) * C::NB; };
+      bool hole = false;
+      for (int i = threadIdx.x; i < (2 * count + 8) * C::NB; i += kThreads) {
+        const int blk = s0 * C::NB + i, last = min(blk_end, s1 * C::NB);
+        const BlockRef r = block_ref(c, it.b, kvh, blk, last);
+        hole |= blk < last && r.bid < 0;
+        s_bid[i] = r.bid;
+        s_ks[i] = r.ks;
+        s_vs[i] = r.vs;
       }
-    };
-    auto scores = [&]() __attribute__((always_inline)) {
-      constexpr int N = C::KT * C::STEPS;
-      auto load = [&](int i) __attribute__((always_inline)) {
-        return as_bf16x8(ld16(k_ops + ((i % C::KT * C::STEPS + i / C::KT) * 64 + lane) * 16));
+      const bool holes = __syncthreads_or(hole);
+
+      // ---- DMA of a tile's codes -----------------------------------------
+      // This wave's blocks of tile j (DMA KiB i of the wave: KiB 4 i + wave of the tile).
+      struct Bids { int b[C::DMA]; };
+      auto bids_of = [&](int j) __attribute__((always_inline)) {
+        Bids x;
+#pragma unroll
+        for (int i = 0; i < C::DMA; ++i) x.b[i] = s_bid[first_block(j) + (i * kGroupWaves + wave) / kKib];
+        return x;
       };
-      bf16x8_t k[N];
+      auto uniform = [&](Bids x) __attribute__((always_inline)) {
 #pragma unroll
-      for (int x = 0; x < C::KT; ++x) sc[x] = f32x16{};
+        for (int i = 0; i < C::DMA; ++i) x.b[i] = __builtin_amdgcn_readfirstlane(x.b[i]);
+        return x;
+      };
+      auto dma = [&](bool isv, int j, const Bids& x) __attribute__((always_inline)) {
+        unsigned char* dst = (isv ? v_raw : k_raw) + (j & 1) * C::RAW + wave * 1024;
+        const uint8_t* pages = (isv ? c.v_pages : c.k_pages) + wave % kKib * 1024;
 #pragma unroll
-      for (int i = 0; i < C::AHEAD && i < N; ++i) k[i] = load(i);
+        for (int i = 0; i < C::DMA; ++i) {
+          const u32x4 rsrc = buffer_rsrc(pages + (static_cast<size_t>(static_cast<uint32_t>(max(x.b[i], 0))) * (kScaleRows * D)),
+                                         x.b[i] >= 0 ? 1024 : 0);
+          dma16_to_lds(rsrc, isv ? static_cast<int>(ul * 16) : k_off, dst + i * kGroupWaves * 1024);
+        }
+      };
+
+      // ---- codes -> operands ----------------------------------------------
+      // K: a thread takes KI 16-code pieces of one row, kStep apart.
+      constexpr int kStep = kGroup / C::BN;
+      struct RawK { u32x4 w[C::KI]; float sc; };
+      auto load_k = [&](int j) __attribute__((always_inline)) {
+        RawK x;
+        const unsigned char* raw = k_raw + (j & 1) * C::RAW;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (i + C::AHEAD < N) k[i + C::AHEAD] = load(i + C::AHEAD);
-        sc[i % C::KT] = mfma32(k[i], q[i / C::KT], sc[i % C::KT]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    };
-    auto softmax = [&](int j) __attribute__((always_inline)) {
-      const int tile = tile_of(j);
-      if (is_masked(tile)) {
-        const unsigned held = held_blocks(tile);
-        const int rel = lim - tile * C::BN - 4 * hf;
+        for (int i = 0; i < C::KI; ++i) x.w[i] = ld16(raw + (kStep < 8 ? k_from ^ (i * kStep * 16) : k_from + i * kStep * 16));
+        x.sc = s_ks[first_block(j) + cr / kScaleRows];
+        return x;
+      };
+      auto store_k = [&](const RawK& x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < C::KI; ++i) {
+          const u32x4 w = x.w[i];
+          unsigned char* dst = k_ops + k_to + i * kStep * 1024;
+          *reinterpret_cast<u32x4*>(dst) = u32x4{fp8x2_to_bf16x2<false>(w[0], x.sc), fp8x2_to_bf16x2<true>(w[0], x.sc),
+                                                 fp8x2_to_bf16x2<false>(w[1], x.sc), fp8x2_to_bf16x2<true>(w[1], x.sc)};
+          *reinterpret_cast<u32x4*>(dst + 512) = u32x4{fp8x2_to_bf16x2<false>(w[2], x.sc), fp8x2_to_bf16x2<true>(w[2], x.sc),
+                                                       fp8x2_to_bf16x2<false>(w[3], x.sc), fp8x2_to_bf16x2<true>(w[3], x.sc)};
+        }
+      };
+      // V: a thread takes 8 keys x 4 dims, the keys 16 (oc / 2) + 4 (oc % 2) + {0..3, 8..11}.
+      struct RawV { uint32_t v[8]; float sc; };
+      auto load_v = [&](int j) __attribute__((always_inline)) {
+        RawV x;
+        const unsigned char* raw = v_raw + (j & 1) * C::RAW + v_from;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x.v[e] = *reinterpret_cast<const uint32_t*>(raw + ((e & 3) + 8 * (e >> 2)) * D);
+        x.sc = s_vs[first_block(j) + (oc >> 1)];
+        return x;
+      };
+      auto store_v = [&](RawV& x, int j, bool masked) __attribute__((always_inline)) {
+        if (masked) {
+          // 0 times NaN is NaN: a masked row must not carry one into the product.
+          // NaN codes are taken out and remembered by dim; the epilogue puts NaN
+          // into the rows that attend the first.
+          const uint32_t keep = s_bid[first_block(j) + (oc >> 1)] >= 0 ? 0xffffffffu : 0u;
+          uint32_t seen = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t n = nan_codes(x.v[e]) >> 7;
+            seen |= n & keep;
+            x.v[e] &= keep & ~(n * 0xffu);
+          }
+          if (seen) {
+            const unsigned char* raw = v_raw + (j & 1) * C::RAW + v_from;
+            const int key = s0 * C::BN + first_block(j) * kScaleRows + 16 * (oc >> 1) + 4 * (oc & 1);
+#pragma unroll 1
+            for (int e = 0; e < 32; ++e) {
+              const int r = (e >> 2 & 3) + 8 * (e >> 4);
+              if ((raw[r * D + (e & 3)] & 0x7f) == 0x7f) atomicMin(&s_nan[4 * dq + (e & 3)], key + r);
+            }
+          }
+        }
+        u32x4 w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t lo = __builtin_amdgcn_perm(x.v[2 * e + 1], x.v[2 * e], 0x05010400u);
+          const uint32_t hi = __builtin_amdgcn_perm(x.v[2 * e + 1], x.v[2 * e], 0x07030602u);
+          w[0][e] = fp8x2_to_bf16x2<false>(lo, x.sc);
+          w[1][e] = fp8x2_to_bf16x2<true>(lo, x.sc);
+          w[2][e] = fp8x2_to_bf16x2<false>(hi, x.sc);
+          w[3][e] = fp8x2_to_bf16x2<true>(hi, x.sc);
+        }
+        // byte i of the quad: the next part, or for D = 64 the other half of this one
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<u32x4*>(v_ops + v_to + (D == 64 ? (i >> 1) * 1024 + (i & 1) * 256 : i * 1024)) = w[i];
+      };
+      const bool v_threads = D != 64 || wave < 2;     // whole waves
+
+      // ---- products ----------------------------------------------------------
+      // Operands are read AHEAD ahead of the products that take them; the schedule
+      // barriers keep it so (left alone, the compiler reads them all first, and
+      // spills).
+      auto pv = [&]() __attribute__((always_inline)) {
+        constexpr int N = 2 * C::KT * C::DT;
+        bf16x8_t v[N];
+#pragma unroll
+        for (int i = 0; i < C::AHEAD && i < N; ++i) v[i] = as_bf16x8(ld16(v_ops + (i * 64 + lane) * 16));
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (i + C::AHEAD < N) v[i + C::AHEAD] = as_bf16x8(ld16(v_ops + ((i + C::AHEAD) * 64 + lane) * 16));
+          const int s = i / C::DT, d = i % C::DT;
+          o[d] = mfma32(v[i], as_bf16x8(p[s >> 1][s & 1]), o[d]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      auto scores = [&]() __attribute__((always_inline)) {
+        constexpr int N = C::KT * C::STEPS;
+        auto load = [&](int i) __attribute__((always_inline)) {
+          return as_bf16x8(ld16(k_ops + ((i % C::KT * C::STEPS + i / C::KT) * 64 + lane) * 16));
+        };
+        bf16x8_t k[N];
+#pragma unroll
+        for (int i = 0; i < C::AHEAD && i < N; ++i) k[i] = load(i);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (i + C::AHEAD < N) k[i + C::AHEAD] = load(i + C::AHEAD);
+          const int st = i / C::KT;
+          const bf16x8_t qs = st >= C::QL ? q[st >= C::QL ? st - C::QL : 0]
+                                          : as_bf16x8(ld16(s_q + ((wave * C::QL + st) * 64 + lane) * 16));
+          sc[i % C::KT] = mfma32(k[i], qs, i < C::KT ? f32x16{} : sc[i % C::KT]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      auto softmax = [&](int j, bool masked) __attribute__((always_inline)) {
+        if (masked) {
+          const int rel = lim - s0 * C::BN - first_block(j) * kScaleRows - 4 * hf;
+#pragma unroll
+          for (int k = 0; k < C::KT; ++k) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const int rb = s_bid[first_block(j) + 2 * k + g] >= 0 ? rel : -1;
+#pragma unroll
+              for (int i = 8 * g; i < 8 * g + 8; ++i)
+                if (32 * k + 8 * (i >> 2) + (i & 3) >= rb) sc[k][i] = -INFINITY;
+            }
+          }
+        }
+        float top = sc[0][0];
 #pragma unroll
         for (int k = 0; k < C::KT; ++k) {
 #pragma unroll
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[k][i]);
+        }
+        top = half_max(top) * a.scale_log2;
+        if (__ballot(top > m + kLazyLog2)) {
+          const float mn = fmaxf(m, top);
+          const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+          m = mn;
+          l *= alpha;
+#pragma unroll
+          for (int d = 0; d < C::DT; ++d) o[d] *= alpha;
+        }
+        const float nm = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+        for (int k = 0; k < C::KT; ++k) {
+          float x[16];
+#pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const bool ok = held >> (2 * k + (i >> 3)) & 1;
-            if (!(ok && 32 * k + 8 * (i >> 2) + (i & 3) < rel)) sc[k][i] = -INFINITY;
+            x[i] = fast_exp2(fmaf(sc[k][i], a.scale_log2, nm));
+            l += x[i];
           }
+          // P is rounded to bf16 once (half a step, 2^-8 of each weight, at random): its
+          // sum of two, as the decode takes, would double this product.
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[k][0][i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+            p[k][1][i] = pack_bf16x2(x[8 + 2 * i], x[9 + 2 * i]);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) pin(p[k][i]);    // made in this phase, not where the next one uses it
         }
-      }
-      float top = sc[0][0];
-#pragma unroll
-      for (int k = 0; k < C::KT; ++k) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[k][i]);
-      }
-      top = half_max(top) * a.scale_log2;
-      if (__ballot(top > m + kLazyLog2)) {
-        const float mn = fmaxf(m, top);
-        const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mn);
-        m = mn;
-        l *= alpha;
-#pragma unroll
-        for (int d = 0; d < C::DT; ++d) o[d] *= alpha;
-      }
-      const float nm = m == -INFINITY ? 0.f : -m;
-#pragma unroll
-      for (int k = 0; k < C::KT; ++k) {
-        float x[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          x[i] = fast_exp2(fmaf(sc[k][i], a.scale_log2, nm));
-          l += x[i];
-        }
-        // P is rounded to bf16 once (2^-9 of each weight, at random): its sum of two,
-        // as the decode takes, would double this product.
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[k][0][i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
-          p[k][1][i] = pack_bf16x2(x[8 + 2 * i], x[9 + 2 * i]);
-        }
-      }
-    };
+      };
+      const int mask_at = min(mask_from, s1);
+      auto masked_tile = [&](int j) __attribute__((always_inline)) { return holes || s0 + 2 * j + grp >= mask_at; };
 
-    // ---- the walk ---------------------------------------------------------------
-    dma(false, 0);
-    dma(true, 0);
-    dma(false, 1);
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm<0>());
-    __syncthreads();
-    convert_k(0);
-    __syncthreads();
-    if (grp == 1) phase_barrier();
-    for (int j = 0; j <= count; ++j) {
-      // M(j)
-      if (j < count) {
-        dma(false, j + 2);
-        dma(true, j + 1);
+      // ---- the walk -------------------------------------------------------------
+      Bids bv = uniform(bids_of(0)), bk;
+      dma(false, 0, bv);
+      dma(true, 0, bv);
+      bk = uniform(bids_of(1));
+      dma(false, 1, bk);
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm<0>());
+      __syncthreads();
+      store_k(load_k(0));
+      Bids next = bids_of(2);      // blocks of the tile whose K goes out next
+      __syncthreads();
+      if (grp == 1) phase_barrier();
+      auto issue = [&](int j) __attribute__((always_inline)) {   // V of tile j + 1, K of j + 2
+        bv = bk;
+        bk = uniform(next);
+        dma(true, j + 1, bv);
+        dma(false, j + 2, bk);
+        next = bids_of(j + 3);
+      };
+      issue(0);
+      scores();
+      for (int j = 0;;) {
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm<2 * C::DMA>());   // all but this phase's DMAs
+        phase_barrier();
+        // V(j)
+        const bool masked = masked_tile(j);
+        if (C::LOAD_FIRST) {
+          const RawK rk = load_k(j + 1);
+          RawV rv;
+          if (v_threads) rv = load_v(j);
+          softmax(j, masked);
+          store_k(rk);
+          if (v_threads) store_v(rv, j, masked);
+        } else {
+          if (v_threads) {
+            RawV rv = load_v(j);
+            store_v(rv, j, masked);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          store_k(load_k(j + 1));
+          __builtin_amdgcn_sched_barrier(0);
+          softmax(j, masked);
+        }
+        phase_barrier();
+        // M(j + 1)
+        ++j;
+        if (j < count) issue(j);
+        pv();
+        if (j == count) break;
+        scores();
       }
-      if (j > 0) pv();
-      if (j < count) scores();
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm<2 * C::DMA>());   // all but this phase's DMAs
-      phase_barrier();
-      // V(j)
-      if (j < count) {
-        advance(tile_of(j));
-        convert_v(j);
-        __builtin_amdgcn_sched_barrier(0);
-        convert_k(j + 1);
-        __builtin_amdgcn_sched_barrier(0);
-        softmax(j);
-      }
-      phase_barrier();
+      if (grp == 0) phase_barrier();
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm<0>());
+      __syncthreads();
     }
-    if (grp == 0) phase_barrier();
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm<0>());
-    __syncthreads();
 
     // ---- the groups' states meet ---------------------------------------------
     {
