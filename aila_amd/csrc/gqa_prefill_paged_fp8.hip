@@ -85,7 +85,7 @@ struct Cfg {
   static constexpr int AHEAD = D == 256 ? 2 : 4;  // LDS operand reads in flight ahead of their MFMAs
   static constexpr int SEG = D == 256 ? 768 : 2048;   // blocks of a segment of keys, looked up at once
   static constexpr int QL = D == 256 ? 5 : 0;     // MFMA steps whose query operand is kept in LDS: the registers do not hold it
-  static constexpr bool LOAD_FIRST = D != 256;    // a vector phase reads its codes before its softmax
+  static constexpr bool LOAD_FIRST = true;    // a vector phase reads its codes before its softmax
   static constexpr int GROUP_LDS = 2 * OPS + 4 * RAW;
   static constexpr int LDS = 2 * GROUP_LDS;
   static_assert(LDS >= kGroupWaves * DT * 16 * 64 * 4, "the groups' outputs meet in LDS");
@@ -601,6 +601,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
         __builtin_amdgcn_s_waitcnt(vmcnt_imm<2 * C::DMA>());   // all but this phase's DMAs
         phase_barrier();
         // V(j)
+        __builtin_amdgcn_s_setprio(0);
         const bool masked = masked_tile(j);
         if (C::LOAD_FIRST) {
           const RawK rk = load_k(j + 1);
@@ -621,6 +622,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
         }
         phase_barrier();
         // M(j + 1)
+        __builtin_amdgcn_s_setprio(1);
         ++j;
         if (j < count) issue(j);
         pv();
