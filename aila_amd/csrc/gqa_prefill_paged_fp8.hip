@@ -82,10 +82,9 @@ struct Cfg {
   static constexpr int RAW = BN * D;              // bytes of a tile as codes
   static constexpr int DMA = RAW / (1024 * kGroupWaves);   // DMA instructions a wave and tile
   static constexpr int KI = BN * CH / kGroup;     // 16-code pieces of K a thread converts
-  static constexpr int AHEAD = D == 256 ? 2 : 4;  // LDS operand reads in flight ahead of their MFMAs
+  static constexpr int AHEAD = D == 256 ? 3 : 4;  // LDS operand reads in flight ahead of their MFMAs
   static constexpr int SEG = D == 256 ? 768 : 2048;   // blocks of a segment of keys, looked up at once
   static constexpr int QL = D == 256 ? 5 : 0;     // MFMA steps whose query operand is kept in LDS: the registers do not hold it
-  static constexpr bool LOAD_FIRST = true;    // a vector phase reads its codes before its softmax
   static constexpr int GROUP_LDS = 2 * OPS + 4 * RAW;
   static constexpr int LDS = 2 * GROUP_LDS;
   static_assert(LDS >= kGroupWaves * DT * 16 * 64 * 4, "the groups' outputs meet in LDS");
@@ -112,6 +111,11 @@ __device__ __forceinline__ float half_sum(float x) {
 __device__ __forceinline__ int here(int x) {
   asm volatile("" : "+v"(x));
   return x;
+}
+
+// acc + the two bf16 of x.
+__device__ __forceinline__ float add_pair(uint32_t x, float acc) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), acc, false);
 }
 
 __device__ __forceinline__ void pin(u32x4& x) { asm volatile("" : "+v"(x)); }
@@ -405,15 +409,16 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
         for (int i = 0; i < C::DMA; ++i) x.b[i] = __builtin_amdgcn_readfirstlane(x.b[i]);
         return x;
       };
-      auto dma = [&](bool isv, int j, const Bids& x) __attribute__((always_inline)) {
+      auto dma_one = [&](bool isv, int j, const Bids& x, int i) __attribute__((always_inline)) {
         unsigned char* dst = (isv ? v_raw : k_raw) + (j & 1) * C::RAW + wave * 1024;
         const uint8_t* pages = (isv ? c.v_pages : c.k_pages) + wave % kKib * 1024;
+        const u32x4 rsrc = buffer_rsrc(pages + (static_cast<size_t>(static_cast<uint32_t>(max(x.b[i], 0))) * (kScaleRows * D)),
+                                       x.b[i] >= 0 ? 1024 : 0);
+        dma16_to_lds(rsrc, isv ? static_cast<int>(ul * 16) : k_off, dst + i * kGroupWaves * 1024);
+      };
+      auto dma = [&](bool isv, int j, const Bids& x) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < C::DMA; ++i) {
-          const u32x4 rsrc = buffer_rsrc(pages + (static_cast<size_t>(static_cast<uint32_t>(max(x.b[i], 0))) * (kScaleRows * D)),
-                                         x.b[i] >= 0 ? 1024 : 0);
-          dma16_to_lds(rsrc, isv ? static_cast<int>(ul * 16) : k_off, dst + i * kGroupWaves * 1024);
-        }
+        for (int i = 0; i < C::DMA; ++i) dma_one(isv, j, x, i);
       };
 
       // ---- codes -> operands ----------------------------------------------
@@ -490,37 +495,42 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
       const bool v_threads = D != 64 || wave < 2;     // whole waves
 
       // ---- products ----------------------------------------------------------
-      // Operands are read AHEAD ahead of the products that take them; the schedule
-      // barriers keep it so (left alone, the compiler reads them all first, and
-      // spills).
-      auto pv = [&]() __attribute__((always_inline)) {
-        constexpr int N = 2 * C::KT * C::DT;
-        bf16x8_t v[N];
+      // A matrix phase: O += V P of the tile before (PV), then S = K Q of this one
+      // (QK), one row of products whose operands are read AHEAD ahead of them. What
+      // else the phase has to do (the next DMAs) goes between the products, a step
+      // every second one, where it costs no time; the schedule barriers keep it all
+      // so (left alone, the compiler reads the operands first, and spills).
+      constexpr int NP = 2 * C::KT * C::DT, NQ = C::KT * C::STEPS;
+      bf16x8_t ahead[C::AHEAD];     // the first operands of QK, read during PV
+      auto load_qk = [&](int i) __attribute__((always_inline)) {
+        return as_bf16x8(ld16(k_ops + ((i % C::KT * C::STEPS + i / C::KT) * 64 + lane) * 16));
+      };
+      auto pv = [&](auto&& step) __attribute__((always_inline)) {
+        auto load = [&](int i) __attribute__((always_inline)) { return as_bf16x8(ld16(v_ops + (i * 64 + lane) * 16)); };
+        bf16x8_t x[NP];
 #pragma unroll
-        for (int i = 0; i < C::AHEAD && i < N; ++i) v[i] = as_bf16x8(ld16(v_ops + (i * 64 + lane) * 16));
+        for (int i = 0; i < C::AHEAD; ++i) x[i] = load(i);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if (i + C::AHEAD < N) v[i + C::AHEAD] = as_bf16x8(ld16(v_ops + ((i + C::AHEAD) * 64 + lane) * 16));
+        for (int i = 0; i < NP; ++i) {
+          if (i + C::AHEAD < NP) x[i + C::AHEAD] = load(i + C::AHEAD);
+          else ahead[i + C::AHEAD - NP] = load_qk(i + C::AHEAD - NP);
           const int s = i / C::DT, d = i % C::DT;
-          o[d] = mfma32(v[i], as_bf16x8(p[s >> 1][s & 1]), o[d]);
+          o[d] = mfma32(x[i], as_bf16x8(p[s >> 1][s & 1]), o[d]);
+          if (i & 1) step(i / 2);
           __builtin_amdgcn_sched_barrier(0);
         }
       };
       auto scores = [&]() __attribute__((always_inline)) {
-        constexpr int N = C::KT * C::STEPS;
-        auto load = [&](int i) __attribute__((always_inline)) {
-          return as_bf16x8(ld16(k_ops + ((i % C::KT * C::STEPS + i / C::KT) * 64 + lane) * 16));
-        };
-        bf16x8_t k[N];
+        bf16x8_t x[NQ];
 #pragma unroll
-        for (int i = 0; i < C::AHEAD && i < N; ++i) k[i] = load(i);
+        for (int i = 0; i < C::AHEAD; ++i) x[i] = ahead[i];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if (i + C::AHEAD < N) k[i + C::AHEAD] = load(i + C::AHEAD);
+        for (int i = 0; i < NQ; ++i) {
+          if (i + C::AHEAD < NQ) x[i + C::AHEAD] = load_qk(i + C::AHEAD);
           const int st = i / C::KT;
           const bf16x8_t qs = st >= C::QL ? q[st >= C::QL ? st - C::QL : 0]
                                           : as_bf16x8(ld16(s_q + ((wave * C::QL + st) * 64 + lane) * 16));
-          sc[i % C::KT] = mfma32(k[i], qs, i < C::KT ? f32x16{} : sc[i % C::KT]);
+          sc[i % C::KT] = mfma32(x[i], qs, i < C::KT ? f32x16{} : sc[i % C::KT]);
           __builtin_amdgcn_sched_barrier(0);
         }
       };
@@ -538,13 +548,16 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
             }
           }
         }
-        float top = sc[0][0];
+        float t0 = sc[0][0], t1 = sc[0][8];     // two chains
 #pragma unroll
         for (int k = 0; k < C::KT; ++k) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[k][i]);
+          for (int i = 0; i < 8; ++i) {
+            t0 = fmaxf(t0, sc[k][i]);
+            t1 = fmaxf(t1, sc[k][8 + i]);
+          }
         }
-        top = half_max(top) * a.scale_log2;
+        const float top = half_max(fmaxf(t0, t1)) * a.scale_log2;
         if (__ballot(top > m + kLazyLog2)) {
           const float mn = fmaxf(m, top);
           const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mn);
@@ -554,24 +567,29 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
           for (int d = 0; d < C::DT; ++d) o[d] *= alpha;
         }
         const float nm = m == -INFINITY ? 0.f : -m;
+        float l1 = 0.f;
 #pragma unroll
         for (int k = 0; k < C::KT; ++k) {
           float x[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            x[i] = fast_exp2(fmaf(sc[k][i], a.scale_log2, nm));
-            l += x[i];
-          }
+          for (int i = 0; i < 16; ++i) x[i] = fast_exp2(fmaf(sc[k][i], a.scale_log2, nm));
           // P is rounded to bf16 once (half a step, 2^-8 of each weight, at random): its
-          // sum of two, as the decode takes, would double this product.
+          // sum of two, as the decode takes, would double this product. The sum is
+          // taken of the rounded weights, in fp32, so that they add up to 1.
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             p[k][0][i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
             p[k][1][i] = pack_bf16x2(x[8 + 2 * i], x[9 + 2 * i]);
           }
 #pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            l = add_pair(p[k][0][i], l);
+            l1 = add_pair(p[k][1][i], l1);
+          }
+#pragma unroll
           for (int i = 0; i < 2; ++i) pin(p[k][i]);    // made in this phase, not where the next one uses it
         }
+        l += l1;
       };
       const int mask_at = min(mask_from, s1);
       auto masked_tile = [&](int j) __attribute__((always_inline)) { return holes || s0 + 2 * j + grp >= mask_at; };
@@ -588,14 +606,23 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
       Bids next = bids_of(2);      // blocks of the tile whose K goes out next
       __syncthreads();
       if (grp == 1) phase_barrier();
-      auto issue = [&](int j) __attribute__((always_inline)) {   // V of tile j + 1, K of j + 2
-        bv = bk;
-        bk = uniform(next);
-        dma(true, j + 1, bv);
-        dma(false, j + 2, bk);
-        next = bids_of(j + 3);
+      // In M(j): V of tile j + 1 and K of j + 2 (past the last tile: empty blocks).
+      auto issue = [&](int j, int step) __attribute__((always_inline)) {
+        if (step == 0) {
+          bv = bk;
+          bk = uniform(next);
+        } else if (step <= C::DMA) {
+          dma_one(true, j + 1, bv, step - 1);
+        } else if (step <= 2 * C::DMA) {
+          dma_one(false, j + 2, bk, step - 1 - C::DMA);
+        } else if (step == 2 * C::DMA + 1) {
+          next = bids_of(j + 3);
+        }
       };
-      issue(0);
+#pragma unroll
+      for (int step = 0; step < 2 * C::DMA + 2; ++step) issue(0, step);
+#pragma unroll
+      for (int i = 0; i < C::AHEAD; ++i) ahead[i] = load_qk(i);
       scores();
       for (int j = 0;;) {
         __builtin_amdgcn_s_waitcnt(vmcnt_imm<2 * C::DMA>());   // all but this phase's DMAs
@@ -603,29 +630,17 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
         // V(j)
         __builtin_amdgcn_s_setprio(0);
         const bool masked = masked_tile(j);
-        if (C::LOAD_FIRST) {
-          const RawK rk = load_k(j + 1);
-          RawV rv;
-          if (v_threads) rv = load_v(j);
-          softmax(j, masked);
-          store_k(rk);
-          if (v_threads) store_v(rv, j, masked);
-        } else {
-          if (v_threads) {
-            RawV rv = load_v(j);
-            store_v(rv, j, masked);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          store_k(load_k(j + 1));
-          __builtin_amdgcn_sched_barrier(0);
-          softmax(j, masked);
-        }
+        const RawK rk = load_k(j + 1);
+        RawV rv;
+        if (v_threads) rv = load_v(j);
+        softmax(j, masked);
+        store_k(rk);
+        if (v_threads) store_v(rv, j, masked);
         phase_barrier();
         // M(j + 1)
         __builtin_amdgcn_s_setprio(1);
         ++j;
-        if (j < count) issue(j);
-        pv();
+        pv([&](int step) __attribute__((always_inline)) { issue(j, step); });
         if (j == count) break;
         scores();
       }
