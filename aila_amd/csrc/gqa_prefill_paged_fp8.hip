@@ -28,6 +28,7 @@
 #include "paged_fp8.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace aila {
 namespace {
@@ -83,11 +84,11 @@ struct Cfg {
   static constexpr int DMA = RAW / (1024 * kGroupWaves);   // DMA instructions a wave and tile
   static constexpr int KI = BN * CH / kGroup;     // 16-code pieces of K a thread converts
   static constexpr int AHEAD = D == 256 ? 3 : 4;  // LDS operand reads in flight ahead of their MFMAs
-  static constexpr int SEG = D == 256 ? 768 : 2048;   // blocks of a segment of keys, looked up at once
+  static constexpr int SEG = D == 256 ? 704 : 2048;   // blocks of a segment of keys, looked up at once
   static constexpr int QL = D == 256 ? 5 : 0;     // MFMA steps whose query operand is kept in LDS: the registers do not hold it
-  static constexpr int GROUP_LDS = 2 * OPS + 4 * RAW;
-  static constexpr int LDS = 2 * GROUP_LDS;
-  static_assert(LDS >= kGroupWaves * DT * 16 * 64 * 4, "the groups' outputs meet in LDS");
+  static constexpr int LDS = 2 * (2 * OPS + 4 * RAW);
+  static constexpr int XR = D == 256 ? 2 : 1;     // rounds in which the groups exchange their outputs
+  static_assert(2 * OPS >= kGroupWaves * DT / XR * 2 * 1024, "half a group's outputs fit its operands' place");
   static constexpr int REC = kRows * (D + 2);     // floats of a record: {o[rows][D], {m, l}[rows]}
 };
 
@@ -181,13 +182,19 @@ __device__ __forceinline__ bool get_item(const Fp8PrefillArgs& a, int index, Ite
   }
   load_request(a, 0, it);
   const int tiles = (it->n * a.group + kRows - 1) / kRows;
-  const int rank = index / a.splits, cut = index % a.splits;
+  const int rank = a.splits > 1 ? index / a.splits : index, cut = index - rank * a.splits;
   if (rank >= tiles) return false;
   it->r0 = (tiles - 1 - rank) * kRows;
-  const int kt = (tile_end(a, *it) + Cfg<D>::BN - 1) / Cfg<D>::BN;
-  it->t0 = static_cast<int>(static_cast<long>(kt) * cut / a.splits);
-  it->t1 = static_cast<int>(static_cast<long>(kt) * (cut + 1) / a.splits);
-  it->rec = a.splits > 1 ? index : -1;
+  const unsigned kt = (tile_end(a, *it) + Cfg<D>::BN - 1) / Cfg<D>::BN;
+  it->t0 = 0;
+  it->t1 = kt;
+  it->rec = -1;
+  if (a.splits > 1) {
+    const unsigned n = a.splits, each = kt / n, rest = kt % n;   // run i begins at floor(i kt / n)
+    it->t0 = each * cut + rest * cut / n;
+    it->t1 = each * (cut + 1) + rest * (cut + 1) / n;
+    it->rec = index;
+  }
   return true;
 }
 
@@ -315,7 +322,8 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
   using C = Cfg<D>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char s_dyn[];
   __shared__ int s_nan[D];      // first masked-tile key whose V holds NaN in this dim
-  __shared__ float s_ml[kRows][2];
+  __shared__ int s_any_nan;
+  __shared__ float s_ml[2][kRows][2];
   // Blocks of the segment of keys being walked: index in the pool (-1: none), scales.
   __shared__ __attribute__((aligned(16))) int s_bid[C::SEG];
   __shared__ float s_ks[C::SEG], s_vs[C::SEG];
@@ -324,11 +332,11 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
   const int t = threadIdx.x % kGroup, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int l32 = lane & 31, hf = lane >> 5;
-  unsigned char* mine = s_dyn + grp * C::GROUP_LDS;
-  unsigned char* k_ops = mine;
-  unsigned char* v_ops = mine + C::OPS;
-  unsigned char* k_raw = mine + 2 * C::OPS;            // two tiles
-  unsigned char* v_raw = k_raw + 2 * C::RAW;           // two tiles
+  // operands of both groups (the exchange of their outputs at the end), then codes
+  unsigned char* k_ops = s_dyn + grp * 2 * C::OPS;
+  unsigned char* v_ops = k_ops + C::OPS;
+  unsigned char* k_raw = s_dyn + 4 * C::OPS + grp * 4 * C::RAW;   // two tiles
+  unsigned char* v_raw = k_raw + 2 * C::RAW;                      // two tiles
   // This thread's places, in bytes: of its codes in a page (K: pieces exchanged;
   // V: lane * 16), of the codes it converts, and of the operands it makes.
   constexpr int kKib = kScaleRows * D / 1024;          // KiB of a block
@@ -345,11 +353,51 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
   const int v_to = (((oc >> 1) * C::DT + v_dt) * 64 + (oc & 1) * 32 + v_row) * 16;
   const int kvh = static_cast<int>(blockIdx.x) % c.Hkv, wl = static_cast<int>(blockIdx.x) / c.Hkv;
 
-  for (int round = 0;; ++round) {
-    // heavy items go out in order, the next round's in the reverse order
-    const int index = round * a.lanes + (round & 1 ? a.lanes - 1 - wl : wl);
-    Item it;
-    if (!get_item<D>(a, index, &it)) break;   // nor is there a later one
+  // group 1 walks the odd tiles of the segment; block 0 of tile j
+  auto first_block = [&](int j) __attribute__((always_inline)) { return (2 * j + grp) * C::NB; };
+
+  // ---- DMA of a tile's codes -----------------------------------------
+  // This wave's blocks of tile j (DMA KiB i of the wave: KiB 4 i + wave of the tile).
+  struct Bids { int b[C::DMA]; };
+  auto bids_of = [&](int j) __attribute__((always_inline)) {
+    Bids x;
+#pragma unroll
+    for (int i = 0; i < C::DMA; ++i) x.b[i] = s_bid[first_block(j) + (i * kGroupWaves + wave) / kKib];
+    return x;
+  };
+  auto uniform = [&](Bids x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < C::DMA; ++i) x.b[i] = __builtin_amdgcn_readfirstlane(x.b[i]);
+    return x;
+  };
+  auto dma_one = [&](bool isv, int j, const Bids& x, int i) __attribute__((always_inline)) {
+    unsigned char* dst = (isv ? v_raw : k_raw) + (j & 1) * C::RAW + wave * 1024;
+    const uint8_t* pages = (isv ? c.v_pages : c.k_pages) + wave % kKib * 1024;
+    const u32x4 rsrc = buffer_rsrc(pages + (static_cast<size_t>(static_cast<uint32_t>(max(x.b[i], 0))) * (kScaleRows * D)),
+                                   x.b[i] >= 0 ? 1024 : 0);
+    dma16_to_lds(rsrc, isv ? static_cast<int>(ul * 16) : k_off, dst + i * kGroupWaves * 1024);
+  };
+  auto dma = [&](bool isv, int j, const Bids& x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < C::DMA; ++i) dma_one(isv, j, x, i);
+  };
+
+  auto start = [&]() __attribute__((always_inline)) {
+    const Bids x = uniform(bids_of(0));
+    dma(false, 0, x);
+    dma(true, 0, x);
+    dma(false, 1, uniform(bids_of(1)));
+  };
+
+  // heavy items go out in order, the next round's in the reverse order
+  auto item_at = [&](int round) __attribute__((always_inline)) {
+    return round * a.lanes + (round & 1 ? a.lanes - 1 - wl : wl);
+  };
+  Item it;
+  bool more = get_item<D>(a, item_at(0), &it);
+  int seg_b = -1, seg_0 = 0, seg_1 = 0;     // the segment whose blocks are in LDS
+  bool holes = false, primed = false;       // primed: its first DMAs are on the way
+  for (int round = 1; more; ++round) {
     const int rows = it.n * a.group;
     const int row = it.r0 + wave * 32 + l32;          // this lane's query row
     const bool there = row < rows;
@@ -377,49 +425,29 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
 #pragma unroll
     for (int d = 0; d < C::DT; ++d) o[d] = f32x16{};
     float m = -INFINITY, l = 0.f;
-    if (threadIdx.x < D) s_nan[threadIdx.x] = kNoKey;
 
+    if (it.t0 == it.t1) {     // no keys: straight to the output
+      __syncthreads();
+      if (threadIdx.x == 0) s_any_nan = 0;
+    }
     for (int s0 = it.t0; s0 < it.t1; s0 += C::SEG / C::NB - 8) {
       const int s1 = min(it.t1, s0 + C::SEG / C::NB - 8);
       const int count = (s1 - s0 + 1) / 2;         // tiles of a group, the last of group 1 perhaps none
-      // group 1 walks the odd tiles of the segment; block 0 of tile j
-      auto first_block = [&](int j) __attribute__((always_inline)) { return (2 * j + grp) * C::NB; };
-      bool hole = false;
-      for (int i = threadIdx.x; i < (2 * count + 8) * C::NB; i += kThreads) {
-        const int blk = s0 * C::NB + i, last = min(blk_end, s1 * C::NB);
-        const BlockRef r = block_ref(c, it.b, kvh, blk, last);
-        hole |= blk < last && r.bid < 0;
-        s_bid[i] = r.bid;
-        s_ks[i] = r.ks;
-        s_vs[i] = r.vs;
+      const bool reuse = seg_b == it.b && seg_0 == s0 && s1 <= seg_1 && s1 == it.t1 && it.rec < 0;
+      const int last = min(blk_end, s1 * C::NB), fill = (2 * count + 8) * C::NB;
+      if (!reuse) {
+        bool hole = false;
+        for (int i = threadIdx.x; i < fill; i += kThreads) {
+          const int blk = s0 * C::NB + i;
+          const int bid = blk < last ? block_id(c, it.b, kvh, blk) : -1;
+          hole |= blk < last && bid < 0;
+          s_bid[i] = bid;
+        }
+        holes = __syncthreads_or(hole);
+        seg_b = it.b;
+        seg_0 = s0;
+        seg_1 = s1;
       }
-      const bool holes = __syncthreads_or(hole);
-
-      // ---- DMA of a tile's codes -----------------------------------------
-      // This wave's blocks of tile j (DMA KiB i of the wave: KiB 4 i + wave of the tile).
-      struct Bids { int b[C::DMA]; };
-      auto bids_of = [&](int j) __attribute__((always_inline)) {
-        Bids x;
-#pragma unroll
-        for (int i = 0; i < C::DMA; ++i) x.b[i] = s_bid[first_block(j) + (i * kGroupWaves + wave) / kKib];
-        return x;
-      };
-      auto uniform = [&](Bids x) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < C::DMA; ++i) x.b[i] = __builtin_amdgcn_readfirstlane(x.b[i]);
-        return x;
-      };
-      auto dma_one = [&](bool isv, int j, const Bids& x, int i) __attribute__((always_inline)) {
-        unsigned char* dst = (isv ? v_raw : k_raw) + (j & 1) * C::RAW + wave * 1024;
-        const uint8_t* pages = (isv ? c.v_pages : c.k_pages) + wave % kKib * 1024;
-        const u32x4 rsrc = buffer_rsrc(pages + (static_cast<size_t>(static_cast<uint32_t>(max(x.b[i], 0))) * (kScaleRows * D)),
-                                       x.b[i] >= 0 ? 1024 : 0);
-        dma16_to_lds(rsrc, isv ? static_cast<int>(ul * 16) : k_off, dst + i * kGroupWaves * 1024);
-      };
-      auto dma = [&](bool isv, int j, const Bids& x) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < C::DMA; ++i) dma_one(isv, j, x, i);
-      };
 
       // ---- codes -> operands ----------------------------------------------
       // K: a thread takes KI 16-code pieces of one row, kStep apart.
@@ -473,7 +501,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
 #pragma unroll 1
             for (int e = 0; e < 32; ++e) {
               const int r = (e >> 2 & 3) + 8 * (e >> 4);
-              if ((raw[r * D + (e & 3)] & 0x7f) == 0x7f) atomicMin(&s_nan[4 * dq + (e & 3)], key + r);
+              if ((raw[r * D + (e & 3)] & 0x7f) == 0x7f) s_any_nan = 1, atomicMin(&s_nan[4 * dq + (e & 3)], key + r);
             }
           }
         }
@@ -595,13 +623,20 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
       auto masked_tile = [&](int j) __attribute__((always_inline)) { return holes || s0 + 2 * j + grp >= mask_at; };
 
       // ---- the walk -------------------------------------------------------------
-      Bids bv = uniform(bids_of(0)), bk;
-      dma(false, 0, bv);
-      dma(true, 0, bv);
-      bk = uniform(bids_of(1));
-      dma(false, 1, bk);
+      if (!primed) start();
+      if (!reuse) {
+        for (int i = threadIdx.x; i < fill; i += kThreads) {
+          const int bid = s_bid[i];
+          s_ks[i] = bid >= 0 ? c.k_scale[bid] : 0.f;
+          s_vs[i] = bid >= 0 ? c.v_scale[bid] : 0.f;
+        }
+      }
+      primed = false;
+      Bids bv, bk = uniform(bids_of(1));
       __builtin_amdgcn_s_waitcnt(vmcnt_imm<0>());
       __syncthreads();
+      if (threadIdx.x < D && s0 == it.t0) s_nan[threadIdx.x] = kNoKey;
+      if (threadIdx.x == 0 && s0 == it.t0) s_any_nan = 0;
       store_k(load_k(0));
       Bids next = bids_of(2);      // blocks of the tile whose K goes out next
       __syncthreads();
@@ -649,85 +684,118 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
       __syncthreads();
     }
 
-    // ---- the groups' states meet ---------------------------------------------
-    {
-    const int lane = here(threadIdx.x & 63), l32 = lane & 31, hf = lane >> 5;
-    const int row = it.r0 + wave * 32 + l32;
-    const bool there = row < rows;
-    const int tok = there ? row / a.group : 0;
-    const int h = kvh * a.group + row % a.group;
-    l = half_sum(l);
-    float* s_o = reinterpret_cast<float*>(s_dyn);                                    // [wave][part][quad][lane] f32x4
-    if (grp == 1) {
-#pragma unroll
-      for (int d = 0; d < C::DT; ++d) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<f32x4*>(s_o + (((wave * C::DT + d) * 4 + i) * 64 + lane) * 4) =
-              f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-      }
-      if (hf == 0) {
-        s_ml[wave * 32 + l32][0] = m;
-        s_ml[wave * 32 + l32][1] = l;
-      }
+    // ---- the groups' states meet -----------------------------------------------
+    // The next item's first codes are fetched meanwhile, if it walks the same keys.
+    const Item done = it;
+    more = get_item<D>(a, item_at(round), &it);
+    if (more && it.b == seg_b && it.t0 == seg_0 && it.t0 < it.t1 && it.t1 <= seg_1 && it.rec < 0) {
+      start();
+      primed = true;
     }
-    __syncthreads();
-    if (grp == 0) {
-      const float m2 = s_ml[wave * 32 + l32][0], l2 = s_ml[wave * 32 + l32][1];
-      const float mm = fmaxf(m, m2);
-      const float f1 = m == -INFINITY ? 0.f : fast_exp2(m - mm), f2 = m2 == -INFINITY ? 0.f : fast_exp2(m2 - mm);
-      const float ll = f1 * l + f2 * l2;
-      const float inv = it.rec >= 0 ? 1.0f : ll == 0.f ? 0.f : 1.0f / ll;
-      float* rec = it.rec >= 0 ? a.part + (static_cast<size_t>(it.rec) * c.Hkv + kvh) * C::REC : nullptr;
+    l = half_sum(l);
+    const int ln = here(threadIdx.x & 63), row32 = wave * 32 + (ln & 31);
+    if (ln < 32) {
+      s_ml[grp][row32][0] = m;
+      s_ml[grp][row32][1] = l;
+    }
+    // Each group finishes half of the output: quads (4 rows of a part) {0, 1} and
+    // {2, 3}, or, for D = 64, {0, 2} and {1, 3}; the other half it hands over.
+    auto finish = [&](auto gtag) __attribute__((always_inline)) {
+      constexpr int G = decltype(gtag)::value;
+      constexpr int P = C::DT / C::XR;
+      constexpr int kOwn[2] = {D == 64 ? G : 2 * G, D == 64 ? G + 2 : 2 * G + 1};
+      constexpr int kOther[2] = {D == 64 ? 1 - G : 2 - 2 * G, D == 64 ? 3 - G : 3 - 2 * G};
+      unsigned char* give = s_dyn + G * 2 * C::OPS + wave * P * 2048 + ln * 16;
+      const unsigned char* take = s_dyn + (1 - G) * 2 * C::OPS + wave * P * 2048 + ln * 16;
+      float f1 = 0.f, f2 = 0.f, mm = 0.f, ll = 0.f;
 #pragma unroll
-      for (int d = 0; d < C::DT; ++d) {
+      for (int r = 0; r < C::XR; ++r) {
+        if (r > 0) __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(s_o + (((wave * C::DT + d) * 4 + i) * 64 + lane) * 4);
+        for (int d = 0; d < P; ++d) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float y = (o[d][4 * i + e] * f1 + x[e] * f2) * inv;
-            // rows 8 i + 4 hf + e of the part
-            if (s_nan[out_dim<D>(d, 8 * i + 4 * hf + e)] < lim) y = __uint_as_float(0x7fc00000u);
-            o[d][4 * i + e] = y;
+          for (int i = 0; i < 2; ++i) {
+            const f32x16& x = o[r * P + d];
+            *reinterpret_cast<f32x4*>(give + (d * 2 + i) * 1024) =
+                f32x4{x[4 * kOther[i]], x[4 * kOther[i] + 1], x[4 * kOther[i] + 2], x[4 * kOther[i] + 3]};
+          }
+        }
+        __syncthreads();
+        if (r == 0) {
+          const float m2 = s_ml[1 - G][row32][0], l2 = s_ml[1 - G][row32][1];
+          mm = fmaxf(m, m2);
+          f1 = m == -INFINITY ? 0.f : fast_exp2(m - mm);
+          f2 = m2 == -INFINITY ? 0.f : fast_exp2(m2 - mm);
+          ll = f1 * l + f2 * l2;
+          if (done.rec < 0) {
+            const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+            f1 *= inv;
+            f2 *= inv;
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < P; ++d) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(take + (d * 2 + i) * 1024);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y = o[r * P + d][4 * kOwn[i] + e];
+              o[r * P + d][4 * kOwn[i] + e] = y * f1 + x[e] * f2;
+            }
           }
         }
       }
-      if (rec != nullptr) {
+      const int hf = ln >> 5, row = done.r0 + row32;
+      if (s_any_nan) {
+        const int tok = row / a.group;
+        const int lim = max(done.len - done.n + tok + 1, 0);
 #pragma unroll
         for (int d = 0; d < C::DT; ++d) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<f32x4*>(rec + (((wave * C::DT + d) * 4 + i) * 64 + lane) * 4) =
-                f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-        }
-        if (hf == 0) {
-          rec[kRows * D + (wave * 32 + l32) * 2] = mm;
-          rec[kRows * D + (wave * 32 + l32) * 2 + 1] = ll;
-        }
-      } else if (there) {
-        bf16* dst = a.out + (static_cast<size_t>(it.q0 + tok) * a.Hq + h) * D;
-        if constexpr (D == 64) {
-#pragma unroll
           for (int i = 0; i < 2; ++i) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)   // dims 4 m + {0, 1, 2, 3} from rows m and m + 16 of both parts
-              *reinterpret_cast<u32x2*>(dst + 4 * (8 * i + 4 * hf + e)) =
-                  u32x2{pack_bf16x2(o[0][4 * i + e], o[0][8 + 4 * i + e]), pack_bf16x2(o[1][4 * i + e], o[1][8 + 4 * i + e])};
+            for (int e = 0; e < 4; ++e)
+              if (s_nan[out_dim<D>(d, 8 * kOwn[i] + 4 * hf + e)] < lim) o[d][4 * kOwn[i] + e] = __uint_as_float(0x7fc00000u);
           }
+        }
+      }
+      if (done.rec >= 0) {
+        float* rec = a.part + (static_cast<size_t>(done.rec) * c.Hkv + kvh) * C::REC;
+#pragma unroll
+        for (int d = 0; d < C::DT; ++d) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const f32x16& x = o[d];
+            *reinterpret_cast<f32x4*>(rec + (((wave * C::DT + d) * 4 + kOwn[i]) * 64 + ln) * 4) =
+                f32x4{x[4 * kOwn[i]], x[4 * kOwn[i] + 1], x[4 * kOwn[i] + 2], x[4 * kOwn[i] + 3]};
+          }
+        }
+        if (G == 0 && hf == 0) {
+          rec[kRows * D + row32 * 2] = mm;
+          rec[kRows * D + row32 * 2 + 1] = ll;
+        }
+      } else if (row < done.n * a.group) {
+        const unsigned tok = static_cast<unsigned>(row) / static_cast<unsigned>(a.group);
+        bf16* dst = a.out + (static_cast<size_t>(done.q0 + tok) * a.Hq + kvh * a.group + row - tok * a.group) * D;
+        if constexpr (D == 64) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)   // dims 4 m + {0, 1, 2, 3} from rows m and m + 16 of both parts
+            *reinterpret_cast<u32x2*>(dst + 4 * (8 * G + 4 * hf + e)) =
+                u32x2{pack_bf16x2(o[0][4 * G + e], o[0][8 + 4 * G + e]), pack_bf16x2(o[1][4 * G + e], o[1][8 + 4 * G + e])};
         } else {
 #pragma unroll
           for (int g = 0; g < D / 128; ++g) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int i = 8 * G; i < 8 * G + 8; ++i)
               *reinterpret_cast<u32x2*>(dst + 128 * g + 4 * (8 * (i >> 2) + 4 * hf + (i & 3))) =
                   u32x2{pack_bf16x2(o[4 * g][i], o[4 * g + 1][i]), pack_bf16x2(o[4 * g + 2][i], o[4 * g + 3][i])};
           }
         }
       }
-    }
-    }
-    __syncthreads();   // LDS is the next item's
+    };
+    if (grp == 0) finish(std::integral_constant<int, 0>{});
+    else finish(std::integral_constant<int, 1>{});
   }
 }
 

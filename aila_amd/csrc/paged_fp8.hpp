@@ -63,15 +63,18 @@ struct BlockRef {
   int bid;
   float ks, vs;
 };
+// Index of a sequence's block in the pool; -1: its table entry is no page.
+__device__ __forceinline__ int block_id(const PagedFp8& c, int b, int head, int blk) {
+  const int p = blk / c.page_blocks;
+  const int page = c.table[static_cast<size_t>(b) * c.max_pages + p];
+  return page >= 0 && page < c.num_pages ? (page * c.Hkv + head) * c.page_blocks + blk - p * c.page_blocks : -1;
+}
 __device__ __forceinline__ BlockRef block_ref(const PagedFp8& c, int b, int head, int blk, int blk_end) {
   BlockRef r{-1, 0.f, 0.f};
-  if (blk < blk_end) {
-    const int page = c.table[static_cast<size_t>(b) * c.max_pages + blk / c.page_blocks];
-    if (page >= 0 && page < c.num_pages) {
-      r.bid = (page * c.Hkv + head) * c.page_blocks + blk % c.page_blocks;
-      r.ks = c.k_scale[r.bid];
-      r.vs = c.v_scale[r.bid];
-    }
+  if (blk < blk_end) r.bid = block_id(c, b, head, blk);
+  if (r.bid >= 0) {
+    r.ks = c.k_scale[r.bid];
+    r.vs = c.v_scale[r.bid];
   }
   return r;
 }
