@@ -400,22 +400,21 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
   for (int round = 1; more; ++round) {
     const int rows = it.n * a.group;
     const int row = it.r0 + wave * 32 + l32;          // this lane's query row
-    const bool there = row < rows;
-    const int tok = there ? row / a.group : 0;
-    const int lim = there ? max(it.len - it.n + tok + 1, 0) : 0;    // keys it attends
-    // tiles from this one on hold keys that not all rows attend (rows past the
-    // request's are computed, whatever they give, and not stored)
+    // rows past the request's are computed like its last and not stored
+    const int tok = min(row, rows - 1) / a.group;
+    const int lim = max(it.len - it.n + tok + 1, 0);  // keys the row attends
+    // tiles from this one on hold keys that not all rows attend
     const int mask_from = max(it.len - it.n + it.r0 / a.group + 1, 0) / C::BN;
     const int blk_end = (tile_end(a, it) + kScaleRows - 1) / kScaleRows;
 
     // ---- state ---------------------------------------------------------------
     bf16x8_t q[C::STEPS - C::QL];
     {
-      const bf16* src = a.q + static_cast<size_t>(it.q0 + tok) * a.q_stride + static_cast<size_t>(kvh * a.group + row % a.group) * D + 8 * hf;
+      const bf16* src = a.q + static_cast<size_t>(it.q0 + tok) * a.q_stride +
+                        static_cast<size_t>(kvh * a.group + min(row, rows - 1) - tok * a.group) * D + 8 * hf;
 #pragma unroll
       for (int s = 0; s < C::STEPS; ++s) {
-        u32x4 w = {0u, 0u, 0u, 0u};
-        if (there) w = ld16(src + 16 * s);
+        const u32x4 w = ld16(src + 16 * s);
         if (s >= C::QL) q[s - C::QL] = as_bf16x8(w);
         else if (grp == 0) *reinterpret_cast<u32x4*>(s_q + ((wave * C::QL + s) * 64 + lane) * 16) = w;   // read behind barriers
       }
@@ -463,13 +462,11 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
       };
       auto store_k = [&](const RawK& x) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < C::KI; ++i) {
-          const u32x4 w = x.w[i];
-          unsigned char* dst = k_ops + k_to + i * kStep * 1024;
-          *reinterpret_cast<u32x4*>(dst) = u32x4{fp8x2_to_bf16x2<false>(w[0], x.sc), fp8x2_to_bf16x2<true>(w[0], x.sc),
-                                                 fp8x2_to_bf16x2<false>(w[1], x.sc), fp8x2_to_bf16x2<true>(w[1], x.sc)};
-          *reinterpret_cast<u32x4*>(dst + 512) = u32x4{fp8x2_to_bf16x2<false>(w[2], x.sc), fp8x2_to_bf16x2<true>(w[2], x.sc),
-                                                       fp8x2_to_bf16x2<false>(w[3], x.sc), fp8x2_to_bf16x2<true>(w[3], x.sc)};
+        for (int i = 0; i < 2 * C::KI; ++i) {
+          const uint32_t lo = x.w[i >> 1][2 * (i & 1)], hi = x.w[i >> 1][2 * (i & 1) + 1];
+          *reinterpret_cast<u32x4*>(k_ops + k_to + (i >> 1) * kStep * 1024 + (i & 1) * 512) =
+              u32x4{fp8x2_to_bf16x2<false>(lo, x.sc), fp8x2_to_bf16x2<true>(lo, x.sc), fp8x2_to_bf16x2<false>(hi, x.sc),
+                    fp8x2_to_bf16x2<true>(hi, x.sc)};
         }
       };
       // V: a thread takes 8 keys x 4 dims, the keys 16 (oc / 2) + 4 (oc % 2) + {0..3, 8..11}.
@@ -482,29 +479,29 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
         x.sc = s_vs[first_block(j) + (oc >> 1)];
         return x;
       };
-      auto store_v = [&](RawV& x, int j, bool masked) __attribute__((always_inline)) {
-        if (masked) {
-          // 0 times NaN is NaN: a masked row must not carry one into the product.
-          // NaN codes are taken out and remembered by dim; the epilogue puts NaN
-          // into the rows that attend the first.
-          const uint32_t keep = s_bid[first_block(j) + (oc >> 1)] >= 0 ? 0xffffffffu : 0u;
-          uint32_t seen = 0;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t n = nan_codes(x.v[e]) >> 7;
-            seen |= n & keep;
-            x.v[e] &= keep & ~(n * 0xffu);
-          }
-          if (seen) {
-            const unsigned char* raw = v_raw + (j & 1) * C::RAW + v_from;
-            const int key = s0 * C::BN + first_block(j) * kScaleRows + 16 * (oc >> 1) + 4 * (oc & 1);
-#pragma unroll 1
-            for (int e = 0; e < 32; ++e) {
-              const int r = (e >> 2 & 3) + 8 * (e >> 4);
-              if ((raw[r * D + (e & 3)] & 0x7f) == 0x7f) s_any_nan = 1, atomicMin(&s_nan[4 * dq + (e & 3)], key + r);
-            }
-          }
-        }
+      auto clean_v = [&](RawV& x, int j) __attribute__((always_inline)) {
+                  // 0 times NaN is NaN: a masked row must not carry one into the product.
+                  // NaN codes are taken out and remembered by dim; the epilogue puts NaN
+                  // into the rows that attend the first.
+                  const uint32_t keep = s_bid[first_block(j) + (oc >> 1)] >= 0 ? 0xffffffffu : 0u;
+                  uint32_t seen = 0;
+        #pragma unroll
+                  for (int e = 0; e < 8; ++e) {
+                    const uint32_t n = nan_codes(x.v[e]) >> 7;
+                    seen |= n & keep;
+                    x.v[e] &= keep & ~(n * 0xffu);
+                  }
+                  if (seen) {
+                    const unsigned char* raw = v_raw + (j & 1) * C::RAW + v_from;
+                    const int key = s0 * C::BN + first_block(j) * kScaleRows + 16 * (oc >> 1) + 4 * (oc & 1);
+        #pragma unroll 1
+                    for (int e = 0; e < 32; ++e) {
+                      const int r = (e >> 2 & 3) + 8 * (e >> 4);
+                      if ((raw[r * D + (e & 3)] & 0x7f) == 0x7f) s_any_nan = 1, atomicMin(&s_nan[4 * dq + (e & 3)], key + r);
+                    }
+                  }
+      };
+      auto store_v = [&](const RawV& x) __attribute__((always_inline)) {
         u32x4 w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -515,7 +512,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
           w[2][e] = fp8x2_to_bf16x2<false>(hi, x.sc);
           w[3][e] = fp8x2_to_bf16x2<true>(hi, x.sc);
         }
-        // byte i of the quad: the next part, or for D = 64 the other half of this one
+        // dim i of the quad: the next part, or for D = 64 the other half of this one
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<u32x4*>(v_ops + v_to + (D == 64 ? (i >> 1) * 1024 + (i & 1) * 256 : i * 1024)) = w[i];
@@ -662,7 +659,9 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
       for (int j = 0;;) {
         __builtin_amdgcn_s_waitcnt(vmcnt_imm<2 * C::DMA>());   // all but this phase's DMAs
         phase_barrier();
-        // V(j)
+        // V(j): reads its codes, then softmax, then the operands change. (Converting
+        // between the products of the matrix phase instead took as long: the vector
+        // ALU, which both waves of a SIMD share, is what a phase waits for.)
         __builtin_amdgcn_s_setprio(0);
         const bool masked = masked_tile(j);
         const RawK rk = load_k(j + 1);
@@ -670,7 +669,10 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
         if (v_threads) rv = load_v(j);
         softmax(j, masked);
         store_k(rk);
-        if (v_threads) store_v(rv, j, masked);
+        if (v_threads) {
+          if (masked) clean_v(rv, j);
+          store_v(rv);
+        }
         phase_barrier();
         // M(j + 1)
         __builtin_amdgcn_s_setprio(1);
