@@ -423,21 +423,25 @@ def copy_to_cache(new_kv, cache, start_pos: int, stream=None):
 _SCALE_ROWS = 16   # rows of a page that share a scale
 
 
-def _same_device(stream, *tensors):
-    """The tensors' one device has to be the one whose stream the call runs on."""
+# As above, the common call tests everything in one expression (dtype, shape,
+# layout, alignment, and that every tensor is on the call's device); only if that
+# fails do these functions find out what is wrong and say it.
+def _device_of(stream):
     import torch
+    return torch.cuda.current_device() if stream is None else stream.device_index
+
+
+def _same_device(dev, *tensors):
+    """The tensors' one device has to be the one whose stream the call runs on."""
     for t in tensors:
-        if t is not None and t.get_device() != tensors[0].get_device():
-            raise ValueError(f"tensors on different devices: {tensors[0].device} and {t.device}")
-    dev = torch.cuda.current_device() if stream is None else stream.device_index
-    if tensors[0].get_device() != dev:
-        raise ValueError(f"tensors on {tensors[0].device}, but the call's stream is on cuda:{dev}: "
-                         "make it inside torch.cuda.device(...)")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensor on {t.device}, but the call's stream is on cuda:{dev}: "
+                             "make it inside torch.cuda.device(...), with all tensors there")
 
 
 def _need_rows(t, tokens, heads, dim, name):
     """[tokens, heads, dim] bf16 whose tokens may be strided (views of a fused
-    projection row); returns the token stride in elements."""
+    projection row)."""
     import torch
     if t is None:
         raise ValueError(f"{name} is required")
@@ -450,25 +454,51 @@ def _need_rows(t, tokens, heads, dim, name):
     st = t.stride()
     if st[2] != 1 or (heads > 1 and st[1] != dim):
         raise ValueError(f"{name}: strides {st}, expected a token's [{heads}, {dim}] values to be contiguous")
-    step = st[0] if tokens > 1 else max(heads * dim, st[0])
-    if step < heads * dim or step % 8:
-        raise ValueError(f"{name}: token stride {step} must be a multiple of 8 and at least {heads * dim}")
+    if tokens > 1 and (st[0] < heads * dim or st[0] % 8):
+        raise ValueError(f"{name}: token stride {st[0]} must be a multiple of 8 and at least {heads * dim}")
     if t.data_ptr() % 16:
         raise ValueError(f"{name} must be 16-byte aligned")
-    return step
+
+
+def _token_stride(t, tokens, heads, dim):
+    """Elements between tokens of a [tokens, heads, dim] view, or 0 if it is not
+    one that the kernels take."""
+    a, b, c = t.stride()
+    if c != 1 or (b != dim and heads > 1):
+        return 0
+    if tokens == 1:
+        return heads * dim
+    return a if a >= heads * dim and not a % 8 else 0
 
 
 def _need_pages(k_pages, v_pages, k_scale, v_scale):
-    """Checks the four arrays of an 8-bit paged cache; returns (num_pages, Hkv, page_size, D)."""
+    """Checks the four arrays of an 8-bit paged cache."""
     import torch
     if k_pages is None or k_pages.dim() != 4:
         raise ValueError("k_pages must be [num_pages, Hkv, page_size, D]")
-    P, Hkv, page_size, D = shape = tuple(k_pages.shape)
+    P, Hkv, page_size, _ = shape = tuple(k_pages.shape)
+    if page_size % _SCALE_ROWS:
+        raise ValueError(f"k_pages: page_size {page_size} must be a multiple of {_SCALE_ROWS}")
     _need(k_pages, torch.float8_e4m3fn, shape, "k_pages")
     _need(v_pages, torch.float8_e4m3fn, shape, "v_pages")
     _need(k_scale, torch.float32, (P, Hkv, page_size // _SCALE_ROWS), "k_scale", align=4)
     _need(v_scale, torch.float32, (P, Hkv, page_size // _SCALE_ROWS), "v_scale", align=4)
-    return shape
+
+
+def _pages_ok(torch, dev, kp, vp, ks, vs):
+    """(k_pages.shape, pointers of the four) if all is as it has to be, else None."""
+    shape = kp.shape
+    if len(shape) != 4:
+        return None
+    f8, f32 = torch.float8_e4m3fn, torch.float32
+    p = kp.data_ptr(), vp.data_ptr(), ks.data_ptr(), vs.data_ptr()
+    if kp.dtype is f8 and vp.dtype is f8 and ks.dtype is f32 and vs.dtype is f32 and vp.shape == shape \
+            and ks.shape == vs.shape == (shape[0], shape[1], shape[2] // _SCALE_ROWS) and not shape[2] % _SCALE_ROWS \
+            and not (p[0] | p[1]) & 15 and not (p[2] | p[3]) & 3 and kp.is_contiguous() and vp.is_contiguous() \
+            and ks.is_contiguous() and vs.is_contiguous() \
+            and kp.get_device() == vp.get_device() == ks.get_device() == vs.get_device() == dev:
+        return shape, p
+    return None
 
 
 def _new_out(make, stream):
@@ -511,23 +541,37 @@ def kv_pages_reserve(cached_lens, new_lens, block_table, free_pages, free_count,
     import torch
     B, max_pages = block_table.shape
     i32 = torch.int32
-    _need(cached_lens, i32, (B,), "cached_lens", align=4)
-    _need(new_lens, i32, (B,), "new_lens", align=4)
-    _need(block_table, i32, (B, max_pages), "block_table", align=4)
-    _need(free_pages, i32, (free_pages.numel(),), "free_pages", align=4)
-    _need(free_count, i32, (1,), "free_count", align=4)
-    _need(slots, i32, (slots.numel(),), "slots", align=4)
     if query_start is None:
         query_start = _new_out(lambda: torch.empty(B + 1, dtype=i32, device=block_table.device), stream)
     if seq_lens is None:
         seq_lens = _new_out(lambda: torch.empty(B, dtype=i32, device=block_table.device), stream)
-    _need(query_start, i32, (B + 1,), "query_start", align=4)
-    _need(seq_lens, i32, (B,), "seq_lens", align=4)
-    _same_device(stream, block_table, cached_lens, new_lens, free_pages, free_count, slots, query_start, seq_lens)
-    rc = lib().aila_hip_kv_pages_reserve(_ptr(cached_lens), _ptr(new_lens), _ptr(block_table), _ptr(free_pages),
-                                         _ptr(free_count), _ptr(query_start), _ptr(seq_lens), _ptr(slots), B, max_pages,
-                                         int(page_size), free_pages.numel(), slots.numel(), _stream(stream))
-    _check(rc, "aila_hip_kv_pages_reserve")
+    dev = _device_of(stream)
+    num_pages, max_tokens = free_pages.numel(), slots.numel()
+    one = (B,)
+    if not (cached_lens.dtype is i32 and new_lens.dtype is i32 and block_table.dtype is i32 and free_pages.dtype is i32
+            and free_count.dtype is i32 and slots.dtype is i32 and query_start.dtype is i32 and seq_lens.dtype is i32
+            and cached_lens.shape == new_lens.shape == seq_lens.shape == one and query_start.shape == (B + 1,)
+            and free_count.shape == (1,) and free_pages.shape == (num_pages,) and slots.shape == (max_tokens,)
+            and cached_lens.is_contiguous() and new_lens.is_contiguous() and block_table.is_contiguous()
+            and free_pages.is_contiguous() and slots.is_contiguous() and query_start.is_contiguous()
+            and seq_lens.is_contiguous() and cached_lens.get_device() == new_lens.get_device() == block_table.get_device()
+            == free_pages.get_device() == free_count.get_device() == slots.get_device() == query_start.get_device()
+            == seq_lens.get_device() == dev):
+        _need(cached_lens, i32, one, "cached_lens", align=4)
+        _need(new_lens, i32, one, "new_lens", align=4)
+        _need(block_table, i32, (B, max_pages), "block_table", align=4)
+        _need(free_pages, i32, (num_pages,), "free_pages", align=4)
+        _need(free_count, i32, (1,), "free_count", align=4)
+        _need(slots, i32, (max_tokens,), "slots", align=4)
+        _need(query_start, i32, (B + 1,), "query_start", align=4)
+        _need(seq_lens, i32, one, "seq_lens", align=4)
+        _same_device(dev, block_table, cached_lens, new_lens, free_pages, free_count, slots, query_start, seq_lens)
+    rc = lib().aila_hip_kv_pages_reserve(cached_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
+                                         free_pages.data_ptr(), free_count.data_ptr(), query_start.data_ptr(),
+                                         seq_lens.data_ptr(), slots.data_ptr(), B, max_pages, int(page_size), num_pages,
+                                         max_tokens, _stream(stream))
+    if rc:
+        _check(rc, "aila_hip_kv_pages_reserve")
     return query_start, seq_lens, slots
 
 
@@ -536,14 +580,22 @@ def kv_pages_release(release, block_table, free_pages, free_count, stream=None):
     free stack; their table entries become -1."""
     import torch
     B, max_pages = block_table.shape
-    _need(release, torch.int32, (B,), "release", align=4)
-    _need(block_table, torch.int32, (B, max_pages), "block_table", align=4)
-    _need(free_pages, torch.int32, (free_pages.numel(),), "free_pages", align=4)
-    _need(free_count, torch.int32, (1,), "free_count", align=4)
-    _same_device(stream, block_table, release, free_pages, free_count)
-    rc = lib().aila_hip_kv_pages_release(_ptr(release), _ptr(block_table), _ptr(free_pages), _ptr(free_count), B,
-                                         max_pages, free_pages.numel(), _stream(stream))
-    _check(rc, "aila_hip_kv_pages_release")
+    i32 = torch.int32
+    dev = _device_of(stream)
+    num_pages = free_pages.numel()
+    if not (release.dtype is i32 and block_table.dtype is i32 and free_pages.dtype is i32 and free_count.dtype is i32
+            and release.shape == (B,) and free_pages.shape == (num_pages,) and free_count.shape == (1,)
+            and release.is_contiguous() and block_table.is_contiguous() and free_pages.is_contiguous()
+            and release.get_device() == block_table.get_device() == free_pages.get_device() == free_count.get_device() == dev):
+        _need(release, i32, (B,), "release", align=4)
+        _need(block_table, i32, (B, max_pages), "block_table", align=4)
+        _need(free_pages, i32, (num_pages,), "free_pages", align=4)
+        _need(free_count, i32, (1,), "free_count", align=4)
+        _same_device(dev, block_table, release, free_pages, free_count)
+    rc = lib().aila_hip_kv_pages_release(release.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(),
+                                         free_count.data_ptr(), B, max_pages, num_pages, _stream(stream))
+    if rc:
+        _check(rc, "aila_hip_kv_pages_release")
 
 
 def kv_append_paged_fp8(k_new, v_new, k_pages, v_pages, k_scale, v_scale, slots, stream=None):
@@ -552,40 +604,104 @@ def kv_append_paged_fp8(k_new, v_new, k_pages, v_pages, k_scale, v_scale, slots,
     page_size, D] float8_e4m3fn, k_scale/v_scale [num_pages, Hkv,
     page_size / 16] float32. The tokens may be strided (both alike)."""
     import torch
-    P, Hkv, page_size, D = _need_pages(k_pages, v_pages, k_scale, v_scale)
+    dev = _device_of(stream)
     T = slots.numel()
-    _need(slots, torch.int32, (T,), "slots", align=4)
-    step = _need_rows(k_new, T, Hkv, D, "k_new")
-    if _need_rows(v_new, T, Hkv, D, "v_new") != step and T > 1:
-        raise ValueError(f"k_new and v_new: token strides {step} and {v_new.stride(0)} differ")
-    _same_device(stream, k_pages, v_pages, k_scale, v_scale, k_new, v_new, slots)
-    rc = lib().aila_hip_kv_append_paged_fp8(_ptr(k_new), _ptr(v_new), step, _ptr(k_pages), _ptr(v_pages), _ptr(k_scale),
-                                            _ptr(v_scale), _ptr(slots), T, Hkv, D, page_size, P, _stream(stream))
-    _check(rc, "aila_hip_kv_append_paged_fp8")
+    bf = torch.bfloat16
+    pages = _pages_ok(torch, dev, k_pages, v_pages, k_scale, v_scale) if k_pages is not None else None
+    ok = pages is not None and k_new is not None and v_new is not None
+    if ok:
+        (P, Hkv, page_size, D), (kp, vp, ks, vs) = pages
+        kn, vn = k_new.data_ptr(), v_new.data_ptr()
+        ok = k_new.dtype is bf and v_new.dtype is bf and slots.dtype is torch.int32 and k_new.shape == v_new.shape == (T, Hkv, D) \
+            and slots.shape == (T,) and slots.is_contiguous() and not (kn | vn) & 15 \
+            and k_new.get_device() == v_new.get_device() == slots.get_device() == dev
+        if ok:
+            step = _token_stride(k_new, T, Hkv, D)
+            ok = step and step == _token_stride(v_new, T, Hkv, D)
+    if not ok:
+        _need_pages(k_pages, v_pages, k_scale, v_scale)
+        P, Hkv, page_size, D = k_pages.shape
+        _need(slots, torch.int32, (T,), "slots", align=4)
+        _need_rows(k_new, T, Hkv, D, "k_new")
+        _need_rows(v_new, T, Hkv, D, "v_new")
+        if k_new.stride(0) != v_new.stride(0):
+            raise ValueError(f"k_new and v_new: token strides {k_new.stride(0)} and {v_new.stride(0)} differ")
+        _same_device(dev, k_pages, v_pages, k_scale, v_scale, k_new, v_new, slots)
+        raise ValueError("kv_append_paged_fp8: bad tensors")
+    rc = lib().aila_hip_kv_append_paged_fp8(kn, vn, step, kp, vp, ks, vs, slots.data_ptr(), T, Hkv, D, page_size, P,
+                                            _stream(stream))
+    if rc:
+        _check(rc, "aila_hip_kv_append_paged_fp8")
 
 
 def kv_read_paged_fp8(k_pages, v_pages, k_scale, v_scale, slots, k_out=None, v_out=None, stream=None):
     """Rows `slots` (int32 [T]; zeros for -1) of an 8-bit paged cache as the
     values they stand for -> (k, v) [T, Hkv, D] bf16."""
     import torch
-    P, Hkv, page_size, D = _need_pages(k_pages, v_pages, k_scale, v_scale)
+    dev = _device_of(stream)
     T = slots.numel()
-    _need(slots, torch.int32, (T,), "slots", align=4)
+    bf = torch.bfloat16
+    pages = _pages_ok(torch, dev, k_pages, v_pages, k_scale, v_scale) if k_pages is not None else None
+    if pages is None:
+        _need_pages(k_pages, v_pages, k_scale, v_scale)
+        _same_device(dev, k_pages, v_pages, k_scale, v_scale)
+        raise ValueError("kv_read_paged_fp8: bad cache tensors")
+    (P, Hkv, page_size, D), (kp, vp, ks, vs) = pages
+    shape = (T, Hkv, D)
     if k_out is None:
-        k_out = _new_out(lambda: torch.empty((T, Hkv, D), dtype=torch.bfloat16, device=k_pages.device), stream)
+        k_out = _new_out(lambda: torch.empty(shape, dtype=bf, device=k_pages.device), stream)
     if v_out is None:
-        v_out = _new_out(lambda: torch.empty((T, Hkv, D), dtype=torch.bfloat16, device=k_pages.device), stream)
-    _need(k_out, torch.bfloat16, (T, Hkv, D), "k_out")
-    _need(v_out, torch.bfloat16, (T, Hkv, D), "v_out")
-    _same_device(stream, k_pages, v_pages, k_scale, v_scale, slots, k_out, v_out)
-    rc = lib().aila_hip_kv_read_paged_fp8(_ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), _ptr(slots),
-                                          _ptr(k_out), _ptr(v_out), T, Hkv, D, page_size, P, _stream(stream))
-    _check(rc, "aila_hip_kv_read_paged_fp8")
+        v_out = _new_out(lambda: torch.empty(shape, dtype=bf, device=k_pages.device), stream)
+    ko, vo = k_out.data_ptr(), v_out.data_ptr()
+    if not (k_out.dtype is bf and v_out.dtype is bf and slots.dtype is torch.int32 and k_out.shape == v_out.shape == shape
+            and slots.shape == (T,) and slots.is_contiguous() and k_out.is_contiguous() and v_out.is_contiguous()
+            and not (ko | vo) & 15 and k_out.get_device() == v_out.get_device() == slots.get_device() == dev):
+        _need(slots, torch.int32, (T,), "slots", align=4)
+        _need(k_out, bf, shape, "k_out")
+        _need(v_out, bf, shape, "v_out")
+        _same_device(dev, slots, k_out, v_out)
+    rc = lib().aila_hip_kv_read_paged_fp8(kp, vp, ks, vs, slots.data_ptr(), ko, vo, T, Hkv, D, page_size, P, _stream(stream))
+    if rc:
+        _check(rc, "aila_hip_kv_read_paged_fp8")
     return k_out, v_out
 
 
 def gqa_decode_paged_fp8_workspace_size(B: int, Hq: int, Hkv: int, D: int, max_len: int) -> int:
     return int(lib().aila_hip_gqa_decode_paged_fp8_workspace_size(B, Hq, Hkv, D, max_len))
+
+
+def _attention_args(q, k_pages, v_pages, k_scale, v_scale, block_table, query_start, seq_lens, out, workspace, stream, B):
+    """Checks what both attention calls take; returns the token stride of q, the
+    cache's shape and pointers, out and the workspace's pointer and size."""
+    import torch
+    dev = _device_of(stream)
+    T, Hq, D = q.shape
+    bf, i32 = torch.bfloat16, torch.int32
+    if out is None:
+        out = _new_out(lambda: torch.empty((T, Hq, D), dtype=q.dtype, device=q.device), stream)
+    pages = _pages_ok(torch, dev, k_pages, v_pages, k_scale, v_scale) if k_pages is not None else None
+    step = _token_stride(q, T, Hq, D)
+    if not (pages is not None and step and q.dtype is bf and out.dtype is bf and block_table.dtype is i32 and seq_lens.dtype is i32
+            and pages[0][3] == D and out.shape == q.shape and seq_lens.shape == (B,) and block_table.shape[0] == B
+            and len(block_table.shape) == 2 and out.is_contiguous() and block_table.is_contiguous() and seq_lens.is_contiguous()
+            and not (q.data_ptr() | out.data_ptr()) & 15
+            and q.get_device() == out.get_device() == block_table.get_device() == seq_lens.get_device() == dev
+            and (query_start is None or (query_start.dtype is i32 and query_start.shape == (B + 1,) and query_start.is_contiguous()
+                                         and query_start.get_device() == dev))
+            and (workspace is None or (workspace.get_device() == dev and workspace.is_contiguous()))):
+        _need_pages(k_pages, v_pages, k_scale, v_scale)
+        _need_rows(q, T, Hq, k_pages.shape[3], "q")
+        _need(block_table, i32, (B, block_table.shape[1]), "block_table", align=4)
+        _need(seq_lens, i32, (B,), "seq_lens", align=4)
+        if query_start is not None:
+            _need(query_start, i32, (B + 1,), "query_start", align=4)
+        _need(out, bf, (T, Hq, D), "out")
+        _workspace_bytes(workspace)
+        _same_device(dev, q, k_pages, v_pages, k_scale, v_scale, block_table, query_start, seq_lens, out, workspace)
+        raise ValueError("bad tensors")
+    if workspace is None:
+        return step, pages, out, None, 0
+    return step, pages, out, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def gqa_decode_paged_fp8(q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, max_len: int, out=None,
@@ -596,22 +712,14 @@ def gqa_decode_paged_fp8(q, k_pages, v_pages, k_scale, v_scale, block_table, seq
     [B,Hq,D]. workspace: uint8 device tensor (see
     gqa_decode_paged_fp8_workspace_size), or None for one workgroup per
     sequence and KV head."""
-    import torch
     B, Hq, D = q.shape
-    P, Hkv, page_size, Dk = _need_pages(k_pages, v_pages, k_scale, v_scale)
-    max_pages = block_table.shape[1]
-    step = _need_rows(q, B, Hq, Dk, "q")
-    _need(block_table, torch.int32, (B, max_pages), "block_table", align=4)
-    _need(seq_lens, torch.int32, (B,), "seq_lens", align=4)
-    if out is None:
-        out = _new_out(lambda: torch.empty((B, Hq, D), dtype=q.dtype, device=q.device), stream)
-    _need(out, torch.bfloat16, (B, Hq, D), "out")
-    ws_bytes = _workspace_bytes(workspace)
-    _same_device(stream, q, k_pages, v_pages, k_scale, v_scale, block_table, seq_lens, out, workspace)
-    rc = lib().aila_hip_gqa_decode_paged_fp8(_ptr(q), step, _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale),
-                                             _ptr(out), _ptr(workspace), ws_bytes, B, Hq, Hkv, D, page_size, P,
-                                             _ptr(block_table), max_pages, int(max_len), _ptr(seq_lens), _stream(stream))
-    _check(rc, "aila_hip_gqa_decode_paged_fp8")
+    step, ((P, Hkv, page_size, _), (kp, vp, ks, vs)), out, ws, ws_bytes = _attention_args(
+        q, k_pages, v_pages, k_scale, v_scale, block_table, None, seq_lens, out, workspace, stream, B)
+    rc = lib().aila_hip_gqa_decode_paged_fp8(q.data_ptr(), step, kp, vp, ks, vs, out.data_ptr(), ws, ws_bytes, B, Hq, Hkv, D,
+                                             page_size, P, block_table.data_ptr(), block_table.shape[1], int(max_len),
+                                             seq_lens.data_ptr(), _stream(stream))
+    if rc:
+        _check(rc, "aila_hip_gqa_decode_paged_fp8")
     return out
 
 
@@ -624,25 +732,20 @@ def gqa_prefill_paged_fp8(q, k_pages, v_pages, k_scale, v_scale, block_table, qu
     """Causal attention of a ragged batch over an 8-bit paged cache that holds
     the new rows already. q [T,Hq,D] bf16, request b's tokens at query_start[b]
     .. query_start[b+1] (int32 [B+1]); seq_lens int32 [B] counts the rows after
-    them -> out [T,Hq,D] (rows from query_start[B] on are not touched)."""
-    import torch
+    them -> out [T,Hq,D] (rows from query_start[B] on are not touched).
+    workspace: uint8 device tensor (see gqa_prefill_paged_fp8_workspace_size);
+    None: one request, or one after the other, and no key split."""
     T, Hq, D = q.shape
-    P, Hkv, page_size, Dk = _need_pages(k_pages, v_pages, k_scale, v_scale)
     B, max_pages = block_table.shape
-    step = _need_rows(q, T, Hq, Dk, "q")
-    _need(block_table, torch.int32, (B, max_pages), "block_table", align=4)
-    _need(query_start, torch.int32, (B + 1,), "query_start", align=4)
-    _need(seq_lens, torch.int32, (B,), "seq_lens", align=4)
-    if out is None:
-        out = _new_out(lambda: torch.empty((T, Hq, D), dtype=q.dtype, device=q.device), stream)
-    _need(out, torch.bfloat16, (T, Hq, D), "out")
-    ws_bytes = _workspace_bytes(workspace)
-    _same_device(stream, q, k_pages, v_pages, k_scale, v_scale, block_table, query_start, seq_lens, out, workspace)
-    rc = lib().aila_hip_gqa_prefill_paged_fp8(_ptr(q), step, _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale),
-                                              _ptr(out), _ptr(workspace), ws_bytes, T, B, Hq, Hkv, D, page_size, P,
-                                              _ptr(block_table), max_pages, int(max_len), _ptr(query_start),
-                                              _ptr(seq_lens), _stream(stream))
-    _check(rc, "aila_hip_gqa_prefill_paged_fp8")
+    if query_start is None:
+        raise ValueError("query_start is required")
+    step, ((P, Hkv, page_size, _), (kp, vp, ks, vs)), out, ws, ws_bytes = _attention_args(
+        q, k_pages, v_pages, k_scale, v_scale, block_table, query_start, seq_lens, out, workspace, stream, B)
+    rc = lib().aila_hip_gqa_prefill_paged_fp8(q.data_ptr(), step, kp, vp, ks, vs, out.data_ptr(), ws, ws_bytes, T, B, Hq, Hkv,
+                                              D, page_size, P, block_table.data_ptr(), max_pages, int(max_len),
+                                              query_start.data_ptr(), seq_lens.data_ptr(), _stream(stream))
+    if rc:
+        _check(rc, "aila_hip_gqa_prefill_paged_fp8")
     return out
 
 

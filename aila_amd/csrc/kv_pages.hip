@@ -36,15 +36,16 @@ __device__ __forceinline__ T block_scan(T x, T* s_wave, T* total) {
   __syncthreads();   // s_wave of the scan before is read
   if (lane == 63) s_wave[wave] = x;
   __syncthreads();
-  T before = 0, all = 0;
+  // every wave adds up the waves' sums for itself, lane w those up to wave w
+  T y = lane < kPlanWaves ? s_wave[lane] : 0;
 #pragma unroll
-  for (int w = 0; w < kPlanWaves; ++w) {
-    const T v = s_wave[w];
-    if (w < wave) before += v;
-    all += v;
+  for (int off = 1; off < kPlanWaves; off <<= 1) {
+    const T z = __shfl_up(y, off);
+    if (lane >= off) y += z;
   }
-  *total = all;
-  return x + before;
+  *total = __shfl(y, kPlanWaves - 1);
+  const T before = __shfl(y, max(wave - 1, 0));
+  return wave > 0 ? x + before : x;
 }
 
 // The last b with start[b] <= x, for start[0] = 0 <= x < start[n] (entries of
@@ -58,18 +59,17 @@ __device__ __forceinline__ int find_request(const int* start, int n, int x) {
   return lo;
 }
 
-struct Lens { long c, n; bool fits; };
+struct Lens { int c, n; bool fits; };
 __device__ __forceinline__ Lens load_lens(const int* cached, const int* fresh, int b, long max_rows) {
   Lens l{cached[b], fresh[b], false};
   if (l.c < 0 || l.n < 0) return Lens{0, 0, false};   // absent
-  l.fits = l.c + l.n <= max_rows;
+  l.fits = static_cast<long>(l.c) + l.n <= max_rows;
   return l;
 }
 
-__device__ __forceinline__ int slot_of(const int* table, int max_pages, int page_size, int num_pages, int b, int row) {
-  const int page = table[static_cast<size_t>(b) * max_pages + row / page_size];
-  return page >= 0 && page < num_pages ? page * page_size + row % page_size : -1;
-}
+// Entries of the flat list whose pages are kept in LDS, and free pages that are
+// fetched before it is known how many are needed.
+constexpr int kFlatPages = 4096;
 
 __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
     const int* __restrict__ cached, const int* __restrict__ fresh, int* table, const int* __restrict__ free_pages,
@@ -80,12 +80,17 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
   int* s_flat = s_start + B + 1;        // [B + 1] first entry of each request's pages
   int* s_first = s_flat + B + 1;        // [B] holes before the request's
   int* s_last = s_first + B;            // [B] holes up to its end
+  int* s_rows = s_last + B;             // [B] rows it holds
+  int* s_ok = s_rows + B;               // [B] its rows fit the table; then: it is admitted
   __shared__ long s_wl[kPlanWaves];
   __shared__ int s_wi[kPlanWaves];
   __shared__ int s_taken;
+  __shared__ int s_top[kPlanThreads];   // the free pages nearest the top
+  __shared__ int s_page[kFlatPages];    // page of each entry of the flat list
   const int tid = threadIdx.x;
   const long max_rows = static_cast<long>(max_pages) * page_size;
   const int have = min(max(*free_count, 0), num_pages);
+  s_top[tid] = tid < have ? free_pages[have - 1 - tid] : -1;
 
   // ---- tokens and table entries of each request ---------------------------
   long tok0 = 0;
@@ -94,7 +99,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
     const int b = b0 + tid;
     Lens l{0, 0, false};
     if (b < B) l = load_lens(cached, fresh, b, max_rows);
-    const int np = l.fits ? static_cast<int>((l.c + l.n + page_size - 1) / page_size - l.c / page_size) : 0;
+    const int np = l.fits ? static_cast<int>((static_cast<long>(l.c) + l.n + page_size - 1) / page_size) - l.c / page_size : 0;
     long all_tok;
     int all_np;
     const long tok = tok0 + block_scan<long>(l.n, s_wl, &all_tok);
@@ -103,6 +108,8 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
       s_start[b + 1] = static_cast<int>(min(tok, 0x7fffffffL));
       s_flat[b + 1] = flat;
       s_first[b] = s_last[b] = 0;
+      s_rows[b] = l.c;
+      s_ok[b] = l.fits;
     }
     tok0 += all_tok;
     flat0 += all_np;
@@ -116,15 +123,20 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
   for (int b = tid; b <= B; b += kPlanThreads) query_start[b] = s_start[b];
 
   // ---- holes among the entries, in order of request and page --------------
+  auto entry_of = [&](int f, int* b) __attribute__((always_inline)) {
+    *b = find_request(s_flat, B, f);
+    return table + static_cast<size_t>(*b) * max_pages + s_rows[*b] / page_size + f - s_flat[*b];
+  };
+  const bool in_lds = flat0 <= kFlatPages;
   int holes0 = 0;
   for (int f0 = 0; f0 < flat0; f0 += kPlanThreads) {
     const int f = f0 + tid;
-    int b = 0, hole = 0;
+    int b = 0, page = 0;
     if (f < flat0) {
-      b = find_request(s_flat, B, f);
-      const int p = cached[b] / page_size + f - s_flat[b];
-      hole = table[static_cast<size_t>(b) * max_pages + p] < 0;
+      page = *entry_of(f, &b);
+      if (in_lds) s_page[f] = page;
     }
+    const int hole = page < 0;
     int all;
     const int incl = holes0 + block_scan<int>(hole, s_wi, &all);
     if (f < flat0) {
@@ -138,32 +150,31 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
   // Admitted: its rows fit the table, its tokens the batch, its holes the pool.
   // Both sums only grow, so the admitted requests that take pages come first
   // among those that need any, and the k-th hole takes the k-th page from the top.
-  auto admitted = [&](int b, bool fits) __attribute__((always_inline)) {
-    return fits && s_start[b + 1] <= max_tokens && (s_last[b] == s_first[b] || s_last[b] <= have);
-  };
+  for (int b = tid; b < B; b += kPlanThreads) {
+    const int ok = s_ok[b] && s_start[b + 1] <= max_tokens && (s_last[b] == s_first[b] || s_last[b] <= have);
+    s_ok[b] = ok;
+    seq_lens[b] = ok ? s_rows[b] + (s_start[b + 1] - s_start[b]) : 0;
+    if (ok && s_last[b] != s_first[b]) atomicMax(&s_taken, s_last[b]);
+  }
+  __syncthreads();
   int carry = 0;
   for (int f0 = 0; f0 < flat0; f0 += kPlanThreads) {
     const int f = f0 + tid;
     int b = 0, hole = 0, *entry = nullptr;
     if (f < flat0) {
-      b = find_request(s_flat, B, f);
-      entry = table + static_cast<size_t>(b) * max_pages + cached[b] / page_size + f - s_flat[b];
-      hole = *entry < 0;
+      entry = entry_of(f, &b);
+      hole = (in_lds ? s_page[f] : *entry) < 0;
     }
     int all;
     const int k = carry + block_scan<int>(hole, s_wi, &all) - 1;
-    if (hole && admitted(b, true)) {   // only requests that fit have entries here
-      *entry = free_pages[have - 1 - k];
-      if (k + 1 == s_last[b]) atomicMax(&s_taken, k + 1);
+    if (hole && s_ok[b]) {
+      const int page = k < kPlanThreads ? s_top[k] : free_pages[have - 1 - k];
+      *entry = page;
+      if (in_lds) s_page[f] = page;
     }
     carry += all;
   }
-  for (int b = tid; b < B; b += kPlanThreads) {
-    const Lens l = load_lens(cached, fresh, b, max_rows);
-    const bool ok = admitted(b, l.fits);
-    seq_lens[b] = ok ? static_cast<int>(l.c + l.n) : 0;
-  }
-  __syncthreads();   // the table's new entries, for this workgroup
+  __syncthreads();   // the new pages, for this workgroup
   if (tid == 0) *free_count = have - s_taken;
 
   // ---- slots ---------------------------------------------------------------
@@ -172,9 +183,11 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
     int slot = -1;
     if (t < total) {
       const int b = find_request(s_start, B, t);
-      const Lens l = load_lens(cached, fresh, b, max_rows);
-      if (admitted(b, l.fits))
-        slot = slot_of(table, max_pages, page_size, num_pages, b, static_cast<int>(l.c) + t - s_start[b]);
+      if (s_ok[b]) {
+        const int row = s_rows[b] + t - s_start[b], p = row / page_size;
+        const int page = in_lds ? s_page[s_flat[b] + p - s_rows[b] / page_size] : table[static_cast<size_t>(b) * max_pages + p];
+        if (page >= 0 && page < num_pages) slot = page * page_size + row - p * page_size;
+      }
     }
     slots[t] = slot;
   }
@@ -196,55 +209,89 @@ __global__ __launch_bounds__(256) void kv_pages_slots_kernel(const int* __restri
   const int c = cached[b];
   // an admitted request of new tokens has rows; a refused one's length is 0
   const bool ok = seq_lens[b] > 0;
-  for (long t = static_cast<long>(q0) + t0; t < q1; t += step)
-    slots[t] = ok ? slot_of(table, max_pages, page_size, num_pages, b, c + static_cast<int>(t - q0)) : -1;
+  for (long t = static_cast<long>(q0) + t0; t < q1; t += step) {
+    int slot = -1;
+    if (ok) {
+      const int row = c + static_cast<int>(t - q0), p = row / page_size;
+      const int page = table[static_cast<size_t>(b) * max_pages + p];
+      if (page >= 0 && page < num_pages) slot = page * page_size + row - p * page_size;
+    }
+    slots[t] = slot;
+  }
 }
 
-// Entries of flagged rows go onto the stack in order of request and page. A
-// wave counts a row's entries; the rows' counts are summed; a wave then writes
-// its row's entries behind those of the rows before.
+// Entries of flagged rows go onto the stack in order of request and page. The
+// flagged rows are listed; a wave counts a row's entries, 512 at a time, the
+// counts are summed, and a wave then writes its row's entries behind those of
+// the rows before. Up to 16 rows of up to 512 entries are read once.
+constexpr int kRowChunk = 8;    // entries of a lane
+
 __global__ __launch_bounds__(kPlanThreads) void kv_pages_release_kernel(const int* __restrict__ release, int* table,
                                                                         int* free_pages, int* free_count, int B,
                                                                         int max_pages, int num_pages) {
   extern __shared__ int s_dyn[];
-  int* s_at = s_dyn;   // [B + 1]
+  int* s_row = s_dyn;          // [B] the flagged rows
+  int* s_at = s_row + B;       // [B + 1] entries of those before
   __shared__ int s_wi[kPlanWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int have = min(max(*free_count, 0), num_pages);
-  for (int b = wave; b < B; b += kPlanWaves) {
-    int n = 0;
-    if (release[b] != 0)
-      for (int p = lane; p < max_pages; p += 64) n += table[static_cast<size_t>(b) * max_pages + p] >= 0;
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) n += __shfl_xor(n, off);
-    if (lane == 0) s_at[b + 1] = n;
+  int rows = 0;
+  for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    const int flag = b < B && release[b] != 0;
+    int all;
+    const int incl = rows + block_scan<int>(flag, s_wi, &all);
+    if (flag) s_row[incl - 1] = b;
+    rows += all;
   }
   if (tid == 0) s_at[0] = 0;
   __syncthreads();
+  int v[kRowChunk];
+  auto read = [&](const int* row, int p0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kRowChunk; ++i) {
+      const int p = p0 + 64 * i + lane;
+      v[i] = p < max_pages ? row[p] : -1;
+    }
+  };
+  auto row_of = [&](int k) __attribute__((always_inline)) { return table + static_cast<size_t>(s_row[k]) * max_pages; };
+  for (int k = wave; k < rows; k += kPlanWaves) {
+    int n = 0;
+    for (int p0 = 0; p0 < max_pages; p0 += 64 * kRowChunk) {
+      read(row_of(k), p0);
+#pragma unroll
+      for (int i = 0; i < kRowChunk; ++i) n += __popcll(__ballot(v[i] >= 0));
+    }
+    if (lane == 0) s_at[k + 1] = n;
+  }
+  __syncthreads();
   int sum = 0;
-  for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
-    const int b = b0 + tid;
-    const int n = b < B ? s_at[b + 1] : 0;
+  for (int k0 = 0; k0 < rows; k0 += kPlanThreads) {
+    const int k = k0 + tid;
+    const int n = k < rows ? s_at[k + 1] : 0;
     int all;
     const int incl = sum + block_scan<int>(n, s_wi, &all);
-    if (b < B) s_at[b + 1] = incl;
+    if (k < rows) s_at[k + 1] = incl;
     sum += all;
   }
   __syncthreads();
-  for (int b = wave; b < B; b += kPlanWaves) {
-    if (s_at[b + 1] == s_at[b]) continue;
-    int at = have + s_at[b];
-    for (int p0 = 0; p0 < max_pages; p0 += 64) {
-      const int p = p0 + lane;
-      int* entry = table + static_cast<size_t>(b) * max_pages + p;
-      const int page = p < max_pages ? *entry : -1;
-      const unsigned long long held = __ballot(page >= 0);
-      if (page >= 0) {
-        const int k = at + __popcll(held & ((1ull << lane) - 1));
-        if (k < num_pages) free_pages[k] = page;
-        *entry = -1;
+  const bool once = rows <= kPlanWaves && max_pages <= 64 * kRowChunk;
+  for (int k = wave; k < rows; k += kPlanWaves) {
+    if (s_at[k + 1] == s_at[k]) continue;
+    int at = have + s_at[k];
+    int* row = row_of(k);
+    for (int p0 = 0; p0 < max_pages; p0 += 64 * kRowChunk) {
+      if (!once) read(row, p0);
+#pragma unroll
+      for (int i = 0; i < kRowChunk; ++i) {
+        const unsigned long long held = __ballot(v[i] >= 0);
+        if (v[i] >= 0) {
+          const int j = at + __popcll(held & ((1ull << lane) - 1));
+          if (j < num_pages) free_pages[j] = v[i];
+          row[p0 + 64 * i + lane] = -1;
+        }
+        at += __popcll(held);
       }
-      at += __popcll(held);
     }
   }
   if (tid == 0) *free_count = min(have + sum, num_pages);
@@ -273,7 +320,7 @@ extern "C" int aila_hip_kv_pages_reserve(const int* cached_lens, const int* new_
   AILA_REQUIRE(max_tokens > 0, "kv_pages_reserve: max_tokens=%d must be positive", max_tokens);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool in_plan = max_tokens <= kSlotsInPlan;
-  const size_t lds = static_cast<size_t>(4 * B + 2) * sizeof(int);
+  const size_t lds = static_cast<size_t>(6 * B + 2) * sizeof(int);
   hipLaunchKernelGGL(kv_pages_reserve_kernel, dim3(1), dim3(kPlanThreads), lds, st, cached_lens, new_lens, block_table,
                      free_pages, free_count, query_start, seq_lens, slots, B, max_pages, page_size, num_pages,
                      max_tokens, in_plan ? 1 : 0);
@@ -291,7 +338,7 @@ extern "C" int aila_hip_kv_pages_release(const int* release, int* block_table, i
   AILA_REQUIRE(max_pages > 0 && static_cast<long>(max_pages) * B < (1L << 31), "kv_pages_release: bad max_pages=%d",
                max_pages);
   AILA_REQUIRE(num_pages > 0, "kv_pages_release: num_pages=%d must be positive", num_pages);
-  hipLaunchKernelGGL(kv_pages_release_kernel, dim3(1), dim3(kPlanThreads), static_cast<size_t>(B + 1) * sizeof(int),
+  hipLaunchKernelGGL(kv_pages_release_kernel, dim3(1), dim3(kPlanThreads), static_cast<size_t>(2 * B + 1) * sizeof(int),
                      static_cast<hipStream_t>(stream), release, block_table, free_pages, free_count, B, max_pages,
                      num_pages);
   return check_launch("kv_pages_release");

@@ -193,7 +193,8 @@ def _reserve_both(cached, new, table, free, count, page, cap):
 @pytest.mark.parametrize("B,page,mp,P,most,new,cap", [
     (1, 16, 4, 4, 60, 1, 1), (1, 64, 2, 3, 0, 128, 128), (3, 16, 8, 20, 100, 30, 64), (32, 64, 64, 900, 3000, 3, 300),
     (257, 16, 40, 5000, 600, 20, 2700), (1024, 16, 8, 8000, 100, 1, 1024), (1025, 48, 4, 2500, 150, 5, 20000),
-    (2048, 16, 6, 9000, 90, 2, 8193), (5, 128, 300, 1000, 20000, 9000, 40000), (40, 16, 30, 300, 400, 90, 2000)])
+    (2048, 16, 6, 9000, 90, 2, 8193), (5, 128, 300, 1000, 20000, 9000, 40000), (40, 16, 30, 300, 400, 90, 2000),
+    (40, 16, 1200, 30000, 19000, 100, 6000), (20, 16, 500, 9000, 7900, 3, 40)])
 def test_reserve_and_release(B, page, mp, P, most, new, cap):
     """Ordinary steps, pools and batches too small for all, requests absent, rows
     that exceed the table, repeated calls and rows taken back."""
