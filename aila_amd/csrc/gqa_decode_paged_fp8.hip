@@ -32,7 +32,8 @@ struct Fp8DecodeArgs {
   const bf16* q;
   long q_stride;                       // elements between sequences' queries
   bf16* out;
-  float* part;                         // null: one workgroup per (sequence, head)
+  float* part;                         // records; null: one workgroup per (sequence, head)
+  int* units;                          // [B + 1] for the merge: units of the sequences before
   const int* seq_lens;
   int B, Hq, group, tile, chunks;      // query heads per KV head; per workgroup; workgroups per KV head
   int max_len;
@@ -99,6 +100,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void gqa_decode_paged_f
     scan_units(a, s_pre);
     const int units = s_pre[a.B] * heads, groups = min(static_cast<int>(gridDim.x), units);
     const int w = blockIdx.x;
+    if (w == 0)
+      for (int i = threadIdx.x; i <= a.B; i += kThreads) a.units[i] = s_pre[i];
     if (w >= groups) return;
     u = share_begin(w, units, groups);
     u1 = share_begin(w + 1, units, groups);
@@ -215,26 +218,29 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void gqa_decode_paged_f
   }
 }
 
+// The workgroups [w0, w1] that walked a (sequence, head).
+__device__ __forceinline__ void holders(const PagedFp8& c, const Fp8DecodeArgs& a, int b, int hc, int launched, int* w0, int* w1) {
+  const int heads = c.Hkv * a.chunks, before = a.units[b], nu = a.units[b + 1] - before;
+  const int units = a.units[a.B] * heads, groups = min(launched, units);
+  const int first = before * heads + hc * nu;
+  // workgroup w holds unit x: the largest w with w U / W < x + 1
+  *w0 = static_cast<int>((static_cast<long>(first + 1) * groups - 1) / units);
+  *w1 = static_cast<int>((static_cast<long>(first + nu) * groups - 1) / units);
+}
+
 // Joins the records of a (sequence, head) that several workgroups walked:
-// o = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i. One workgroup a query
-// head and 64 head dims: 16 columns of 4 dims, 16 record phases.
+// o = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i. Few sequences, many
+// records each: a workgroup takes a query head's 64 dims, 16 columns of 4 dims
+// and 16 record phases.
 template <int D>
 __global__ __launch_bounds__(256) void gqa_decode_paged_fp8_merge_kernel(PagedFp8 c, Fp8DecodeArgs a, int launched) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char s_dyn[];
-  int* s_pre = reinterpret_cast<int*>(s_dyn);
   __shared__ f32x4 s_a[16][16];
   __shared__ float s_m[16], s_l[16];
-  const int heads = c.Hkv * a.chunks;
   const int b = blockIdx.y, hq = blockIdx.x;
   const int kvh = hq / a.group, in = hq % a.group;
   const int hc = kvh * a.chunks + in / a.tile, h = in % a.tile;
-  scan_units(a, s_pre);
-  const int units = s_pre[a.B] * heads, groups = min(launched, units);
-  const int nu = s_pre[b + 1] - s_pre[b];
-  const int first = s_pre[b] * heads + hc * nu;
-  // the workgroup that holds unit x: the largest w with w U / W < x + 1
-  auto holder = [&](int x) { return static_cast<int>((static_cast<long>(x + 1) * groups - 1) / units); };
-  const int w0 = holder(first), w1 = holder(first + nu - 1);
+  int w0, w1;
+  holders(c, a, b, hc, launched, &w0, &w1);
   if (w0 == w1) return;   // one workgroup wrote the output
   const int col = threadIdx.x & 15, ph = threadIdx.x >> 4;
   const int d = blockIdx.z * 64 + 4 * col;
@@ -275,6 +281,36 @@ __global__ __launch_bounds__(256) void gqa_decode_paged_fp8_merge_kernel(PagedFp
   }
 }
 
+// The same for many sequences, few records each: a workgroup takes a
+// (sequence, head), a thread 4 dims of a query head.
+template <int D>
+__global__ __launch_bounds__(256) void gqa_decode_paged_fp8_merge_few_kernel(PagedFp8 c, Fp8DecodeArgs a, int launched) {
+  const int b = blockIdx.y, hc = blockIdx.x;
+  int w0, w1;
+  holders(c, a, b, hc, launched, &w0, &w1);
+  if (w0 == w1) return;
+  const int kvh = hc / a.chunks, chunk = hc % a.chunks;
+  const int gv = min(a.tile, a.group - chunk * a.tile);
+  for (int i = threadIdx.x; i < gv * (D / 4); i += 256) {
+    const int h = i / (D / 4), d = i % (D / 4) * 4;
+    f32x4 A = {0.f, 0.f, 0.f, 0.f};
+    float M = -INFINITY, L = 0.f;
+    for (int w = w0; w <= w1; ++w) {
+      const float* r = a.part + ((static_cast<size_t>(w) * 2 + (w == w0 ? 1 : 0)) * a.tile + h) * (D + kRecTail);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(r + d);
+      const float m = r[D], l = r[D + 1];
+      const float mn = fmaxf(M, m);
+      const float fo = M == -INFINITY ? 0.f : fast_exp2(M - mn), fn = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+      A = A * fo + x * fn;
+      L = L * fo + l * fn;
+      M = mn;
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    *reinterpret_cast<u32x2*>(a.out + (static_cast<size_t>(b) * a.Hq + kvh * a.group + chunk * a.tile + h) * D + d) =
+        u32x2{pack_bf16x2(A[0] * inv, A[1] * inv), pack_bf16x2(A[2] * inv, A[3] * inv)};
+  }
+}
+
 // Query heads of a workgroup and workgroups per KV head.
 void head_tiles(int group, int* tile, int* chunks) {
   *chunks = (group + kMaxTile - 1) / kMaxTile;
@@ -282,15 +318,19 @@ void head_tiles(int group, int* tile, int* chunks) {
 }
 
 size_t record_bytes(int tile, int D) { return static_cast<size_t>(2) * tile * (D + kRecTail) * sizeof(float); }
+// The unit counts stand before the records.
+size_t units_bytes(int B) { return (static_cast<size_t>(B + 1) * sizeof(int) + 255) / 256 * 256; }
 
 template <int D>
 int launch(const PagedFp8& c, const Fp8DecodeArgs& a, int groups, hipStream_t st) {
   const size_t lds = (static_cast<size_t>(kWaves) * a.tile * (D + 2)) * sizeof(float) +
                      (a.part ? static_cast<size_t>(a.B + 1) * sizeof(int) : 0);
   hipLaunchKernelGGL((gqa_decode_paged_fp8_kernel<D>), dim3(groups), dim3(kThreads), lds, st, c, a);
-  if (a.part)
-    hipLaunchKernelGGL((gqa_decode_paged_fp8_merge_kernel<D>), dim3(a.Hq, a.B, D / 64), dim3(256),
-                       static_cast<size_t>(a.B + 1) * sizeof(int), st, c, a, groups);
+  const int heads = c.Hkv * a.chunks;
+  if (a.part && a.B * heads >= 64)
+    hipLaunchKernelGGL((gqa_decode_paged_fp8_merge_few_kernel<D>), dim3(heads, a.B), dim3(256), 0, st, c, a, groups);
+  else if (a.part)
+    hipLaunchKernelGGL((gqa_decode_paged_fp8_merge_kernel<D>), dim3(a.Hq, a.B, D / 64), dim3(256), 0, st, c, a, groups);
   return check_launch("gqa_decode_paged_fp8");
 }
 
@@ -310,7 +350,7 @@ extern "C" size_t aila_hip_gqa_decode_paged_fp8_workspace_size(int B, int Hq, in
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || max_len < 0) return 0;
   int tile, chunks;
   head_tiles(Hq / Hkv, &tile, &chunks);
-  return split_groups(B, Hkv * chunks, max_len, D) * record_bytes(tile, D);
+  return units_bytes(B) + std::max(2L, split_groups(B, Hkv * chunks, max_len, D)) * record_bytes(tile, D);
 }
 
 extern "C" int aila_hip_gqa_decode_paged_fp8(const void* q, long q_stride, const void* k_pages, const void* v_pages,
@@ -348,14 +388,26 @@ extern "C" int aila_hip_gqa_decode_paged_fp8(const void* q, long q_stride, const
   AILA_REQUIRE(static_cast<long>(B) * heads * ((max_len + kUnit - 1) / kUnit + 1) < (1L << 31),
                "gqa_decode_paged_fp8: B=%d sequences of up to %d rows and %d heads are too many", B, max_len, heads);
   long groups = static_cast<long>(B) * heads;
-  if (workspace != nullptr && max_len > kUnit) {
+  // One workgroup per (sequence, head) where that is faster than a split and its
+  // merge (us, whole / split): up to 6 units a sequence (D = 64: 8, D = 256: 4;
+  // one sequence, 16/8 heads, D = 128: 612 rows 7.7 / 9.2, 900 9.6 / 8.9; D = 256:
+  // 450 11.3 / 11.4, 612 12.3 / 11.5; D = 64: 900 7.4 / 8.1, 1300 8.9 / 8.1), and
+  // where they fill the CUs, up to 4096 rows (D = 256: 2048): lengths between 5 and
+  // 100% of the bound, 64 sequences, D = 128: 2000 rows 37.8 / 47.1, 4000 68.9 /
+  // 68.1, 16000 260 / 198; D = 256: 2000 39.1 / 52.1, 4000 70.9 / 67.8.
+  const int few = (D == 64 ? 8 : D == 128 ? 6 : 4) * kUnit, many = D == 256 ? 2048 : 4096;
+  const bool whole = max_len <= few || (groups >= 256 && max_len <= many);
+  if (workspace != nullptr) {
     AILA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "gqa_decode_paged_fp8: workspace must be 16-byte aligned");
     const size_t rec = record_bytes(a.tile, D);
-    if (workspace_bytes < 2 * rec)
-      return set_error(AILA_HIP_EWORKSPACE, "gqa_decode_paged_fp8: workspace %zu bytes holds < 2 workgroups' records (%zu bytes each)",
-                       workspace_bytes, rec);
-    groups = std::min<long>(split_groups(B, heads, max_len, D), static_cast<long>(workspace_bytes / rec));
-    a.part = static_cast<float*>(workspace);
+    if (workspace_bytes < units_bytes(B) + 2 * rec)
+      return set_error(AILA_HIP_EWORKSPACE, "gqa_decode_paged_fp8: workspace %zu bytes, %zu are the least", workspace_bytes,
+                       units_bytes(B) + 2 * rec);
+    if (!whole) {
+      groups = std::min<long>(split_groups(B, heads, max_len, D), static_cast<long>((workspace_bytes - units_bytes(B)) / rec));
+      a.units = static_cast<int*>(workspace);
+      a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + units_bytes(B));
+    }
   }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   switch (D) {

@@ -40,6 +40,7 @@ constexpr int kRows = 32 * kGroupWaves;    // query rows of a tile
 constexpr int kMaxSequences = 4096;
 constexpr int kCus = 256;
 constexpr int kNoKey = 0x7fffffff;
+constexpr int kThinRows = 16;              // a tile of so few rows is walked by single waves
 
 
 struct Fp8PrefillArgs {
@@ -228,19 +229,18 @@ __device__ __forceinline__ T plan_scan(T x, T* s_wave, T* total) {
 }
 
 __global__ __launch_bounds__(kPlanThreads) void gqa_prefill_paged_fp8_plan_kernel(Fp8PrefillArgs a, int key_tile) {
-  extern __shared__ int s_first[];     // [B + 1] first tile of each request
+  extern __shared__ int s_dyn_plan[];
+  int* s_first = s_dyn_plan;          // [B + 1] first tile of each request
+  int* s_n = s_first + a.B + 1;       // [B] tokens
+  int* s_len = s_n + a.B;             // [B] rows
   __shared__ int s_wave[kPlanThreads / 64];
   __shared__ long s_wave_l[kPlanThreads / 64];
   __shared__ int s_bucket[kBuckets];
-  __shared__ unsigned long long s_sum;
   const int tid = threadIdx.x;
   PlanItem* items = reinterpret_cast<PlanItem*>(a.plan + kPlanHead);
   PlanCut* cuts_of = reinterpret_cast<PlanCut*>(items + plan_items(a.T, a.B, a.group, a.lanes));
   s_bucket[tid] = 0;
-  if (tid == 0) {
-    s_first[0] = 0;
-    s_sum = 0;
-  }
+  if (tid == 0) s_first[0] = 0;
   // malformed starts may overlap: no more tiles than the list holds
   const long most = plan_items(a.T, a.B, a.group, 0);
   long all_tiles = 0;
@@ -250,65 +250,89 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_prefill_paged_fp8_plan_kerne
     if (b < a.B) load_request(a, b, &it);
     long all;
     const long incl = all_tiles + plan_scan<long>((it.n * a.group + kRows - 1) / kRows, s_wave_l, &all);
-    if (b < a.B) s_first[b + 1] = static_cast<int>(min(incl, most));
+    if (b < a.B) {
+      s_first[b + 1] = static_cast<int>(min(incl, most));
+      s_n[b] = it.n;
+      s_len[b] = it.len;
+    }
     all_tiles += all;
   }
   const int tiles = static_cast<int>(min(all_tiles, most));
   __syncthreads();
-  auto tile = [&](int f, Item* it) __attribute__((always_inline)) {   // -> key tiles
+  // Tile f: its request, first row, key tiles and what walking them costs, in
+  // quarters of a key tile: one of at most kThinRows rows is walked by single
+  // waves, each its own keys.
+  struct Tile { int b, r0, kt, cost; };
+  auto tile = [&](int f) __attribute__((always_inline)) {
     int lo = 0, hi = a.B;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (s_first[mid] <= f) lo = mid; else hi = mid;
     }
-    load_request(a, lo, it);
-    it->r0 = (f - s_first[lo]) * kRows;
-    return (tile_end(a, *it) + key_tile - 1) / key_tile;
+    Tile x;
+    x.b = lo;
+    x.r0 = (f - s_first[lo]) * kRows;
+    Item it{};
+    it.n = s_n[lo];
+    it.len = s_len[lo];
+    it.r0 = x.r0;
+    x.kt = (tile_end(a, it) + key_tile - 1) / key_tile;
+    x.cost = it.n * a.group - x.r0 <= kThinRows ? x.kt : 4 * x.kt;
+    return x;
   };
-  unsigned long long sum = 0;
-  for (int f = tid; f < tiles; f += kPlanThreads) {
-    Item it;
-    sum += tile(f, &it);
+  Tile mine{};      // the first round's, which is all there are as a rule
+  if (tid < tiles) mine = tile(tid);
+  auto tile_at = [&](int f) __attribute__((always_inline)) { return f < kPlanThreads ? mine : tile(f); };
+  long sum = 0;
+  for (int f0 = 0; f0 < tiles; f0 += kPlanThreads) {
+    const int f = f0 + tid;
+    long all;
+    plan_scan<long>(f < tiles ? tile_at(f).cost : 0, s_wave_l, &all);
+    sum += all;
   }
-  atomicAdd(&s_sum, sum);
-  __syncthreads();
-  const int share = max(kMinRun, static_cast<int>((s_sum + a.lanes - 1) / a.lanes));
-  auto bucket = [&](int size) __attribute__((always_inline)) {   // large sizes first
-    return kBuckets - 1 - static_cast<int>(static_cast<long>(size) * (kBuckets - 1) / share);
+  const int share = max(4 * kMinRun, static_cast<int>((sum + a.lanes - 1) / a.lanes));
+  auto cuts_for = [&](const Tile& x) __attribute__((always_inline)) { return max(1, (x.cost + share - 1) / share); };
+  // run i of a tile's key tiles, large runs' buckets first
+  auto run_begin = [&](const Tile& x, int cuts, int i) __attribute__((always_inline)) {
+    return x.kt / cuts * i + x.kt % cuts * i / cuts;
+  };
+  auto bucket = [&](const Tile& x, int cuts) __attribute__((always_inline)) {
+    return kBuckets - 1 - static_cast<int>(static_cast<long>(x.cost / cuts) * (kBuckets - 1) / share);
   };
   for (int f = tid; f < tiles; f += kPlanThreads) {
-    Item it;
-    const int kt = tile(f, &it), cuts = max(1, (kt + share - 1) / share);
-    for (int i = 0; i < cuts; ++i)
-      atomicAdd(&s_bucket[bucket(static_cast<int>(static_cast<long>(kt) * (i + 1) / cuts - static_cast<long>(kt) * i / cuts))], 1);
+    const Tile x = tile_at(f);
+    const int cuts = cuts_for(x);
+    atomicAdd(&s_bucket[bucket(x, cuts)], cuts);
   }
   __syncthreads();
-  const int mine = s_bucket[tid];
+  const int count = s_bucket[tid];
   int total;
-  const int incl = plan_scan<int>(mine, s_wave, &total);
-  s_bucket[tid] = incl - mine;
+  const int incl = plan_scan<int>(count, s_wave, &total);
+  s_bucket[tid] = incl - count;
   __syncthreads();
   // Which workgroup an item goes to depends on the order within a bucket, its
   // result does not: records are numbered by the tiles' order.
   int recs = 0, cut_tiles = 0;
   for (int f0 = 0; f0 < tiles; f0 += kPlanThreads) {
     const int f = f0 + tid;
-    Item it{};
-    int kt = 0, cuts = 0;
+    Tile x{};
+    int cuts = 0;
     if (f < tiles) {
-      kt = tile(f, &it);
-      cuts = max(1, (kt + share - 1) / share);
+      x = tile_at(f);
+      cuts = cuts_for(x);
     }
-    const int cut = cuts > 1;
-    int all_r, all_c;
-    const int rec = recs + plan_scan<int>(cut ? cuts : 0, s_wave, &all_r) - (cut ? cuts : 0);
-    const int slot = cut_tiles + plan_scan<int>(cut, s_wave, &all_c) - cut;
-    recs += all_r;
-    cut_tiles += all_c;
-    if (cut) cuts_of[slot] = PlanCut{it.b, it.r0, rec, cuts};
-    for (int i = 0; i < cuts; ++i) {
-      const int t0 = static_cast<int>(static_cast<long>(kt) * i / cuts), t1 = static_cast<int>(static_cast<long>(kt) * (i + 1) / cuts);
-      items[atomicAdd(&s_bucket[bucket(t1 - t0)], 1)] = PlanItem{it.b, it.r0, t0, t1, cut ? rec + i : -1};
+    // both sums in one: fewer than 2^15 tiles are cut, into fewer than 2^16 runs
+    const int cut = cuts > 1 ? cuts << 15 | 1 : 0;
+    int all;
+    const int before = plan_scan<int>(cut, s_wave, &all) - cut;
+    const int rec = recs + (before >> 15), slot = cut_tiles + (before & 0x7fff);
+    recs += all >> 15;
+    cut_tiles += all & 0x7fff;
+    if (cut) cuts_of[slot] = PlanCut{x.b, x.r0, rec, cuts};
+    if (cuts > 0) {
+      int at = atomicAdd(&s_bucket[bucket(x, cuts)], cuts);
+      for (int i = 0; i < cuts; ++i, ++at)
+        items[at] = PlanItem{x.b, x.r0, run_begin(x, cuts, i), run_begin(x, cuts, i + 1), cut ? rec + i : -1};
     }
   }
   if (tid == 0) {
@@ -317,7 +341,108 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_prefill_paged_fp8_plan_kerne
   }
 }
 
+// Place in a record of head dim d of query row r < 32.
 template <int D>
+__device__ __forceinline__ int record_at(int r, int d) {
+  const int j = d & 3;
+  const int dt = D == 64 ? j >> 1 : j + 4 * (d >> 7), m = D == 64 ? (d >> 2) + 16 * (j & 1) : (d & 127) >> 2;
+  return ((dt * 4 + (m >> 3)) * 64 + (m >> 2 & 1) * 32 + r) * 4 + (m & 3);
+}
+
+// A tile of up to 16 rows (a decoding request's token, the rest of a prompt): no
+// use of the codes but one, so nothing is staged. Each of the workgroup's 8
+// waves walks every eighth strip of 32 keys as the decode kernel does, and
+// their states meet in LDS (s_o: 16 * 8 * D floats).
+template <int D>
+__device__ __forceinline__ void thin_item(const PagedFp8& c, const Fp8PrefillArgs& a, const Item& it, int kvh, float* s_o,
+                                          float* s_ml) {
+  constexpr int kWaves = kThreads / 64;
+  constexpr int kDepth = D == 256 ? 1 : 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m16 = lane & 15, g4 = lane >> 4;
+  const int rows = it.n * a.group - it.r0;
+  const int row = it.r0 + min(m16, rows - 1);
+  const int tok = row / a.group;
+  const int lim = max(it.len - it.n + tok + 1, 0);
+  const int first = max(it.len - it.n + it.r0 / a.group + 1, 0);   // keys that every row attends
+  const bf16* src = a.q + static_cast<size_t>(it.q0 + tok) * a.q_stride + static_cast<size_t>(kvh * a.group + row - tok * a.group) * D;
+  bf16x8_t q[D / 32];
+#pragma unroll
+  for (int ks = 0; ks < D / 32; ++ks) q[ks] = as_bf16x8(ld16(src + 64 * (ks >> 1) + 16 * g4 + 8 * (ks & 1)));
+  Column<D> col;
+  clear_column(col);
+  const int row0 = it.t0 * Cfg<D>::BN + 32 * wave;
+  const int end = min(it.t1 * Cfg<D>::BN, tile_end(a, it));
+  const int ns = row0 < end ? (end - row0 + 32 * kWaves - 1) / (32 * kWaves) : 0;
+  const int blk_end = (end + kScaleRows - 1) / kScaleRows;
+  for (int n0 = 0; n0 < ns; n0 += 32) {
+    const BlockRef mine = block_ref(c, it.b, kvh, row0 / kScaleRows + (n0 + (lane >> 1)) * (2 * kWaves) + (lane & 1), blk_end);
+    const int n1 = min(ns - n0, 32);
+    auto load = [&](Strip<D>& s, int n) __attribute__((always_inline)) {
+      const bool in = n < n1;
+      const int ba = __builtin_amdgcn_readlane(mine.bid, 2 * n & 63), bb = __builtin_amdgcn_readlane(mine.bid, (2 * n + 1) & 63);
+      load_strip<D, true>(s, c, in ? ba : -1, in ? bb : -1, m16, g4);
+    };
+    Strip<D> s[kDepth];
+#pragma unroll
+    for (int i = 0; i < kDepth - 1; ++i) load(s[i], i);
+    for (int n = 0; n < n1; n += kDepth) {
+#pragma unroll
+      for (int i = 0; i < kDepth; ++i) {
+        if (n + i < n1) {
+          load(s[(i + kDepth - 1) % kDepth], n + i + kDepth - 1);
+          const int ba = __builtin_amdgcn_readlane(mine.bid, 2 * (n + i)), bb = __builtin_amdgcn_readlane(mine.bid, 2 * (n + i) + 1);
+          const int at = row0 + (n0 + n + i) * 32 * kWaves;
+          strip_step<D>(col, s[i], q, readlane_f(mine.ks, 2 * (n + i)) * a.scale_log2, readlane_f(mine.ks, 2 * (n + i) + 1) * a.scale_log2,
+                        readlane_f(mine.vs, 2 * (n + i)), readlane_f(mine.vs, 2 * (n + i) + 1),
+                        at + 32 > min(end, first) || (ba | bb) < 0, at, min(lim, end), ba >= 0, bb >= 0, g4);
+        }
+      }
+    }
+  }
+  const float l = xrow4_sum(col.l);
+  __syncthreads();     // the item before has been written
+  float* mine_o = s_o + (wave * 16 + m16) * D;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) mine_o[(D / 16) * (4 * g4 + i) + t] = col.acc[t][i];
+  }
+  if (g4 == 0) {
+    s_ml[(wave * 16 + m16) * 2] = col.m;
+    s_ml[(wave * 16 + m16) * 2 + 1] = l;
+  }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < rows * D; idx += kThreads) {
+    const int r = idx / D, d = idx % D;
+    float M = -INFINITY, A = 0.f, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, s_ml[(w * 16 + r) * 2]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float mw = s_ml[(w * 16 + r) * 2];
+      const float f = mw == -INFINITY ? 0.f : fast_exp2(mw - M);
+      A += f * s_o[(w * 16 + r) * D + d];
+      L += f * s_ml[(w * 16 + r) * 2 + 1];
+    }
+    if (it.rec >= 0) {
+      float* rec = a.part + (static_cast<size_t>(it.rec) * c.Hkv + kvh) * Cfg<D>::REC;
+      rec[record_at<D>(r, d)] = A;
+      if (d == 0) {
+        rec[kRows * D + r * 2] = M;
+        rec[kRows * D + r * 2 + 1] = L;
+      }
+    } else {
+      const int rr = it.r0 + r, tk = rr / a.group;
+      a.out[(static_cast<size_t>(it.q0 + tk) * a.Hq + kvh * a.group + rr - tk * a.group) * D + d] = f2bf(L == 0.f ? 0.f : A / L);
+    }
+  }
+  __syncthreads();     // LDS is the next item's
+}
+
+// THIN: the items may be thin ones. (A kernel that never meets one is a variant of
+// its own: the thin walk's registers cost the other's loop 5-9%.)
+template <int D, bool THIN>
 __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(PagedFp8 c, Fp8PrefillArgs a) {
   using C = Cfg<D>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char s_dyn[];
@@ -399,6 +524,11 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
   bool holes = false, primed = false;       // primed: its first DMAs are on the way
   for (int round = 1; more; ++round) {
     const int rows = it.n * a.group;
+    if (THIN && rows - it.r0 <= kThinRows) {
+      thin_item<D>(c, a, it, kvh, reinterpret_cast<float*>(s_dyn), &s_ml[0][0][0]);
+      more = get_item<D>(a, item_at(round), &it);
+      continue;
+    }
     const int row = it.r0 + wave * 32 + l32;          // this lane's query row
     // rows past the request's are computed like its last and not stored
     const int tok = min(row, rows - 1) / a.group;
@@ -690,7 +820,8 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
     // The next item's first codes are fetched meanwhile, if it walks the same keys.
     const Item done = it;
     more = get_item<D>(a, item_at(round), &it);
-    if (more && it.b == seg_b && it.t0 == seg_0 && it.t0 < it.t1 && it.t1 <= seg_1 && it.rec < 0) {
+    if (more && it.b == seg_b && it.t0 == seg_0 && it.t0 < it.t1 && it.t1 <= seg_1 && it.rec < 0 &&
+        !(THIN && it.n * a.group - it.r0 <= kThinRows)) {
       start();
       primed = true;
     }
@@ -880,7 +1011,12 @@ int launch(PagedFp8 c, Fp8PrefillArgs a, void* workspace, size_t workspace_bytes
   const size_t need = workspace_need<D>(a.T, a.B, c.Hkv, a.group, a.max_len, &a.lanes, &a.splits);
   const int tiles = static_cast<int>((static_cast<long>(a.T) * a.group + kRows - 1) / kRows);
   auto walk = [&](const PagedFp8& cache, const Fp8PrefillArgs& args) {
-    hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D>), dim3(args.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, cache, args);
+    // one request's last tile may be thin too, but is one of many then
+    const bool thin = a.B > 1 || static_cast<long>(a.T) * a.group <= kThinRows;
+    if (thin)
+      hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D, true>), dim3(args.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, cache, args);
+    else
+      hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D, false>), dim3(args.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, cache, args);
   };
   auto merge = [&](int cut_tiles) {
     hipLaunchKernelGGL((gqa_prefill_paged_fp8_merge_kernel<D>), dim3(cut_tiles, c.Hkv, 4 * (D > 128 ? D / 128 : 1)), dim3(256), 0,
@@ -906,7 +1042,7 @@ int launch(PagedFp8 c, Fp8PrefillArgs a, void* workspace, size_t workspace_bytes
       return set_error(AILA_HIP_EWORKSPACE, "gqa_prefill_paged_fp8: a workspace of %zu bytes, %zu are needed", workspace_bytes, need);
     a.plan = static_cast<int*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan_bytes(a.T, a.B, a.group, a.lanes));
-    hipLaunchKernelGGL(gqa_prefill_paged_fp8_plan_kernel, dim3(1), dim3(kPlanThreads), static_cast<size_t>(a.B + 1) * sizeof(int), st, a,
+    hipLaunchKernelGGL(gqa_prefill_paged_fp8_plan_kernel, dim3(1), dim3(kPlanThreads), static_cast<size_t>(3 * a.B + 1) * sizeof(int), st, a,
                        Cfg<D>::BN);
     walk(c, a);
     merge(a.lanes);

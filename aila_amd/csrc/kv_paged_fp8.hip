@@ -34,10 +34,20 @@ __device__ __forceinline__ uint32_t pack_fp8x4(float a, float b, float c, float 
   return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true));
 }
 
+template <int CTRL>
+__device__ __forceinline__ int dpp_i(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xF, 0xF, false);
+}
+// Maximum of the wave's values, in every lane.
 __device__ __forceinline__ int wave_max(int x) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x = max(x, __shfl_xor(x, off));
-  return x;
+  x = max(x, dpp_i<kDppQuadXor1>(x));
+  x = max(x, dpp_i<kDppQuadXor2>(x));
+  x = max(x, dpp_i<kDppRowHalfMirror>(x));
+  x = max(x, dpp_i<kDppRowMirror>(x));
+  const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  x = max(static_cast<int>(a[0]), static_cast<int>(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return max(static_cast<int>(b[0]), static_cast<int>(b[1]));
 }
 
 // Grid (ceil(T / tile), ceil(Hkv / 2)); wave w: K or V (w & 1) of head
@@ -60,22 +70,22 @@ __global__ __launch_bounds__(kThreads) void kv_append_paged_fp8_kernel(
   const int t0 = static_cast<int>(blockIdx.x) * tile;
   const int rr = lane / LR, c8 = (lane % LR) * 8;
 
-  // tokens of the tile that begin a run: lane i looks at token t0 + i
-  const int ti = t0 + lane;
-  const int slot_i = ti < T ? slots[ti] : -1;
-  const int slot_b = ti > 0 && ti <= T ? slots[ti - 1] : -1;
-  const bool begins = lane < tile && slot_i >= 0 && slot_i < num_slots &&
-                      !(slot_b >= 0 && slot_b + 1 == slot_i && slot_i % kScaleRows != 0);
+  // Lane i holds the slot of token t0 + i - 1: a tile's runs end 31 tokens after
+  // its begin at most.
+  const int ti = t0 + lane - 1;
+  const int win = ti >= 0 && ti < T && lane < 2 * kScaleRows + 1 ? slots[ti] : -1;
+  const int before = __shfl_up(win, 1);
+  const bool begins = lane >= 1 && lane <= tile && win >= 0 && win < num_slots &&
+                      !(before >= 0 && before + 1 == win && win % kScaleRows != 0);
   unsigned long long todo = __ballot(begins);
   while (todo) {
     const int i = __builtin_ctzll(todo);
     todo &= todo - 1;
-    const int t = t0 + i;
-    const int slot = __shfl(slot_i, i);
+    const int t = t0 + i - 1;
+    const int slot = __builtin_amdgcn_readlane(win, i);
     const int r0 = slot % kScaleRows;
-    // the run: lane j compares token t + j's slot
-    const int next = lane < kScaleRows && t + lane < T ? slots[t + lane] : -1;
-    const unsigned long long off = ~__ballot(lane < kScaleRows - r0 && next == slot + lane);
+    // the run: the tokens from i on whose slots go on, to the block's end
+    const unsigned long long off = ~(__ballot(lane >= i && lane - i < kScaleRows - r0 && win == slot + (lane - i)) >> i);
     const int n = __builtin_ctzll(off);      // 1 .. 16 - r0
 
     u32x4 x[NI];

@@ -58,7 +58,7 @@ def test_refusals(name, args, bad):
 
 def test_workspace_sizes():
     f = aila_amd.gqa_decode_paged_fp8_workspace_size
-    assert f(1, 16, 8, 128, 612) == 8 * 5 * 2 * 2 * 132 * 4        # a record pair for each 128 rows of each KV head
+    assert f(1, 16, 8, 128, 612) == 256 + 8 * 5 * 2 * 2 * 132 * 4  # a record pair for each 128 rows of each KV head, and the counts
     assert f(64, 40, 8, 128, 4000) == f(64, 40, 8, 128, 32768)     # as many as the device holds
     assert f(0, 16, 8, 128, 612) == f(1, 16, 0, 128, 612) == f(1, 15, 8, 128, 612) == f(1, 16, 8, 128, -1) == 0
     assert aila_amd.gqa_prefill_paged_fp8_workspace_size(0, 1, 16, 8, 128, 100) == 0
