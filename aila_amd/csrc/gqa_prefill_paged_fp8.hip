@@ -42,7 +42,6 @@ constexpr int kCus = 256;
 constexpr int kNoKey = 0x7fffffff;
 constexpr int kThinRows = 16;              // a tile of so few rows is walked by single waves
 
-
 struct Fp8PrefillArgs {
   const bf16* q;
   long q_stride;
@@ -290,7 +289,8 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_prefill_paged_fp8_plan_kerne
     plan_scan<long>(f < tiles ? tile_at(f).cost : 0, s_wave_l, &all);
     sum += all;
   }
-  const int share = max(4 * kMinRun, static_cast<int>((sum + a.lanes - 1) / a.lanes));
+  // (no tile costs 2^28: T * group and max_len are at most 2^30)
+  const int share = static_cast<int>(min(max(4L * kMinRun, (sum + a.lanes - 1) / a.lanes), 1L << 28));
   auto cuts_for = [&](const Tile& x) __attribute__((always_inline)) { return max(1, (x.cost + share - 1) / share); };
   // run i of a tile's key tiles, large runs' buckets first
   auto run_begin = [&](const Tile& x, int cuts, int i) __attribute__((always_inline)) {
@@ -609,27 +609,30 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
         x.sc = s_vs[first_block(j) + (oc >> 1)];
         return x;
       };
+      // 0 times NaN is NaN: a masked row must not carry one into the product. NaN
+      // codes are taken out and remembered by dim; the epilogue puts NaN into the
+      // rows that attend the first.
       auto clean_v = [&](RawV& x, int j) __attribute__((always_inline)) {
-                  // 0 times NaN is NaN: a masked row must not carry one into the product.
-                  // NaN codes are taken out and remembered by dim; the epilogue puts NaN
-                  // into the rows that attend the first.
-                  const uint32_t keep = s_bid[first_block(j) + (oc >> 1)] >= 0 ? 0xffffffffu : 0u;
-                  uint32_t seen = 0;
-        #pragma unroll
-                  for (int e = 0; e < 8; ++e) {
-                    const uint32_t n = nan_codes(x.v[e]) >> 7;
-                    seen |= n & keep;
-                    x.v[e] &= keep & ~(n * 0xffu);
-                  }
-                  if (seen) {
-                    const unsigned char* raw = v_raw + (j & 1) * C::RAW + v_from;
-                    const int key = s0 * C::BN + first_block(j) * kScaleRows + 16 * (oc >> 1) + 4 * (oc & 1);
-        #pragma unroll 1
-                    for (int e = 0; e < 32; ++e) {
-                      const int r = (e >> 2 & 3) + 8 * (e >> 4);
-                      if ((raw[r * D + (e & 3)] & 0x7f) == 0x7f) s_any_nan = 1, atomicMin(&s_nan[4 * dq + (e & 3)], key + r);
-                    }
-                  }
+        const uint32_t keep = s_bid[first_block(j) + (oc >> 1)] >= 0 ? 0xffffffffu : 0u;
+        uint32_t seen = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t n = nan_codes(x.v[e]) >> 7;
+          seen |= n & keep;
+          x.v[e] &= keep & ~(n * 0xffu);
+        }
+        if (seen) {
+          const unsigned char* raw = v_raw + (j & 1) * C::RAW + v_from;
+          const int key = s0 * C::BN + first_block(j) * kScaleRows + 16 * (oc >> 1) + 4 * (oc & 1);
+#pragma unroll 1
+          for (int e = 0; e < 32; ++e) {
+            const int r = (e >> 2 & 3) + 8 * (e >> 4);
+            if ((raw[r * D + (e & 3)] & 0x7f) == 0x7f) {
+              s_any_nan = 1;
+              atomicMin(&s_nan[4 * dq + (e & 3)], key + r);
+            }
+          }
+        }
       };
       auto store_v = [&](const RawV& x) __attribute__((always_inline)) {
         u32x4 w[4];

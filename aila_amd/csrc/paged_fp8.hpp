@@ -39,10 +39,6 @@ __device__ __forceinline__ void fp8x16_to_bf16(const u32x4& w, bf16x8_t& lo, bf1
                        fp8x2_to_bf16x2<true>(w[3])});
 }
 
-}  // namespace aila
-
-namespace aila {
-
 // What the attention kernels are given of the cache and its tables.
 struct PagedFp8 {
   const uint8_t* k_pages;
@@ -170,8 +166,9 @@ __device__ __forceinline__ void v_tiles(const uint32_t (&v)[8], bf16x8_t (&t)[4]
 // One strip into a column's softmax. `row` is the strip's first row; if masked,
 // a column attends rows < lim of the blocks that have a page (ok_a, ok_b).
 // ka, kb: the K scales times log2(e) / sqrt(D). The V scales go into P, where
-// they are exact. P goes in as the sum of two bf16 (16 bits): one would double the output's rounding error, and the
-// matrix cores are idle most of the time here.
+// they are exact. P goes in as the sum of two bf16 (16 bits): one
+// would double the output's rounding error, and the matrix cores are idle most of
+// the time here.
 //
 // A masked row's P is 0, but 0 times NaN is NaN, and a masked row may hold
 // anything. So a masked strip's NaN codes are taken out of V; where there are

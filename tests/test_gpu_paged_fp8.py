@@ -364,6 +364,184 @@ def test_large_scores(big):
     _check(got, q.expand(5, Hq, D), (kp, vp, ks, vs), table, [0, 5], [L], L, 2.0 ** -8)
 
 
+def _check_tokens(got, q, cache, table, starts, lens, max_len, tokens):
+    """As _check, for some of a batch's tokens: {request: its tokens}."""
+    for b, some in tokens.items():
+        L, a, n = min(lens[b], max_len), starts[b], starts[b + 1] - starts[b]
+        k, held = ref.gather(cache[0], cache[2], table[b], L)
+        v, _ = ref.gather(cache[1], cache[3], table[b], L)
+        for i in sorted({x % n for x in some}):
+            out, mag, big = ref.attention(q[a + i:a + i + 1], k, v, held, L - n + 1 + i)
+            tol = ref.attention_tolerance(out, mag, big, L, q.shape[2], 2.0 ** -8)
+            off = (got[a + i:a + i + 1].double() - out).abs() / tol
+            assert off.max() <= 1, (b, i, off.max().item())
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,page,new,lens", [
+    # one request: more keys than a workgroup looks up at once, with and without runs
+    (64, 8, 2, 16, [5], [40000]), (128, 4, 1, 64, [4], [35000]), (128, 4, 4, 64, [130], [33001]), (256, 8, 2, 64, [9], [12000]),
+    (256, 2, 2, 48, [200], [23077]), (64, 4, 4, 32, [700], [1500]), (128, 32, 2, 16, [150], [150]),
+    # batches: runs of odd lengths, tokens beside prompts, ends of prompts with few rows
+    (128, 8, 2, 64, [300, 1, 700, 2], [33000, 40000, 700, 5]), (64, 6, 2, 16, [129, 1, 1, 44], [2129, 9000, 31, 20011]),
+    (256, 16, 2, 32, [17, 3, 65, 1], [11100, 4097, 65, 12000]), (128, 2, 2, 16, [129, 257, 385, 8], [129, 777, 385, 3001]),
+    (64, 1, 1, 16, [128, 145, 1, 0, 16], [128, 145, 20000, 0, 16]), (256, 4, 4, 16, [130, 1, 140], [130, 7000, 6001])])
+def test_prefill_of_long_requests(D, Hq, Hkv, page, new, lens):
+    import torch
+    import aila_amd as A
+    B = len(lens)
+    P = sum(-(-n // page) for n in lens) + 3
+    cache = _cache(P, Hkv, page, D, D + Hq)
+    table = _table(lens, page, P, D + page)
+    max_len = table.shape[1] * page
+    starts = [0] + [int(x) for x in np.cumsum(new)]
+    T = starts[-1]
+    g = torch.Generator(device="cuda").manual_seed(Hq)
+    q = torch.randn((T, Hq, D), generator=g, device="cuda").to(torch.bfloat16)
+    some = {b: (0, 1, new[b] // 2, -2, -1) for b in range(B) if new[b]}
+    size = A.gqa_prefill_paged_fp8_workspace_size(T, B, Hq, Hkv, D, max_len)
+    for ws in (torch.empty(size, dtype=torch.uint8, device="cuda"), None):
+        out = A.gqa_prefill_paged_fp8(q, *cache, table, _i32(starts), _i32(lens), max_len, workspace=ws)
+        _check_tokens(out, q, cache, table, starts, lens, max_len, some)
+
+
+@pytest.mark.parametrize("B,D,Hq,Hkv", [(1300, 64, 2, 1), (4096, 128, 2, 2), (1100, 256, 4, 1)])
+def test_prefill_of_many_requests(B, D, Hq, Hkv):
+    """More tiles than the list's threads, most of them of one token; every request
+    against the decode of the same rows where it has one token."""
+    import torch
+    import aila_amd as A
+    page, rng = 16, np.random.default_rng(B)
+    lens = [int(x) for x in rng.integers(0, 60, B)]
+    lens[7], lens[B - 3] = 3001, 1500
+    new = [min(n, int(x)) for n, x in zip(lens, rng.choice([0, 1, 1, 1, 2, 17, 40], B))]
+    new[7], new[B - 3] = 1, 400
+    P = sum(-(-n // page) for n in lens) + 3
+    cache = _cache(P, Hkv, page, D, B)
+    table = _table(lens, page, P, B, extra=0)
+    max_len = table.shape[1] * page
+    starts = [0] + [int(x) for x in np.cumsum(new)]
+    T = starts[-1]
+    q = torch.randn((T, Hq, D), generator=torch.Generator(device="cuda").manual_seed(B), device="cuda").to(torch.bfloat16)
+    ws = torch.empty(A.gqa_prefill_paged_fp8_workspace_size(T, B, Hq, Hkv, D, max_len), dtype=torch.uint8, device="cuda")
+    out = A.gqa_prefill_paged_fp8(q, *cache, table, _i32(starts), _i32(lens), max_len, workspace=ws)
+    some = {b: (0, -1) for b in [7, B - 3] + [int(x) for x in rng.choice(B, 60)] if new[b]}
+    _check_tokens(out, q, cache, table, starts, lens, max_len, some)
+    ones = [b for b in range(B) if new[b] == 1]
+    at = torch.tensor([starts[b] for b in ones], device="cuda")
+    one = A.gqa_decode_paged_fp8(q[at], *cache, table[torch.tensor(ones, device="cuda")].contiguous(), _i32([lens[b] for b in ones]), max_len)
+    # half a step of bf16 each, and weights rounded to 2^-8 at most before values below 2 * 2^2
+    assert ((one.double() - out[at].double()).abs() <= 2.0 ** -7 * one.double().abs() * (1 + 2.0 ** -7) + 2.0 ** -8 * 8).all()
+
+
+@pytest.mark.parametrize("B,D,Hq,Hkv,page,most,max_len", [(20, 128, 8, 4, 32, 6000, 8000), (70, 64, 16, 1, 16, 5000, 6000), (9, 256, 32, 8, 64, 3000, 5000),
+                                                          (4096, 64, 2, 1, 16, 40, 48), (300, 128, 20, 1, 16, 500, 5000)])
+def test_decode_of_many_sequences(B, D, Hq, Hkv, page, most, max_len):
+    """Splits with few records each, and one workgroup per sequence and head."""
+    import torch
+    import aila_amd as A
+    rng = np.random.default_rng(B)
+    lens = [int(x) for x in rng.integers(0, most + 1, B)]
+    lens[1], lens[B // 2] = most, 0
+    P = sum(-(-n // page) for n in lens) + 3
+    cache = _cache(P, Hkv, page, D, B)
+    table = _table(lens, page, P, B, extra=-(-max_len // page) - -(-most // page))
+    q = torch.randn((B, Hq, D), generator=torch.Generator(device="cuda").manual_seed(B), device="cuda").to(torch.bfloat16)
+    size = A.gqa_decode_paged_fp8_workspace_size(B, Hq, Hkv, D, max_len)
+    some = [1, B // 2, B - 1] + [int(x) for x in rng.choice(B, 12)]
+    for ws in (torch.empty(size, dtype=torch.uint8, device="cuda"), None):
+        got = A.gqa_decode_paged_fp8(q, *cache, table, _i32(lens), max_len, workspace=ws)
+        for b in some:
+            _check(got[b:b + 1], q[b:b + 1], cache, table[b:b + 1], [0, 1], lens[b:b + 1], max_len, 2.0 ** -16)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_nan_rows_of_a_long_request(D):
+    """A NaN that lies behind some tokens of a chunk, far from the start: shown where
+    it is attended, in its dim, and nowhere else; with the keys walked in one run
+    and in several, for a tile's rows and for single rows."""
+    import torch
+    import aila_amd as A
+    page, L, Hq, Hkv = 16, 14000, 4, 2
+    P = L // page + 2
+    for n in (300, 5):
+        cache = _cache(P, Hkv, page, D, 5)
+        table = _table([L, 1], page, P, 6)
+        at = L - 1 - n // 2
+        cache[1].view(torch.uint8)[int(table[0, at // page]), 1, at % page, 11] = F8_NAN
+        q = torch.randn((n + 1, Hq, D), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(torch.bfloat16)
+        first = n - (L - at)           # the token whose own row it is
+        for B in (1, 2):
+            starts, lens = [0, n, n + 1][:B + 1], [L, 1][:B]
+            size = A.gqa_prefill_paged_fp8_workspace_size(n + 1, B, Hq, Hkv, D, L)
+            for ws in (torch.empty(size, dtype=torch.uint8, device="cuda"), None):
+                out = A.gqa_prefill_paged_fp8(q, *cache, table[:B], _i32(starts), _i32(lens), L, workspace=ws)[:n]
+                want = torch.zeros((n, Hq, D), dtype=torch.bool, device="cuda")
+                want[first:, 2:, 11] = True
+                assert torch.equal(torch.isnan(out), want), (n, B, ws is None)
+
+
+def test_two_streams_with_workspaces_of_their_own():
+    """Calls that overlap in time: each has its workspace, and both give what they
+    give alone."""
+    import torch
+    import aila_amd as A
+    D, Hq, Hkv, page, lens, new = 128, 8, 2, 16, [9000, 500, 40], [300, 1, 40]
+    P = sum(-(-n // page) for n in lens) + 3
+    cache, table = _cache(P, Hkv, page, D, 1), _table(lens, page, P, 2)
+    max_len, T = table.shape[1] * page, sum(new)
+    starts, seq = _i32([0] + [int(x) for x in np.cumsum(new)]), _i32(lens)
+    q = torch.randn((T, Hq, D), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(torch.bfloat16)
+    sizes = (A.gqa_prefill_paged_fp8_workspace_size(T, 3, Hq, Hkv, D, max_len), A.gqa_decode_paged_fp8_workspace_size(3, Hq, Hkv, D, max_len))
+
+    def both(stream, wp, wd):
+        a = A.gqa_prefill_paged_fp8(q, *cache, table, starts, seq, max_len, workspace=wp, stream=stream)
+        return a, A.gqa_decode_paged_fp8(q[:3], *cache, table, seq, max_len, workspace=wd, stream=stream)
+
+    ws = [[torch.empty(n, dtype=torch.uint8, device="cuda") for n in sizes] for _ in range(2)]
+    want = both(None, *ws[0])
+    st = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in st:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [both(s, *w) for _ in range(4) for s, w in zip(st, ws)]
+    for s in st:
+        s.synchronize()
+    for a, d in got:
+        assert torch.equal(a, want[0]) and torch.equal(d, want[1])
+
+
+def test_graphs_that_share_a_workspace():
+    """Two captured calls of other shapes over one workspace, replayed in turn on a
+    stream, with eager calls between."""
+    import torch
+    import aila_amd as A
+    D, Hq, Hkv, page, lens, new = 128, 8, 2, 16, [9000, 500, 40], [300, 1, 40]
+    P = sum(-(-n // page) for n in lens) + 3
+    cache, table = _cache(P, Hkv, page, D, 1), _table(lens, page, P, 2)
+    max_len, T = table.shape[1] * page, sum(new)
+    starts, seq = _i32([0] + [int(x) for x in np.cumsum(new)]), _i32(lens)
+    q = torch.randn((T, Hq, D), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(torch.bfloat16)
+    size = max(A.gqa_prefill_paged_fp8_workspace_size(T, 3, Hq, Hkv, D, max_len), A.gqa_decode_paged_fp8_workspace_size(3, Hq, Hkv, D, max_len))
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    qd = q[:3].contiguous()
+    outs = torch.zeros_like(q), torch.zeros_like(qd)
+    calls = (lambda o: A.gqa_prefill_paged_fp8(q, *cache, table, starts, seq, max_len, out=o, workspace=ws),
+             lambda o: A.gqa_decode_paged_fp8(qd, *cache, table, seq, max_len, out=o, workspace=ws))
+    want = [f(torch.zeros_like(o)).clone() for f, o in zip(calls, outs)]
+    graphs = []
+    for f, o in zip(calls, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            f(o)
+        graphs.append(g)
+    for n in range(3):
+        for g, f, o, w in zip(graphs, calls, outs, want):
+            o.zero_()
+            g.replay()
+            eager = f(torch.zeros_like(o))
+            torch.cuda.synchronize()
+            assert torch.equal(o, w) and torch.equal(eager, w), n
+
+
 # ------------------------------------------------------------- used together --
 class _Server:
     """The step of a serving loop: lengths -> tables and slots -> rows -> attention."""

@@ -61,7 +61,17 @@ def test_workspace_sizes():
     assert f(1, 16, 8, 128, 612) == 256 + 8 * 5 * 2 * 2 * 132 * 4  # a record pair for each 128 rows of each KV head, and the counts
     assert f(64, 40, 8, 128, 4000) == f(64, 40, 8, 128, 32768)     # as many as the device holds
     assert f(0, 16, 8, 128, 612) == f(1, 16, 0, 128, 612) == f(1, 15, 8, 128, 612) == f(1, 16, 8, 128, -1) == 0
-    assert aila_amd.gqa_prefill_paged_fp8_workspace_size(0, 1, 16, 8, 128, 100) == 0
+    f = aila_amd.gqa_prefill_paged_fp8_workspace_size
+    assert f(0, 1, 16, 8, 128, 100) == f(9, 1, 16, 8, 96, 100) == f(9, 0, 16, 8, 128, 100) == f(9, 1, 16, 8, 128, -1) == 0
+    assert f(5000, 1, 16, 8, 128, 9000) == 0                       # tiles enough: no runs
+    assert f(128, 1, 16, 8, 128, 9000) == 2 * 16 * 8 * 128 * 130 * 4    # 2 tiles a head, 16 runs each
+    assert f(9, 2, 16, 8, 128, 9000) > 2 * 32 * 8 * 128 * 130 * 4  # a list, and the runs of 32 workgroups a head
+
+
+def test_a_batch_needs_its_whole_workspace():
+    need = aila_amd.gqa_prefill_paged_fp8_workspace_size(9, 2, 4, 2, 128, 300)
+    rc, msg = _rc("gqa_prefill_paged_fp8", PREFILL, ws_bytes=need - 1)
+    assert rc == -4 and str(need) in msg
 
 
 # ---- the binding's own checks, with stand-ins for device tensors -----------------------------
