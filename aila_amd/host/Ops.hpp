@@ -50,6 +50,41 @@ void attention_decode_paged(Context& ctx, Tensor& q, Tensor& k_pages, Tensor& v_
                             Tensor& seq_lens, Tensor& output, int num_heads, int num_kv_heads, int head_dim,
                             int max_len, Tensor* exact_partials_buf = nullptr);
 
+// The paged cache in 8 bits (additions; see aila_hip.h for what each does):
+// k_pages/v_pages [num_pages, Hkv, page_size, D] u8 (e4m3 codes), k_scale/v_scale
+// [num_pages, Hkv, page_size / 16] f32. Lengths, tables, starts and slots are s32
+// tensors on the device; a serving step is reserve, then per layer copy_to_cache
+// and attention, and release when a request has ended.
+//
+// Pages and slots of the requests' new tokens: cached_lens/new_lens/seq_lens
+// [B], block_table [B, max_pages], free_pages [num_pages], free_count [1],
+// query_start [B + 1], slots [max_tokens].
+void kv_pages_reserve(Context& ctx, Tensor& cached_lens, Tensor& new_lens, Tensor& block_table, Tensor& free_pages,
+                      Tensor& free_count, int page_size, Tensor& slots, Tensor& query_start, Tensor& seq_lens);
+
+// Gives the pages of the rows b with ended[b] != 0 back.
+void kv_pages_release(Context& ctx, Tensor& ended, Tensor& block_table, Tensor& free_pages, Tensor& free_count);
+
+// copy_to_cache for both of new_k/new_v [T, Hkv*D] bf16, quantised, by slots [T].
+void copy_to_cache_paged_fp8(Context& ctx, Tensor& new_k, Tensor& new_v, Tensor& k_pages, Tensor& v_pages,
+                             Tensor& k_scale, Tensor& v_scale, Tensor& slots);
+
+// The rows of slots [T] as the bf16 values they stand for, k_out/v_out [T, Hkv*D].
+void read_cache_paged_fp8(Context& ctx, Tensor& k_pages, Tensor& v_pages, Tensor& k_scale, Tensor& v_scale,
+                          Tensor& slots, Tensor& k_out, Tensor& v_out);
+
+// attention_decode_paged over the 8-bit pages; workspace: any dtype, at least
+// two records (aila_hip_gqa_decode_paged_fp8_workspace_size), or null.
+void attention_decode_paged_fp8(Context& ctx, Tensor& q, Tensor& k_pages, Tensor& v_pages, Tensor& k_scale,
+                                Tensor& v_scale, Tensor& block_table, Tensor& seq_lens, Tensor& output, int num_heads,
+                                int max_len, Tensor* workspace = nullptr);
+
+// attention_prefill_cached over the 8-bit pages for a ragged batch: q/output
+// [T, Hq*D], request b's tokens [query_start[b], query_start[b + 1]).
+void attention_prefill_paged_fp8(Context& ctx, Tensor& q, Tensor& k_pages, Tensor& v_pages, Tensor& k_scale,
+                                 Tensor& v_scale, Tensor& block_table, Tensor& query_start, Tensor& seq_lens,
+                                 Tensor& output, int num_heads, int max_len, Tensor* workspace = nullptr);
+
 // Causal prefill over the current chunk (Ops.hpp:271-282). q [S, Hq*D],
 // k/v [S, Hkv*D]; output [S, Hq*D]. scores_buf is accepted and unused (no
 // [H, S, S] score matrix is materialised).

@@ -112,6 +112,139 @@ void attention_decode_paged(Context& ctx, Tensor& q, Tensor& k_pages, Tensor& v_
         "attention_decode_paged");
 }
 
+namespace {
+
+const int* s32(const Tensor& t, const char* name, int64_t least) {
+  need_dtype(t, DType::s32, name);
+  if (t.numel() < least) throw std::runtime_error(std::string(name) + ": too few elements");
+  return static_cast<const int*>(t.data());
+}
+
+// An 8-bit paged cache's sizes, checked against each other.
+struct PagesFp8 {
+  int num_pages, Hkv, page_size, D;
+  const float *k_scale, *v_scale;
+};
+PagesFp8 pages_fp8(const Tensor& k_pages, const Tensor& v_pages, const Tensor& k_scale, const Tensor& v_scale,
+                   const char* what) {
+  need_dtype(k_pages, DType::u8, what);
+  need_dtype(v_pages, DType::u8, what);
+  need_dtype(k_scale, DType::f32, what);
+  need_dtype(v_scale, DType::f32, what);
+  if (k_pages.ndim() != 4 || v_pages.shape() != k_pages.shape())
+    throw std::runtime_error(std::string(what) + ": k_pages and v_pages must be [num_pages, Hkv, page_size, D]");
+  const PagesFp8 p{static_cast<int>(k_pages.shape(0)), static_cast<int>(k_pages.shape(1)), static_cast<int>(k_pages.shape(2)),
+                   static_cast<int>(k_pages.shape(3)), static_cast<const float*>(k_scale.data()),
+                   static_cast<const float*>(v_scale.data())};
+  const std::vector<int64_t> want = {p.num_pages, p.Hkv, p.page_size / 16};
+  if (k_scale.shape() != want || v_scale.shape() != want)
+    throw std::runtime_error(std::string(what) + ": k_scale and v_scale must be [num_pages, Hkv, page_size / 16]");
+  return p;
+}
+
+// Tokens of a [T, width] bf16 tensor.
+int rows_of(const Tensor& t, int64_t width, const char* name) {
+  need_dtype(t, DType::bf16, name);
+  if (t.ndim() < 1 || t.numel() != t.shape(0) * width) throw std::runtime_error(std::string(name) + ": wrong row size");
+  return static_cast<int>(t.shape(0));
+}
+
+}  // namespace
+
+void kv_pages_reserve(Context& ctx, Tensor& cached_lens, Tensor& new_lens, Tensor& block_table, Tensor& free_pages,
+                      Tensor& free_count, int page_size, Tensor& slots, Tensor& query_start, Tensor& seq_lens) {
+  need_dtype(block_table, DType::s32, "kv_pages_reserve block_table");
+  if (block_table.ndim() != 2) throw std::runtime_error("kv_pages_reserve block_table: must be [B, max_pages]");
+  const int B = static_cast<int>(block_table.shape(0));
+  const int* cached = s32(cached_lens, "kv_pages_reserve cached_lens", B);
+  const int* fresh = s32(new_lens, "kv_pages_reserve new_lens", B);
+  const int* pool = s32(free_pages, "kv_pages_reserve free_pages", 1);
+  s32(free_count, "kv_pages_reserve free_count", 1);
+  s32(slots, "kv_pages_reserve slots", 1);
+  s32(query_start, "kv_pages_reserve query_start", B + 1);
+  s32(seq_lens, "kv_pages_reserve seq_lens", B);
+  check(aila_hip_kv_pages_reserve(cached, fresh, block_table.data_as<int>(), pool, free_count.data_as<int>(),
+                                  query_start.data_as<int>(), seq_lens.data_as<int>(), slots.data_as<int>(), B,
+                                  static_cast<int>(block_table.shape(1)), page_size, static_cast<int>(free_pages.numel()),
+                                  static_cast<int>(slots.numel()), ctx.stream()),
+        "kv_pages_reserve");
+}
+
+void kv_pages_release(Context& ctx, Tensor& ended, Tensor& block_table, Tensor& free_pages, Tensor& free_count) {
+  need_dtype(block_table, DType::s32, "kv_pages_release block_table");
+  if (block_table.ndim() != 2) throw std::runtime_error("kv_pages_release block_table: must be [B, max_pages]");
+  const int B = static_cast<int>(block_table.shape(0));
+  const int* flags = s32(ended, "kv_pages_release ended", B);
+  s32(free_pages, "kv_pages_release free_pages", 1);
+  s32(free_count, "kv_pages_release free_count", 1);
+  check(aila_hip_kv_pages_release(flags, block_table.data_as<int>(), free_pages.data_as<int>(), free_count.data_as<int>(), B,
+                                  static_cast<int>(block_table.shape(1)), static_cast<int>(free_pages.numel()), ctx.stream()),
+        "kv_pages_release");
+}
+
+void copy_to_cache_paged_fp8(Context& ctx, Tensor& new_k, Tensor& new_v, Tensor& k_pages, Tensor& v_pages,
+                             Tensor& k_scale, Tensor& v_scale, Tensor& slots) {
+  const PagesFp8 p = pages_fp8(k_pages, v_pages, k_scale, v_scale, "copy_to_cache_paged_fp8");
+  const int T = rows_of(new_k, int64_t{p.Hkv} * p.D, "copy_to_cache_paged_fp8 new_k");
+  if (rows_of(new_v, int64_t{p.Hkv} * p.D, "copy_to_cache_paged_fp8 new_v") != T)
+    throw std::runtime_error("copy_to_cache_paged_fp8: new_k and new_v differ in rows");
+  check(aila_hip_kv_append_paged_fp8(new_k.data(), new_v.data(), static_cast<long>(p.Hkv) * p.D, k_pages.data(), v_pages.data(),
+                                     k_scale.data_as<float>(), v_scale.data_as<float>(),
+                                     s32(slots, "copy_to_cache_paged_fp8 slots", T), T, p.Hkv, p.D, p.page_size, p.num_pages,
+                                     ctx.stream()),
+        "copy_to_cache_paged_fp8");
+}
+
+void read_cache_paged_fp8(Context& ctx, Tensor& k_pages, Tensor& v_pages, Tensor& k_scale, Tensor& v_scale,
+                          Tensor& slots, Tensor& k_out, Tensor& v_out) {
+  const PagesFp8 p = pages_fp8(k_pages, v_pages, k_scale, v_scale, "read_cache_paged_fp8");
+  const int T = rows_of(k_out, int64_t{p.Hkv} * p.D, "read_cache_paged_fp8 k_out");
+  if (rows_of(v_out, int64_t{p.Hkv} * p.D, "read_cache_paged_fp8 v_out") != T)
+    throw std::runtime_error("read_cache_paged_fp8: k_out and v_out differ in rows");
+  check(aila_hip_kv_read_paged_fp8(k_pages.data(), v_pages.data(), p.k_scale, p.v_scale, s32(slots, "read_cache_paged_fp8 slots", T),
+                                   k_out.data(), v_out.data(), T, p.Hkv, p.D, p.page_size, p.num_pages, ctx.stream()),
+        "read_cache_paged_fp8");
+}
+
+void attention_decode_paged_fp8(Context& ctx, Tensor& q, Tensor& k_pages, Tensor& v_pages, Tensor& k_scale,
+                                Tensor& v_scale, Tensor& block_table, Tensor& seq_lens, Tensor& output, int num_heads,
+                                int max_len, Tensor* workspace) {
+  const PagesFp8 p = pages_fp8(k_pages, v_pages, k_scale, v_scale, "attention_decode_paged_fp8");
+  const int B = rows_of(q, int64_t{num_heads} * p.D, "attention_decode_paged_fp8 q");
+  if (rows_of(output, int64_t{num_heads} * p.D, "attention_decode_paged_fp8 output") != B)
+    throw std::runtime_error("attention_decode_paged_fp8: q and output differ in rows");
+  need_dtype(block_table, DType::s32, "attention_decode_paged_fp8 block_table");
+  if (block_table.ndim() != 2 || block_table.shape(0) != B)
+    throw std::runtime_error("attention_decode_paged_fp8 block_table: must be [B, max_pages]");
+  const bool ws = workspace && workspace->valid();
+  check(aila_hip_gqa_decode_paged_fp8(q.data(), static_cast<long>(num_heads) * p.D, k_pages.data(), v_pages.data(), p.k_scale,
+                                      p.v_scale, output.data(), ws ? workspace->data() : nullptr,
+                                      ws ? workspace->size_bytes() : 0, B, num_heads, p.Hkv, p.D, p.page_size, p.num_pages,
+                                      block_table.data_as<int>(), static_cast<int>(block_table.shape(1)), max_len,
+                                      s32(seq_lens, "attention_decode_paged_fp8 seq_lens", B), ctx.stream()),
+        "attention_decode_paged_fp8");
+}
+
+void attention_prefill_paged_fp8(Context& ctx, Tensor& q, Tensor& k_pages, Tensor& v_pages, Tensor& k_scale,
+                                 Tensor& v_scale, Tensor& block_table, Tensor& query_start, Tensor& seq_lens,
+                                 Tensor& output, int num_heads, int max_len, Tensor* workspace) {
+  const PagesFp8 p = pages_fp8(k_pages, v_pages, k_scale, v_scale, "attention_prefill_paged_fp8");
+  const int T = rows_of(q, int64_t{num_heads} * p.D, "attention_prefill_paged_fp8 q");
+  if (rows_of(output, int64_t{num_heads} * p.D, "attention_prefill_paged_fp8 output") != T)
+    throw std::runtime_error("attention_prefill_paged_fp8: q and output differ in rows");
+  need_dtype(block_table, DType::s32, "attention_prefill_paged_fp8 block_table");
+  if (block_table.ndim() != 2) throw std::runtime_error("attention_prefill_paged_fp8 block_table: must be [B, max_pages]");
+  const int B = static_cast<int>(block_table.shape(0));
+  const bool ws = workspace && workspace->valid();
+  check(aila_hip_gqa_prefill_paged_fp8(q.data(), static_cast<long>(num_heads) * p.D, k_pages.data(), v_pages.data(), p.k_scale,
+                                       p.v_scale, output.data(), ws ? workspace->data() : nullptr,
+                                       ws ? workspace->size_bytes() : 0, T, B, num_heads, p.Hkv, p.D, p.page_size, p.num_pages,
+                                       block_table.data_as<int>(), static_cast<int>(block_table.shape(1)), max_len,
+                                       s32(query_start, "attention_prefill_paged_fp8 query_start", B + 1),
+                                       s32(seq_lens, "attention_prefill_paged_fp8 seq_lens", B), ctx.stream()),
+        "attention_prefill_paged_fp8");
+}
+
 void attention_prefill(Context& ctx, Tensor& q, Tensor& k, Tensor& v, Tensor& output,
                        Tensor& scores_buf, int seq_len, int num_heads, int num_kv_heads,
                        int head_dim) {

@@ -375,7 +375,9 @@ int aila_hip_kv_read_paged_fp8(const void* k_pages, const void* v_pages,
  * KV head), B <= 4096. Softmax scale 1/sqrt(D).
  * The work is shared evenly by the workgroups whatever the lengths are;
  * workspace_size bytes let as many work as the device holds, a smaller
- * workspace fewer, and NULL one per sequence and KV head (no split). */
+ * workspace fewer (2 records at least, else AILA_HIP_EWORKSPACE), and NULL one
+ * per sequence and KV head (no split). Calls that may overlap in time (other
+ * streams, graphs replayed side by side) need workspaces of their own. */
 size_t aila_hip_gqa_decode_paged_fp8_workspace_size(int B, int Hq, int Hkv,
                                                     int D, int max_len);
 int aila_hip_gqa_decode_paged_fp8(const void* q, long q_stride,
@@ -399,7 +401,11 @@ int aila_hip_gqa_decode_paged_fp8(const void* q, long q_stride,
  *            max_len); none: 0. Tokens from query_start[B] on are not touched.
  * Other arguments as aila_hip_gqa_decode_paged_fp8. T is the number of rows of
  * q and out; query_start must not decrease nor pass T (what passes it is not
- * computed). */
+ * computed).
+ * The workspace holds the list of a batch's work (B > 1) and the records of
+ * tiles whose keys are split. B > 1: workspace_size bytes, less is
+ * AILA_HIP_EWORKSPACE; NULL runs one request after the other, unsplit. B = 1:
+ * less than workspace_size (0 where nothing is split), or NULL, runs unsplit. */
 size_t aila_hip_gqa_prefill_paged_fp8_workspace_size(int T, int B, int Hq,
                                                      int Hkv, int D,
                                                      int max_len);

@@ -1,6 +1,9 @@
 """GPU parity of the 8-bit paged KV cache (kv_pages_*, kv_*_paged_fp8,
 gqa_*_paged_fp8) against plain forms in 64 bits: tables, codes and scales bit for
 bit, attention within a bound derived from its roundings."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -696,3 +699,12 @@ def test_offsets_beyond_32_bits():
     got = A.gqa_prefill_paged_fp8(q, *cache, table, _i32([0, L, 2 * L]), _i32([L, L]), L)
     assert torch.equal(got, A.gqa_prefill_paged_fp8(q, *small, there, _i32([0, L, 2 * L]), _i32([L, L]), L))
     _check(got[rows], q[rows], tuple(small), there, range(3), [L, L], L, 2.0 ** -8)
+
+
+def test_cpp_ops():
+    """The C++ forms (tests/cpp/test_paged_fp8.cpp)."""
+    exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "test_paged_fp8")
+    assert os.path.exists(exe), "build first: python -c 'import __graft_entry__ as g; g.build()'"
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=100)
+    print(r.stdout)
+    assert r.returncode == 0 and "ALL OK" in r.stdout, r.stdout + r.stderr
