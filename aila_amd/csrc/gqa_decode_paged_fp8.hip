@@ -6,7 +6,12 @@
 // of a KV head (up to 16: the columns of the matrix instructions), so each code
 // is read from HBM once. Codes go from memory to registers, are converted to
 // bf16 there (exact) and feed the matrix cores; nothing passes through LDS but
-// the waves' results. Bound by the bytes of K and V.
+// the waves' results. Bound by the bytes of K and V: 8 ragged sequences of up to
+// 32768 rows (4 KV heads, D = 256) 68 us = 6.1 TB/s and 4.6 us of merge, 64 of up
+// to 4001 (8 KV heads of 5 query heads, D = 128) 76 us = 5.3 TB/s; a large copy
+// reaches 4.7, a pure read 7.1. One sequence of 32768 rows is 17 us (4.0 TB/s):
+// a workgroup's share is 4 units there, and start-up and the end of the waves are
+// half of it.
 //
 // Split: the rows of all sequences and KV heads form one line, in units of 128
 // rows (a strip of 32 for each of the 4 waves), and every workgroup takes an
@@ -82,7 +87,10 @@ __device__ __forceinline__ int share_begin(int w, int units, int groups) {
 
 template <int D>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void gqa_decode_paged_fp8_kernel(PagedFp8 c, Fp8DecodeArgs a) {
-  constexpr int kDepth = 3;    // strips of a wave in registers
+  // Strips of a wave in registers: one is worked on while the next arrives. (Three:
+  // 8 sequences of 32768, D = 256, 57.2 us in a graph against 55.2, 8 of 8000, 32/8,
+  // D = 128, 24.7 against 23.4. Two workgroups a CU at D = 256 instead spill: 85.)
+  constexpr int kDepth = 2;
   extern __shared__ __attribute__((aligned(16))) unsigned char s_dyn[];
   float* s_acc = reinterpret_cast<float*>(s_dyn);             // [kWaves][tile][D]
   float* s_ml = s_acc + kWaves * a.tile * D;                  // [kWaves][tile][2]
@@ -327,7 +335,9 @@ int launch(const PagedFp8& c, const Fp8DecodeArgs& a, int groups, hipStream_t st
                      (a.part ? static_cast<size_t>(a.B + 1) * sizeof(int) : 0);
   hipLaunchKernelGGL((gqa_decode_paged_fp8_kernel<D>), dim3(groups), dim3(kThreads), lds, st, c, a);
   const int heads = c.Hkv * a.chunks;
-  if (a.part && a.B * heads >= 64)
+  // us of decode and merge, the kernel for few records / the other: 64 (sequence,
+  // head)s 27.9 / 24.7, 128 36.1 / 35.0, 256 107.1 / 108.0
+  if (a.part && a.B * heads >= 256)
     hipLaunchKernelGGL((gqa_decode_paged_fp8_merge_few_kernel<D>), dim3(heads, a.B), dim3(256), 0, st, c, a, groups);
   else if (a.part)
     hipLaunchKernelGGL((gqa_decode_paged_fp8_merge_kernel<D>), dim3(a.Hq, a.B, D / 64), dim3(256), 0, st, c, a, groups);

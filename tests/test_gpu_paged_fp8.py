@@ -141,9 +141,9 @@ def test_append_rounds_every_bf16_value():
     assert torch.equal(v, -k)
 
 
-@pytest.mark.parametrize("T", [1, 2047, 2049, 5003])
+@pytest.mark.parametrize("T", [1, 256, 257, 1023, 1025, 2047, 2049, 5003])
 def test_append_of_a_long_prompt(T):
-    """Above and below the batch size where a workgroup takes 16 tokens."""
+    """Above and below the batch sizes where a workgroup takes more tokens."""
     import torch
     import aila_amd as A
     H, page, D = 3, 64, 64
@@ -153,6 +153,32 @@ def test_append_of_a_long_prompt(T):
     start = 37                       # the first run begins inside a block
     perm = np.random.default_rng(T).permutation(P)
     slots = [int(perm[(start + i) // page]) * page + (start + i) % page for i in range(T)]
+    k, v = (torch.randn((T, H, D), generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    want = [ref.Cache(kp, ks), ref.Cache(vp, vs)]
+    A.kv_append_paged_fp8(k, v, kp, vp, ks, vs, _i32(slots))
+    for c, t, pages, scale in zip(want, (k, v), (kp, vp), (ks, vs)):
+        c.append(t.double().cpu().numpy(), slots)
+        assert np.array_equal(pages.float().double().cpu().numpy(), c.val)
+        assert np.array_equal(scale.double().cpu().numpy(), c.scale)
+
+
+@pytest.mark.parametrize("T", [64, 300, 1500, 2500])
+def test_append_of_single_tokens_and_short_runs(T):
+    """Runs of one to five tokens, so that a workgroup's tile holds many and they
+    go on behind its end."""
+    import torch
+    import aila_amd as A
+    H, page, D = 2, 16, 128
+    g = torch.Generator(device="cuda").manual_seed(T)
+    kp, vp, ks, vs = _cache(T, H, page, D, T)
+    slots, p = [], 0
+    while len(slots) < T:
+        n = min(1 + p * 7 % 5, T - len(slots))
+        r = p * 5 % (page - n + 1)
+        slots += [p * page + r + i for i in range(n)]
+        if p % 11 == 3 and len(slots) < T:
+            slots.append(-1)
+        p += 1
     k, v = (torch.randn((T, H, D), generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
     want = [ref.Cache(kp, ks), ref.Cache(vp, vs)]
     A.kv_append_paged_fp8(k, v, kp, vp, ks, vs, _i32(slots))
