@@ -527,7 +527,8 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
   };
   Item it;
   bool more = get_item<D>(a, item_at(0), &it);
-  int seg_b = -1, seg_0 = 0, seg_1 = 0;     // the segment whose blocks are in LDS
+  int seg_b = -1, seg_0 = 0, seg_1 = 0;     // the segment whose blocks are in LDS: key tiles,
+  int seg_last = 0;                         // and the last block looked up (the tile may end in a later one)
   bool holes = false, primed = false;       // primed: its first DMAs are on the way
   for (int round = 1; more; ++round) {
     const int rows = it.n * a.group;
@@ -569,8 +570,8 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
     for (int s0 = it.t0; s0 < it.t1; s0 += C::SEG / C::NB - 8) {
       const int s1 = min(it.t1, s0 + C::SEG / C::NB - 8);
       const int count = (s1 - s0 + 1) / 2;         // tiles of a group, the last of group 1 perhaps none
-      const bool reuse = seg_b == it.b && seg_0 == s0 && s1 <= seg_1 && s1 == it.t1 && it.rec < 0;
       const int last = min(blk_end, s1 * C::NB), fill = (2 * count + 8) * C::NB;
+      const bool reuse = seg_b == it.b && seg_0 == s0 && s1 <= seg_1 && last <= seg_last && s1 == it.t1 && it.rec < 0;
       if (!reuse) {
         bool hole = false;
         for (int i = threadIdx.x; i < fill; i += kThreads) {
@@ -583,6 +584,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
         seg_b = it.b;
         seg_0 = s0;
         seg_1 = s1;
+        seg_last = last;
       }
 
       // ---- codes -> operands ----------------------------------------------
@@ -831,7 +833,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
     const Item done = it;
     more = get_item<D>(a, item_at(round), &it);
     if (more && it.b == seg_b && it.t0 == seg_0 && it.t0 < it.t1 && it.t1 <= seg_1 && it.rec < 0 &&
-        !(THIN && it.n * a.group - it.r0 <= kThinRows)) {
+        (tile_end(a, it) + kScaleRows - 1) / kScaleRows <= seg_last && !(THIN && it.n * a.group - it.r0 <= kThinRows)) {
       start();
       primed = true;
     }

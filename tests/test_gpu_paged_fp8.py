@@ -462,6 +462,33 @@ def test_prefill_of_many_requests(B, D, Hq, Hkv):
     assert ((one.double() - out[at].double()).abs() <= 2.0 ** -7 * one.double().abs() * (1 + 2.0 ** -7) + 2.0 ** -8 * 8).all()
 
 
+@pytest.mark.parametrize("D,Hq,Hkv,new,lens", [(64, 1024, 128, [100, 3], [333, 3]), (128, 768, 128, [90, 70], [517, 300]), (256, 512, 64, [60, 61, 2], [161, 460, 9])])
+def test_tiles_that_end_in_one_key_tile(D, Hq, Hkv, new, lens):
+    """One or two workgroups a KV head walk all tiles of a batch, many of which have
+    equally many key tiles but not the same last block, in any order; the requests
+    alone give the same bits."""
+    import torch
+    import aila_amd as A
+    page, B = 16, len(lens)
+    P = sum(-(-n // page) for n in lens) + 3
+    cache = _cache(P, Hkv, page, D, 7)
+    table = _table(lens, page, P, 8)
+    max_len = table.shape[1] * page
+    starts = [0] + [int(x) for x in np.cumsum(new)]
+    q = torch.randn((starts[-1], Hq, D), generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").to(torch.bfloat16)
+    ws = torch.empty(A.gqa_prefill_paged_fp8_workspace_size(starts[-1], B, Hq, Hkv, D, max_len), dtype=torch.uint8, device="cuda")
+    want = A.gqa_prefill_paged_fp8(q, *cache, table, _i32(starts), _i32(lens), max_len)
+    for _ in range(10):
+        got = A.gqa_prefill_paged_fp8(q, *cache, table, _i32(starts), _i32(lens), max_len, workspace=ws)
+        assert torch.equal(got, want)
+    few = [h for h in range(0, Hkv, Hkv // 4)]            # some heads against the definition
+    g = Hq // Hkv
+    heads = [h * g + i for h in few for i in range(g)]
+    small = [x[:, few].contiguous() if x.dtype == torch.float32 else x.view(torch.uint8)[:, few].contiguous().view(x.dtype) for x in cache]
+    _check_tokens(got[:, heads].contiguous(), q[:, heads].contiguous(), small, table, starts, lens, max_len,
+                  {b: (0, n // 3, n // 2, -1) for b, n in enumerate(new)})
+
+
 @pytest.mark.parametrize("B,D,Hq,Hkv,page,most,max_len", [(20, 128, 8, 4, 32, 6000, 8000), (70, 64, 16, 1, 16, 5000, 6000), (9, 256, 32, 8, 64, 3000, 5000),
                                                           (4096, 64, 2, 1, 16, 40, 48), (300, 128, 20, 1, 16, 500, 5000)])
 def test_decode_of_many_sequences(B, D, Hq, Hkv, page, most, max_len):
