@@ -31,7 +31,7 @@
 // 8191 tokens, 16 / 4 heads, D = 256: 505-530 us (1.04-1.09 PFLOP/s; a large bf16
 // product reaches 1.19 here); 2048 tokens, 32 / 8, D = 128: 47 us; 250 tokens after
 // 7900, D = 256: 48 us and 9 us of merge; 3 prompts of up to 600 tokens after 3000
-// rows beside 29 single tokens, 40 / 8, D = 128: 7 us of plan, 128 us and 4.6 us.
+// rows beside 29 single tokens, 40 / 8, D = 128: 5.4 us of plan, 128 us and 4.6 us.
 #include "paged_fp8.hpp"
 
 #include <algorithm>
@@ -209,11 +209,9 @@ __device__ __forceinline__ bool get_item(const Fp8PrefillArgs& a, int index, Ite
 // number of key tiles: a tile of query rows with more of them than that share
 // is cut into equal runs of at most a share, and the items are sorted by size,
 // so that the workgroups, which take them forth and back, fill up evenly.
-constexpr int kPlanThreads = 1024;
 constexpr int kMinRun = 8;      // key tiles; shorter runs cost more in records than they gain
-constexpr int kBuckets = 1024;
 
-template <typename T>
+template <int NT, typename T>
 __device__ __forceinline__ T plan_scan(T x, T* s_wave, T* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -226,7 +224,7 @@ __device__ __forceinline__ T plan_scan(T x, T* s_wave, T* total) {
   __syncthreads();
   T before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kPlanThreads / 64; ++w) {
+  for (int w = 0; w < NT / 64; ++w) {
     if (w < wave) before += s_wave[w];
     all += s_wave[w];
   }
@@ -234,13 +232,15 @@ __device__ __forceinline__ T plan_scan(T x, T* s_wave, T* total) {
   return x + before;   // inclusive
 }
 
-__global__ __launch_bounds__(kPlanThreads) void gqa_prefill_paged_fp8_plan_kernel(Fp8PrefillArgs a, int key_tile) {
+template <int NT>
+__global__ __launch_bounds__(NT) void gqa_prefill_paged_fp8_plan_kernel(Fp8PrefillArgs a, int key_tile) {
+  constexpr int kBuckets = NT;
   extern __shared__ int s_dyn_plan[];
   int* s_first = s_dyn_plan;          // [B + 1] first tile of each request
   int* s_n = s_first + a.B + 1;       // [B] tokens
   int* s_len = s_n + a.B;             // [B] rows
-  __shared__ int s_wave[kPlanThreads / 64];
-  __shared__ long s_wave_l[kPlanThreads / 64];
+  __shared__ int s_wave[NT / 64];
+  __shared__ long s_wave_l[NT / 64];
   __shared__ int s_bucket[kBuckets];
   const int tid = threadIdx.x;
   PlanItem* items = reinterpret_cast<PlanItem*>(a.plan + kPlanHead);
@@ -250,12 +250,12 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_prefill_paged_fp8_plan_kerne
   // malformed starts may overlap: no more tiles than the list holds
   const long most = plan_items(a.T, a.B, a.group, 0);
   long all_tiles = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
+  for (int b0 = 0; b0 < a.B; b0 += NT) {
     const int b = b0 + tid;
     Item it{};
     if (b < a.B) load_request(a, b, &it);
     long all;
-    const long incl = all_tiles + plan_scan<long>((it.n * a.group + kRows - 1) / kRows, s_wave_l, &all);
+    const long incl = all_tiles + plan_scan<NT, long>((it.n * a.group + kRows - 1) / kRows, s_wave_l, &all);
     if (b < a.B) {
       s_first[b + 1] = static_cast<int>(min(incl, most));
       s_n[b] = it.n;
@@ -288,12 +288,12 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_prefill_paged_fp8_plan_kerne
   };
   Tile mine{};      // the first round's, which is all there are as a rule
   if (tid < tiles) mine = tile(tid);
-  auto tile_at = [&](int f) __attribute__((always_inline)) { return f < kPlanThreads ? mine : tile(f); };
+  auto tile_at = [&](int f) __attribute__((always_inline)) { return f < NT ? mine : tile(f); };
   long sum = 0;
-  for (int f0 = 0; f0 < tiles; f0 += kPlanThreads) {
+  for (int f0 = 0; f0 < tiles; f0 += NT) {
     const int f = f0 + tid;
     long all;
-    plan_scan<long>(f < tiles ? tile_at(f).cost : 0, s_wave_l, &all);
+    plan_scan<NT, long>(f < tiles ? tile_at(f).cost : 0, s_wave_l, &all);
     sum += all;
   }
   // (no tile costs 2^28: T * group and max_len are at most 2^30)
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_prefill_paged_fp8_plan_kerne
   auto bucket = [&](const Tile& x, int cuts) __attribute__((always_inline)) {
     return kBuckets - 1 - static_cast<int>(static_cast<long>(x.cost / cuts) * (kBuckets - 1) / share);
   };
-  for (int f = tid; f < tiles; f += kPlanThreads) {
+  for (int f = tid; f < tiles; f += NT) {
     const Tile x = tile_at(f);
     const int cuts = cuts_for(x);
     atomicAdd(&s_bucket[bucket(x, cuts)], cuts);
@@ -314,13 +314,13 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_prefill_paged_fp8_plan_kerne
   __syncthreads();
   const int count = s_bucket[tid];
   int total;
-  const int incl = plan_scan<int>(count, s_wave, &total);
+  const int incl = plan_scan<NT, int>(count, s_wave, &total);
   s_bucket[tid] = incl - count;
   __syncthreads();
   // Which workgroup an item goes to depends on the order within a bucket, its
   // result does not: records are numbered by the tiles' order.
   int recs = 0, cut_tiles = 0;
-  for (int f0 = 0; f0 < tiles; f0 += kPlanThreads) {
+  for (int f0 = 0; f0 < tiles; f0 += NT) {
     const int f = f0 + tid;
     Tile x{};
     int cuts = 0;
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_prefill_paged_fp8_plan_kerne
     // both sums in one: fewer than 2^15 tiles are cut, into fewer than 2^16 runs
     const int cut = cuts > 1 ? cuts << 15 | 1 : 0;
     int all;
-    const int before = plan_scan<int>(cut, s_wave, &all) - cut;
+    const int before = plan_scan<NT, int>(cut, s_wave, &all) - cut;
     const int rec = recs + (before >> 15), slot = cut_tiles + (before & 0x7fff);
     recs += all >> 15;
     cut_tiles += all & 0x7fff;
@@ -1054,8 +1054,13 @@ int launch(PagedFp8 c, Fp8PrefillArgs a, void* workspace, size_t workspace_bytes
       return set_error(AILA_HIP_EWORKSPACE, "gqa_prefill_paged_fp8: a workspace of %zu bytes, %zu are needed", workspace_bytes, need);
     a.plan = static_cast<int*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan_bytes(a.T, a.B, a.group, a.lanes));
-    hipLaunchKernelGGL(gqa_prefill_paged_fp8_plan_kernel, dim3(1), dim3(kPlanThreads), static_cast<size_t>(3 * a.B + 1) * sizeof(int), st, a,
-                       Cfg<D>::BN);
+    auto plan = [&](auto kernel, int threads) {
+      hipLaunchKernelGGL(kernel, dim3(1), dim3(threads), static_cast<size_t>(3 * a.B + 1) * sizeof(int), st, a, Cfg<D>::BN);
+    };
+    // a thread a tile; few tiles: 4 waves, whose sums and barriers are shorter (us, a batch of
+    // 32 with 91 tiles: 5.4 against 7.1)
+    if (a.B <= 256 && plan_items(a.T, a.B, a.group, 0) <= 256) plan(gqa_prefill_paged_fp8_plan_kernel<256>, 256);
+    else plan(gqa_prefill_paged_fp8_plan_kernel<1024>, 1024);
     walk(c, a);
     merge(a.lanes);
   }

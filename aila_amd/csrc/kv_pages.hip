@@ -14,7 +14,7 @@
 // LDS and the cost is latency: the chain of lengths -> table entries -> slots,
 // three dependent round trips to memory (the free pages nearest the top of the
 // stack are fetched beside the lengths), and four sums over the workgroup.
-// 32 requests of 4096 rows and 245 new tokens: 7.5 us, of which a launch is 2;
+// 32 requests of 4096 rows and 245 new tokens: 6.3 us, of which a launch is 2;
 // 256 requests, 16-row pages, 9000 new tokens in a pool too small for them:
 // 11.7 us, and 2.9 us for a second launch that fills the slots. Release: 4.0 and
 // 5.8 us.
@@ -24,7 +24,7 @@ namespace aila {
 namespace {
 
 constexpr int kMaxRequests = 2048;   // their prefix sums live in LDS
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024;   // of a large batch
 constexpr int kPlanWaves = kPlanThreads / 64;
 // Slots that the planning workgroup fills itself; more are a second launch's (us,
 // 32 requests, itself / second launch: 1024 slots 7.9 / 9.0, 4096 10.5 / 9.1, 16384
@@ -32,8 +32,9 @@ constexpr int kPlanWaves = kPlanThreads / 64;
 constexpr int kSlotsInPlan = 2048;
 
 // Inclusive sum over the workgroup's threads; `total` gets the sum of all.
-template <typename T>
+template <int NT, typename T>
 __device__ __forceinline__ T block_scan(T x, T* s_wave, T* total) {
+  constexpr int kWaves = NT / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -44,13 +45,13 @@ __device__ __forceinline__ T block_scan(T x, T* s_wave, T* total) {
   if (lane == 63) s_wave[wave] = x;
   __syncthreads();
   // every wave adds up the waves' sums for itself, lane w those up to wave w
-  T y = lane < kPlanWaves ? s_wave[lane] : 0;
+  T y = lane < kWaves ? s_wave[lane] : 0;
 #pragma unroll
-  for (int off = 1; off < kPlanWaves; off <<= 1) {
+  for (int off = 1; off < kWaves; off <<= 1) {
     const T z = __shfl_up(y, off);
     if (lane >= off) y += z;
   }
-  *total = __shfl(y, kPlanWaves - 1);
+  *total = __shfl(y, kWaves - 1);
   const T before = __shfl(y, max(wave - 1, 0));
   return wave > 0 ? x + before : x;
 }
@@ -78,7 +79,8 @@ __device__ __forceinline__ Lens load_lens(const int* cached, const int* fresh, i
 // fetched before it is known how many are needed.
 constexpr int kFlatPages = 4096;
 
-__global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
+template <int NT>
+__global__ __launch_bounds__(NT) void kv_pages_reserve_kernel(
     const int* __restrict__ cached, const int* __restrict__ fresh, int* table, const int* __restrict__ free_pages,
     int* free_count, int* __restrict__ query_start, int* __restrict__ seq_lens, int* __restrict__ slots, int B,
     int max_pages, int page_size, int num_pages, int max_tokens, int fill_slots) {
@@ -89,10 +91,10 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
   int* s_last = s_first + B;            // [B] holes up to its end
   int* s_rows = s_last + B;             // [B] rows it holds
   int* s_ok = s_rows + B;               // [B] its rows fit the table; then: it is admitted
-  __shared__ long s_wl[kPlanWaves];
-  __shared__ int s_wi[kPlanWaves];
+  __shared__ long s_wl[NT / 64];
+  __shared__ int s_wi[NT / 64];
   __shared__ int s_taken;
-  __shared__ int s_top[kPlanThreads];   // the free pages nearest the top
+  __shared__ int s_top[NT];   // the free pages nearest the top
   __shared__ int s_page[kFlatPages];    // page of each entry of the flat list
   const int tid = threadIdx.x;
   const long max_rows = static_cast<long>(max_pages) * page_size;
@@ -102,15 +104,15 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
   // ---- tokens and table entries of each request ---------------------------
   long tok0 = 0;
   int flat0 = 0;
-  for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
+  for (int b0 = 0; b0 < B; b0 += NT) {
     const int b = b0 + tid;
     Lens l{0, 0, false};
     if (b < B) l = load_lens(cached, fresh, b, max_rows);
     const int np = l.fits ? static_cast<int>((static_cast<long>(l.c) + l.n + page_size - 1) / page_size) - l.c / page_size : 0;
     long all_tok;
     int all_np;
-    const long tok = tok0 + block_scan<long>(l.n, s_wl, &all_tok);
-    const int flat = flat0 + block_scan<int>(np, s_wi, &all_np);
+    const long tok = tok0 + block_scan<NT, long>(l.n, s_wl, &all_tok);
+    const int flat = flat0 + block_scan<NT, int>(np, s_wi, &all_np);
     if (b < B) {
       s_start[b + 1] = static_cast<int>(min(tok, 0x7fffffffL));
       s_flat[b + 1] = flat;
@@ -127,7 +129,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
   }
   __syncthreads();
   const int total = s_start[B];
-  for (int b = tid; b <= B; b += kPlanThreads) query_start[b] = s_start[b];
+  for (int b = tid; b <= B; b += NT) query_start[b] = s_start[b];
 
   // ---- holes among the entries, in order of request and page --------------
   auto entry_of = [&](int f, int* b) __attribute__((always_inline)) {
@@ -136,7 +138,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
   };
   const bool in_lds = flat0 <= kFlatPages;
   int holes0 = 0;
-  for (int f0 = 0; f0 < flat0; f0 += kPlanThreads) {
+  for (int f0 = 0; f0 < flat0; f0 += NT) {
     const int f = f0 + tid;
     int b = 0, page = 0;
     if (f < flat0) {
@@ -145,7 +147,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
     }
     const int hole = page < 0;
     int all;
-    const int incl = holes0 + block_scan<int>(hole, s_wi, &all);
+    const int incl = holes0 + block_scan<NT, int>(hole, s_wi, &all);
     if (f < flat0) {
       if (f == s_flat[b]) s_first[b] = incl - hole;
       if (f + 1 == s_flat[b + 1]) s_last[b] = incl;
@@ -157,7 +159,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
   // Admitted: its rows fit the table, its tokens the batch, its holes the pool.
   // Both sums only grow, so the admitted requests that take pages come first
   // among those that need any, and the k-th hole takes the k-th page from the top.
-  for (int b = tid; b < B; b += kPlanThreads) {
+  for (int b = tid; b < B; b += NT) {
     const int ok = s_ok[b] && s_start[b + 1] <= max_tokens && (s_last[b] == s_first[b] || s_last[b] <= have);
     s_ok[b] = ok;
     seq_lens[b] = ok ? s_rows[b] + (s_start[b + 1] - s_start[b]) : 0;
@@ -165,7 +167,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
   }
   __syncthreads();
   int carry = 0;
-  for (int f0 = 0; f0 < flat0; f0 += kPlanThreads) {
+  for (int f0 = 0; f0 < flat0; f0 += NT) {
     const int f = f0 + tid;
     int b = 0, hole = 0, *entry = nullptr;
     if (f < flat0) {
@@ -173,9 +175,9 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
       hole = (in_lds ? s_page[f] : *entry) < 0;
     }
     int all;
-    const int k = carry + block_scan<int>(hole, s_wi, &all) - 1;
+    const int k = carry + block_scan<NT, int>(hole, s_wi, &all) - 1;
     if (hole && s_ok[b]) {
-      const int page = k < kPlanThreads ? s_top[k] : free_pages[have - 1 - k];
+      const int page = k < NT ? s_top[k] : free_pages[have - 1 - k];
       *entry = page;
       if (in_lds) s_page[f] = page;
     }
@@ -186,7 +188,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_reserve_kernel(
 
   // ---- slots ---------------------------------------------------------------
   if (!fill_slots) return;
-  for (int t = tid; t < max_tokens; t += kPlanThreads) {
+  for (int t = tid; t < max_tokens; t += NT) {
     int slot = -1;
     if (t < total) {
       const int b = find_request(s_start, B, t);
@@ -247,7 +249,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_release_kernel(const in
     const int b = b0 + tid;
     const int flag = b < B && release[b] != 0;
     int all;
-    const int incl = rows + block_scan<int>(flag, s_wi, &all);
+    const int incl = rows + block_scan<kPlanThreads, int>(flag, s_wi, &all);
     if (flag) s_row[incl - 1] = b;
     rows += all;
   }
@@ -277,7 +279,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_release_kernel(const in
     const int k = k0 + tid;
     const int n = k < rows ? s_at[k + 1] : 0;
     int all;
-    const int incl = sum + block_scan<int>(n, s_wi, &all);
+    const int incl = sum + block_scan<kPlanThreads, int>(n, s_wi, &all);
     if (k < rows) s_at[k + 1] = incl;
     sum += all;
   }
@@ -328,9 +330,15 @@ extern "C" int aila_hip_kv_pages_reserve(const int* cached_lens, const int* new_
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool in_plan = max_tokens <= kSlotsInPlan;
   const size_t lds = static_cast<size_t>(6 * B + 2) * sizeof(int);
-  hipLaunchKernelGGL(kv_pages_reserve_kernel, dim3(1), dim3(kPlanThreads), lds, st, cached_lens, new_lens, block_table,
-                     free_pages, free_count, query_start, seq_lens, slots, B, max_pages, page_size, num_pages,
-                     max_tokens, in_plan ? 1 : 0);
+  auto plan = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(threads), lds, st, cached_lens, new_lens, block_table, free_pages, free_count,
+                       query_start, seq_lens, slots, B, max_pages, page_size, num_pages, max_tokens, in_plan ? 1 : 0);
+  };
+  // Few requests and slots: 4 waves, whose sums and barriers are shorter (us, 256 /
+  // 1024 threads: 32 requests, 32 slots 6.3 / 7.8, 512 6.9 / 7.8, 2048 10.6 / 8.8; 256
+  // requests, 512 slots 7.8 / 8.6, 1024 9.4 / 8.7; 512 of one 12.0 / 9.1).
+  if (B <= 256 && max_tokens <= 512) plan(kv_pages_reserve_kernel<256>, 256);
+  else plan(kv_pages_reserve_kernel<kPlanThreads>, kPlanThreads);
   if (!in_plan)
     hipLaunchKernelGGL(kv_pages_slots_kernel, dim3(B + 1, 4), dim3(256), 0, st, cached_lens, block_table, query_start,
                        seq_lens, slots, B, max_pages, page_size, num_pages, max_tokens);
