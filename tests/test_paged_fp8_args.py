@@ -40,7 +40,7 @@ PAGES = [dict(H=0), dict(H=-1), dict(page=0), dict(page=24), dict(page=-16), dic
                                                   dict(mp=1 << 21, B=1024))]
     + [("kv_append_paged_fp8", APPEND, b) for b in (*PAGES, dict(k=None), dict(v=None), dict(slots=None), dict(T=0), dict(stride=255), dict(stride=248),
                                                     dict(stride=260), dict(k=P16 + 8), dict(v=P16 + 2))]
-    + [("kv_read_paged_fp8", READ, b) for b in (*PAGES, dict(slots=None), dict(ko=None), dict(vo=None), dict(T=0), dict(ko=P16 + 8), dict(vo=P16 + 8))]
+    + [("kv_read_paged_fp8", READ, b) for b in (*PAGES, dict(slots=None), dict(ko=None), dict(vo=None), dict(T=0), dict(T=1 << 30), dict(ko=P16 + 8), dict(vo=P16 + 8))]
     + [("gqa_decode_paged_fp8", DECODE, b) for b in (
         *PAGES, dict(q=None), dict(out=None), dict(table=None), dict(lens=None), dict(B=0), dict(B=4097), dict(Hq=0), dict(Hq=5), dict(stride=504),
         dict(stride=516), dict(q=P16 + 8), dict(out=P16 + 8), dict(mp=0), dict(mp=1 << 27), dict(max_len=-1), dict(max_len=321), dict(ws=P16 + 8),
