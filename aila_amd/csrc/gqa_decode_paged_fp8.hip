@@ -399,14 +399,17 @@ extern "C" int aila_hip_gqa_decode_paged_fp8(const void* q, long q_stride, const
                "gqa_decode_paged_fp8: B=%d sequences of up to %d rows and %d heads are too many", B, max_len, heads);
   long groups = static_cast<long>(B) * heads;
   // One workgroup per (sequence, head) where that is faster than a split and its
-  // merge (us, whole / split): up to 6 units a sequence (D = 64: 8, D = 256: 4;
-  // one sequence, 16/8 heads, D = 128: 612 rows 7.7 / 9.2, 900 9.6 / 8.9; D = 256:
-  // 450 11.3 / 11.4, 612 12.3 / 11.5; D = 64: 900 7.4 / 8.1, 1300 8.9 / 8.1), and
-  // where they fill the CUs, up to 4096 rows (D = 256: 2048): lengths between 5 and
-  // 100% of the bound, 64 sequences, D = 128: 2000 rows 37.8 / 47.1, 4000 68.9 /
-  // 68.1, 16000 260 / 198; D = 256: 2000 39.1 / 52.1, 4000 70.9 / 67.8.
-  const int few = (D == 64 ? 8 : D == 128 ? 6 : 4) * kUnit, many = D == 256 ? 2048 : 4096;
-  const bool whole = max_len <= few || (groups >= 256 && max_len <= many);
+  // merge: up to 6 units a sequence (D = 64: 8, D = 256: 4), and the longer the more
+  // of the CUs they fill, up to 4096 rows (D = 256: 2048) where they fill all. us in
+  // a graph, whole / split, lengths between 5 and 100% of the bound. D = 128, 8 heads:
+  // 1 sequence of 768 rows 7.9 / 8.7, 900 9.2 / 8.7; 8 of 1024 11.2 / 11.4, 1300 13.7 /
+  // 11.8; 16 of 1024 11.6 / 16.0, 2000 19.0 / 18.8, 3000 25.8 / 20.4; 64 of 2000 30.2 /
+  // 41.2, 4000 57.2 / 56.7, 8000 108 / 101. D = 64, 8 heads: 1 of 1024 7.4 / 7.7, 1300
+  // 9.0 / 7.8; 16 of 2000 12.4 / 13.8, 3000 16.6 / 14.8; 64 of 4000 29.9 / 35.3. D = 256,
+  // 4 heads: 1 of 512 10.9 / 11.1, 612 13.0 / 11.2; 32 of 1024 19.6 / 26.6, 2000 32.8 /
+  // 32.6; 64 of 2000 35.4 / 44.0, 4000 65.7 / 61.7.
+  const long few = (D == 64 ? 8 : D == 128 ? 6 : 4) * kUnit, many = D == 256 ? 2048 : 4096;
+  const bool whole = max_len <= std::max(few, many * std::min(groups, 256L) / 256);
   if (workspace != nullptr) {
     AILA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "gqa_decode_paged_fp8: workspace must be 16-byte aligned");
     const size_t rec = record_bytes(a.tile, D);
