@@ -35,6 +35,7 @@
 #include "paged_fp8.hpp"
 
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 namespace aila {
@@ -209,7 +210,10 @@ __device__ __forceinline__ bool get_item(const Fp8PrefillArgs& a, int index, Ite
 // number of key tiles: a tile of query rows with more of them than that share
 // is cut into equal runs of at most a share, and the items are sorted by size,
 // so that the workgroups, which take them forth and back, fill up evenly.
-constexpr int kMinRun = 8;      // key tiles; shorter runs cost more in records than they gain
+// Shorter runs cost more in records than they gain: key tiles in a batch, keys of one
+// request (us, D = 128, 32 / 8: 8 requests of 32 tokens and up to 1200 rows, 4 tiles
+// 35.3, 8 31.4; one of 32 after 1200, 256 keys 16.6, 512 19.4; of 5000, 22.3 and 22.5).
+constexpr int kMinRun = 8, kMinKeys = 256;
 
 template <int NT, typename T>
 __device__ __forceinline__ T plan_scan(T x, T* s_wave, T* total) {
@@ -242,6 +246,7 @@ __global__ __launch_bounds__(NT) void gqa_prefill_paged_fp8_plan_kernel(Fp8Prefi
   __shared__ int s_wave[NT / 64];
   __shared__ long s_wave_l[NT / 64];
   __shared__ int s_bucket[kBuckets];
+  __shared__ int s_share[16], s_runs[16], s_cost[kCus];
   const int tid = threadIdx.x;
   PlanItem* items = reinterpret_cast<PlanItem*>(a.plan + kPlanHead);
   PlanCut* cuts_of = reinterpret_cast<PlanCut*>(items + plan_items(a.T, a.B, a.group, a.lanes));
@@ -296,8 +301,36 @@ __global__ __launch_bounds__(NT) void gqa_prefill_paged_fp8_plan_kernel(Fp8Prefi
     plan_scan<NT, long>(f < tiles ? tile_at(f).cost : 0, s_wave_l, &all);
     sum += all;
   }
-  // (no tile costs 2^28: T * group and max_len are at most 2^30)
-  const int share = static_cast<int>(min(max(4L * kMinRun, (sum + a.lanes - 1) / a.lanes), 1L << 28));
+  // The share: an equal part of the whole, but where all tiles can run at once, the
+  // smallest of some that leaves no more runs than workgroups (a run too many would
+  // wait for another to end: 8 requests of 32 tokens and up to 5000 rows, 16 / 4, D =
+  // 256: 85 -> 57 us). The last always does: a run a tile, and sum / share more.
+  // (No tile costs 2^28: T * group and max_len are at most 2^30.)
+  constexpr int kShares = 9;
+  if (tid < kShares) {
+    const long even = max(4L * kMinRun, (sum + a.lanes - 1) / a.lanes);
+    const long x = tid < kShares - 1 ? even + even * tid / 8 : max(even, sum / max(1, a.lanes - tiles) + 1);
+    s_share[tid] = static_cast<int>(min(x, 1L << 28));
+  }
+  const bool one_round = tiles <= a.lanes;      // fewer than the threads
+  if (one_round && tid < tiles) s_cost[tid] = mine.cost;
+  __syncthreads();
+  int share = s_share[0];
+  if (one_round) {
+    for (int k = tid >> 6; k < kShares; k += NT / 64) {
+      int runs = 0;
+      for (int f = tid & 63; f < tiles; f += 64) runs += max(1, (s_cost[f] + s_share[k] - 1) / s_share[k]);
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) runs += __shfl_xor(runs, off);
+      if ((tid & 63) == 0) s_runs[k] = runs;
+    }
+    __syncthreads();
+    int pick = INT_MAX;
+#pragma unroll
+    for (int k = 0; k < kShares; ++k)
+      if (s_runs[k] <= a.lanes) pick = min(pick, s_share[k]);
+    if (pick != INT_MAX) share = pick;
+  }
   auto cuts_for = [&](const Tile& x) __attribute__((always_inline)) { return max(1, (x.cost + share - 1) / share); };
   // run i of a tile's key tiles, large runs' buckets first
   auto run_begin = [&](const Tile& x, int cuts, int i) __attribute__((always_inline)) {
@@ -906,6 +939,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
         }
       }
       if (done.rec >= 0) {
+        if (done.r0 + wave * 32 >= done.n * a.group) return;     // no rows: not read
         float* rec = a.part + (static_cast<size_t>(done.rec) * c.Hkv + kvh) * C::REC;
 #pragma unroll
         for (int d = 0; d < C::DT; ++d) {
@@ -974,16 +1008,41 @@ __global__ __launch_bounds__(256) void gqa_prefill_paged_fp8_merge_kernel(PagedF
   const size_t step = static_cast<size_t>(c.Hkv) * C::REC;
   const float* r0 = a.part + (static_cast<size_t>(rec) * c.Hkv + kvh) * C::REC;
   const float* ml = r0 + kRows * D + (wave * 32 + l32) * 2;
+  // kBatch records at a time, their loads all in flight (past the last: the last
+  // again, with weight 0).
+  constexpr int kBatch = 4;
   float M = -INFINITY, L = 0.f;
-  for (int x = 0; x < cuts; ++x) M = fmaxf(M, ml[x * step]);
   f32x4 o[4] = {};
-  for (int x = 0; x < cuts; ++x) {
-    const float m = ml[x * step], f = m == -INFINITY ? 0.f : fast_exp2(m - M);
-    L += f * ml[x * step + 1];
+  for (int x0 = 0; x0 < cuts; x0 += kBatch) {
+    float m[kBatch], l[kBatch];
+    f32x4 v[kBatch][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int dt = D == 64 ? e >> 1 : 4 * g + e, quad = D == 64 ? i + 2 * (e & 1) : i;
-      o[e] += f * *reinterpret_cast<const f32x4*>(r0 + x * step + (((wave * C::DT + dt) * 4 + quad) * 64 + lane) * 4);
+    for (int y = 0; y < kBatch; ++y) {
+      const size_t at = min(x0 + y, cuts - 1) * step;
+      m[y] = x0 + y < cuts ? ml[at] : -INFINITY;
+      l[y] = ml[at + 1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int dt = D == 64 ? e >> 1 : 4 * g + e, quad = D == 64 ? i + 2 * (e & 1) : i;
+        v[y][e] = *reinterpret_cast<const f32x4*>(r0 + at + (((wave * C::DT + dt) * 4 + quad) * 64 + lane) * 4);
+      }
+    }
+    float top = M;
+#pragma unroll
+    for (int y = 0; y < kBatch; ++y) top = fmaxf(top, m[y]);
+    const float f0 = M == -INFINITY ? 0.f : fast_exp2(M - top);
+    M = top;
+    L *= f0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= f0;
+#pragma unroll
+    for (int y = 0; y < kBatch; ++y) {
+      if (x0 + y < cuts) {
+        const float f = m[y] == -INFINITY ? 0.f : fast_exp2(m[y] - M);
+        L += f * l[y];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += f * v[y][e];
+      }
     }
   }
   const float inv = L == 0.f ? 0.f : 1.0f / L;
@@ -995,13 +1054,13 @@ __global__ __launch_bounds__(256) void gqa_prefill_paged_fp8_merge_kernel(PagedF
 }
 
 // Workgroups per KV head, and key runs of one request's tiles: enough that all
-// CUs have one, none shorter than kMinRun key tiles where the length is the bound.
+// CUs have one, none shorter than kMinKeys where the length is the bound.
 void shape(int T, int B, int Hkv, int group, int key_tile, int max_len, int* lanes, int* splits) {
   const int tiles = static_cast<int>((static_cast<long>(T) * group + kRows - 1) / kRows);
   *lanes = std::max(1, kCus / Hkv);
   *splits = 1;
   if (B == 1 && tiles < *lanes) {
-    const int runs = std::max(1, (max_len + key_tile - 1) / key_tile / kMinRun);
+    const int runs = std::max(1, max_len / kMinKeys);
     *splits = std::min(*lanes / tiles, runs);
   }
 }
