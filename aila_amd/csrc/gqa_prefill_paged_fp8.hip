@@ -30,7 +30,7 @@
 //
 // 8191 tokens, 16 / 4 heads, D = 256: 505-530 us (1.04-1.09 PFLOP/s; a large bf16
 // product reaches 1.19 here); 2048 tokens, 32 / 8, D = 128: 47 us; 250 tokens after
-// 7900, D = 256: 48 us and 9 us of merge; 3 prompts of up to 600 tokens after 3000
+// 7900, D = 256: 47 us and 7 us of merge; 3 prompts of up to 600 tokens after 3000
 // rows beside 29 single tokens, 40 / 8, D = 128: 5.4 us of plan, 128 us and 4.6 us.
 #include "paged_fp8.hpp"
 
