@@ -537,7 +537,9 @@ def kv_pages_reserve(cached_lens, new_lens, block_table, free_pages, free_count,
     free_pages int32 [num_pages], a stack whose entries [0, free_count[0]) are
     free; slots int32 [max_tokens] (written whole). -> (query_start [B+1],
     seq_lens [B], slots). seq_lens is 0 for requests that did not fit the
-    table, the batch or the free pages; their slots are -1."""
+    table, the batch or the free pages; their slots are -1, and the rows and
+    pages that they had stay theirs: the next call's cached_lens are
+    torch.where(seq_lens > 0, seq_lens, cached_lens), not seq_lens."""
     import torch
     B, max_pages = block_table.shape
     i32 = torch.int32

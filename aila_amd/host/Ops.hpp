@@ -58,7 +58,9 @@ void attention_decode_paged(Context& ctx, Tensor& q, Tensor& k_pages, Tensor& v_
 //
 // Pages and slots of the requests' new tokens: cached_lens/new_lens/seq_lens
 // [B], block_table [B, max_pages], free_pages [num_pages], free_count [1],
-// query_start [B + 1], slots [max_tokens].
+// query_start [B + 1], slots [max_tokens]. A request that was not admitted gets
+// seq_lens 0 and keeps its rows: the next step's cached_lens are seq_lens where
+// that is above 0, else what they were.
 void kv_pages_reserve(Context& ctx, Tensor& cached_lens, Tensor& new_lens, Tensor& block_table, Tensor& free_pages,
                       Tensor& free_count, int page_size, Tensor& slots, Tensor& query_start, Tensor& seq_lens);
 

@@ -311,8 +311,14 @@ int aila_hip_copy_to_cache(const void* new_kv, void* cache, int S,
  *                     query_start[b+1]) of the batch, the sum of new_lens before
  *                     (requests that are not admitted keep their place;
  *                     saturates at 2^31 - 1).
- *   seq_lens[B]       out: cached_lens[b] + new_lens[b], or 0 if not admitted.
- *                     May not be the array of cached_lens or new_lens.
+ *   seq_lens[B]       out: cached_lens[b] + new_lens[b], or 0 if not admitted
+ *                     in this call. 0 does not say that the request holds no
+ *                     rows: a request of cached_lens[b] rows that finds no free
+ *                     page keeps them and its pages. The lengths of the next
+ *                     call are seq_lens[b] > 0 ? seq_lens[b] : cached_lens[b];
+ *                     with a bare copy of seq_lens its next token would be
+ *                     written over its first row. May not be the array of
+ *                     cached_lens or new_lens.
  *   slots[max_tokens] out: the slot of each token; -1 for tokens of requests
  *                     that are not admitted and behind the last.
  * The table entries that request b's new rows need (pages cached / page_size
@@ -322,7 +328,8 @@ int aila_hip_copy_to_cache(const void* new_kv, void* cache, int S,
  * admitted if its rows fit the table, its tokens fit max_tokens, and, where it
  * needs pages, the free pages cover its need and that of every request before
  * it whose rows fit. Requests that are not admitted leave table and stack
- * alone. Calls on one stack must not overlap in time. */
+ * alone, and may be asked for again once pages have been given back. Calls on
+ * one stack must not overlap in time. */
 int aila_hip_kv_pages_reserve(const int* cached_lens, const int* new_lens,
                               int* block_table, const int* free_pages,
                               int* free_count, int* query_start, int* seq_lens,
