@@ -397,6 +397,9 @@ extern "C" int aila_hip_gqa_decode_paged_fp8(const void* q, long q_stride, const
   const int heads = Hkv * a.chunks;
   AILA_REQUIRE(static_cast<long>(B) * heads * ((max_len + kUnit - 1) / kUnit + 1) < (1L << 31),
                "gqa_decode_paged_fp8: B=%d sequences of up to %d rows and %d heads are too many", B, max_len, heads);
+  // one workgroup each without a split: fewer than 2^32 threads, the most of a launch
+  AILA_REQUIRE(static_cast<long>(B) * heads * kThreads < (1L << 32), "gqa_decode_paged_fp8: B=%d sequences of %d heads are too many",
+               B, heads);
   long groups = static_cast<long>(B) * heads;
   // One workgroup per (sequence, head) where that is faster than a split and its
   // merge: up to 6 units a sequence (D = 64: 8, D = 256: 4), and the longer the more

@@ -215,7 +215,8 @@ extern "C" int aila_hip_kv_append_paged_fp8(const void* k_new, const void* v_new
   AILA_REQUIRE(k_new && v_new && slots, "kv_append_paged_fp8: null pointer");
   if (int rc = check_paged_fp8("kv_append_paged_fp8", k_pages, v_pages, k_scale, v_scale, Hkv, D, page_size, num_pages))
     return rc;
-  AILA_REQUIRE(T > 0 && T <= (1 << 30), "kv_append_paged_fp8: bad T=%d", T);
+  // 16 tokens a workgroup at least where T is large: fewer than 2^32 threads, the most of a launch
+  AILA_REQUIRE(T > 0 && T <= (1 << 28) - kScaleRows, "kv_append_paged_fp8: T=%d outside [1, 2^28 - 16]", T);
   AILA_REQUIRE(new_stride >= static_cast<long>(Hkv) * D && new_stride % 8 == 0,
                "kv_append_paged_fp8: token stride %ld must be a multiple of 8 and hold Hkv * D = %ld values", new_stride,
                static_cast<long>(Hkv) * D);
@@ -248,11 +249,12 @@ extern "C" int aila_hip_kv_read_paged_fp8(const void* k_pages, const void* v_pag
   AILA_REQUIRE(slots && k_out && v_out, "kv_read_paged_fp8: null pointer");
   if (int rc = check_paged_fp8("kv_read_paged_fp8", k_pages, v_pages, k_scale, v_scale, Hkv, D, page_size, num_pages))
     return rc;
-  AILA_REQUIRE(T > 0 && T <= (1 << 30), "kv_read_paged_fp8: bad T=%d", T);
+  AILA_REQUIRE(T > 0, "kv_read_paged_fp8: bad T=%d", T);
   AILA_REQUIRE(reinterpret_cast<uintptr_t>(k_out) % 16 == 0 && reinterpret_cast<uintptr_t>(v_out) % 16 == 0,
                "kv_read_paged_fp8: k_out and v_out must be 16-byte aligned");
-  AILA_REQUIRE(static_cast<long>(T) * Hkv < (1L << 31), "kv_read_paged_fp8: T=%d rows of %d heads are too many", T, Hkv);
+  // a thread 8 values: fewer than 2^32 of them, the most of a launch
   const long n = static_cast<long>(T) * Hkv * (D / 8);
+  AILA_REQUIRE(n < (1L << 32) - kThreads, "kv_read_paged_fp8: T=%d rows of %d heads are too many for one call", T, Hkv);
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((n + kThreads - 1) / kThreads)), dim3(kThreads), 0,
                        static_cast<hipStream_t>(stream), static_cast<const uint8_t*>(k_pages),

@@ -357,7 +357,7 @@ int aila_hip_kv_pages_release(const int* release, int* block_table,
  *       not count for a), saturated beyond 448 (at e = 119 only).
  * If e exceeds the block's exponent, the rows before the run are requantised to
  * it (exact but for underflow). Rows behind the run are left as they were and
- * are not valid until written. */
+ * are not valid until written. T <= 2^28 - 16. */
 int aila_hip_kv_append_paged_fp8(const void* k_new, const void* v_new,
                                  long new_stride, void* k_pages, void* v_pages,
                                  float* k_scale, float* v_scale,
@@ -366,7 +366,7 @@ int aila_hip_kv_append_paged_fp8(const void* k_new, const void* v_new,
 
 /* Read rows back by slot, as the values they stand for: k_out/v_out [T, Hkv, D]
  * bf16; zeros for slots outside the pool. (Handing a sequence to the bf16 entry
- * points, export, inspection.) */
+ * points, export, inspection.) T * Hkv * D below 2^35 - 2^11. */
 int aila_hip_kv_read_paged_fp8(const void* k_pages, const void* v_pages,
                                const float* k_scale, const float* v_scale,
                                const int* slots, void* k_out, void* v_out,
@@ -379,7 +379,8 @@ int aila_hip_kv_read_paged_fp8(const void* k_pages, const void* v_pages,
  * of 8); out [B, Hq, D] bf16. Sequence b attends rows [0, min(seq_lens[b],
  * max_len)); none: 0. Rows whose table entry is outside [0, num_pages) are
  * masked. Any integer Hq / Hkv (one workgroup serves up to 16 query heads of a
- * KV head), B <= 4096. Softmax scale 1/sqrt(D).
+ * KV head), B <= 4096, and fewer than 2^24 such workgroups without a split.
+ * Softmax scale 1/sqrt(D).
  * The work is shared evenly by the workgroups whatever the lengths are;
  * workspace_size bytes let as many work as the device holds, a smaller
  * workspace fewer (2 records at least, else AILA_HIP_EWORKSPACE), and NULL one

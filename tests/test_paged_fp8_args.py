@@ -180,3 +180,12 @@ def test_plain_append_and_reserve():
     t, n, starts, lens, slots = ref.reserve([3, 0, 16], [2, 20, 0], [[5, -1], [-1, -1], [7, -1]], [1], 1, 16, 30)
     assert (t, n, lens) == ([[5, -1], [-1, -1], [7, -1]], 1, [5, 0, 16]) and slots[2:] == [-1] * 28
     assert ref.release([0, 1, 1], [[5, -1], [3, 2], [-1, 1]], [9, 0, 0, 0], 1) == ([[5, -1], [-1, -1], [-1, -1]], [9, 3, 2, 1], 4)
+
+
+@pytest.mark.parametrize("name,args,bad", [
+    ("kv_append_paged_fp8", APPEND, dict(T=1 << 28)), ("kv_append_paged_fp8", APPEND, dict(T=(1 << 28) - 15)),
+    ("kv_read_paged_fp8", READ, dict(T=1 << 26, H=4)), ("kv_read_paged_fp8", READ, dict(T=2**31 - 1, H=1)),
+    ("gqa_decode_paged_fp8", DECODE, dict(B=4096, H=4096, Hq=4096, stride=4096 * 128))])
+def test_calls_of_more_threads_than_a_launch_has(name, args, bad):
+    rc, msg = _rc(name, args, **bad)
+    assert rc == -1 and msg.startswith(name + ":"), (rc, msg)
