@@ -711,9 +711,11 @@ def gqa_decode_paged_fp8(q, k_pages, v_pages, k_scale, v_scale, block_table, seq
     """Decode over an 8-bit paged cache. q [B,Hq,D] bf16 (sequences may be
     strided); the cache as kv_append_paged_fp8; block_table int32 [B,
     max_pages]; seq_lens int32 [B] (taken as max_len where larger) -> out
-    [B,Hq,D]. workspace: uint8 device tensor (see
-    gqa_decode_paged_fp8_workspace_size), or None for one workgroup per
-    sequence and KV head."""
+    [B,Hq,D]. Row b of q is sequence b's, which is the order of
+    kv_pages_reserve's tokens only if each request adds exactly one (else gather
+    q[query_start[:B].clamp(max=T - 1)], or call gqa_prefill_paged_fp8).
+    workspace: uint8 device tensor (see gqa_decode_paged_fp8_workspace_size), or
+    None for one workgroup per sequence and KV head."""
     B, Hq, D = q.shape
     step, ((P, Hkv, page_size, _), (kp, vp, ks, vs)), out, ws, ws_bytes = _attention_args(
         q, k_pages, v_pages, k_scale, v_scale, block_table, None, seq_lens, out, workspace, stream, B)

@@ -75,7 +75,8 @@ void copy_to_cache_paged_fp8(Context& ctx, Tensor& new_k, Tensor& new_v, Tensor&
 void read_cache_paged_fp8(Context& ctx, Tensor& k_pages, Tensor& v_pages, Tensor& k_scale, Tensor& v_scale,
                           Tensor& slots, Tensor& k_out, Tensor& v_out);
 
-// attention_decode_paged over the 8-bit pages; workspace: any dtype, at least
+// attention_decode_paged over the 8-bit pages, row b of q being request b's (the
+// tokens of kv_pages_reserve where every request adds one); workspace: any dtype, at least
 // two records (aila_hip_gqa_decode_paged_fp8_workspace_size), or null.
 void attention_decode_paged_fp8(Context& ctx, Tensor& q, Tensor& k_pages, Tensor& v_pages, Tensor& k_scale,
                                 Tensor& v_scale, Tensor& block_table, Tensor& seq_lens, Tensor& output, int num_heads,

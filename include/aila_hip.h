@@ -376,11 +376,15 @@ int aila_hip_kv_read_paged_fp8(const void* k_pages, const void* v_pages,
 /* Single-token GQA decode over the 8-bit pages (the 8-bit form of
  * aila_hip_gqa_decode_paged; ops::attention_decode, src/ops/AttentionOps.cpp:
  * 499-643). q: sequence b's [Hq, D] bf16 at + b * q_stride elements (a multiple
- * of 8); out [B, Hq, D] bf16. Sequence b attends rows [0, min(seq_lens[b],
- * max_len)); none: 0. Rows whose table entry is outside [0, num_pages) are
- * masked. Any integer Hq / Hkv (one workgroup serves up to 16 query heads of a
- * KV head), B <= 4096, and fewer than 2^24 such workgroups without a split.
- * Softmax scale 1/sqrt(D).
+ * of 8); out [B, Hq, D] bf16. Row b of q and out is sequence b's: the order of
+ * the tokens of aila_hip_kv_pages_reserve only where every request adds exactly
+ * one token. In a batch with absent or idle requests (no new token) the later
+ * tokens stand earlier: gather the rows min(query_start[b], T - 1), or call
+ * aila_hip_gqa_prefill_paged_fp8, which takes such batches as they are.
+ * Sequence b attends rows [0, min(seq_lens[b], max_len)); none: 0. Rows whose
+ * table entry is outside [0, num_pages) are masked. Any integer Hq / Hkv (one
+ * workgroup serves up to 16 query heads of a KV head), B <= 4096, and fewer than
+ * 2^24 such workgroups without a split. Softmax scale 1/sqrt(D).
  * The work is shared evenly by the workgroups whatever the lengths are;
  * workspace_size bytes let as many work as the device holds, a smaller
  * workspace fewer (2 records at least, else AILA_HIP_EWORKSPACE), and NULL one

@@ -88,3 +88,34 @@ def test_a_running_request_without_a_page(decode):
             assert all(torch.equal(x[:k], y[:k]) for x, y in zip(rows[b], s.held(b, want[b]))), (n, b)
             seen += k
     assert want == [-1, 34, 34] and seen > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,max_len", [(64, 96), (128, 4800), (256, 96)])
+def test_a_batch_with_idle_requests(D, max_len):
+    """Absent and idle requests have no token in the batch, a refused one keeps its
+    place: prefill takes the batch as it is, decode its rows gathered by the starts."""
+    import torch
+    import aila_amd as A
+    from test_gpu_paged_fp8 import _cache, _check, _i32, _table
+    B, Hq, Hkv, page, P = 8, 8, 2, 16, 40
+    held = [50, 33, 20, 16, 0, 45, 31, 12]       # the last idle one's start is the batch's end
+    cache = _cache(P, Hkv, page, D, 4)
+    table = _table(held, page, P, 5, extra=max_len // page - 4)
+    cached, new = _i32([50, -33, 20, 16, 0, 45, 31, 12]), _i32([1, 1, 0, 1, 0, 1, 1, 0])
+    count, slots = _i32([0]), _i32([9] * 4)
+    starts, lens, _ = A.kv_pages_reserve(cached, new, table, _i32([0] * P), count, page, slots)
+    assert starts.tolist() == [0, 1, 1, 1, 2, 2, 3, 4, 4] and lens.tolist() == [51, 0, 20, 0, 0, 46, 32, 12]       # request 3 finds no page
+    qkv = torch.randn((4, Hq + 2 * Hkv, D), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(torch.bfloat16)
+    q, k, v = qkv.split([Hq, Hkv, Hkv], 1)
+    A.kv_append_paged_fp8(k, v, *cache, slots)
+    ws = torch.empty(max(A.gqa_decode_paged_fp8_workspace_size(B, Hq, Hkv, D, max_len), A.gqa_prefill_paged_fp8_workspace_size(4, B, Hq, Hkv, D, max_len)),
+                     dtype=torch.uint8, device="cuda")
+    got = A.gqa_prefill_paged_fp8(q, *cache, table, starts, lens, max_len, workspace=ws)
+    _check(got, q, cache, table, starts.tolist(), lens.tolist(), max_len, 2.0 ** -8)
+    rows = q[starts[:B].long().clamp(max=3)]
+    got = A.gqa_decode_paged_fp8(rows, *cache, table, lens, max_len, workspace=ws)
+    _check(got, rows, cache, table, range(B + 1), lens.tolist(), max_len, 2.0 ** -16)
+    for b, n in ((0, 51), (5, 46), (6, 32)):      # the rows that the gathered tokens wrote
+        at = int(table[b, (n - 1) // page]) * page + (n - 1) % page
+        assert slots[starts[b]].item() == at
