@@ -16,7 +16,8 @@
 // Split: the rows of all sequences and KV heads form one line, in units of 128
 // rows (a strip of 32 for each of the 4 waves), and every workgroup takes an
 // equal piece of it, whatever the lengths are: a ragged batch keeps every CU
-// busy until the end. A piece that covers a (sequence, head) whole writes its
+// busy until the end. Whether to split is the host's choice, which knows the
+// bound of the lengths alone. A piece that covers a (sequence, head) whole writes its
 // output; the others write records {acc[D], m, l}, at most two a workgroup, and
 // the merge kernel joins those of each (sequence, head).
 #include "paged_fp8.hpp"
@@ -87,9 +88,10 @@ __device__ __forceinline__ int share_begin(int w, int units, int groups) {
 
 template <int D>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void gqa_decode_paged_fp8_kernel(PagedFp8 c, Fp8DecodeArgs a) {
-  // Strips of a wave in registers: one is worked on while the next arrives. (Three:
-  // 8 sequences of 32768, D = 256, 57.2 us in a graph against 55.2, 8 of 8000, 32/8,
-  // D = 128, 24.7 against 23.4. Two workgroups a CU at D = 256 instead spill: 85.)
+  // Strips of a wave in registers: one is worked on while the next arrives. (us a
+  // call, merge included, in a graph that changes its inputs. Three: 8 ragged
+  // sequences of up to 32768, 16/4, D = 256, 75.6 against 73.3; 8 of 8000, 32/8, D =
+  // 128, 32.0 against 31.0. Two workgroups a CU at D = 256 instead spill: 109.8.)
   constexpr int kDepth = 2;
   extern __shared__ __attribute__((aligned(16))) unsigned char s_dyn[];
   float* s_acc = reinterpret_cast<float*>(s_dyn);             // [kWaves][tile][D]
@@ -410,7 +412,10 @@ extern "C" int aila_hip_gqa_decode_paged_fp8(const void* q, long q_stride, const
   // 41.2, 4000 57.2 / 56.7, 8000 108 / 101. D = 64, 8 heads: 1 of 1024 7.4 / 7.7, 1300
   // 9.0 / 7.8; 16 of 2000 12.4 / 13.8, 3000 16.6 / 14.8; 64 of 4000 29.9 / 35.3. D = 256,
   // 4 heads: 1 of 512 10.9 / 11.1, 612 13.0 / 11.2; 32 of 1024 19.6 / 26.6, 2000 32.8 /
-  // 32.6; 64 of 2000 35.4 / 44.0, 4000 65.7 / 61.7.
+  // 32.6; 64 of 2000 35.4 / 44.0, 4000 65.7 / 61.7. The bound is all that the rule sees:
+  // one long sequence among short ones pays for it (32 / 8, D = 128, one of 4096 rows
+  // and 31 of 100, 32.5 / 22.2; 16 / 4, D = 256, one of 2048 and 63 of 100, 33.1 / 23.1),
+  // and so do short sequences under a loose bound (32 of up to 1024, 14.6 / 22.8).
   const long few = (D == 64 ? 8 : D == 128 ? 6 : 4) * kUnit, many = D == 256 ? 2048 : 4096;
   const bool whole = max_len <= std::max(few, many * std::min(groups, 256L) / 256);
   if (workspace != nullptr) {

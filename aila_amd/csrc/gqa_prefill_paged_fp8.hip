@@ -29,9 +29,10 @@
 // where the vector phase does, for 1056 cycles of products.
 //
 // 8191 tokens, 16 / 4 heads, D = 256: 505-530 us (1.04-1.09 PFLOP/s; a large bf16
-// product reaches 1.19 here); 2048 tokens, 32 / 8, D = 128: 47 us; 250 tokens after
-// 7900, D = 256: 47 us and 7 us of merge; 3 prompts of up to 600 tokens after 3000
-// rows beside 29 single tokens, 40 / 8, D = 128: 5.4 us of plan, 128 us and 4.6 us.
+// product reaches 1.19 here); 2048 tokens, 32 / 8, D = 128: 47-49 us; 250 tokens after
+// 7900, D = 256: 50-51 us with 7 us of merge; 3 prompts of up to 600 tokens after 3000
+// rows beside 29 single tokens, 40 / 8, D = 128: 138-141 us with 5.5 us of plan and
+// 4.7 us of merge.
 #include "paged_fp8.hpp"
 
 #include <algorithm>
@@ -48,7 +49,12 @@ constexpr int kRows = 32 * kGroupWaves;    // query rows of a tile
 constexpr int kMaxSequences = 4096;
 constexpr int kCus = 256;
 constexpr int kNoKey = 0x7fffffff;
-constexpr int kThinRows = 16;              // a tile of so few rows is walked by single waves
+// A tile of so few rows is walked by single waves (us a call, so / as the others, in a
+// graph that changes its inputs. 32 requests of 1 token after up to 3000 rows: 32 / 8,
+// D = 64 28.1 / 50.3, D = 128 42.4 / 65.8, 16 / 4, D = 256 58.5 / 74.0; 8 after up to
+// 30000, D = 256 101.6 / 129.2; one after 5000, D = 128 20.2 / 25.4, D = 256 26.8 / 29.2;
+// its 4 tokens after 30000, 16 rows, D = 256 47.0 / 45.7, the one case that loses).
+constexpr int kThinRows = 16;
 
 struct Fp8PrefillArgs {
   const bf16* q;
@@ -1054,8 +1060,12 @@ __global__ __launch_bounds__(256) void gqa_prefill_paged_fp8_merge_kernel(PagedF
 }
 
 // Workgroups per KV head, and key runs of one request's tiles: enough that all
-// CUs have one, none shorter than kMinKeys where the length is the bound.
-void shape(int T, int B, int Hkv, int group, int key_tile, int max_len, int* lanes, int* splits) {
+// CUs have one, none shorter than kMinKeys where the length is the bound. As many
+// runs for each tile, so a number of tiles a little above the workgroups', or above a
+// half of them, leaves CUs without one (us, 16 / 4, D = 256 after 14000 rows, 64
+// workgroups a head: 32 tiles 240, 33 367, 64 466, 65 757; 32 / 8, D = 128, 32
+// workgroups: 32 tiles 242, 33 412).
+void shape(int T, int B, int Hkv, int group, int max_len, int* lanes, int* splits) {
   const int tiles = static_cast<int>((static_cast<long>(T) * group + kRows - 1) / kRows);
   *lanes = std::max(1, kCus / Hkv);
   *splits = 1;
@@ -1067,7 +1077,7 @@ void shape(int T, int B, int Hkv, int group, int key_tile, int max_len, int* lan
 
 template <int D>
 size_t workspace_need(int T, int B, int Hkv, int group, int max_len, int* lanes, int* splits) {
-  shape(T, B, Hkv, group, Cfg<D>::BN, max_len, lanes, splits);
+  shape(T, B, Hkv, group, max_len, lanes, splits);
   const size_t rec = static_cast<size_t>(Cfg<D>::REC) * sizeof(float) * Hkv;
   if (B == 1) {
     const size_t tiles = (static_cast<size_t>(T) * group + kRows - 1) / kRows;

@@ -9,8 +9,8 @@
 // wave owns a run for one head and one of K and V, so block and scale have one
 // writer, and it is bound by the bytes: 2 in and 1 out a value. A long prompt of
 // 8191 tokens, 4 heads, D = 256: 15-17 us for 50 MB (a large copy reaches 4.7
-// TB/s, 10.6 us); reading the rows back 10.5 us for the same. 32 single tokens,
-// 8 heads, D = 128: 3.6 and 3.3 us, which are the launch and the chain slot ->
+// TB/s, 10.6 us); reading the rows back 9.9 us for the same. 32 single tokens,
+// 8 heads, D = 128: 3.7 and 3.0 us, which are the launch and the chain slot ->
 // rows and block -> codes.
 #include "paged_fp8.hpp"
 
@@ -227,7 +227,11 @@ extern "C" int aila_hip_kv_append_paged_fp8(const void* k_new, const void* v_new
   // single tokens / prompt, 8 heads, D = 128, tiles of 1, 4, 8 and 16 tokens:
   // T = 32 3.2/3.3, 6.0/3.3, 11.1/3.4, 20.8/4.5; 512 6.3/8.3, 7.3/4.2, 10.4/3.6,
   // 18.0/4.5; 1024 10.1/14.1, 10.3/5.9, 12.4/4.3, 18.4/4.5; 2048 18.1/25.0,
-  // 16.5/9.2, 18.6/5.9, 22.0/5.4; 4096 32.9/45.8, 29.3/15.3, 29.9/9.3, 34.3/8.3.
+  // 16.5/9.2, 18.6/5.9, 22.0/5.4; 4096 32.9/45.8, 29.3/15.3, 29.9/9.3, 34.3/8.3. T is
+  // all that the host knows: single tokens that stand together in a large T take the
+  // long tiles too, and a wave stores up to 16 runs in a row (32 of them padded to
+  // 4096 31.4 us, to 256 4.5; 30 behind prompts of 3 x 1300 tokens 24.3, prompts of as
+  // many alone 9.6).
   const int tile = T <= 256 ? 1 : T <= 1024 ? 4 : T <= 2048 ? 8 : kScaleRows;
   const dim3 grid((T + tile - 1) / tile, (Hkv + 1) / 2);
   auto go = [&](auto kernel) {

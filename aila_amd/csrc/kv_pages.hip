@@ -14,9 +14,9 @@
 // LDS and the cost is latency: the chain of lengths -> table entries -> slots,
 // three dependent round trips to memory (the free pages nearest the top of the
 // stack are fetched beside the lengths), and four sums over the workgroup.
-// 32 requests of 4096 rows and 245 new tokens: 6.3 us, of which a launch is 2;
+// 32 requests of 4096 rows and 245 new tokens: 6.1 us, of which a launch is 2;
 // 256 requests, 16-row pages, 9000 new tokens in a pool too small for them:
-// 11.7 us, and 2.9 us for a second launch that fills the slots. Release: 4.0 and
+// 11.8 us, and 3.9 us for a second launch that fills the slots. Release: 3.9 and
 // 5.8 us.
 #include "common.hpp"
 

@@ -384,11 +384,15 @@ int aila_hip_kv_read_paged_fp8(const void* k_pages, const void* v_pages,
  * Sequence b attends rows [0, min(seq_lens[b], max_len)); none: 0. Rows whose
  * table entry is outside [0, num_pages) are masked. Any integer Hq / Hkv (one
  * workgroup serves up to 16 query heads of a KV head), B <= 4096, and fewer than
- * 2^24 such workgroups without a split. Softmax scale 1/sqrt(D).
- * The work is shared evenly by the workgroups whatever the lengths are;
- * workspace_size bytes let as many work as the device holds, a smaller
- * workspace fewer (2 records at least, else AILA_HIP_EWORKSPACE), and NULL one
- * per sequence and KV head (no split). Calls that may overlap in time (other
+ * 2^24 such workgroups without a split. Softmax scale 1/sqrt(D). Sums are held
+ * in fp32, of weights of up to 2^8: the largest |V| times the rows attended has
+ * to stay below 2^120.
+ * With a workspace the rows of all sequences are shared evenly by the workgroups,
+ * whatever the lengths are, where max_len is above a bound that grows with B *
+ * Hkv up to 4096 (D = 256: 2048); below it, and with NULL, each sequence and KV
+ * head is one workgroup's (no split). workspace_size bytes let as many work as
+ * the device holds, a smaller workspace fewer (2 records at least, else
+ * AILA_HIP_EWORKSPACE). Calls that may overlap in time (other
  * streams, graphs replayed side by side) need workspaces of their own. */
 size_t aila_hip_gqa_decode_paged_fp8_workspace_size(int B, int Hq, int Hkv,
                                                     int D, int max_len);
@@ -411,6 +415,8 @@ int aila_hip_gqa_decode_paged_fp8(const void* q, long q_stride,
  *            them. Token query_start[b] + i, of n = query_start[b+1] -
  *            query_start[b], attends rows [0, L - n + i], L = min(seq_lens[b],
  *            max_len); none: 0. Tokens from query_start[B] on are not touched.
+ * The softmax weights are rounded to bf16 (2^-8 of each at most) before they meet
+ * V; where few tokens are walked as the decode does, to 2^-16.
  * Other arguments as aila_hip_gqa_decode_paged_fp8. T is the number of rows of
  * q and out; query_start must not decrease nor pass T (what passes it is not
  * computed).
