@@ -52,6 +52,14 @@ _SIGS = {
     "aila_hip_gqa_prefill_paged_fp8_workspace_size": ([_I, _I, _I, _I, _I, _I], _SZ),
     "aila_hip_gqa_prefill_paged_fp8": ([_P, _L, _P, _P, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _I, _I, _I, _P, _I, _I,
                                         _P, _P, _P], _I),
+    "aila_hip_prepare_qkv_paged_fp8": ([_P, _L, _L, _P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I,
+                                        _I, _I, _I, _I, _I, _F, _P, _F, _P], _I),
+    "aila_hip_gqa_tree_paged_fp8_workspace_size": ([_I, _I, _I, _I, _I, _I, _I], _SZ),
+    "aila_hip_gqa_tree_paged_fp8": ([_P, _L, _P, _P, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _I, _I, _I, _P, _I, _I, _P, _P, _P,
+                                     _I, _P], _I),
+    "aila_hip_kv_keep_paged_fp8": ([_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P], _I),
+    "aila_hip_kv_pages_trim": ([_P, _P, _P, _P, _I, _I, _I, _I, _P], _I),
+    "aila_hip_kv_copy_paged_fp8": ([_P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P], _I),
     "aila_hip_deltanet_decode": ([_P, _P, _P, _P, _P, _P, _P, _P, _P,
                                   _I, _I, _I, _I, _I, _F, _F, _P], _I),
     "aila_hip_deltanet_prefill_workspace_size": ([_I, _I, _I, _I, _I], _SZ),
@@ -751,6 +759,234 @@ def gqa_prefill_paged_fp8(q, k_pages, v_pages, k_scale, v_scale, block_table, qu
     if rc:
         _check(rc, "aila_hip_gqa_prefill_paged_fp8")
     return out
+
+
+# ---------------------- drafts, forks and trims over the 8-bit paged cache ----
+def _head_strides(t, tokens, heads, dim):
+    """(token, head) strides of a [tokens, heads, dim] view whose heads may stand
+    apart, or (0, 0) if it is not one that the kernels take."""
+    a, b, c = t.stride()
+    if heads == 1:
+        b = dim
+    if tokens == 1:
+        a = (heads - 1) * b + dim
+        a += -a % 8
+    ok = c == 1 and b >= dim and not b % 8 and a >= (heads - 1) * b + dim and not a % 8
+    return (a, b) if ok else (0, 0)
+
+
+def prepare_qkv_paged_fp8(q, k, v, k_pages, v_pages, k_scale, v_scale, slots, positions, q_norm=None, k_norm=None,
+                          rotary_dim=None, theta: float = 1e6, eps: float = 1e-6, sections=None, inv_freq=None, q_out=None,
+                          stream=None):
+    """Between a layer's projection and its attention over an 8-bit paged cache.
+    q [T,Hq,D], k/v [T,Hkv,D] bf16 (tokens may be strided, q's heads too: a view
+    of packed q|gate rows); per-head RMSNorm of q and k with weights q_norm,
+    k_norm [D] bf16 (None: 1); the first rotary_dim dims (None: D; a multiple
+    of 8, 0: none) turned at positions int32 [T], or [3,T]: the t, h and w
+    streams of interleaved mRoPE with ``sections`` (t, h, w); k and v quantised
+    into the rows ``slots`` (int32 [T], -1: skip) as kv_append_paged_fp8 does
+    -> q_out [T,Hq,D] bf16 (may be q itself, if contiguous). inv_freq: float32
+    [rotary_dim/2] in place of theta^(-2d/rotary_dim)."""
+    import torch
+    dev = _device_of(stream)
+    T, Hq, D = q.shape
+    bf, i32 = torch.bfloat16, torch.int32
+    rot = D if rotary_dim is None else int(rotary_dim)
+    if q_out is None:
+        q_out = _new_out(lambda: torch.empty((T, Hq, D), dtype=bf, device=q.device), stream)
+    pages = _pages_ok(torch, dev, k_pages, v_pages, k_scale, v_scale) if k_pages is not None else None
+    ok = pages is not None and k is not None and v is not None
+    streams = 0 if positions is None else 1 if positions.dim() == 1 else 3
+    if ok:
+        (P, Hkv, page_size, _), (kp, vp, ks, vs) = pages
+        qs, qh = _head_strides(q, T, Hq, D)
+        ok = qs and pages[0][3] == D and k.shape == v.shape == (T, Hkv, D) and q.dtype is bf and k.dtype is bf and v.dtype is bf \
+            and q_out.dtype is bf and q_out.shape == (T, Hq, D) and q_out.is_contiguous() and slots.dtype is i32 \
+            and slots.shape == (T,) and slots.is_contiguous() \
+            and not (q.data_ptr() | k.data_ptr() | v.data_ptr() | q_out.data_ptr()) & 15 \
+            and q.get_device() == k.get_device() == v.get_device() == q_out.get_device() == slots.get_device() == dev
+    if ok:
+        k_step, v_step = _token_stride(k, T, Hkv, D), _token_stride(v, T, Hkv, D)
+        ok = k_step and v_step \
+            and (q_norm is None or (q_norm.dtype is bf and q_norm.shape == (D,) and q_norm.is_contiguous() and q_norm.get_device() == dev)) \
+            and (k_norm is None or (k_norm.dtype is bf and k_norm.shape == (D,) and k_norm.is_contiguous() and k_norm.get_device() == dev)) \
+            and (positions is None or (positions.dtype is i32 and positions.shape == ((T,) if streams == 1 else (3, T))
+                                       and positions.is_contiguous() and positions.get_device() == dev)) \
+            and (inv_freq is None or (inv_freq.dtype is torch.float32 and inv_freq.shape == (rot // 2,) and inv_freq.is_contiguous()
+                                      and inv_freq.get_device() == dev))
+    if not ok:
+        _need_pages(k_pages, v_pages, k_scale, v_scale)
+        P, Hkv, page_size, _ = k_pages.shape
+        _need_rows(k, T, Hkv, k_pages.shape[3], "k")
+        _need_rows(v, T, Hkv, k_pages.shape[3], "v")
+        if not q.is_cuda or q.dtype != bf or D != k_pages.shape[3] or q.data_ptr() % 16:
+            raise ValueError(f"q: {q.dtype} of head dim {D} on {q.device}, expected 16-byte aligned bfloat16 device data of {k_pages.shape[3]}")
+        if not _head_strides(q, T, Hq, D)[0]:
+            raise ValueError(f"q: strides {q.stride()}, expected contiguous dims, and tokens and heads multiples of 8 apart")
+        _need(q_out, bf, (T, Hq, D), "q_out")
+        _need(slots, i32, (T,), "slots", align=4)
+        for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+            if t is not None:
+                _need(t, bf, (D,), name)
+        if positions is not None:
+            _need(positions, i32, (T,) if streams == 1 else (3, T), "positions", align=4)
+        if inv_freq is not None:
+            _need(inv_freq, torch.float32, (rot // 2,), "inv_freq", align=4)
+        _same_device(dev, q, k, v, k_pages, v_pages, k_scale, v_scale, q_out, slots, q_norm, k_norm, positions, inv_freq)
+        raise ValueError("prepare_qkv_paged_fp8: bad tensors")
+    if streams == 3 and sections is None:
+        raise ValueError("positions [3, T] need sections (t, h, w)")
+    pos = _ptr(positions)
+    _, sh, sw = (0, 0, 0) if streams != 3 else (int(x) for x in sections)
+    rc = lib().aila_hip_prepare_qkv_paged_fp8(
+        q.data_ptr(), qs, qh, k.data_ptr(), k_step, v.data_ptr(), v_step, q_out.data_ptr(), _ptr(q_norm), _ptr(k_norm), kp, vp, ks, vs,
+        slots.data_ptr(), pos, pos + 4 * T if streams == 3 else None, pos + 8 * T if streams == 3 else None, sh, sw, T, Hq, Hkv, D,
+        page_size, P, rot, float(theta), _ptr(inv_freq), float(eps), _stream(stream))
+    if rc:
+        _check(rc, "aila_hip_prepare_qkv_paged_fp8")
+    return q_out
+
+
+def gqa_tree_paged_fp8_workspace_size(T: int, B: int, Hq: int, Hkv: int, D: int, max_len: int, mask_words: int) -> int:
+    return int(lib().aila_hip_gqa_tree_paged_fp8_workspace_size(T, B, Hq, Hkv, D, max_len, mask_words))
+
+
+def gqa_tree_paged_fp8(q, k_pages, v_pages, k_scale, v_scale, block_table, query_start, seq_lens, tree_mask, max_len: int,
+                       out=None, workspace=None, stream=None):
+    """Attention of drafted trees over an 8-bit paged cache that holds the
+    drafted rows already. Arguments as gqa_prefill_paged_fp8; tree_mask int64
+    [T, W], W <= 64: token i of a request attends its rows before the draft and
+    the drafted token j if bit j % 64 of tree_mask[i, j // 64] is set (its own
+    bit too, if it is to attend itself). A request has 64 W tokens at most.
+    workspace: uint8 device tensor (see gqa_tree_paged_fp8_workspace_size), or
+    None: no key split."""
+    import torch
+    T, Hq, D = q.shape
+    B, max_pages = block_table.shape
+    if query_start is None:
+        raise ValueError("query_start is required")
+    if tree_mask is None or tree_mask.dim() != 2:
+        raise ValueError("tree_mask must be [T, words]")
+    words = tree_mask.shape[1]
+    step, ((P, Hkv, page_size, _), (kp, vp, ks, vs)), out, ws, ws_bytes = _attention_args(
+        q, k_pages, v_pages, k_scale, v_scale, block_table, query_start, seq_lens, out, workspace, stream, B)
+    if not (tree_mask.dtype is torch.int64 and tree_mask.shape[0] == T and tree_mask.is_contiguous()
+            and tree_mask.get_device() == q.get_device()):
+        _need(tree_mask, torch.int64, (T, words), "tree_mask", align=8)
+        _same_device(q.get_device(), tree_mask)
+    rc = lib().aila_hip_gqa_tree_paged_fp8(q.data_ptr(), step, kp, vp, ks, vs, out.data_ptr(), ws, ws_bytes, T, B, Hq, Hkv, D,
+                                           page_size, P, block_table.data_ptr(), max_pages, int(max_len), query_start.data_ptr(),
+                                           seq_lens.data_ptr(), tree_mask.data_ptr(), words, _stream(stream))
+    if rc:
+        _check(rc, "aila_hip_gqa_tree_paged_fp8")
+    return out
+
+
+def _layer_pointers(caches, dev):
+    """(layers, shape of a cache, the four host arrays of device pointers) of one
+    cache (k_pages, v_pages, k_scale, v_scale) or a list of such."""
+    import torch
+    if not caches:
+        raise ValueError("no caches")
+    if torch.is_tensor(caches[0]):
+        caches = [caches]
+    shape, ptrs = None, []
+    for kp, vp, ks, vs in caches:
+        got = _pages_ok(torch, dev, kp, vp, ks, vs)
+        if got is None or (shape is not None and got[0] != shape):
+            _need_pages(kp, vp, ks, vs)
+            _same_device(dev, kp, vp, ks, vs)
+            raise ValueError(f"caches: pages {tuple(kp.shape)} beside {tuple(shape)}" if shape is not None else "bad cache tensors")
+        shape = got[0]
+        ptrs.append(got[1])
+    n = len(ptrs)
+    return n, shape, [(_P * n)(*(p[i] for p in ptrs)) for i in range(4)]
+
+
+def kv_keep_paged_fp8(caches, block_table, cached_lens, kept, kept_lens, lens=None, stream=None):
+    """Keep the accepted rows of drafts, in all layers: row cached_lens[b] +
+    kept[b, i] of request b becomes row cached_lens[b] + i for i < kept_lens[b].
+    caches: one (k_pages, v_pages, k_scale, v_scale) or a list of them, a layer
+    each, of one shape; cached_lens int32 [B] (rows before the draft; negative:
+    absent), kept int32 [B, max_kept] (rising in each row), kept_lens int32 [B]
+    -> lens int32 [B], cached_lens + kept_lens."""
+    import torch
+    dev = _device_of(stream)
+    B, max_pages = block_table.shape
+    i32 = torch.int32
+    if kept.dim() != 2:
+        raise ValueError("kept must be [B, max_kept]")
+    most = kept.shape[1]
+    if lens is None:
+        lens = _new_out(lambda: torch.empty(B, dtype=i32, device=block_table.device), stream)
+    n, (P, Hkv, page_size, D), ptrs = _layer_pointers(caches, dev)
+    one = (B,)
+    if not (block_table.dtype is i32 and cached_lens.dtype is i32 and kept.dtype is i32 and kept_lens.dtype is i32 and lens.dtype is i32
+            and cached_lens.shape == kept_lens.shape == lens.shape == one and kept.shape[0] == B and block_table.is_contiguous()
+            and cached_lens.is_contiguous() and kept.is_contiguous() and kept_lens.is_contiguous() and lens.is_contiguous()
+            and block_table.get_device() == cached_lens.get_device() == kept.get_device() == kept_lens.get_device()
+            == lens.get_device() == dev):
+        _need(block_table, i32, (B, max_pages), "block_table", align=4)
+        _need(cached_lens, i32, one, "cached_lens", align=4)
+        _need(kept, i32, (B, most), "kept", align=4)
+        _need(kept_lens, i32, one, "kept_lens", align=4)
+        _need(lens, i32, one, "lens", align=4)
+        _same_device(dev, block_table, cached_lens, kept, kept_lens, lens)
+    rc = lib().aila_hip_kv_keep_paged_fp8(*ptrs, n, block_table.data_ptr(), cached_lens.data_ptr(), kept.data_ptr(),
+                                          kept_lens.data_ptr(), lens.data_ptr(), B, most, Hkv, D, page_size, P, max_pages, _stream(stream))
+    if rc:
+        _check(rc, "aila_hip_kv_keep_paged_fp8")
+    return lens
+
+
+def kv_pages_trim(lens, block_table, free_pages, free_count, page_size: int, stream=None):
+    """Push the pages behind each request's rows (lens int32 [B]; negative: leave
+    the row alone) back onto the free stack; their table entries become -1."""
+    import torch
+    B, max_pages = block_table.shape
+    i32 = torch.int32
+    dev = _device_of(stream)
+    num_pages = free_pages.numel()
+    if not (lens.dtype is i32 and block_table.dtype is i32 and free_pages.dtype is i32 and free_count.dtype is i32
+            and lens.shape == (B,) and free_pages.shape == (num_pages,) and free_count.shape == (1,)
+            and lens.is_contiguous() and block_table.is_contiguous() and free_pages.is_contiguous()
+            and lens.get_device() == block_table.get_device() == free_pages.get_device() == free_count.get_device() == dev):
+        _need(lens, i32, (B,), "lens", align=4)
+        _need(block_table, i32, (B, max_pages), "block_table", align=4)
+        _need(free_pages, i32, (num_pages,), "free_pages", align=4)
+        _need(free_count, i32, (1,), "free_count", align=4)
+        _same_device(dev, block_table, lens, free_pages, free_count)
+    rc = lib().aila_hip_kv_pages_trim(lens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), B,
+                                      max_pages, int(page_size), num_pages, _stream(stream))
+    if rc:
+        _check(rc, "aila_hip_kv_pages_trim")
+
+
+def kv_copy_paged_fp8(caches, block_table, src, dst, lens, max_len: int, stream=None):
+    """Copy rows [0, lens[i]) (int32 [n], taken as max_len where larger) of row
+    src[i] of block_table to the pages of row dst[i] (int32 [n] each), in all
+    layers (caches as kv_keep_paged_fp8): forks, whose pages kv_pages_reserve
+    has taken. Whole blocks of 16 rows are copied."""
+    import torch
+    dev = _device_of(stream)
+    B, max_pages = block_table.shape
+    i32 = torch.int32
+    n, (P, Hkv, page_size, D), ptrs = _layer_pointers(caches, dev)
+    pairs = src.numel()
+    one = (pairs,)
+    if not (block_table.dtype is i32 and src.dtype is i32 and dst.dtype is i32 and lens.dtype is i32
+            and src.shape == dst.shape == lens.shape == one and block_table.is_contiguous() and src.is_contiguous()
+            and dst.is_contiguous() and lens.is_contiguous()
+            and block_table.get_device() == src.get_device() == dst.get_device() == lens.get_device() == dev):
+        _need(block_table, i32, (B, max_pages), "block_table", align=4)
+        _need(src, i32, one, "src", align=4)
+        _need(dst, i32, one, "dst", align=4)
+        _need(lens, i32, one, "lens", align=4)
+        _same_device(dev, block_table, src, dst, lens)
+    rc = lib().aila_hip_kv_copy_paged_fp8(*ptrs, n, block_table.data_ptr(), src.data_ptr(), dst.data_ptr(), lens.data_ptr(), pairs,
+                                          int(max_len), B, Hkv, D, page_size, P, max_pages, _stream(stream))
+    if rc:
+        _check(rc, "aila_hip_kv_copy_paged_fp8")
 
 
 # ------------------------------------------------------------ DeltaNet ----

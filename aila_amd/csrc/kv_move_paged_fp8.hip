@@ -1,0 +1,254 @@
+// Rows of the 8-bit paged KV cache moved inside it, in all layers at once: the
+// accepted rows of a draft to its front, and a request's rows to the pages of its
+// forks. Codes are moved as they are, or times a power of two where the block
+// that they come to has a larger scale (exact but for underflow): nothing is
+// quantised again from a rounded value.
+#include "paged_fp8.hpp"
+
+#include <algorithm>
+
+namespace aila {
+namespace {
+
+constexpr int kMaxLayers = 64;    // of a launch: their pointers are kernel arguments
+struct Layers {
+  uint8_t* pages[2 * kMaxLayers];   // K and V of layer 0, of layer 1, ...
+  float* scale[2 * kMaxLayers];
+};
+
+__device__ __forceinline__ uint32_t scale_codes(uint32_t w, float f) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+  const int x = __builtin_amdgcn_cvt_pk_fp8_f32(lo[0] * f, lo[1] * f, 0, false);
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * f, hi[1] * f, x, true));
+}
+
+struct KeepArgs {
+  const int* table;
+  const int* cached;
+  const int* kept;        // [B, most]
+  const int* kept_lens;
+  int* lens;              // null: written by another launch
+  int B, most, max_pages, num_pages, Hkv, page_size;
+};
+
+// One wave: K or V of one head of one request and layer. Blocks from the one of
+// the first row that moves, in order: a row comes from behind its place (kept
+// indices rise), so a block that has been written holds no later block's source.
+constexpr int kKeepThreads = 256;
+constexpr int kNone = kMinScaleExp - 1;
+template <int D>
+__global__ __launch_bounds__(kKeepThreads) void kv_keep_paged_fp8_kernel(Layers ly, KeepArgs a) {
+  constexpr int LR = D / 16;                // lanes of a row, 16 codes each
+  constexpr int RI = 64 / LR;               // rows of an instruction
+  constexpr int NI = kScaleRows / RI;       // instructions of a block
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = blockIdx.y;
+  const int hv = static_cast<int>(blockIdx.x) * (kKeepThreads / 64) + wave;   // head, K or V
+  const int cached = a.cached[b];
+  const long max_rows = static_cast<long>(a.max_pages) * a.page_size;
+  int n = min(max(a.kept_lens[b], 0), a.most);
+  if (cached < 0) n = 0;
+  else n = static_cast<int>(min(static_cast<long>(n), max(max_rows - cached, 0L)));
+  if (a.lens != nullptr && blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.lens[b] = cached + n;
+  if (hv >= 2 * a.Hkv || n == 0) return;
+  const int* kept = a.kept + static_cast<size_t>(b) * a.most;
+  int first = n;      // rows before it stay where they are
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    const int i = i0 + lane;
+    const unsigned long long off = __ballot(i < n && kept[i] != i);
+    if (off) {
+      first = i0 + __builtin_ctzll(off);
+      break;
+    }
+  }
+  if (first == n) return;
+  const int head = hv >> 1, arr = 2 * blockIdx.z + (hv & 1);
+  uint8_t* pages = ly.pages[arr];
+  float* scale = ly.scale[arr];
+  const int* row_table = a.table + static_cast<size_t>(b) * a.max_pages;
+  const int page_blocks = a.page_size / kScaleRows;
+  // block of a row in the pool, -1: none
+  auto block_of = [&](long row) __attribute__((always_inline)) -> int {
+    if (row < 0 || row >= max_rows) return -1;
+    const int r = static_cast<int>(row), p = r / a.page_size;
+    const int page = row_table[p];
+    return page >= 0 && page < a.num_pages ? (page * a.Hkv + head) * page_blocks + (r - p * a.page_size) / kScaleRows : -1;
+  };
+  const int rr = lane / LR, c16 = lane % LR * 16;
+  const int end = cached + n;
+  for (int at = (cached + first) / kScaleRows * kScaleRows; at < end; at += kScaleRows) {
+    const int bid = block_of(at);
+    if (bid < 0) continue;
+    uint8_t* block = pages + static_cast<size_t>(bid) * (kScaleRows * D);
+    const int held = held_exp(scale[bid]);
+    u32x4 w[NI];
+    int e_from[NI];
+    bool moves[NI], stays[NI];
+    int top = kNone;
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+      const int j = k * RI + rr, row = at + j, i = row - cached;
+      stays[k] = i < first;
+      moves[k] = !stays[k] && i < n;
+      w[k] = u32x4{0u, 0u, 0u, 0u};
+      e_from[k] = held;
+      if (moves[k]) {
+        const long src = static_cast<long>(cached) + kept[i];
+        const int sb = kept[i] < 0 ? -1 : block_of(src);
+        moves[k] = sb >= 0;
+        if (sb >= 0) {
+          e_from[k] = held_exp(scale[sb]);
+          w[k] = ld16(pages + static_cast<size_t>(sb) * (kScaleRows * D) + (src % kScaleRows) * D + c16);
+        }
+      } else if (stays[k]) {
+        w[k] = ld16(block + j * D + c16);
+      }
+      if (moves[k] || stays[k]) top = max(top, e_from[k]);
+    }
+    const int e = wave_max(top);
+    if (e == kNone) continue;     // no row of it is in range
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+      if (moves[k] || (stays[k] && e != held)) {
+        if (e != e_from[k]) {
+          const float f = pow2f(e_from[k] - e);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) w[k][x] = scale_codes(w[k][x], f);
+        }
+        *reinterpret_cast<u32x4*>(block + (k * RI + rr) * D + c16) = w[k];
+      }
+    }
+    if (lane == 0) scale[bid] = pow2f(e);
+  }
+}
+
+struct CopyArgs {
+  const int* table;
+  const int* src;
+  const int* dst;
+  const int* lens;
+  int B, max_pages, num_pages, Hkv, page_size, max_len;
+  int parts;              // workgroups of a page
+};
+
+// One workgroup: a part of a page of one pair, K or V of one layer. A page of all
+// heads is contiguous; of the last one the blocks behind the rows are left out.
+constexpr int kCopyThreads = 256;
+constexpr int kCopyBytes = 32768;     // of a workgroup
+template <int D>
+__global__ __launch_bounds__(kCopyThreads) void kv_copy_paged_fp8_kernel(Layers ly, CopyArgs a) {
+  const int p = static_cast<int>(blockIdx.x) / a.parts, part = static_cast<int>(blockIdx.x) % a.parts;
+  const int len = min(a.lens[blockIdx.y], a.max_len);
+  const int rows = min(len - p * a.page_size, a.page_size);
+  if (rows <= 0) return;
+  const int from = a.src[blockIdx.y], to = a.dst[blockIdx.y];
+  if (from < 0 || from >= a.B || to < 0 || to >= a.B) return;
+  const int sp = a.table[static_cast<size_t>(from) * a.max_pages + p], dp = a.table[static_cast<size_t>(to) * a.max_pages + p];
+  if (sp < 0 || sp >= a.num_pages || dp < 0 || dp >= a.num_pages || sp == dp) return;
+  const int page_blocks = a.page_size / kScaleRows, blocks = (rows + kScaleRows - 1) / kScaleRows;
+  const size_t bytes = static_cast<size_t>(a.Hkv) * a.page_size * D;
+  const uint8_t* s = ly.pages[blockIdx.z] + sp * bytes;
+  uint8_t* d = ly.pages[blockIdx.z] + dp * bytes;
+  const int pieces = static_cast<int>(bytes / 16);      // D of a block
+  const int end = min(pieces, (part + 1) * (kCopyBytes / 16));
+  for (int i = part * (kCopyBytes / 16) + threadIdx.x; i < end; i += kCopyThreads)
+    if (i / D % page_blocks < blocks) *reinterpret_cast<u32x4*>(d + static_cast<size_t>(i) * 16) = ld16(s + static_cast<size_t>(i) * 16);
+  if (part == 0) {
+    const float* ss = ly.scale[blockIdx.z] + static_cast<size_t>(sp) * a.Hkv * page_blocks;
+    float* ds = ly.scale[blockIdx.z] + static_cast<size_t>(dp) * a.Hkv * page_blocks;
+    for (int i = threadIdx.x; i < a.Hkv * page_blocks; i += kCopyThreads)
+      if (i % page_blocks < blocks) ds[i] = ss[i];
+  }
+}
+
+// The host's arrays of the layers' pointers, checked; layers [l0, l0 + n) of them.
+int check_layers(const char* what, const void* const* k_pages, const void* const* v_pages, const float* const* k_scale,
+                 const float* const* v_scale, int layers, int Hkv, int D, int page_size, int num_pages) {
+  AILA_REQUIRE(k_pages && v_pages && k_scale && v_scale, "%s: null pointer", what);
+  AILA_REQUIRE(layers > 0, "%s: layers=%d must be positive", what, layers);
+  for (int l = 0; l < layers; ++l)
+    if (int rc = check_paged_fp8(what, k_pages[l], v_pages[l], k_scale[l], v_scale[l], Hkv, D, page_size, num_pages)) return rc;
+  return AILA_HIP_OK;
+}
+Layers some_layers(void* const* k_pages, void* const* v_pages, float* const* k_scale, float* const* v_scale, int l0, int n) {
+  Layers ly{};
+  for (int l = 0; l < n; ++l) {
+    ly.pages[2 * l] = static_cast<uint8_t*>(k_pages[l0 + l]);
+    ly.pages[2 * l + 1] = static_cast<uint8_t*>(v_pages[l0 + l]);
+    ly.scale[2 * l] = k_scale[l0 + l];
+    ly.scale[2 * l + 1] = v_scale[l0 + l];
+  }
+  return ly;
+}
+
+}  // namespace
+}  // namespace aila
+
+extern "C" int aila_hip_kv_keep_paged_fp8(void* const* k_pages, void* const* v_pages, float* const* k_scale,
+                                          float* const* v_scale, int layers, const int* block_table,
+                                          const int* cached_lens, const int* kept, const int* kept_lens, int* lens, int B,
+                                          int max_kept, int Hkv, int D, int page_size, int num_pages, int max_pages,
+                                          void* stream) {
+  using namespace aila;
+  AILA_REQUIRE(block_table && cached_lens && kept && kept_lens && lens, "kv_keep_paged_fp8: null pointer");
+  if (int rc = check_layers("kv_keep_paged_fp8", k_pages, v_pages, k_scale, v_scale, layers, Hkv, D, page_size, num_pages)) return rc;
+  AILA_REQUIRE(B > 0 && B <= 65535, "kv_keep_paged_fp8: B=%d outside [1, 65535]", B);
+  AILA_REQUIRE(max_kept > 0 && max_kept <= 65536, "kv_keep_paged_fp8: max_kept=%d outside [1, 65536]", max_kept);
+  AILA_REQUIRE(max_pages > 0 && static_cast<long>(max_pages) * page_size <= (1L << 30), "kv_keep_paged_fp8: bad max_pages=%d",
+               max_pages);
+  AILA_REQUIRE(lens != cached_lens && lens != kept_lens, "kv_keep_paged_fp8: the lengths going out may not overwrite those coming in");
+  KeepArgs a{block_table, cached_lens, kept, kept_lens, lens, B, max_kept, max_pages, num_pages, Hkv, page_size};
+  const unsigned gx = (2 * Hkv + kKeepThreads / 64 - 1) / (kKeepThreads / 64);
+  // fewer than 2^32 threads, the most of a launch
+  const long fit = ((1L << 32) - 1) / kKeepThreads / gx / B;
+  AILA_REQUIRE(fit > 0, "kv_keep_paged_fp8: B=%d requests of %d heads are too many", B, Hkv);
+  const int step = static_cast<int>(std::min<long>(kMaxLayers, fit));
+  for (int l0 = 0; l0 < layers; l0 += step) {
+    const int n = std::min(step, layers - l0);
+    const Layers ly = some_layers(k_pages, v_pages, k_scale, v_scale, l0, n);
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(gx, B, n), dim3(kKeepThreads), 0, static_cast<hipStream_t>(stream), ly, a);
+    };
+    if (D == 64) go(kv_keep_paged_fp8_kernel<64>);
+    else if (D == 128) go(kv_keep_paged_fp8_kernel<128>);
+    else go(kv_keep_paged_fp8_kernel<256>);
+    a.lens = nullptr;
+  }
+  return check_launch("kv_keep_paged_fp8");
+}
+
+extern "C" int aila_hip_kv_copy_paged_fp8(void* const* k_pages, void* const* v_pages, float* const* k_scale,
+                                          float* const* v_scale, int layers, const int* block_table, const int* src,
+                                          const int* dst, const int* lens, int n, int max_len, int B, int Hkv, int D,
+                                          int page_size, int num_pages, int max_pages, void* stream) {
+  using namespace aila;
+  AILA_REQUIRE(block_table && src && dst && lens, "kv_copy_paged_fp8: null pointer");
+  if (int rc = check_layers("kv_copy_paged_fp8", k_pages, v_pages, k_scale, v_scale, layers, Hkv, D, page_size, num_pages)) return rc;
+  AILA_REQUIRE(B > 0 && n > 0 && n <= 65535, "kv_copy_paged_fp8: bad B=%d or n=%d pairs (at most 65535)", B, n);
+  AILA_REQUIRE(max_pages > 0 && static_cast<long>(max_pages) * page_size <= (1L << 30), "kv_copy_paged_fp8: bad max_pages=%d",
+               max_pages);
+  AILA_REQUIRE(max_len >= 0 && max_len <= max_pages * page_size, "kv_copy_paged_fp8: max_len=%d outside [0, %d]", max_len,
+               max_pages * page_size);
+  const long bytes = static_cast<long>(Hkv) * page_size * D;
+  AILA_REQUIRE(bytes < (1L << 31), "kv_copy_paged_fp8: a page of %ld bytes is too large", bytes);
+  if (max_len == 0) return AILA_HIP_OK;
+  CopyArgs a{block_table, src, dst, lens, B, max_pages, num_pages, Hkv, page_size, max_len,
+             static_cast<int>((bytes + kCopyBytes - 1) / kCopyBytes)};
+  const long gx = static_cast<long>((max_len + page_size - 1) / page_size) * a.parts;
+  const long fit = ((1L << 32) - 1) / kCopyThreads / gx / n / 2;
+  AILA_REQUIRE(fit > 0, "kv_copy_paged_fp8: %d pairs of up to %d rows are too many", n, max_len);
+  const int step = static_cast<int>(std::min<long>(kMaxLayers, fit));
+  for (int l0 = 0; l0 < layers; l0 += step) {
+    const int m = std::min(step, layers - l0);
+    const Layers ly = some_layers(k_pages, v_pages, k_scale, v_scale, l0, m);
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(gx), n, 2 * m), dim3(kCopyThreads), 0,
+                         static_cast<hipStream_t>(stream), ly, a);
+    };
+    if (D == 64) go(kv_copy_paged_fp8_kernel<64>);
+    else if (D == 128) go(kv_copy_paged_fp8_kernel<128>);
+    else go(kv_copy_paged_fp8_kernel<256>);
+  }
+  return check_launch("kv_copy_paged_fp8");
+}

@@ -26,34 +26,6 @@ __device__ __forceinline__ int scale_exp(int mag) {
   return min(max(e, kMinScaleExp), kMaxScaleExp);
 }
 
-// x * 2^-e as a value to be rounded to e4m3: saturated (at kMaxScaleExp alone
-// a finite x exceeds 448), NaN for what is not finite (e4m3 has no infinity).
-__device__ __forceinline__ float to_code_range(float x, float inv) {
-  const float y = fminf(fmaxf(x * inv, -kE4m3Max), kE4m3Max);
-  return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : y;
-}
-
-__device__ __forceinline__ uint32_t pack_fp8x4(float a, float b, float c, float d) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true));
-}
-
-template <int CTRL>
-__device__ __forceinline__ int dpp_i(int x) {
-  return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xF, 0xF, false);
-}
-// Maximum of the wave's values, in every lane.
-__device__ __forceinline__ int wave_max(int x) {
-  x = max(x, dpp_i<kDppQuadXor1>(x));
-  x = max(x, dpp_i<kDppQuadXor2>(x));
-  x = max(x, dpp_i<kDppRowHalfMirror>(x));
-  x = max(x, dpp_i<kDppRowMirror>(x));
-  const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  x = max(static_cast<int>(a[0]), static_cast<int>(a[1]));
-  const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  return max(static_cast<int>(b[0]), static_cast<int>(b[1]));
-}
-
 // Grid (ceil(T / tile), ceil(Hkv / 2)); wave w: K or V (w & 1) of head
 // 2 * blockIdx.y + w / 2, the runs that begin in the workgroup's `tile` tokens.
 template <int D>

@@ -306,6 +306,72 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_release_kernel(const in
   if (tid == 0) *free_count = min(have + sum, num_pages);
 }
 
+// Entries from lens[b] rows on go onto the stack in order of request and page.
+// As the release, but every row is looked at, from the page behind its rows.
+__global__ __launch_bounds__(kPlanThreads) void kv_pages_trim_kernel(const int* __restrict__ lens, int* table,
+                                                                     int* free_pages, int* free_count, int B,
+                                                                     int max_pages, int page_size, int num_pages) {
+  extern __shared__ int s_dyn[];
+  int* s_from = s_dyn;         // [B] first entry looked at
+  int* s_at = s_from + B;      // [B + 1] entries of the rows before
+  __shared__ int s_wi[kPlanWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int have = min(max(*free_count, 0), num_pages);
+  for (int b = tid; b < B; b += kPlanThreads) {
+    const int len = lens[b];
+    s_from[b] = len < 0 ? max_pages : min(len / page_size + (len % page_size > 0 ? 1 : 0), max_pages);
+  }
+  if (tid == 0) s_at[0] = 0;
+  __syncthreads();
+  int v[kRowChunk];
+  auto read = [&](const int* row, int p0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kRowChunk; ++i) {
+      const int p = p0 + 64 * i + lane;
+      v[i] = p < max_pages ? row[p] : -1;
+    }
+  };
+  for (int b = wave; b < B; b += kPlanWaves) {
+    int n = 0;
+    for (int p0 = s_from[b]; p0 < max_pages; p0 += 64 * kRowChunk) {
+      read(table + static_cast<size_t>(b) * max_pages, p0);
+#pragma unroll
+      for (int i = 0; i < kRowChunk; ++i) n += __popcll(__ballot(v[i] >= 0));
+    }
+    if (lane == 0) s_at[b + 1] = n;
+  }
+  __syncthreads();
+  int sum = 0;
+  for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    const int n = b < B ? s_at[b + 1] : 0;
+    int all;
+    const int incl = sum + block_scan<kPlanThreads, int>(n, s_wi, &all);
+    if (b < B) s_at[b + 1] = incl;
+    sum += all;
+  }
+  __syncthreads();
+  for (int b = wave; b < B; b += kPlanWaves) {
+    if (s_at[b + 1] == s_at[b]) continue;
+    int at = have + s_at[b];
+    int* row = table + static_cast<size_t>(b) * max_pages;
+    for (int p0 = s_from[b]; p0 < max_pages; p0 += 64 * kRowChunk) {
+      read(row, p0);
+#pragma unroll
+      for (int i = 0; i < kRowChunk; ++i) {
+        const unsigned long long held = __ballot(v[i] >= 0);
+        if (v[i] >= 0) {
+          const int j = at + __popcll(held & ((1ull << lane) - 1));
+          if (j < num_pages) free_pages[j] = v[i];
+          row[p0 + 64 * i + lane] = -1;
+        }
+        at += __popcll(held);
+      }
+    }
+  }
+  if (tid == 0) *free_count = min(have + sum, num_pages);
+}
+
 }  // namespace
 }  // namespace aila
 
@@ -357,4 +423,18 @@ extern "C" int aila_hip_kv_pages_release(const int* release, int* block_table, i
                      static_cast<hipStream_t>(stream), release, block_table, free_pages, free_count, B, max_pages,
                      num_pages);
   return check_launch("kv_pages_release");
+}
+
+extern "C" int aila_hip_kv_pages_trim(const int* lens, int* block_table, int* free_pages, int* free_count, int B,
+                                      int max_pages, int page_size, int num_pages, void* stream) {
+  using namespace aila;
+  AILA_REQUIRE(lens && block_table && free_pages && free_count, "kv_pages_trim: null pointer");
+  AILA_REQUIRE(B > 0 && B <= kMaxRequests, "kv_pages_trim: B=%d outside [1, %d]", B, kMaxRequests);
+  AILA_REQUIRE(page_size > 0 && page_size % 16 == 0, "kv_pages_trim: page_size=%d must be a positive multiple of 16", page_size);
+  AILA_REQUIRE(max_pages > 0 && static_cast<long>(max_pages) * B < (1L << 31), "kv_pages_trim: bad max_pages=%d", max_pages);
+  AILA_REQUIRE(num_pages > 0, "kv_pages_trim: num_pages=%d must be positive", num_pages);
+  hipLaunchKernelGGL(kv_pages_trim_kernel, dim3(1), dim3(kPlanThreads), static_cast<size_t>(2 * B + 1) * sizeof(int),
+                     static_cast<hipStream_t>(stream), lens, block_table, free_pages, free_count, B, max_pages, page_size,
+                     num_pages);
+  return check_launch("kv_pages_trim");
 }

@@ -1,0 +1,345 @@
+// What stands between a layer's fused projection and its attention over the 8-bit
+// paged cache, for a ragged batch of tokens: per-head RMSNorm of q and k, rotation
+// at each token's own position, k and v quantised into the pages.
+//
+//   y = x / sqrt(mean(x^2) + eps) * w
+//   (y_d, y_{d + rot/2}) turned by p theta^(-2 d / rot), d < rot / 2
+//
+// in fp32, rounded once: q to bf16, k by the append's rule to e4m3 (the calls for
+// one step each round k to bf16 twice on its way there). An angle is a product in
+// fp64 of whole turns, taken modulo 1 there: at position 2^20 an fp32 product is
+// off by 2^-4 radians.
+//
+// A lane holds dims 4 s .. 4 s + 3 of both halves of the rotated part (or of the
+// rest), so a pair is never apart, at two 8-byte loads instead of one of 16.
+#include "paged_fp8.hpp"
+
+namespace aila {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+
+struct TurnTable {
+  double f[kMaxRopePairs];     // turns a position
+};
+
+struct PrepareArgs {
+  const bf16 *q, *k, *v;
+  long q_stride, q_head_stride, k_stride, v_stride;
+  bf16* q_out;
+  const bf16 *q_norm, *k_norm;     // null: 1
+  uint8_t *k_pages, *v_pages;
+  float *k_scale, *v_scale;
+  const int* slots;
+  const int *pos_t, *pos_h, *pos_w;
+  int section_h, section_w;
+  const float* inv_freq;
+  int T, tile, Hq, Hkv, page_size, num_slots, rot;
+  int kv_groups;       // workgroups that store rows; the others take a token's queries each
+  float eps;
+};
+
+template <int LR>
+__device__ __forceinline__ float row_sum(float x) {
+  x += dpp_f<kDppQuadXor1>(x);
+  x += dpp_f<kDppQuadXor2>(x);
+  x += dpp_f<kDppRowHalfMirror>(x);
+  if constexpr (LR >= 16) x += dpp_f<kDppRowMirror>(x);
+  if constexpr (LR >= 32) {
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+  }
+  return x;
+}
+
+// A lane's place in a row: dims lo .. lo + 3 and hi .. hi + 3, which are turned
+// pairwise (pairs j .. j + 3) if `turns`.
+struct Place { int lo, hi, j; bool turns; };
+template <int D>
+__device__ __forceinline__ Place place_of(int s, int rot) {
+  const int x = 4 * s, half = rot / 2;
+  return x < half ? Place{x, x + half, x, true} : Place{x + half, x + D / 2, x, false};
+}
+
+struct Turn { float c[4], s[4]; };
+__device__ __forceinline__ Turn turn_of(const PrepareArgs& a, const TurnTable& tt, const Place& p, int token) {
+  Turn r;
+  const int pt = a.pos_t[token];
+  int ph = pt, pw = pt;
+  if (a.pos_h != nullptr) {
+    ph = a.pos_h[token];
+    pw = a.pos_w[token];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = p.j + i, m = j % 3, n = j / 3;
+    int pos = pt;
+    pos = m == 1 && n < a.section_h ? ph : pos;
+    pos = m == 2 && n < a.section_w ? pw : pos;
+    const double f = a.inv_freq != nullptr ? static_cast<double>(a.inv_freq[j]) * 0.15915494309189535 : tt.f[j];
+    double t = static_cast<double>(pos) * f;
+    t -= __builtin_rint(t);
+    sincospif(2.0f * static_cast<float>(t), &r.s[i], &r.c[i]);
+  }
+  return r;
+}
+
+__device__ __forceinline__ void load4(const bf16* p, float* f) {
+  const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+  f[0] = __uint_as_float(w[0] << 16);
+  f[1] = __uint_as_float(w[0] & 0xffff0000u);
+  f[2] = __uint_as_float(w[1] << 16);
+  f[3] = __uint_as_float(w[1] & 0xffff0000u);
+}
+__device__ __forceinline__ void load_weights(const bf16* w, const Place& p, float* f) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = 1.0f;
+  if (w != nullptr) {
+    load4(w + p.lo, f);
+    load4(w + p.hi, f + 4);
+  }
+}
+
+// x: a lane's 8 values of a head, normalised and turned in place.
+template <int D>
+__device__ __forceinline__ void norm_turn(float* x, const float* w, const Turn& t, bool turns, float eps) {
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+  const float r = 1.0f / sqrtf(row_sum<D / 8>(ss) * (1.0f / D) + eps);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+  if (turns) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = x[i], b = x[4 + i];
+      x[i] = a * t.c[i] - b * t.s[i];
+      x[4 + i] = fmaf(a, t.s[i], b * t.c[i]);
+    }
+  }
+}
+
+// The queries of one token.
+template <int D>
+__device__ __forceinline__ void prepare_queries(const PrepareArgs& a, const TurnTable& tt, int token) {
+  constexpr int LR = D / 8, RI = 64 / LR;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Place p = place_of<D>(lane % LR, a.rot);
+  float w[8];
+  load_weights(a.q_norm, p, w);
+  Turn t{};
+  if (p.turns) t = turn_of(a, tt, p, token);
+  const bf16* src = a.q + static_cast<size_t>(token) * a.q_stride;
+  bf16* dst = a.q_out + static_cast<size_t>(token) * a.Hq * D;
+  for (int h0 = wave * RI; h0 < a.Hq; h0 += kWaves * RI) {
+    const int h = min(h0 + lane / LR, a.Hq - 1);
+    float x[8];
+    load4(src + h * a.q_head_stride + p.lo, x);
+    load4(src + h * a.q_head_stride + p.hi, x + 4);
+    norm_turn<D>(x, w, t, p.turns, a.eps);
+    if (h0 + lane / LR < a.Hq) {
+      *reinterpret_cast<u32x2*>(dst + h * D + p.lo) = u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+      *reinterpret_cast<u32x2*>(dst + h * D + p.hi) = u32x2{pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+    }
+  }
+}
+
+// Smallest e with a <= 448 * 2^e (448 = 1.75 * 2^8) for the fp32 of these bits, bounded.
+__device__ __forceinline__ int scale_exp_f32(int bits) {
+  const int e = (bits >> 23) - 127 - 8 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0);
+  return min(max(e, kMinScaleExp), kMaxScaleExp);
+}
+
+// Rows into the pages: as the append (a wave takes K or V of a head, the runs that
+// begin in its tile of tokens), K normalised and turned on the way.
+template <int D>
+__device__ __forceinline__ void prepare_rows(const PrepareArgs& a, const TurnTable& tt, int bx, int by) {
+  constexpr int LR = D / 8;
+  constexpr int RI = 64 / LR;
+  constexpr int NI = kScaleRows / RI;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int head = by * 2 + (wave >> 1);
+  if (head >= a.Hkv) return;
+  const bool isv = wave & 1;
+  const bf16* src = (isv ? a.v : a.k) + static_cast<size_t>(head) * D;
+  const long stride = isv ? a.v_stride : a.k_stride;
+  uint8_t* pages = isv ? a.v_pages : a.k_pages;
+  float* scale = isv ? a.v_scale : a.k_scale;
+  const int t0 = bx * a.tile;
+  const int rr = lane / LR, s = lane % LR;
+  Place p = place_of<D>(s, a.rot);
+  if (isv) p = Place{8 * s, 8 * s + 4, 0, false};
+  float w[8];
+  load_weights(isv ? nullptr : a.k_norm, p, w);
+
+  // Lane i holds the slot of token t0 + i - 1: a tile's runs end 31 tokens after
+  // its begin at most.
+  const int ti = t0 + lane - 1;
+  const int win = ti >= 0 && ti < a.T && lane < 2 * kScaleRows + 1 ? a.slots[ti] : -1;
+  const int before = __shfl_up(win, 1);
+  const bool begins = lane >= 1 && lane <= a.tile && win >= 0 && win < a.num_slots &&
+                      !(before >= 0 && before + 1 == win && win % kScaleRows != 0);
+  unsigned long long todo = __ballot(begins);
+  while (todo) {
+    const int i = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    const int t = t0 + i - 1;
+    const int slot = __builtin_amdgcn_readlane(win, i);
+    const int r0 = slot % kScaleRows;
+    // the run: the tokens from i on whose slots go on, to the block's end
+    const unsigned long long off = ~(__ballot(lane >= i && lane - i < kScaleRows - r0 && win == slot + (lane - i)) >> i);
+    const int n = __builtin_ctzll(off);      // 1 .. 16 - r0
+
+    const int page = slot / a.page_size, blk = slot % a.page_size / kScaleRows;
+    const size_t bid = (static_cast<size_t>(page) * a.Hkv + head) * (a.page_size / kScaleRows) + blk;
+    uint8_t* block = pages + bid * (kScaleRows * D);
+    const int held = held_exp(scale[bid]);
+    float x[NI][8];
+    int top = 0;
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+      const int j = min(k * RI + rr, n - 1);      // past the last: its copy
+      const bf16* row = src + static_cast<size_t>(t + j) * stride;
+      load4(row + p.lo, x[k]);
+      load4(row + p.hi, x[k] + 4);
+    }
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+      if (k * RI >= n) break;
+      if (!isv) {
+        Turn r{};
+        if (p.turns) r = turn_of(a, tt, p, t + min(k * RI + rr, n - 1));
+        norm_turn<D>(x[k], w, r, p.turns, a.eps);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int m = __float_as_uint(x[k][e]) & 0x7fffffff;
+        if (m < 0x7f800000) top = max(top, m);
+      }
+    }
+    int e = scale_exp_f32(wave_max(top));
+    if (r0 > 0) {
+      if (e > held) {
+        // requantise rows [0, r0): x 2^(held - e) is exact but for underflow
+        const float f = pow2f(held - e);
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+          const int j = k * RI + rr;
+          if (j < r0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t* at = reinterpret_cast<uint32_t*>(block + j * D + (h ? p.hi : p.lo));
+              const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(*at, false);
+              const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(*at, true);
+              *at = pack_fp8x4(lo[0] * f, lo[1] * f, hi[0] * f, hi[1] * f);
+            }
+          }
+        }
+      }
+      e = max(e, held);
+    }
+    const float inv = pow2f(-e);
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+      const int j = k * RI + rr;
+      if (j < n) {
+        float f[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) f[y] = to_code_range(x[k][y], inv);
+        *reinterpret_cast<uint32_t*>(block + (r0 + j) * D + p.lo) = pack_fp8x4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<uint32_t*>(block + (r0 + j) * D + p.hi) = pack_fp8x4(f[4], f[5], f[6], f[7]);
+      }
+    }
+    if (lane == 0) scale[bid] = pow2f(e);
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads) void prepare_qkv_paged_fp8_kernel(PrepareArgs a, TurnTable tt) {
+  const int x = blockIdx.x;
+  if (x < a.kv_groups) {
+    const int pairs = (a.Hkv + 1) / 2;
+    prepare_rows<D>(a, tt, x / pairs, x % pairs);
+  } else {
+    prepare_queries<D>(a, tt, x - a.kv_groups);
+  }
+}
+
+// Turns a position of each pair: theta^(-2 j / rot) / (2 pi).
+const TurnTable& turn_table(float theta, int rot) {
+  thread_local float last_theta = 0.f;
+  thread_local int last_rot = -1;
+  thread_local TurnTable t{};
+  if (theta != last_theta || rot != last_rot) {
+    for (int j = 0; j < rot / 2; ++j)
+      t.f[j] = std::pow(static_cast<double>(theta), -2.0 * j / rot) * 0.15915494309189535;
+    last_theta = theta;
+    last_rot = rot;
+  }
+  return t;
+}
+
+}  // namespace
+}  // namespace aila
+
+extern "C" int aila_hip_prepare_qkv_paged_fp8(const void* q, long q_stride, long q_head_stride, const void* k,
+                                              long k_stride, const void* v, long v_stride, void* q_out,
+                                              const void* q_norm_w, const void* k_norm_w, void* k_pages, void* v_pages,
+                                              float* k_scale, float* v_scale, const int* slots, const int* positions,
+                                              const int* pos_h, const int* pos_w, int section_h, int section_w, int T,
+                                              int Hq, int Hkv, int D, int page_size, int num_pages, int rotary_dim,
+                                              float theta, const float* inv_freq, float eps, void* stream) {
+  using namespace aila;
+  const char* what = "prepare_qkv_paged_fp8";
+  AILA_REQUIRE(q && k && v && q_out && slots, "%s: null pointer", what);
+  if (int rc = check_paged_fp8(what, k_pages, v_pages, k_scale, v_scale, Hkv, D, page_size, num_pages)) return rc;
+  AILA_REQUIRE(Hq > 0 && Hq <= 65535, "%s: bad Hq=%d", what, Hq);
+  AILA_REQUIRE(rotary_dim >= 0 && rotary_dim <= D && rotary_dim % 8 == 0, "%s: rotary_dim=%d must be a multiple of 8 up to D=%d", what,
+               rotary_dim, D);
+  AILA_REQUIRE(rotary_dim == 0 || positions != nullptr, "%s: positions are required", what);
+  AILA_REQUIRE((pos_h == nullptr) == (pos_w == nullptr), "%s: pos_h and pos_w go together", what);
+  AILA_REQUIRE(section_h >= 0 && section_w >= 0, "%s: bad sections h=%d w=%d", what, section_h, section_w);
+  AILA_REQUIRE(rotary_dim == 0 || inv_freq != nullptr || theta > 0.f, "%s: theta=%g must be positive", what, static_cast<double>(theta));
+  AILA_REQUIRE(q_head_stride >= D && q_head_stride % 8 == 0 && q_stride % 8 == 0 && q_stride >= (Hq - 1) * q_head_stride + D,
+               "%s: query strides %ld (token) and %ld (head) must be multiples of 8 and hold %d heads of %d", what, q_stride,
+               q_head_stride, Hq, D);
+  AILA_REQUIRE(k_stride >= static_cast<long>(Hkv) * D && k_stride % 8 == 0 && v_stride >= static_cast<long>(Hkv) * D && v_stride % 8 == 0,
+               "%s: token strides %ld (k) and %ld (v) must be multiples of 8 and hold Hkv * D = %ld values", what, k_stride, v_stride,
+               static_cast<long>(Hkv) * D);
+  const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                        reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(q_norm_w) | reinterpret_cast<uintptr_t>(k_norm_w);
+  AILA_REQUIRE(all % 16 == 0, "%s: q, k, v, q_out and the weights must be 16-byte aligned", what);
+  const int tile = T <= 256 ? 1 : T <= 1024 ? 4 : T <= 2048 ? 8 : kScaleRows;
+  // fewer than 2^32 threads, the most of a launch
+  const long kv_groups = (static_cast<long>(T) + tile - 1) / tile * ((Hkv + 1) / 2);
+  AILA_REQUIRE(T > 0 && T <= (1 << 30) && (kv_groups + T) * kThreads < (1L << 32), "%s: T=%d tokens are none or too many for one call", what, T);
+  PrepareArgs a{};
+  a.q = static_cast<const bf16*>(q);
+  a.k = static_cast<const bf16*>(k);
+  a.v = static_cast<const bf16*>(v);
+  a.q_stride = q_stride; a.q_head_stride = q_head_stride; a.k_stride = k_stride; a.v_stride = v_stride;
+  a.q_out = static_cast<bf16*>(q_out);
+  a.q_norm = static_cast<const bf16*>(q_norm_w);
+  a.k_norm = static_cast<const bf16*>(k_norm_w);
+  a.k_pages = static_cast<uint8_t*>(k_pages);
+  a.v_pages = static_cast<uint8_t*>(v_pages);
+  a.k_scale = k_scale; a.v_scale = v_scale;
+  a.slots = slots;
+  a.pos_t = positions; a.pos_h = pos_h; a.pos_w = pos_w;
+  a.section_h = section_h; a.section_w = section_w;
+  a.inv_freq = inv_freq;
+  a.T = T; a.tile = tile; a.Hq = Hq; a.Hkv = Hkv; a.page_size = page_size; a.num_slots = num_pages * page_size;
+  a.rot = rotary_dim;
+  a.kv_groups = static_cast<int>(kv_groups);
+  a.eps = eps;
+  static const TurnTable none{};
+  const TurnTable& tt = rotary_dim > 0 && inv_freq == nullptr ? turn_table(theta, rotary_dim) : none;
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(kv_groups + T)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a, tt);
+  };
+  if (D == 64) go(prepare_qkv_paged_fp8_kernel<64>);
+  else if (D == 128) go(prepare_qkv_paged_fp8_kernel<128>);
+  else go(prepare_qkv_paged_fp8_kernel<256>);
+  return check_launch(what);
+}

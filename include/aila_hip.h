@@ -438,6 +438,128 @@ int aila_hip_gqa_prefill_paged_fp8(const void* q, long q_stride,
                                    const int* query_start, const int* seq_lens,
                                    void* stream);
 
+/* ------------------------- drafts, forks, trims (8-bit paged cache) --- */
+
+/* A step that verifies trees of drafted tokens: reserve (new_lens: the drafts) ->
+ * prepare -> tree attention in every layer; the caller's sampler then picks a path
+ * of each tree; keep moves its rows together in all layers, and trim gives the
+ * pages behind them back. The reference decodes one token a step and has no
+ * counterpart. */
+
+/* Between a layer's projection and its attention, T tokens of any requests: q and
+ * k normalised per head and rotated, k and v quantised into the rows `slots` (the
+ * work of ops::decode_prepare_qkv_partial and of ops::head_rms_norm +
+ * ops::apply_rope_partial + ops::copy_to_cache, src/ops/ElementwiseOps.cpp:33-103,
+ * 555-705, NormOps.cpp:277-321).
+ *   y = x / sqrt(mean(x^2) + eps) * w, w = q_norm_w / k_norm_w [D] bf16 (NULL: 1)
+ *   dims d and d + rotary_dim / 2 of y are turned by p * theta^(-2 d / rotary_dim)
+ *   (inv_freq, device float[rotary_dim / 2]: by p * inv_freq[d]), d < rotary_dim / 2
+ * The angle is exact to 2^-52 of itself before it is reduced, and there is one
+ * rounding: q to bf16, k by the rule of aila_hip_kv_append_paged_fp8, which holds
+ * for the (unrounded) y here; v as there.
+ *   q        head h of token t at + t * q_stride + h * q_head_stride elements
+ *            (multiples of 8: the queries of a packed q|gate row have head stride
+ *            2 D); q_out [T, Hq, D] (may be q, where that is [T, Hq, D])
+ *   k, v     [Hkv, D] of token t at + t * k_stride, t * v_stride elements
+ *   slots    int[T], as aila_hip_kv_append_paged_fp8; -1: k and v are skipped
+ *   positions  p of each token, int[T] (NULL where rotary_dim is 0). With pos_h and
+ *            pos_w (int[T] each) pair d turns with pos_h if d % 3 == 1 and d / 3 <
+ *            section_h, with pos_w if d % 3 == 2 and d / 3 < section_w, else with
+ *            positions (the streams of aila_hip_rope_pos).
+ *   rotary_dim a multiple of 8 up to D; 0: no rotation. */
+int aila_hip_prepare_qkv_paged_fp8(const void* q, long q_stride,
+                                   long q_head_stride, const void* k,
+                                   long k_stride, const void* v, long v_stride,
+                                   void* q_out, const void* q_norm_w,
+                                   const void* k_norm_w, void* k_pages,
+                                   void* v_pages, float* k_scale,
+                                   float* v_scale, const int* slots,
+                                   const int* positions, const int* pos_h,
+                                   const int* pos_w, int section_h,
+                                   int section_w, int T, int Hq, int Hkv, int D,
+                                   int page_size, int num_pages, int rotary_dim,
+                                   float theta, const float* inv_freq, float eps,
+                                   void* stream);
+
+/* Attention of drafted trees: aila_hip_gqa_prefill_paged_fp8, but token
+ * query_start[b] + i, of n = query_start[b+1] - query_start[b], attends the rows
+ * [0, L - n) and of the drafted rows L - n + j those whose bit j is set in its mask;
+ * none: 0. L = min(seq_lens[b], max_len).
+ *   tree_mask  [T, mask_words] 64-bit words, 8-byte aligned; bit j % 64 of word j /
+ *              64. A token attends itself only if its own bit is set. mask_words <=
+ *              64. A request's tokens from the (64 * mask_words)-th on have no mask
+ *              and are not computed.
+ * Tokens from query_start[B] on are not touched. The softmax weights are rounded to
+ * bf16 (2^-8 of each at most) before they meet V. Sums are held in fp32, of weights
+ * of up to 2^8: the largest value that a block of V can hold (448 times its scale)
+ * times the rows attended has to stay below 2^120. Other arguments as
+ * aila_hip_gqa_prefill_paged_fp8.
+ * The workspace holds the records of the items whose keys are split: workspace_size
+ * bytes let as many workgroups work as the device holds, a smaller workspace fewer
+ * (2 records at least, else AILA_HIP_EWORKSPACE), and NULL none but one for each
+ * request, KV head and 256 query rows (D = 256: 128). Calls that may overlap in time
+ * need workspaces of their own. */
+size_t aila_hip_gqa_tree_paged_fp8_workspace_size(int T, int B, int Hq, int Hkv,
+                                                  int D, int max_len,
+                                                  int mask_words);
+int aila_hip_gqa_tree_paged_fp8(const void* q, long q_stride,
+                                const void* k_pages, const void* v_pages,
+                                const float* k_scale, const float* v_scale,
+                                void* out, void* workspace,
+                                size_t workspace_bytes, int T, int B, int Hq,
+                                int Hkv, int D, int page_size, int num_pages,
+                                const int* block_table, int max_pages,
+                                int max_len, const int* query_start,
+                                const int* seq_lens, const void* tree_mask,
+                                int mask_words, void* stream);
+
+/* Keep the accepted rows of drafts: row cached_lens[b] + kept[b * max_kept + i] of
+ * request b becomes row cached_lens[b] + i, for i < kept_lens[b], in `layers` caches
+ * at once (k_pages .. v_scale: host arrays of their device pointers; every cache has
+ * num_pages pages of one table).
+ *   cached_lens[b]  rows before the draft; negative: the request is absent
+ *   kept        int[B, max_kept], each request's drafted tokens that stay, rising
+ *               (entries past kept_lens[b] are not read as rows). max_kept <= 65536.
+ *   lens[B]     out: cached_lens[b] + kept_lens[b] (of at most max_kept, and within
+ *               the table); cached_lens[b] where that is negative. May not be the
+ *               array of cached_lens or kept_lens.
+ * Rows up to the first that moves stay untouched. A block of 16 rows that rows move
+ * into gets the largest of the scales that its rows come from: its own for rows
+ * before the first moved one, the source's for each moved row. Codes move as they
+ * are, or times the power of two between the scales: exact but for underflow. Rows
+ * behind lens[b] are not valid any more. A row whose index or page is out of range is
+ * left as it was. */
+int aila_hip_kv_keep_paged_fp8(void* const* k_pages, void* const* v_pages,
+                               float* const* k_scale, float* const* v_scale,
+                               int layers, const int* block_table,
+                               const int* cached_lens, const int* kept,
+                               const int* kept_lens, int* lens, int B,
+                               int max_kept, int Hkv, int D, int page_size,
+                               int num_pages, int max_pages, void* stream);
+
+/* Give back the pages behind each request's rows: the entries p >= lens[b] /
+ * page_size (rounded up) of row b of block_table that hold a page (>= 0) are pushed
+ * onto the stack in order of request and page and become -1. lens[b] < 0: the row is
+ * left alone. B <= 2048. Calls on one stack must not overlap in time. */
+int aila_hip_kv_pages_trim(const int* lens, int* block_table, int* free_pages,
+                           int* free_count, int B, int max_pages, int page_size,
+                           int num_pages, void* stream);
+
+/* Copy requests' rows, in `layers` caches at once (as aila_hip_kv_keep_paged_fp8):
+ * rows [0, min(lens[i], max_len)) of row src[i] of block_table to the pages of row
+ * dst[i], for i < n (<= 65535): a fork of a prompt, whose pages
+ * aila_hip_kv_pages_reserve has taken (cached_lens 0, new_lens the rows). Whole
+ * blocks of 16 rows are copied, codes and scales; rows behind them stay as they were.
+ * Pairs, rows and pages out of range are skipped. No row may be dst twice, nor src
+ * and dst of different pairs. */
+int aila_hip_kv_copy_paged_fp8(void* const* k_pages, void* const* v_pages,
+                               float* const* k_scale, float* const* v_scale,
+                               int layers, const int* block_table,
+                               const int* src, const int* dst, const int* lens,
+                               int n, int max_len, int B, int Hkv, int D,
+                               int page_size, int num_pages, int max_pages,
+                               void* stream);
+
 /* ----------------------------------------------------------- DeltaNet --- */
 
 /* One Gated DeltaNet decode step (the recurrence of
