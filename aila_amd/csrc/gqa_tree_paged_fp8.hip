@@ -16,13 +16,13 @@
 namespace aila {
 namespace {
 
-constexpr int kTiles = 2;              // column tiles of a wave
+constexpr int kWaves = 8;
+constexpr int kThreads = 64 * kWaves;
 constexpr int kMaxSequences = 4096;    // their unit counts live in LDS
 constexpr int kRecTail = 4;
 constexpr int kCus = 256;
-// D = 256: a wave's columns and strips take more than half of a SIMD's registers.
-template <int D> constexpr int kWavesOf = D == 256 ? 4 : 8;
-template <int D> constexpr int kCap = kWavesOf<D> * kTiles;   // column tiles of a workgroup
+template <int D> constexpr int kTiles = D == 256 ? 1 : 2;     // column tiles of a wave
+template <int D> constexpr int kCap = kWaves * kTiles<D>;     // column tiles of a workgroup
 template <int D> constexpr int kAccStride = D + 4;            // of a column in LDS, padded
 
 struct TreeArgs {
@@ -43,20 +43,28 @@ struct TreeArgs {
 };
 
 // What a request's columns are cut into. An item is up to kCap column tiles of a
-// KV head and all keys; its tiles are spread over `lanes` waves (a power of two),
-// and the workgroup's other waves take other keys, so that a unit - a strip of 32
-// keys for each wave - costs the same whatever the number of columns.
+// KV head and all keys; its tiles are spread over 1, 2, 4 or 8 lanes of waves, the
+// workgroup's other waves take other keys, so that a unit - a strip of 32 keys for
+// each wave - costs the same whatever the number of columns. Full items first; of
+// the rest, more than 3/4 of an item is one, else it is half an item and what is
+// left over, or less than that: of 9 tiles in 16 places 7 would idle.
 struct Shape {
   int q0, n, len;      // first token, tokens that are computed, rows
   int base;            // first drafted row
-  int tiles;           // column tiles of an item
-  int items;           // of a KV head
-  int lanes_log2;
-  int units;           // of an item
+  int full;            // items of kCap tiles (the last may be short of them)
+  int half, rest;      // tiles of the others, 0: there is none
 };
 
 template <int D>
-__device__ __forceinline__ int unit_rows(const Shape& s) { return (32 * kWavesOf<D>) >> s.lanes_log2; }
+__device__ __forceinline__ int lanes_log2(int tiles) {
+  const int lanes = (tiles + kTiles<D> - 1) / kTiles<D>;
+  return lanes <= 1 ? 0 : 32 - __builtin_clz(lanes - 1);
+}
+template <int D>
+__device__ __forceinline__ int item_units(int tiles, int len) {
+  const int rows = (32 * kWaves) >> lanes_log2<D>(tiles);
+  return max(1, (len + rows - 1) / rows);      // an output without keys is written too
+}
 
 template <int D>
 __device__ __forceinline__ Shape shape_of(const TreeArgs& a, int b) {
@@ -67,13 +75,57 @@ __device__ __forceinline__ Shape shape_of(const TreeArgs& a, int b) {
   s.base = s.len - s.n;
   s.n = min(s.n, 32 * a.words32);   // those behind have no mask
   const int all = (s.n * a.group + 15) / 16;
-  s.items = (all + kCap<D> - 1) / kCap<D>;
-  s.tiles = s.items > 0 ? (all + s.items - 1) / s.items : 0;
-  const int lanes = (s.tiles + kTiles - 1) / kTiles;
-  s.lanes_log2 = lanes <= 1 ? 0 : 32 - __builtin_clz(lanes - 1);
-  s.units = max(1, (s.len + unit_rows<D>(s) - 1) / unit_rows<D>(s));   // an output without keys is written too
+  s.full = all / kCap<D>;
+  s.rest = all % kCap<D>;
+  s.half = 0;
+  if (4 * s.rest > 3 * kCap<D>) {
+    ++s.full;
+    s.rest = 0;
+  } else if (2 * s.rest > kCap<D>) {
+    s.half = kCap<D> / 2;
+    s.rest -= s.half;
+  }
   return s;
 }
+// Units of a KV head.
+template <int D>
+__device__ __forceinline__ int head_units(const Shape& s) {
+  int n = s.full > 0 ? s.full * item_units<D>(kCap<D>, s.len) : 0;
+  if (s.half > 0) n += item_units<D>(s.half, s.len);
+  if (s.rest > 0) n += item_units<D>(s.rest, s.len);
+  return n;
+}
+
+// An item: its first tile, its tiles, its units and its KV head's units before it.
+struct Item { int tile0, tiles, units, before; };
+template <int D>
+__device__ __forceinline__ Item item_at(const Shape& s, int index) {
+  Item it;
+  const int u = item_units<D>(kCap<D>, s.len);
+  it.tile0 = min(index, s.full) * kCap<D>;
+  it.before = min(index, s.full) * u;
+  it.tiles = kCap<D>;
+  it.units = u;
+  if (index >= s.full) {
+    const bool second = s.half > 0 && index > s.full;
+    it.tiles = s.half > 0 && !second ? s.half : s.rest;
+    it.units = item_units<D>(it.tiles, s.len);
+    if (second) {
+      it.tile0 += s.half;
+      it.before += item_units<D>(s.half, s.len);
+    }
+  }
+  return it;
+}
+// The item that holds unit `at` of a KV head.
+template <int D>
+__device__ __forceinline__ Item item_of_unit(const Shape& s, int at) {
+  const int u = item_units<D>(kCap<D>, s.len);
+  int index = at / u;
+  if (index >= s.full) index = s.full + (s.half > 0 && at - s.full * u >= item_units<D>(s.half, s.len) ? 1 : 0);
+  return item_at<D>(s, index);
+}
+__device__ __forceinline__ int item_count(const Shape& s) { return s.full + (s.half > 0) + (s.rest > 0); }
 
 // s_pre[b] = units of a KV head of the requests before b, for b <= B.
 template <int D>
@@ -84,10 +136,7 @@ __device__ __forceinline__ void scan_units(const TreeArgs& a, int* s_pre) {
     for (int b0 = 0; b0 < a.B; b0 += 64) {
       const int b = b0 + lane;
       int n = 0;
-      if (b < a.B) {
-        const Shape s = shape_of<D>(a, b);
-        n = s.items * s.units;
-      }
+      if (b < a.B) n = head_units<D>(shape_of<D>(a, b));
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) {
         const int y = __shfl_up(n, off);
@@ -134,13 +183,46 @@ __device__ __forceinline__ uint32_t attended(const TreeArgs& a, size_t words_at,
   return left >= 32 ? keep : left > 0 ? keep & ((1u << left) - 1) : 0u;
 }
 
-// One strip of 32 keys into N column tiles. ka, kb: the K scales times log2(e) /
-// sqrt(D); ea, eb: the exponents of the V scales. masked: keep[t] holds the rows
-// that tile t's column of this lane attends.
-template <int D, int N>
-__device__ __forceinline__ void tree_step(Column<D>* c, Strip<D>& s, const bf16x8_t (*q)[D / 32], float ka, float kb, int ea,
-                                          int eb, bool masked, const uint32_t* keep, int g4) {
-  f32x4 sa[N], sb[N];
+// Codes of a strip of 32 keys, as Strip. K and V have registers of one strip each:
+// the next strip's K goes out when this one's scores are made, its V when this one's
+// products are.
+template <int D, bool V>
+__device__ __forceinline__ void load_codes(Strip<D>& s, const uint8_t* pages, int bid_a, int bid_b, int m16, int g4) {
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int bid = x ? bid_b : bid_a;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(pages) + static_cast<size_t>(max(bid, 0)) * (kScaleRows * D), 0, bid >= 0 ? kScaleRows * D : 0, kBufferRsrcWord3);
+    if constexpr (!V) {
+#pragma unroll
+      for (int kk = 0; kk < D / 64; ++kk) s.k[x][kk] = __builtin_amdgcn_raw_buffer_load_b128(r, m16 * D + 16 * g4 + 64 * kk, 0, 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = (4 * g4 + j) * D + m16 * (D / 16);
+        if constexpr (D == 256) {
+          const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s.v[4 * x + j][i] = w[i];
+        } else if constexpr (D == 128) {
+          const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0);
+          s.v[4 * x + j][0] = w[0];
+          s.v[4 * x + j][1] = w[1];
+        } else {
+          s.v[4 * x + j][0] = __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
+        }
+      }
+    }
+  }
+}
+
+// What a strip's blocks contribute: K scales times log2(e) / sqrt(D), exponents of
+// the V scales.
+struct Scales { float ka, kb; int ea, eb; };
+
+template <int D>
+__device__ __forceinline__ void make_scores(f32x4* sa, f32x4* sb, const Strip<D>& s, const bf16x8_t (*q)[D / 32]) {
+  constexpr int N = kTiles<D>;
 #pragma unroll
   for (int t = 0; t < N; ++t) sa[t] = sb[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -152,69 +234,81 @@ __device__ __forceinline__ void tree_step(Column<D>* c, Strip<D>& s, const bf16x
     for (int t = 0; t < N; ++t) {
       sa[t] = mfma16x16x32(alo, q[t][2 * kk], sa[t]);
       sb[t] = mfma16x16x32(blo, q[t][2 * kk], sb[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
       sa[t] = mfma16x16x32(ahi, q[t][2 * kk + 1], sa[t]);
       sb[t] = mfma16x16x32(bhi, q[t][2 * kk + 1], sb[t]);
     }
   }
-  // A masked row's weight is 0, but 0 times NaN is NaN, and a masked row may hold
-  // anything: a masked strip's NaN codes are taken out of V, and where there are any
-  // a second product counts those that each column attends, and puts the NaN back.
-  if (masked) {
+}
+
+// keep[t]: the rows that tile t's column of this lane attends.
+template <int D>
+__device__ __forceinline__ void mask_scores(f32x4* sa, f32x4* sb, const uint32_t* keep, int g4) {
 #pragma unroll
-    for (int t = 0; t < N; ++t) {
+  for (int t = 0; t < kTiles<D>; ++t) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (!(keep[t] >> (4 * g4 + j) & 1)) sa[t][j] = -INFINITY;
-        if (!(keep[t] >> (16 + 4 * g4 + j) & 1)) sb[t][j] = -INFINITY;
+    for (int j = 0; j < 4; ++j) {
+      if (!(keep[t] >> (4 * g4 + j) & 1)) sa[t][j] = -INFINITY;
+      if (!(keep[t] >> (16 + 4 * g4 + j) & 1)) sb[t][j] = -INFINITY;
+    }
+  }
+}
+
+// A masked row's weight is 0, but 0 times NaN is NaN, and a masked row may hold
+// anything: a masked strip's NaN codes are taken out of V, and where there are any
+// a second product counts those that each column attends, and puts the NaN back.
+template <int D>
+__device__ __forceinline__ void mend_values(Column<D>* c, Strip<D>& s, const uint32_t* keep, int g4) {
+  uint32_t seen = 0;
+#pragma unroll
+  for (int w = 0; w < D / 64; ++w) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) seen |= nan_codes(s.v[j][w]);
+  }
+  if (__ballot(seen != 0) == 0) return;
+#pragma unroll
+  for (int w = 0; w < D / 64; ++w) {
+    uint32_t one[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t n = nan_codes(s.v[j][w]) >> 7;
+      one[j] = n * 0x38u;      // the code of 1
+      s.v[j][w] &= ~(n * 0xffu);
+    }
+    bf16x8_t vt[4];
+    v_tiles(one, vt);
+#pragma unroll
+    for (int t = 0; t < kTiles<D>; ++t) {
+      u32x4 pa;   // 1 where the column attends the row
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t k = keep[t] >> ((e < 2 ? 0 : 16) + 4 * g4 + 2 * (e & 1));
+        pa[e] = (k & 1 ? 0x3f80u : 0u) | (k & 2 ? 0x3f800000u : 0u);
       }
-    }
-    uint32_t seen = 0;
 #pragma unroll
-    for (int w = 0; w < D / 64; ++w) {
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 n = mfma16x16x32(vt[i], as_bf16x8(pa), f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-      for (int j = 0; j < 8; ++j) seen |= nan_codes(s.v[j][w]);
-    }
-    if (__ballot(seen != 0)) {
-#pragma unroll
-      for (int w = 0; w < D / 64; ++w) {
-        uint32_t one[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t n = nan_codes(s.v[j][w]) >> 7;
-          one[j] = n * 0x38u;      // the code of 1
-          s.v[j][w] &= ~(n * 0xffu);
-        }
-        bf16x8_t vt[4];
-        v_tiles(one, vt);
-#pragma unroll
-        for (int t = 0; t < N; ++t) {
-          u32x4 pa;   // 1 where the column attends the row
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t k = keep[t] >> ((e < 2 ? 0 : 16) + 4 * g4 + 2 * (e & 1));
-            pa[e] = (k & 1 ? 0x3f80u : 0u) | (k & 2 ? 0x3f800000u : 0u);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const f32x4 n = mfma16x16x32(vt[i], as_bf16x8(pa), f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-            for (int j = 0; j < 4; ++j)   // n[j] is 0 or at least 1
-              c[t].acc[4 * w + i][j] = __uint_as_float(__float_as_uint(c[t].acc[4 * w + i][j]) |
-                                                       ((0u - min(__float_as_uint(n[j]), 1u)) & 0x7fc00000u));
-          }
-        }
+        for (int j = 0; j < 4; ++j)   // n[j] is 0 or at least 1
+          c[t].acc[4 * w + i][j] = __uint_as_float(__float_as_uint(c[t].acc[4 * w + i][j]) |
+                                                   ((0u - min(__float_as_uint(n[j]), 1u)) & 0x7fc00000u));
       }
     }
   }
-  // The V scales go into the exponents, and out of the weights' sums again. A weight
-  // is rounded to bf16 once (half a step, 2^-8 of it, at random); the sums are taken
-  // of the rounded ones, in fp32, so that they add up to 1.
-  u32x4 p[N];
+}
+
+// Scores to weights p. The V scales go into the exponents, and out of the weights'
+// sums again. A weight is rounded to bf16 once (half a step, 2^-8 of it, at random);
+// the sums are taken of the rounded ones, in fp32, so that they add up to 1.
+template <int D>
+__device__ __forceinline__ void make_weights(u32x4* p, Column<D>* c, const f32x4* sa, const f32x4* sb, const Scales& x) {
 #pragma unroll
-  for (int t = 0; t < N; ++t) {
+  for (int t = 0; t < kTiles<D>; ++t) {
     const float ta = fmaxf(fmaxf(sa[t][0], sa[t][1]), fmaxf(sa[t][2], sa[t][3]));
     const float tb = fmaxf(fmaxf(sb[t][0], sb[t][1]), fmaxf(sb[t][2], sb[t][3]));
-    const float top = xrow4_max(fmaxf(ta * ka, tb * kb));
+    const float top = xrow4_max(fmaxf(ta * x.ka, tb * x.kb));
     // the reference maximum moves only when a row exceeds it by 2^8
     if (__ballot(top > c[t].m + kLazyLog2)) {
       const float mn = fmaxf(c[t].m, top);
@@ -225,15 +319,19 @@ __device__ __forceinline__ void tree_step(Column<D>* c, Strip<D>& s, const bf16x
       for (int i = 0; i < D / 16; ++i) c[t].acc[i] *= alpha;
     }
     const float ref = c[t].m == -INFINITY ? 0.f : c[t].m;
-    const float ra = static_cast<float>(ea) - ref, rb = static_cast<float>(eb) - ref;
+    const float ra = static_cast<float>(x.ea) - ref, rb = static_cast<float>(x.eb) - ref;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      p[t][e] = pack_bf16x2(fast_exp2(fmaf(sa[t][2 * e], ka, ra)), fast_exp2(fmaf(sa[t][2 * e + 1], ka, ra)));
-      p[t][2 + e] = pack_bf16x2(fast_exp2(fmaf(sb[t][2 * e], kb, rb)), fast_exp2(fmaf(sb[t][2 * e + 1], kb, rb)));
+      p[t][e] = pack_bf16x2(fast_exp2(fmaf(sa[t][2 * e], x.ka, ra)), fast_exp2(fmaf(sa[t][2 * e + 1], x.ka, ra)));
+      p[t][2 + e] = pack_bf16x2(fast_exp2(fmaf(sb[t][2 * e], x.kb, rb)), fast_exp2(fmaf(sb[t][2 * e + 1], x.kb, rb)));
     }
-    c[t].l = fmaf(add_pair(p[t][1], add_pair(p[t][0], 0.f)), pow2f(-ea), c[t].l);
-    c[t].l = fmaf(add_pair(p[t][3], add_pair(p[t][2], 0.f)), pow2f(-eb), c[t].l);
+    c[t].l = fmaf(add_pair(p[t][1], add_pair(p[t][0], 0.f)), pow2f(-x.ea), c[t].l);
+    c[t].l = fmaf(add_pair(p[t][3], add_pair(p[t][2], 0.f)), pow2f(-x.eb), c[t].l);
   }
+}
+
+template <int D>
+__device__ __forceinline__ void add_values(Column<D>* c, const Strip<D>& s, const u32x4* p) {
 #pragma unroll
   for (int w = 0; w < D / 64; ++w) {
     uint32_t v[8];
@@ -244,18 +342,18 @@ __device__ __forceinline__ void tree_step(Column<D>* c, Strip<D>& s, const bf16x
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int t = 0; t < N; ++t) c[t].acc[4 * w + i] = mfma16x16x32(vt[i], as_bf16x8(p[t]), c[t].acc[4 * w + i]);
+      for (int t = 0; t < kTiles<D>; ++t) c[t].acc[4 * w + i] = mfma16x16x32(vt[i], as_bf16x8(p[t]), c[t].acc[4 * w + i]);
     }
   }
 }
 
 template <int D>
-__global__ __launch_bounds__(64 * kWavesOf<D>, 1) void gqa_tree_paged_fp8_kernel(PagedFp8 c, TreeArgs a) {
-  constexpr int kWaves = kWavesOf<D>, kThreads = 64 * kWaves, kStride = kAccStride<D>;
+__global__ __launch_bounds__(kThreads, 1) void gqa_tree_paged_fp8_kernel(PagedFp8 c, TreeArgs a) {
+  constexpr int kStride = kAccStride<D>, kT = kTiles<D>;
   extern __shared__ __attribute__((aligned(16))) unsigned char s_dyn[];
-  float* s_acc = reinterpret_cast<float*>(s_dyn);             // [kWaves][16 kTiles][kStride]
-  float* s_ml = s_acc + kWaves * 16 * kTiles * kStride;       // [kWaves][16 kTiles][2]
-  int* s_pre = reinterpret_cast<int*>(s_ml + kWaves * 16 * kTiles * 2);   // [B + 1]
+  float* s_acc = reinterpret_cast<float*>(s_dyn);             // [kWaves][16 kT][kStride]
+  float* s_ml = s_acc + kWaves * 16 * kT * kStride;           // [kWaves][16 kT][2]
+  int* s_pre = reinterpret_cast<int*>(s_ml + kWaves * 16 * kT * 2);   // [B + 1]
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m16 = lane & 15, g4 = lane >> 4;
@@ -275,43 +373,43 @@ __global__ __launch_bounds__(64 * kWavesOf<D>, 1) void gqa_tree_paged_fp8_kernel
     u1 = share_begin(w + 1, units, groups);
   }
   while (u < u1) {
-    int b, kvh, item, i0, i1;
+    int b, kvh, i0, i1;
     Shape s;
+    Item it;
     if (a.part == nullptr) {
       b = u / (c.Hkv * a.chunks);
       const int hi = u % (c.Hkv * a.chunks);
       kvh = hi / a.chunks;
-      item = hi % a.chunks;
       s = shape_of<D>(a, b);
-      if (item >= s.items) return;
+      if (hi % a.chunks >= item_count(s)) return;
+      it = item_at<D>(s, hi % a.chunks);
       i0 = 0;
-      i1 = s.units;
+      i1 = it.units;
       u = u1;
     } else {
       b = __builtin_amdgcn_readfirstlane(find_request(s_pre, a.B, u / c.Hkv));
       s = shape_of<D>(a, b);
-      const int at = __builtin_amdgcn_readfirstlane(u - s_pre[b] * c.Hkv);
-      const int hi = at / s.units;
-      i0 = at % s.units;
-      i1 = min(s.units, i0 + (u1 - u));
+      const int before = __builtin_amdgcn_readfirstlane(s_pre[b]), per = __builtin_amdgcn_readfirstlane(s_pre[b + 1]) - before;
+      const int at = u - before * c.Hkv;
+      kvh = at / per;
+      it = item_of_unit<D>(s, at - kvh * per);
+      i0 = at - kvh * per - it.before;
+      i1 = min(it.units, i0 + (u1 - u));
       u += i1 - i0;
-      kvh = hi / s.items;
-      item = hi % s.items;
     }
-    const int lanes = 1 << s.lanes_log2;
-    const int rows = unit_rows<D>(s);
-    const int tile0 = item * s.tiles;                                       // of the request's
-    const int cols = s.n * a.group;
-    const int tiles = min(s.tiles, (cols + 15) / 16 - tile0);
-    const int per = (s.tiles + lanes - 1) >> s.lanes_log2;                  // of a wave
+    const int lg = lanes_log2<D>(it.tiles);
+    const int lanes = 1 << lg, rows = (32 * kWaves) >> lg;                  // keys of a unit
+    const int cols = s.n * a.group;                                         // the request's
+    const int tiles = min(it.tiles, (cols + 15) / 16 - it.tile0);
+    const int per = (it.tiles + lanes - 1) >> lg;                           // of a wave
     const int mine = min(max(tiles - (wave & (lanes - 1)) * per, 0), per);
 
-    bf16x8_t q[kTiles][D / 32];
-    size_t words_at[kTiles];
-    Column<D> col[kTiles];
+    bf16x8_t q[kT][D / 32];
+    size_t words_at[kT];
+    Column<D> col[kT];
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      const int x = min(16 * (tile0 + (wave & (lanes - 1)) * per + t) + m16, cols - 1);   // past the last: its copies, not stored
+    for (int t = 0; t < kT; ++t) {
+      const int x = min(16 * (it.tile0 + (wave & (lanes - 1)) * per + t) + m16, cols - 1);   // past the last: its copies, not stored
       const int tok = x / a.group;
       const bf16* src = a.q + static_cast<size_t>(s.q0 + tok) * a.q_stride + static_cast<size_t>(kvh * a.group + x - tok * a.group) * D;
       words_at[t] = static_cast<size_t>(s.q0 + tok) * a.words32;
@@ -321,55 +419,74 @@ __global__ __launch_bounds__(64 * kWavesOf<D>, 1) void gqa_tree_paged_fp8_kernel
     }
 
     // strips of this wave: row0 + rows * n, n < ns
-    const int row0 = i0 * rows + 32 * (wave >> s.lanes_log2);
+    const int row0 = i0 * rows + 32 * (wave >> lg);
     const int end = min(i1 * rows, s.len);
     const int ns = mine > 0 && row0 < end ? (end - row0 + rows - 1) / rows : 0;
     const int blk_end = (end + kScaleRows - 1) / kScaleRows;
+    const int open = min(end, s.base);        // rows that every column attends
     for (int n0 = 0; n0 < ns; n0 += 32) {
       // lane l holds block l % 2 of strip n0 + l / 2
-      const BlockRef ref = block_ref(c, b, kvh, (row0 + (n0 + (lane >> 1)) * rows) / kScaleRows + (lane & 1), blk_end);
+      const int blk = (row0 + (n0 + (lane >> 1)) * rows) / kScaleRows + (lane & 1);
+      const BlockRef ref = block_ref(c, b, kvh, blk, blk_end);
       const int n1 = min(ns - n0, 32);
-      auto load = [&](Strip<D>& x, int n) __attribute__((always_inline)) {
-        const bool in = n < n1;
-        const int ba = __builtin_amdgcn_readlane(ref.bid, 2 * n & 63), bb = __builtin_amdgcn_readlane(ref.bid, (2 * n + 1) & 63);
-        load_strip<D, false>(x, c, in ? ba : -1, in ? bb : -1, m16, g4);
+      Strip<D> x;
+      auto bid = [&](int n, int i) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(ref.bid, (2 * n + i) & 63); };
+      auto load_k = [&](int n) __attribute__((always_inline)) {
+        load_codes<D, false>(x, c.k_pages, n < n1 ? bid(n, 0) : -1, n < n1 ? bid(n, 1) : -1, m16, g4);
       };
-      auto step = [&](Strip<D>& x, int n) __attribute__((always_inline)) {
-        const int ba = __builtin_amdgcn_readlane(ref.bid, 2 * n), bb = __builtin_amdgcn_readlane(ref.bid, 2 * n + 1);
+      auto load_v = [&](int n) __attribute__((always_inline)) {
+        load_codes<D, true>(x, c.v_pages, n < n1 ? bid(n, 0) : -1, n < n1 ? bid(n, 1) : -1, m16, g4);
+      };
+      auto scales = [&](int n) __attribute__((always_inline)) {
         // no page: all rows masked, and -inf times a scale of 0 would be NaN
-        const float ka = (ba >= 0 ? readlane_f(ref.ks, 2 * n) : 1.0f) * a.scale_log2;
-        const float kb = (bb >= 0 ? readlane_f(ref.ks, 2 * n + 1) : 1.0f) * a.scale_log2;
-        const int ea = held_exp(readlane_f(ref.vs, 2 * n)), eb = held_exp(readlane_f(ref.vs, 2 * n + 1));
-        const int row = row0 + (n0 + n) * rows;
-        const bool masked = row + 32 > min(end, s.base) || (ba | bb) < 0;
-        uint32_t keep[kTiles] = {};
-        if (masked) {
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t)
-            keep[t] = attended(a, words_at[t], row, s.base, end) & ((ba >= 0 ? 0xffffu : 0u) | (bb >= 0 ? 0xffff0000u : 0u));
-        }
-        if (mine == kTiles) tree_step<D, kTiles>(col, x, q, ka, kb, ea, eb, masked, keep, g4);
-        else tree_step<D, 1>(col, x, q, ka, kb, ea, eb, masked, keep, g4);
+        Scales r;
+        r.ka = (bid(n, 0) >= 0 ? readlane_f(ref.ks, 2 * n) : 1.0f) * a.scale_log2;
+        r.kb = (bid(n, 1) >= 0 ? readlane_f(ref.ks, 2 * n + 1) : 1.0f) * a.scale_log2;
+        r.ea = held_exp(readlane_f(ref.vs, 2 * n));
+        r.eb = held_exp(readlane_f(ref.vs, 2 * n + 1));
+        return r;
       };
-      Strip<D> x[2];
-      load(x[0], 0);
-      for (int n = 0; n < n1; n += 2) {
+      load_k(0);
+      load_v(0);
+      // the strips whose rows all columns attend, then the others
+      const bool hole = __ballot(blk < blk_end && ref.bid < 0) != 0;
+      const int plain = hole ? 0 : min(n1, max(0, open - row0 - n0 * rows + rows - 32) / rows);
+      f32x4 sa[kT], sb[kT];
+      u32x4 p[kT];
+      int n = 0;
+      for (; n < plain; ++n) {
+        make_scores<D>(sa, sb, x, q);
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(n + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        make_weights<D>(p, col, sa, sb, scales(n));
+        add_values<D>(col, x, p);
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(n + 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      for (; n < n1; ++n) {
+        make_scores<D>(sa, sb, x, q);
+        load_k(n + 1);
+        const int row = row0 + (n0 + n) * rows;
+        const uint32_t held = (bid(n, 0) >= 0 ? 0xffffu : 0u) | (bid(n, 1) >= 0 ? 0xffff0000u : 0u);
+        uint32_t keep[kT];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (n + i < n1) {
-            load(x[1 - i], n + i + 1);
-            step(x[i], n + i);
-          }
-        }
+        for (int t = 0; t < kT; ++t) keep[t] = attended(a, words_at[t], row, s.base, end) & held;
+        mask_scores<D>(sa, sb, keep, g4);
+        mend_values<D>(col, x, keep, g4);
+        make_weights<D>(p, col, sa, sb, scales(n));
+        add_values<D>(col, x, p);
+        load_v(n + 1);
       }
     }
 
     // ---- the waves' results meet ------------------------------------------
     __syncthreads();   // the item before has been read
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
+    for (int t = 0; t < kT; ++t) {
       const float l = xrow4_sum(col[t].l);
-      const int slot = (wave * kTiles + t) * 16 + m16;
+      const int slot = (wave * kT + t) * 16 + m16;
       float* row = s_acc + slot * kStride;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -382,15 +499,15 @@ __global__ __launch_bounds__(64 * kWavesOf<D>, 1) void gqa_tree_paged_fp8_kernel
       }
     }
     __syncthreads();
-    const bool whole = i0 == 0 && i1 == s.units;
+    const bool whole = i0 == 0 && i1 == it.units;
     float* rec = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (i0 == 0 ? 1 : 0)) * a.rec_cols * (D + kRecTail);
-    const int here = min(16 * tiles, cols - 16 * tile0);      // columns of the item
-    const int parts = kWaves >> s.lanes_log2;
+    const int here = min(16 * tiles, cols - 16 * it.tile0);      // columns of the item
+    const int parts = kWaves >> lg;
     for (int idx = threadIdx.x; idx < here * (D / 4); idx += kThreads) {
       const int x = idx / (D / 4), d = idx % (D / 4) * 4;
       const int tile = x >> 4, w0 = tile / per;
-      const int slot0 = (w0 * kTiles + tile - w0 * per) * 16 + (x & 15);
-      const int step = lanes * kTiles * 16;     // the same column, other keys
+      const int slot0 = (w0 * kT + tile - w0 * per) * 16 + (x & 15);
+      const int step = lanes * kT * 16;     // the same column, other keys
       float M = -INFINITY, L = 0.f;
       for (int i = 0; i < parts; ++i) M = fmaxf(M, s_ml[(slot0 + i * step) * 2]);
       f32x4 A = {0.f, 0.f, 0.f, 0.f};
@@ -402,7 +519,7 @@ __global__ __launch_bounds__(64 * kWavesOf<D>, 1) void gqa_tree_paged_fp8_kernel
         L += f * s_ml[slot * 2 + 1];
       }
       if (whole) {
-        const int y = 16 * tile0 + x, tok = y / a.group;
+        const int y = 16 * it.tile0 + x, tok = y / a.group;
         const float inv = L == 0.f ? 0.f : 1.0f / L;
         *reinterpret_cast<u32x2*>(a.out + (static_cast<size_t>(s.q0 + tok) * a.Hq + kvh * a.group + y - tok * a.group) * D + d) =
             u32x2{pack_bf16x2(A[0] * inv, A[1] * inv), pack_bf16x2(A[2] * inv, A[3] * inv)};
@@ -431,17 +548,18 @@ __global__ __launch_bounds__(kMergeThreads) void gqa_tree_paged_fp8_merge_kernel
   const Shape s = shape_of<D>(a, b);
   const int cols = s.n * a.group, x0 = static_cast<int>(blockIdx.z) * kMergeCols;
   if (x0 >= cols) return;
-  const int item = x0 / (16 * s.tiles);
+  const int index = min(x0 / (16 * kCap<D>), s.full);
+  const Item it = item_at<D>(s, index + (index == s.full && s.half > 0 && x0 >= 16 * (s.full * kCap<D> + s.half) ? 1 : 0));
   const int before = a.units[b], units = a.units[a.B] * c.Hkv, groups = min(launched, units);
-  const int first = before * c.Hkv + (kvh * s.items + item) * s.units;
+  const int first = before * c.Hkv + kvh * (a.units[b + 1] - before) + it.before;
   // workgroup w holds unit x: the largest w with w U / W < x + 1
   const int w0 = static_cast<int>((static_cast<long>(first + 1) * groups - 1) / units);
-  const int w1 = static_cast<int>((static_cast<long>(first + s.units) * groups - 1) / units);
+  const int w1 = static_cast<int>((static_cast<long>(first + it.units) * groups - 1) / units);
   if (w0 == w1) return;   // one workgroup wrote the output
   const int d = static_cast<int>(threadIdx.x) % kQuads * 4, x = static_cast<int>(threadIdx.x) / kQuads % kMergeCols;
   const int ph = static_cast<int>(threadIdx.x) / (kQuads * kMergeCols);
   const int y = min(x0 + x, cols - 1);
-  const float* at = a.part + static_cast<size_t>(y - 16 * s.tiles * item) * (D + kRecTail);
+  const float* at = a.part + static_cast<size_t>(y - 16 * it.tile0) * (D + kRecTail);
   const size_t step = static_cast<size_t>(a.rec_cols) * (D + kRecTail);
   f32x4 A = {0.f, 0.f, 0.f, 0.f};
   float M = -INFINITY, L = 0.f;
@@ -488,7 +606,7 @@ Most most_of(int T, int words, int group) {
   Most m;
   m.cols = static_cast<long>(std::min<long>(T, 64L * words)) * group;
   const long tiles = (m.cols + 15) / 16;
-  m.items = static_cast<int>((tiles + kCap<D> - 1) / kCap<D>);
+  m.items = static_cast<int>(tiles / kCap<D> + 2);    // of the rest, two at most
   m.rec_cols = static_cast<int>(16 * std::min<long>(tiles, kCap<D>));
   return m;
 }
@@ -516,7 +634,6 @@ int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t wor
   const Most m = most_of<D>(a.T, words, a.group);
   a.chunks = m.items;
   a.rec_cols = m.rec_cols;
-  constexpr int kThreads = 64 * kWavesOf<D>;
   const long items = static_cast<long>(a.B) * c.Hkv * m.items;
   AILA_REQUIRE(items * most_units(a.max_len) < (1L << 31) && items * kThreads < (1L << 32),
                "gqa_tree_paged_fp8: B=%d requests of up to %ld query rows and %d keys are too many", a.B, m.cols, a.max_len);
@@ -532,7 +649,7 @@ int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t wor
     a.units = static_cast<int*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + units_bytes(a.B));
   }
-  const size_t lds = static_cast<size_t>(kWavesOf<D>) * 16 * kTiles * (kAccStride<D> + 2) * sizeof(float) +
+  const size_t lds = static_cast<size_t>(kWaves) * 16 * kTiles<D> * (kAccStride<D> + 2) * sizeof(float) +
                      (a.part ? static_cast<size_t>(a.B + 1) * sizeof(int) : 0);
   hipLaunchKernelGGL((gqa_tree_paged_fp8_kernel<D>), dim3(groups), dim3(kThreads), lds, st, c, a);
   if (a.part)
