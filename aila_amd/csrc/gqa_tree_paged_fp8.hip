@@ -4,11 +4,16 @@
 //
 // over the rows j < L - n before a request's n drafted tokens, and the drafted
 // rows whose bit is set in token i's mask. The query rows of a KV head are its
-// columns: (token, head) pairs, token-major, in tiles of 16, the columns of the
-// matrix instructions (v_mfma_f32_16x16x32_bf16, products and lane layout as
-// Strip in paged_fp8.hpp). Codes go from memory to registers, are converted to
-// bf16 there (exact, unscaled: the scales are powers of two and go into the
-// softmax's exponents) and serve every tile of the wave.
+// columns: (token, head) pairs, token-major, in tiles of 32, one a wave. Products on
+// v_mfma_f32_32x32x16_bf16, a strip of 32 keys at a time:
+//   S^T = K Q^T     A = 32 keys, B = the wave's 32 columns
+//     lane (m, h) = (l % 32, l / 32) loads 16 codes of key m at 32 kk + 16 h, two
+//     operands of 8 dims; it receives keys 8 a + 4 h + c (a, c < 4) of column m.
+//   O^T += V^T P^T  A = 32 head dims, B = P of 16 keys, in the registers where S^T
+//     left it: step s takes keys 16 s + 4 h + {0..3, 8..11}. A lane loads those
+//     rows' dims [D/32 m, D/32 (m + 1)) and pairs the rows' bytes with v_perm.
+// Codes go from memory to registers and are converted to bf16 there (exact,
+// unscaled: the scales are powers of two and go into the softmax's exponents).
 #include "paged_fp8.hpp"
 
 #include <algorithm>
@@ -16,13 +21,12 @@
 namespace aila {
 namespace {
 
-constexpr int kWaves = 8;
-constexpr int kThreads = 64 * kWaves;
+constexpr int kTile = 32;              // columns of a wave
 constexpr int kMaxSequences = 4096;    // their unit counts live in LDS
 constexpr int kRecTail = 4;
 constexpr int kCus = 256;
-template <int D> constexpr int kTiles = D == 256 ? 1 : 2;     // column tiles of a wave
-template <int D> constexpr int kCap = kWaves * kTiles<D>;     // column tiles of a workgroup
+// D = 256: a wave's columns take more than half of a SIMD's registers.
+template <int D> constexpr int kWaves = D == 256 ? 4 : 8;     // and column tiles of a workgroup
 template <int D> constexpr int kAccStride = D + 4;            // of a column in LDS, padded
 
 struct TreeArgs {
@@ -42,27 +46,23 @@ struct TreeArgs {
   float scale_log2;
 };
 
-// What a request's columns are cut into. An item is up to kCap column tiles of a
-// KV head and all keys; its tiles are spread over 1, 2, 4 or 8 lanes of waves, the
-// workgroup's other waves take other keys, so that a unit - a strip of 32 keys for
+// What a request's columns are cut into. An item is up to kWaves column tiles of a
+// KV head and all keys, a wave for each tile; the workgroup's other waves take other
+// keys (a power of two each), so that a unit - a strip of 32 keys for
 // each wave - costs the same whatever the number of columns. Full items first; of
 // the rest, more than 3/4 of an item is one, else it is half an item and what is
-// left over, or less than that: of 9 tiles in 16 places 7 would idle.
+// left over, or less than that: of 5 tiles in 8 places 3 would idle.
 struct Shape {
   int q0, n, len;      // first token, tokens that are computed, rows
   int base;            // first drafted row
-  int full;            // items of kCap tiles (the last may be short of them)
+  int full;            // items of kWaves tiles (the last may be short of them)
   int half, rest;      // tiles of the others, 0: there is none
 };
 
-template <int D>
-__device__ __forceinline__ int lanes_log2(int tiles) {
-  const int lanes = (tiles + kTiles<D> - 1) / kTiles<D>;
-  return lanes <= 1 ? 0 : 32 - __builtin_clz(lanes - 1);
-}
+__device__ __forceinline__ int lanes_log2(int tiles) { return tiles <= 1 ? 0 : 32 - __builtin_clz(tiles - 1); }
 template <int D>
 __device__ __forceinline__ int item_units(int tiles, int len) {
-  const int rows = (32 * kWaves) >> lanes_log2<D>(tiles);
+  const int rows = (32 * kWaves<D>) >> lanes_log2(tiles);
   return max(1, (len + rows - 1) / rows);      // an output without keys is written too
 }
 
@@ -74,15 +74,15 @@ __device__ __forceinline__ Shape shape_of(const TreeArgs& a, int b) {
   s.len = min(max(a.seq_lens[b], 0), a.max_len);
   s.base = s.len - s.n;
   s.n = min(s.n, 32 * a.words32);   // those behind have no mask
-  const int all = (s.n * a.group + 15) / 16;
-  s.full = all / kCap<D>;
-  s.rest = all % kCap<D>;
+  const int all = (s.n * a.group + kTile - 1) / kTile;
+  s.full = all / kWaves<D>;
+  s.rest = all % kWaves<D>;
   s.half = 0;
-  if (4 * s.rest > 3 * kCap<D>) {
+  if (4 * s.rest > 3 * kWaves<D>) {
     ++s.full;
     s.rest = 0;
-  } else if (2 * s.rest > kCap<D>) {
-    s.half = kCap<D> / 2;
+  } else if (2 * s.rest > kWaves<D>) {
+    s.half = kWaves<D> / 2;
     s.rest -= s.half;
   }
   return s;
@@ -90,7 +90,7 @@ __device__ __forceinline__ Shape shape_of(const TreeArgs& a, int b) {
 // Units of a KV head.
 template <int D>
 __device__ __forceinline__ int head_units(const Shape& s) {
-  int n = s.full > 0 ? s.full * item_units<D>(kCap<D>, s.len) : 0;
+  int n = s.full > 0 ? s.full * item_units<D>(kWaves<D>, s.len) : 0;
   if (s.half > 0) n += item_units<D>(s.half, s.len);
   if (s.rest > 0) n += item_units<D>(s.rest, s.len);
   return n;
@@ -101,10 +101,10 @@ struct Item { int tile0, tiles, units, before; };
 template <int D>
 __device__ __forceinline__ Item item_at(const Shape& s, int index) {
   Item it;
-  const int u = item_units<D>(kCap<D>, s.len);
-  it.tile0 = min(index, s.full) * kCap<D>;
+  const int u = item_units<D>(kWaves<D>, s.len);
+  it.tile0 = min(index, s.full) * kWaves<D>;
   it.before = min(index, s.full) * u;
-  it.tiles = kCap<D>;
+  it.tiles = kWaves<D>;
   it.units = u;
   if (index >= s.full) {
     const bool second = s.half > 0 && index > s.full;
@@ -120,7 +120,7 @@ __device__ __forceinline__ Item item_at(const Shape& s, int index) {
 // The item that holds unit `at` of a KV head.
 template <int D>
 __device__ __forceinline__ Item item_of_unit(const Shape& s, int at) {
-  const int u = item_units<D>(kCap<D>, s.len);
+  const int u = item_units<D>(kWaves<D>, s.len);
   int index = at / u;
   if (index >= s.full) index = s.full + (s.half > 0 && at - s.full * u >= item_units<D>(s.half, s.len) ? 1 : 0);
   return item_at<D>(s, index);
@@ -172,10 +172,10 @@ __device__ __forceinline__ float add_pair(uint32_t x, float acc) {
 
 // The rows [row, row + 32) that a token attends, as bits: those before the draft
 // (row < base), the drafted ones by its mask words, none from len on.
-__device__ __forceinline__ uint32_t attended(const TreeArgs& a, size_t words_at, int row, int base, int len) {
+__device__ __forceinline__ uint32_t attended(const TreeArgs& a, const uint32_t* words, int row, int base, int len) {
   const int o = row - base, i = o >> 5, sh = o & 31;
   auto word = [&](int w) __attribute__((always_inline)) -> uint32_t {
-    return w < 0 ? ~0u : w < a.words32 ? a.mask[words_at + w] : 0u;
+    return w < 0 ? ~0u : w < a.words32 ? words[w] : 0u;
   };
   const uint64_t both = static_cast<uint64_t>(word(i + 1)) << 32 | word(i);
   const uint32_t keep = static_cast<uint32_t>(both >> sh);
@@ -183,180 +183,227 @@ __device__ __forceinline__ uint32_t attended(const TreeArgs& a, size_t words_at,
   return left >= 32 ? keep : left > 0 ? keep & ((1u << left) - 1) : 0u;
 }
 
-// Codes of a strip of 32 keys, as Strip. K and V have registers of one strip each:
-// the next strip's K goes out when this one's scores are made, its V when this one's
-// products are.
-template <int D, bool V>
-__device__ __forceinline__ void load_codes(Strip<D>& s, const uint8_t* pages, int bid_a, int bid_b, int m16, int g4) {
+__device__ __forceinline__ f32x16 mfma32(const bf16x8_t& a, const bf16x8_t& b, const f32x16& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// Max / sum over lanes l and l ^ 32.
+__device__ __forceinline__ float half_max(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// Codes of a strip's K and V, one strip's registers each: the next strip's K goes
+// out when this one's scores are made, its V when this one's products are. A block
+// without a page is read as block 0: all its rows are masked.
+template <int D>
+struct Codes {
+  u32x4 k[D / 32];
+  static constexpr int VW = D == 256 ? 2 : 1;       // words of a row's run of dims
+  uint32_t v[2][VW][8];                             // [step][word][row]
+};
+
+template <int D>
+__device__ __forceinline__ void load_k(Codes<D>& x, const uint8_t* pages, int bid_a, int bid_b, int m32, int hf) {
+  const uint32_t bid = static_cast<uint32_t>(max(m32 < 16 ? bid_a : bid_b, 0));
+  const uint8_t* p = pages + static_cast<size_t>(bid) * (kScaleRows * D) + ((m32 & 15) * D + 16 * hf);
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int bid = x ? bid_b : bid_a;
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(pages) + static_cast<size_t>(max(bid, 0)) * (kScaleRows * D), 0, bid >= 0 ? kScaleRows * D : 0, kBufferRsrcWord3);
-    if constexpr (!V) {
+  for (int kk = 0; kk < D / 32; ++kk) x.k[kk] = ld16(p + 32 * kk);
+}
+
+template <int D>
+__device__ __forceinline__ void load_v(Codes<D>& x, const uint8_t* pages, int bid_a, int bid_b, int m32, int hf) {
+  const uint32_t at = 4 * hf * D + (D == 64 ? 4 * (m32 & 15) : m32 * (D / 32));
 #pragma unroll
-      for (int kk = 0; kk < D / 64; ++kk) s.k[x][kk] = __builtin_amdgcn_raw_buffer_load_b128(r, m16 * D + 16 * g4 + 64 * kk, 0, 0);
-    } else {
+  for (int s = 0; s < 2; ++s) {
+    const uint8_t* p = pages + static_cast<size_t>(static_cast<uint32_t>(max(s ? bid_b : bid_a, 0))) * (kScaleRows * D);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int at = (4 * g4 + j) * D + m16 * (D / 16);
-        if constexpr (D == 256) {
-          const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s.v[4 * x + j][i] = w[i];
-        } else if constexpr (D == 128) {
-          const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0);
-          s.v[4 * x + j][0] = w[0];
-          s.v[4 * x + j][1] = w[1];
-        } else {
-          s.v[4 * x + j][0] = __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
-        }
+    for (int j = 0; j < 8; ++j) {
+      const uint8_t* r = p + at + ((j & 3) + 8 * (j >> 2)) * D;
+      if constexpr (D == 256) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(r);
+        x.v[s][0][j] = w[0];
+        x.v[s][1][j] = w[1];
+      } else {
+        x.v[s][0][j] = *reinterpret_cast<const uint32_t*>(r);
       }
     }
   }
 }
+
+// Head dim of row m of output part dt.
+template <int D>
+__device__ __forceinline__ int out_dim(int dt, int m) {
+  return D == 64 ? 4 * (m & 15) + 2 * dt + (m >> 4) : (D / 32) * m + dt;
+}
+
+// V operands of a step from a word of each of its 8 rows: 4 parts, D = 64: both
+// (the lanes of rows 16 .. 31 take the odd bytes).
+template <int D>
+__device__ __forceinline__ void step_tiles(const uint32_t (&v)[8], bf16x8_t* t, int m32) {
+  if constexpr (D == 64) {
+    const uint32_t sel = m32 < 16 ? 0x06020400u : 0x07030501u;
+    u32x4 o[2];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t w = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], sel);
+      o[0][e] = fp8x2_to_bf16x2<false>(w);
+      o[1][e] = fp8x2_to_bf16x2<true>(w);
+    }
+    t[0] = as_bf16x8(o[0]);
+    t[1] = as_bf16x8(o[1]);
+  } else {
+    bf16x8_t x[4];
+    v_tiles(v, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = x[i];
+  }
+}
+
+// A column's running softmax and its output: o[dt][i] is head dim out_dim(dt, 8 (i /
+// 4) + 4 h + i % 4).
+template <int D>
+struct Tile {
+  f32x16 o[D / 32];
+  float m, l;          // maximum (log2 domain) and this lane's part of the sum
+};
 
 // What a strip's blocks contribute: K scales times log2(e) / sqrt(D), exponents of
 // the V scales.
 struct Scales { float ka, kb; int ea, eb; };
 
 template <int D>
-__device__ __forceinline__ void make_scores(f32x4* sa, f32x4* sb, const Strip<D>& s, const bf16x8_t (*q)[D / 32]) {
-  constexpr int N = kTiles<D>;
+__device__ __forceinline__ f32x16 make_scores(const Codes<D>& x, const bf16x8_t (&q)[D / 16]) {
+  f32x16 sc = {};
 #pragma unroll
-  for (int t = 0; t < N; ++t) sa[t] = sb[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int kk = 0; kk < D / 64; ++kk) {
-    bf16x8_t alo, ahi, blo, bhi;
-    fp8x16_to_bf16(s.k[0][kk], alo, ahi);
-    fp8x16_to_bf16(s.k[1][kk], blo, bhi);
-#pragma unroll
-    for (int t = 0; t < N; ++t) {
-      sa[t] = mfma16x16x32(alo, q[t][2 * kk], sa[t]);
-      sb[t] = mfma16x16x32(blo, q[t][2 * kk], sb[t]);
-    }
-#pragma unroll
-    for (int t = 0; t < N; ++t) {
-      sa[t] = mfma16x16x32(ahi, q[t][2 * kk + 1], sa[t]);
-      sb[t] = mfma16x16x32(bhi, q[t][2 * kk + 1], sb[t]);
-    }
+  for (int kk = 0; kk < D / 32; ++kk) {
+    bf16x8_t lo, hi;
+    fp8x16_to_bf16(x.k[kk], lo, hi);
+    sc = mfma32(lo, q[2 * kk], sc);
+    sc = mfma32(hi, q[2 * kk + 1], sc);
   }
+  return sc;
 }
 
-// keep[t]: the rows that tile t's column of this lane attends.
-template <int D>
-__device__ __forceinline__ void mask_scores(f32x4* sa, f32x4* sb, const uint32_t* keep, int g4) {
+// keep: the rows that this lane's column attends, from row 4 h on.
+__device__ __forceinline__ void mask_scores(f32x16& sc, uint32_t keep) {
 #pragma unroll
-  for (int t = 0; t < kTiles<D>; ++t) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (!(keep[t] >> (4 * g4 + j) & 1)) sa[t][j] = -INFINITY;
-      if (!(keep[t] >> (16 + 4 * g4 + j) & 1)) sb[t][j] = -INFINITY;
-    }
-  }
+  for (int i = 0; i < 16; ++i)
+    if (!(keep >> (8 * (i >> 2) + (i & 3)) & 1)) sc[i] = -INFINITY;
 }
 
 // A masked row's weight is 0, but 0 times NaN is NaN, and a masked row may hold
 // anything: a masked strip's NaN codes are taken out of V, and where there are any
 // a second product counts those that each column attends, and puts the NaN back.
 template <int D>
-__device__ __forceinline__ void mend_values(Column<D>* c, Strip<D>& s, const uint32_t* keep, int g4) {
+__device__ __forceinline__ void mend_values(Tile<D>& c, Codes<D>& x, uint32_t keep, int m32) {
   uint32_t seen = 0;
 #pragma unroll
-  for (int w = 0; w < D / 64; ++w) {
+  for (int s = 0; s < 2; ++s) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) seen |= nan_codes(s.v[j][w]);
+    for (int w = 0; w < Codes<D>::VW; ++w) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) seen |= nan_codes(x.v[s][w][j]);
+    }
   }
   if (__ballot(seen != 0) == 0) return;
 #pragma unroll
-  for (int w = 0; w < D / 64; ++w) {
-    uint32_t one[8];
+  for (int w = 0; w < Codes<D>::VW; ++w) {
+    f32x16 count[4] = {};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t n = nan_codes(s.v[j][w]) >> 7;
-      one[j] = n * 0x38u;      // the code of 1
-      s.v[j][w] &= ~(n * 0xffu);
-    }
-    bf16x8_t vt[4];
-    v_tiles(one, vt);
+    for (int s = 0; s < 2; ++s) {
+      uint32_t one[8];
 #pragma unroll
-    for (int t = 0; t < kTiles<D>; ++t) {
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t n = nan_codes(x.v[s][w][j]) >> 7;
+        one[j] = n * 0x38u;      // the code of 1
+        x.v[s][w][j] &= ~(n * 0xffu);
+      }
       u32x4 pa;   // 1 where the column attends the row
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t k = keep[t] >> ((e < 2 ? 0 : 16) + 4 * g4 + 2 * (e & 1));
+        const uint32_t k = keep >> (16 * s + 8 * (e >> 1) + 2 * (e & 1));
         pa[e] = (k & 1 ? 0x3f80u : 0u) | (k & 2 ? 0x3f800000u : 0u);
       }
+      bf16x8_t vt[4];
+      step_tiles<D>(one, vt, m32);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 n = mfma16x16x32(vt[i], as_bf16x8(pa), f32x4{0.f, 0.f, 0.f, 0.f});
+      for (int i = 0; i < (D == 64 ? 2 : 4); ++i) count[i] = mfma32(vt[i], as_bf16x8(pa), count[i]);
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)   // n[j] is 0 or at least 1
-          c[t].acc[4 * w + i][j] = __uint_as_float(__float_as_uint(c[t].acc[4 * w + i][j]) |
-                                                   ((0u - min(__float_as_uint(n[j]), 1u)) & 0x7fc00000u));
-      }
+    for (int i = 0; i < (D == 64 ? 2 : 4); ++i) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)   // count is 0 or at least 1
+        c.o[4 * w + i][j] = __uint_as_float(__float_as_uint(c.o[4 * w + i][j]) |
+                                            ((0u - min(__float_as_uint(count[i][j]), 1u)) & 0x7fc00000u));
     }
   }
 }
 
-// Scores to weights p. The V scales go into the exponents, and out of the weights'
-// sums again. A weight is rounded to bf16 once (half a step, 2^-8 of it, at random);
-// the sums are taken of the rounded ones, in fp32, so that they add up to 1.
+// Scores to weights p[step]. The V scales go into the exponents, and out of the
+// weights' sums again. A weight is rounded to bf16 once (half a step, 2^-8 of it, at
+// random); the sums are taken of the rounded ones, in fp32, so that they add up to 1.
 template <int D>
-__device__ __forceinline__ void make_weights(u32x4* p, Column<D>* c, const f32x4* sa, const f32x4* sb, const Scales& x) {
+__device__ __forceinline__ void make_weights(u32x4 (&p)[2], Tile<D>& c, const f32x16& sc, const Scales& x) {
+  float ta = sc[0], tb = sc[8];
 #pragma unroll
-  for (int t = 0; t < kTiles<D>; ++t) {
-    const float ta = fmaxf(fmaxf(sa[t][0], sa[t][1]), fmaxf(sa[t][2], sa[t][3]));
-    const float tb = fmaxf(fmaxf(sb[t][0], sb[t][1]), fmaxf(sb[t][2], sb[t][3]));
-    const float top = xrow4_max(fmaxf(ta * x.ka, tb * x.kb));
-    // the reference maximum moves only when a row exceeds it by 2^8
-    if (__ballot(top > c[t].m + kLazyLog2)) {
-      const float mn = fmaxf(c[t].m, top);
-      const float alpha = c[t].m == -INFINITY ? 0.f : fast_exp2(c[t].m - mn);
-      c[t].m = mn;
-      c[t].l *= alpha;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) c[t].acc[i] *= alpha;
-    }
-    const float ref = c[t].m == -INFINITY ? 0.f : c[t].m;
-    const float ra = static_cast<float>(x.ea) - ref, rb = static_cast<float>(x.eb) - ref;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      p[t][e] = pack_bf16x2(fast_exp2(fmaf(sa[t][2 * e], x.ka, ra)), fast_exp2(fmaf(sa[t][2 * e + 1], x.ka, ra)));
-      p[t][2 + e] = pack_bf16x2(fast_exp2(fmaf(sb[t][2 * e], x.kb, rb)), fast_exp2(fmaf(sb[t][2 * e + 1], x.kb, rb)));
-    }
-    c[t].l = fmaf(add_pair(p[t][1], add_pair(p[t][0], 0.f)), pow2f(-x.ea), c[t].l);
-    c[t].l = fmaf(add_pair(p[t][3], add_pair(p[t][2], 0.f)), pow2f(-x.eb), c[t].l);
+  for (int i = 1; i < 8; ++i) {
+    ta = fmaxf(ta, sc[i]);
+    tb = fmaxf(tb, sc[8 + i]);
   }
-}
-
-template <int D>
-__device__ __forceinline__ void add_values(Column<D>* c, const Strip<D>& s, const u32x4* p) {
+  const float top = half_max(fmaxf(ta * x.ka, tb * x.kb));
+  // the reference maximum moves only when a row exceeds it by 2^8
+  if (__ballot(top > c.m + kLazyLog2)) {
+    const float mn = fmaxf(c.m, top);
+    const float alpha = c.m == -INFINITY ? 0.f : fast_exp2(c.m - mn);
+    c.m = mn;
+    c.l *= alpha;
 #pragma unroll
-  for (int w = 0; w < D / 64; ++w) {
-    uint32_t v[8];
+    for (int i = 0; i < D / 32; ++i) c.o[i] *= alpha;
+  }
+  const float ref = c.m == -INFINITY ? 0.f : c.m;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = s.v[j][w];
-    bf16x8_t vt[4];
-    v_tiles(v, vt);
+  for (int s = 0; s < 2; ++s) {
+    const int e = s ? x.eb : x.ea;
+    const float k = s ? x.kb : x.ka, r = static_cast<float>(e) - ref;
+    float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      p[s][i] = pack_bf16x2(fast_exp2(fmaf(sc[8 * s + 2 * i], k, r)), fast_exp2(fmaf(sc[8 * s + 2 * i + 1], k, r)));
+      sum = add_pair(p[s][i], sum);
+    }
+    c.l = fmaf(sum, pow2f(-e), c.l);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void add_values(Tile<D>& c, const Codes<D>& x, const u32x4 (&p)[2], int m32) {
 #pragma unroll
-      for (int t = 0; t < kTiles<D>; ++t) c[t].acc[4 * w + i] = mfma16x16x32(vt[i], as_bf16x8(p[t]), c[t].acc[4 * w + i]);
+  for (int s = 0; s < 2; ++s) {
+#pragma unroll
+    for (int w = 0; w < Codes<D>::VW; ++w) {
+      bf16x8_t vt[4];
+      step_tiles<D>(x.v[s][w], vt, m32);
+#pragma unroll
+      for (int i = 0; i < (D == 64 ? 2 : 4); ++i) c.o[4 * w + i] = mfma32(vt[i], as_bf16x8(p[s]), c.o[4 * w + i]);
     }
   }
 }
 
 template <int D>
-__global__ __launch_bounds__(kThreads, 1) void gqa_tree_paged_fp8_kernel(PagedFp8 c, TreeArgs a) {
-  constexpr int kStride = kAccStride<D>, kT = kTiles<D>;
+__global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(PagedFp8 c, TreeArgs a) {
+  constexpr int kStride = kAccStride<D>, kThreads = 64 * kWaves<D>;
   extern __shared__ __attribute__((aligned(16))) unsigned char s_dyn[];
-  float* s_acc = reinterpret_cast<float*>(s_dyn);             // [kWaves][16 kT][kStride]
-  float* s_ml = s_acc + kWaves * 16 * kT * kStride;           // [kWaves][16 kT][2]
-  int* s_pre = reinterpret_cast<int*>(s_ml + kWaves * 16 * kT * 2);   // [B + 1]
+  float* s_acc = reinterpret_cast<float*>(s_dyn);             // [kWaves][kTile][kStride]
+  float* s_ml = s_acc + kWaves<D> * kTile * kStride;          // [kWaves][kTile][2]
+  int* s_pre = reinterpret_cast<int*>(s_ml + kWaves<D> * kTile * 2);   // [B + 1]
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m16 = lane & 15, g4 = lane >> 4;
+  const int m32 = lane & 31, hf = lane >> 5;
 
   int u, u1;
   if (a.part == nullptr) {
@@ -397,31 +444,31 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_tree_paged_fp8_kernel(PagedFp
       i1 = min(it.units, i0 + (u1 - u));
       u += i1 - i0;
     }
-    const int lg = lanes_log2<D>(it.tiles);
-    const int lanes = 1 << lg, rows = (32 * kWaves) >> lg;                  // keys of a unit
+    const int lg = lanes_log2(it.tiles);
+    const int lanes = 1 << lg, rows = (32 * kWaves<D>) >> lg;               // keys of a unit
     const int cols = s.n * a.group;                                         // the request's
-    const int tiles = min(it.tiles, (cols + 15) / 16 - it.tile0);
-    const int per = (it.tiles + lanes - 1) >> lg;                           // of a wave
-    const int mine = min(max(tiles - (wave & (lanes - 1)) * per, 0), per);
+    const int tile = it.tile0 + (wave & (lanes - 1));
+    const bool mine = (wave & (lanes - 1)) < it.tiles && tile * kTile < cols;
 
-    bf16x8_t q[kT][D / 32];
-    size_t words_at[kT];
-    Column<D> col[kT];
+    // this lane's column; past the last: its copy, not stored
+    const int y0 = min(tile * kTile + m32, cols - 1), tok0 = y0 / a.group;
+    const uint32_t* words = a.mask + static_cast<size_t>(s.q0 + tok0) * a.words32;
+    bf16x8_t q[D / 16];
+    {
+      const bf16* src = a.q + static_cast<size_t>(s.q0 + tok0) * a.q_stride + static_cast<size_t>(kvh * a.group + y0 - tok0 * a.group) * D + 16 * hf;
 #pragma unroll
-    for (int t = 0; t < kT; ++t) {
-      const int x = min(16 * (it.tile0 + (wave & (lanes - 1)) * per + t) + m16, cols - 1);   // past the last: its copies, not stored
-      const int tok = x / a.group;
-      const bf16* src = a.q + static_cast<size_t>(s.q0 + tok) * a.q_stride + static_cast<size_t>(kvh * a.group + x - tok * a.group) * D;
-      words_at[t] = static_cast<size_t>(s.q0 + tok) * a.words32;
-#pragma unroll
-      for (int ks = 0; ks < D / 32; ++ks) q[t][ks] = as_bf16x8(ld16(src + 64 * (ks >> 1) + 16 * g4 + 8 * (ks & 1)));
-      clear_column(col[t]);
+      for (int i = 0; i < D / 16; ++i) q[i] = as_bf16x8(ld16(src + 32 * (i >> 1) + 8 * (i & 1)));
     }
+    Tile<D> col;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) col.o[i] = f32x16{};
+    col.m = -INFINITY;
+    col.l = 0.f;
 
     // strips of this wave: row0 + rows * n, n < ns
     const int row0 = i0 * rows + 32 * (wave >> lg);
     const int end = min(i1 * rows, s.len);
-    const int ns = mine > 0 && row0 < end ? (end - row0 + rows - 1) / rows : 0;
+    const int ns = mine && row0 < end ? (end - row0 + rows - 1) / rows : 0;
     const int blk_end = (end + kScaleRows - 1) / kScaleRows;
     const int open = min(end, s.base);        // rows that every column attends
     for (int n0 = 0; n0 < ns; n0 += 32) {
@@ -429,13 +476,13 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_tree_paged_fp8_kernel(PagedFp
       const int blk = (row0 + (n0 + (lane >> 1)) * rows) / kScaleRows + (lane & 1);
       const BlockRef ref = block_ref(c, b, kvh, blk, blk_end);
       const int n1 = min(ns - n0, 32);
-      Strip<D> x;
+      Codes<D> x;
       auto bid = [&](int n, int i) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(ref.bid, (2 * n + i) & 63); };
-      auto load_k = [&](int n) __attribute__((always_inline)) {
-        load_codes<D, false>(x, c.k_pages, n < n1 ? bid(n, 0) : -1, n < n1 ? bid(n, 1) : -1, m16, g4);
+      auto next_k = [&](int n) __attribute__((always_inline)) {
+        if (n < n1) load_k<D>(x, c.k_pages, bid(n, 0), bid(n, 1), m32, hf);
       };
-      auto load_v = [&](int n) __attribute__((always_inline)) {
-        load_codes<D, true>(x, c.v_pages, n < n1 ? bid(n, 0) : -1, n < n1 ? bid(n, 1) : -1, m16, g4);
+      auto next_v = [&](int n) __attribute__((always_inline)) {
+        if (n < n1) load_v<D>(x, c.v_pages, bid(n, 0), bid(n, 1), m32, hf);
       };
       auto scales = [&](int n) __attribute__((always_inline)) {
         // no page: all rows masked, and -inf times a scale of 0 would be NaN
@@ -446,68 +493,69 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_tree_paged_fp8_kernel(PagedFp
         r.eb = held_exp(readlane_f(ref.vs, 2 * n + 1));
         return r;
       };
-      load_k(0);
-      load_v(0);
+      next_k(0);
+      next_v(0);
       // the strips whose rows all columns attend, then the others
       const bool hole = __ballot(blk < blk_end && ref.bid < 0) != 0;
       const int plain = hole ? 0 : min(n1, max(0, open - row0 - n0 * rows + rows - 32) / rows);
-      f32x4 sa[kT], sb[kT];
-      u32x4 p[kT];
+      u32x4 p[2];
       int n = 0;
       for (; n < plain; ++n) {
-        make_scores<D>(sa, sb, x, q);
+        const f32x16 sc = make_scores<D>(x, q);
         __builtin_amdgcn_sched_barrier(0);
-        load_k(n + 1);
+        next_k(n + 1);
         __builtin_amdgcn_sched_barrier(0);
-        make_weights<D>(p, col, sa, sb, scales(n));
-        add_values<D>(col, x, p);
+        make_weights<D>(p, col, sc, scales(n));
+        add_values<D>(col, x, p, m32);
         __builtin_amdgcn_sched_barrier(0);
-        load_v(n + 1);
+        next_v(n + 1);
         __builtin_amdgcn_sched_barrier(0);
       }
       for (; n < n1; ++n) {
-        make_scores<D>(sa, sb, x, q);
-        load_k(n + 1);
+        f32x16 sc = make_scores<D>(x, q);
+        next_k(n + 1);
         const int row = row0 + (n0 + n) * rows;
         const uint32_t held = (bid(n, 0) >= 0 ? 0xffffu : 0u) | (bid(n, 1) >= 0 ? 0xffff0000u : 0u);
-        uint32_t keep[kT];
-#pragma unroll
-        for (int t = 0; t < kT; ++t) keep[t] = attended(a, words_at[t], row, s.base, end) & held;
-        mask_scores<D>(sa, sb, keep, g4);
-        mend_values<D>(col, x, keep, g4);
-        make_weights<D>(p, col, sa, sb, scales(n));
-        add_values<D>(col, x, p);
-        load_v(n + 1);
+        const uint32_t keep = (attended(a, words, row, s.base, end) & held) >> (4 * hf);
+        mask_scores(sc, keep);
+        mend_values<D>(col, x, keep, m32);
+        make_weights<D>(p, col, sc, scales(n));
+        add_values<D>(col, x, p, m32);
+        next_v(n + 1);
       }
     }
 
     // ---- the waves' results meet ------------------------------------------
     __syncthreads();   // the item before has been read
+    {
+      const float l = half_sum(col.l);
+      float* row = s_acc + (wave * kTile + m32) * kStride;
 #pragma unroll
-    for (int t = 0; t < kT; ++t) {
-      const float l = xrow4_sum(col[t].l);
-      const int slot = (wave * kT + t) * 16 + m16;
-      float* row = s_acc + slot * kStride;
+      for (int i = 0; i < 16; ++i) {
+        const int m = 8 * (i >> 2) + 4 * hf + (i & 3);
+        if constexpr (D == 64) {
+          if (i < 8) *reinterpret_cast<f32x4*>(row + 4 * m) = f32x4{col.o[0][i], col.o[0][i + 8], col.o[1][i], col.o[1][i + 8]};
+        } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d) row[(D / 16) * (4 * g4 + i) + d] = col[t].acc[d][i];
+          for (int w = 0; w < D / 128; ++w)
+            *reinterpret_cast<f32x4*>(row + (D / 32) * m + 4 * w) =
+                f32x4{col.o[4 * w][i], col.o[4 * w + 1][i], col.o[4 * w + 2][i], col.o[4 * w + 3][i]};
+        }
       }
-      if (g4 == 0) {
-        s_ml[slot * 2] = col[t].m;
-        s_ml[slot * 2 + 1] = l;
+      if (hf == 0) {
+        s_ml[(wave * kTile + m32) * 2] = col.m;
+        s_ml[(wave * kTile + m32) * 2 + 1] = l;
       }
     }
     __syncthreads();
     const bool whole = i0 == 0 && i1 == it.units;
     float* rec = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (i0 == 0 ? 1 : 0)) * a.rec_cols * (D + kRecTail);
-    const int here = min(16 * tiles, cols - 16 * it.tile0);      // columns of the item
-    const int parts = kWaves >> lg;
+    const int here = min(kTile * it.tiles, cols - kTile * it.tile0);      // columns of the item
+    const int parts = kWaves<D> >> lg;
     for (int idx = threadIdx.x; idx < here * (D / 4); idx += kThreads) {
       const int x = idx / (D / 4), d = idx % (D / 4) * 4;
-      const int tile = x >> 4, w0 = tile / per;
-      const int slot0 = (w0 * kT + tile - w0 * per) * 16 + (x & 15);
-      const int step = lanes * kT * 16;     // the same column, other keys
+      const int slot0 = x;                      // wave x / kTile
+      const int step = lanes * kTile;           // the same column, other keys
       float M = -INFINITY, L = 0.f;
       for (int i = 0; i < parts; ++i) M = fmaxf(M, s_ml[(slot0 + i * step) * 2]);
       f32x4 A = {0.f, 0.f, 0.f, 0.f};
@@ -519,7 +567,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_tree_paged_fp8_kernel(PagedFp
         L += f * s_ml[slot * 2 + 1];
       }
       if (whole) {
-        const int y = 16 * it.tile0 + x, tok = y / a.group;
+        const int y = kTile * it.tile0 + x, tok = y / a.group;
         const float inv = L == 0.f ? 0.f : 1.0f / L;
         *reinterpret_cast<u32x2*>(a.out + (static_cast<size_t>(s.q0 + tok) * a.Hq + kvh * a.group + y - tok * a.group) * D + d) =
             u32x2{pack_bf16x2(A[0] * inv, A[1] * inv), pack_bf16x2(A[2] * inv, A[3] * inv)};
@@ -548,8 +596,8 @@ __global__ __launch_bounds__(kMergeThreads) void gqa_tree_paged_fp8_merge_kernel
   const Shape s = shape_of<D>(a, b);
   const int cols = s.n * a.group, x0 = static_cast<int>(blockIdx.z) * kMergeCols;
   if (x0 >= cols) return;
-  const int index = min(x0 / (16 * kCap<D>), s.full);
-  const Item it = item_at<D>(s, index + (index == s.full && s.half > 0 && x0 >= 16 * (s.full * kCap<D> + s.half) ? 1 : 0));
+  const int index = min(x0 / (kTile * kWaves<D>), s.full);
+  const Item it = item_at<D>(s, index + (index == s.full && s.half > 0 && x0 >= kTile * (s.full * kWaves<D> + s.half) ? 1 : 0));
   const int before = a.units[b], units = a.units[a.B] * c.Hkv, groups = min(launched, units);
   const int first = before * c.Hkv + kvh * (a.units[b + 1] - before) + it.before;
   // workgroup w holds unit x: the largest w with w U / W < x + 1
@@ -559,7 +607,7 @@ __global__ __launch_bounds__(kMergeThreads) void gqa_tree_paged_fp8_merge_kernel
   const int d = static_cast<int>(threadIdx.x) % kQuads * 4, x = static_cast<int>(threadIdx.x) / kQuads % kMergeCols;
   const int ph = static_cast<int>(threadIdx.x) / (kQuads * kMergeCols);
   const int y = min(x0 + x, cols - 1);
-  const float* at = a.part + static_cast<size_t>(y - 16 * it.tile0) * (D + kRecTail);
+  const float* at = a.part + static_cast<size_t>(y - kTile * it.tile0) * (D + kRecTail);
   const size_t step = static_cast<size_t>(a.rec_cols) * (D + kRecTail);
   f32x4 A = {0.f, 0.f, 0.f, 0.f};
   float M = -INFINITY, L = 0.f;
@@ -605,9 +653,9 @@ template <int D>
 Most most_of(int T, int words, int group) {
   Most m;
   m.cols = static_cast<long>(std::min<long>(T, 64L * words)) * group;
-  const long tiles = (m.cols + 15) / 16;
-  m.items = static_cast<int>(tiles / kCap<D> + 2);    // of the rest, two at most
-  m.rec_cols = static_cast<int>(16 * std::min<long>(tiles, kCap<D>));
+  const long tiles = (m.cols + kTile - 1) / kTile;
+  m.items = static_cast<int>(tiles / kWaves<D> + 2);    // of the rest, two at most
+  m.rec_cols = static_cast<int>(kTile * std::min<long>(tiles, kWaves<D>));
   return m;
 }
 
@@ -634,6 +682,7 @@ int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t wor
   const Most m = most_of<D>(a.T, words, a.group);
   a.chunks = m.items;
   a.rec_cols = m.rec_cols;
+  constexpr int kThreads = 64 * kWaves<D>;
   const long items = static_cast<long>(a.B) * c.Hkv * m.items;
   AILA_REQUIRE(items * most_units(a.max_len) < (1L << 31) && items * kThreads < (1L << 32),
                "gqa_tree_paged_fp8: B=%d requests of up to %ld query rows and %d keys are too many", a.B, m.cols, a.max_len);
@@ -649,7 +698,7 @@ int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t wor
     a.units = static_cast<int*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + units_bytes(a.B));
   }
-  const size_t lds = static_cast<size_t>(kWaves) * 16 * kTiles<D> * (kAccStride<D> + 2) * sizeof(float) +
+  const size_t lds = static_cast<size_t>(kWaves<D>) * kTile * (kAccStride<D> + 2) * sizeof(float) +
                      (a.part ? static_cast<size_t>(a.B + 1) * sizeof(int) : 0);
   hipLaunchKernelGGL((gqa_tree_paged_fp8_kernel<D>), dim3(groups), dim3(kThreads), lds, st, c, a);
   if (a.part)
