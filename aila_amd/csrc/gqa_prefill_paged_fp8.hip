@@ -69,6 +69,8 @@ struct Fp8PrefillArgs {
   int splits;            // one request: key runs a tile is cut into
   int* plan;             // several requests: the items' list (null: one request)
   float scale_log2;
+  const uint32_t* mask;  // drafted trees: [T, words32] bits of the drafted rows that a token attends
+  int words32;
 };
 
 // The list of a ragged batch's items: counts, the items in order of falling
@@ -166,40 +168,49 @@ struct Item {
   int t0, t1;         // key tiles
   int rec;            // record, -1: the run is the tile's only one
   int q0, n, len;     // the request's first token, tokens, rows
+  int base;           // TREE: its first drafted row
 };
 
+// TREE: a request's tokens are a drafted tree, those without mask bits left out.
+template <bool TREE>
 __device__ __forceinline__ void load_request(const Fp8PrefillArgs& a, int b, Item* it) {
   it->b = b;
   it->q0 = min(max(a.query_start[b], 0), a.T);
   it->n = max(min(max(a.query_start[b + 1], 0), a.T) - it->q0, 0);
   it->len = min(max(a.seq_lens[b], 0), a.max_len);
+  if constexpr (TREE) {
+    it->base = it->len - it->n;
+    it->n = min(it->n, 32 * a.words32);
+  }
 }
 
 // Keys that some row of the tile attends.
+template <bool TREE>
 __device__ __forceinline__ int tile_end(const Fp8PrefillArgs& a, const Item& it) {
+  if constexpr (TREE) return it.len;
   return max(it.len - it.n + min(it.n - 1, (it.r0 + kRows - 1) / a.group) + 1, 0);
 }
 
 // Item `index` of a KV head; false: there is none. One request: tiles with more
 // keys first, their keys in `splits` equal runs.
-template <int D>
+template <int D, bool TREE>
 __device__ __forceinline__ bool get_item(const Fp8PrefillArgs& a, int index, Item* it) {
   if (a.plan != nullptr) {
     if (index >= a.plan[0]) return false;
     const PlanItem x = reinterpret_cast<const PlanItem*>(a.plan + kPlanHead)[index];
-    load_request(a, x.b, it);
+    load_request<TREE>(a, x.b, it);
     it->r0 = x.r0;
     it->t0 = x.t0;
     it->t1 = x.t1;
     it->rec = x.rec;
     return true;
   }
-  load_request(a, 0, it);
+  load_request<TREE>(a, 0, it);
   const int tiles = (it->n * a.group + kRows - 1) / kRows;
   const int rank = a.splits > 1 ? index / a.splits : index, cut = index - rank * a.splits;
   if (rank >= tiles) return false;
   it->r0 = (tiles - 1 - rank) * kRows;
-  const unsigned kt = (tile_end(a, *it) + Cfg<D>::BN - 1) / Cfg<D>::BN;
+  const unsigned kt = (tile_end<TREE>(a, *it) + Cfg<D>::BN - 1) / Cfg<D>::BN;
   it->t0 = 0;
   it->t1 = kt;
   it->rec = -1;
@@ -242,7 +253,7 @@ __device__ __forceinline__ T plan_scan(T x, T* s_wave, T* total) {
   return x + before;   // inclusive
 }
 
-template <int NT>
+template <int NT, bool TREE>
 __global__ __launch_bounds__(NT) void gqa_prefill_paged_fp8_plan_kernel(Fp8PrefillArgs a, int key_tile) {
   constexpr int kBuckets = NT;
   extern __shared__ int s_dyn_plan[];
@@ -264,7 +275,7 @@ __global__ __launch_bounds__(NT) void gqa_prefill_paged_fp8_plan_kernel(Fp8Prefi
   for (int b0 = 0; b0 < a.B; b0 += NT) {
     const int b = b0 + tid;
     Item it{};
-    if (b < a.B) load_request(a, b, &it);
+    if (b < a.B) load_request<TREE>(a, b, &it);
     long all;
     const long incl = all_tiles + plan_scan<NT, long>((it.n * a.group + kRows - 1) / kRows, s_wave_l, &all);
     if (b < a.B) {
@@ -293,8 +304,8 @@ __global__ __launch_bounds__(NT) void gqa_prefill_paged_fp8_plan_kernel(Fp8Prefi
     it.n = s_n[lo];
     it.len = s_len[lo];
     it.r0 = x.r0;
-    x.kt = (tile_end(a, it) + key_tile - 1) / key_tile;
-    x.cost = it.n * a.group - x.r0 <= kThinRows ? x.kt : 4 * x.kt;
+    x.kt = (tile_end<TREE>(a, it) + key_tile - 1) / key_tile;
+    x.cost = !TREE && it.n * a.group - x.r0 <= kThinRows ? x.kt : 4 * x.kt;
     return x;
   };
   Tile mine{};      // the first round's, which is all there are as a rule
@@ -418,7 +429,7 @@ __device__ __forceinline__ void thin_item(const PagedFp8& c, const Fp8PrefillArg
   Column<D> col;
   clear_column(col);
   const int row0 = it.t0 * Cfg<D>::BN + 32 * wave;
-  const int end = min(it.t1 * Cfg<D>::BN, tile_end(a, it));
+  const int end = min(it.t1 * Cfg<D>::BN, tile_end<false>(a, it));
   const int ns = row0 < end ? (end - row0 + 32 * kWaves - 1) / (32 * kWaves) : 0;
   const int blk_end = (end + kScaleRows - 1) / kScaleRows;
   for (int n0 = 0; n0 < ns; n0 += 32) {
@@ -486,9 +497,25 @@ __device__ __forceinline__ void thin_item(const PagedFp8& c, const Fp8PrefillArg
   __syncthreads();     // LDS is the next item's
 }
 
+// Whether any key of [key, end) that a row of a drafted tree attends holds NaN in
+// head dim d of V.
+template <int D>
+__device__ __noinline__ bool tree_meets_nan(PagedFp8 c, const uint32_t* words, int words32, int b, int kvh, int base, int key,
+                                            int end, int d) {
+  for (; key < end; ++key) {
+    const int j = key - base;
+    if (j >= 0 && (j >= 32 * words32 || !(words[j >> 5] >> (j & 31) & 1))) continue;
+    const int bid = block_id(c, b, kvh, key / kScaleRows);
+    if (bid < 0) continue;
+    if ((c.v_pages[static_cast<size_t>(bid) * (kScaleRows * D) + key % kScaleRows * D + d] & 0x7f) == 0x7f) return true;
+  }
+  return false;
+}
+
 // THIN: the items may be thin ones. (A kernel that never meets one is a variant of
-// its own: the thin walk's registers cost the other's loop 5-9%.)
-template <int D, bool THIN>
+// its own: the thin walk's registers cost the other's loop 5-9%.) TREE: the rows
+// attend the drafted keys that their masks say.
+template <int D, bool THIN, bool TREE>
 __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(PagedFp8 c, Fp8PrefillArgs a) {
   using C = Cfg<D>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char s_dyn[];
@@ -565,7 +592,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
     return round * a.lanes + (round & 1 ? a.lanes - 1 - wl : wl);
   };
   Item it;
-  bool more = get_item<D>(a, item_at(0), &it);
+  bool more = get_item<D, TREE>(a, item_at(0), &it);
   int seg_b = -1, seg_0 = 0, seg_1 = 0;     // the segment whose blocks are in LDS: key tiles,
   int seg_last = 0;                         // and the last block looked up (the tile may end in a later one)
   bool holes = false, primed = false;       // primed: its first DMAs are on the way
@@ -573,7 +600,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
     const int rows = it.n * a.group;
     if (THIN && rows - it.r0 <= kThinRows) {
       thin_item<D>(c, a, it, kvh, reinterpret_cast<float*>(s_dyn), &s_ml[0][0][0]);
-      more = get_item<D>(a, item_at(round), &it);
+      more = get_item<D, TREE>(a, item_at(round), &it);
       continue;
     }
     const int row = it.r0 + wave * 32 + l32;          // this lane's query row
@@ -581,8 +608,8 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
     const int tok = min(row, rows - 1) / a.group;
     const int lim = max(it.len - it.n + tok + 1, 0);  // keys the row attends
     // tiles from this one on hold keys that not all rows attend
-    const int mask_from = max(it.len - it.n + it.r0 / a.group + 1, 0) / C::BN;
-    const int blk_end = (tile_end(a, it) + kScaleRows - 1) / kScaleRows;
+    const int mask_from = (TREE ? max(it.base, 0) : max(it.len - it.n + it.r0 / a.group + 1, 0)) / C::BN;
+    const int blk_end = (tile_end<TREE>(a, it) + kScaleRows - 1) / kScaleRows;
 
     // ---- state ---------------------------------------------------------------
     bf16x8_t q[C::STEPS - C::QL];
@@ -741,7 +768,18 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
         }
       };
       auto softmax = [&](int j, bool masked) __attribute__((always_inline)) {
-        if (masked) {
+        if (TREE && masked) {
+          const uint32_t* words = a.mask + static_cast<size_t>(it.q0 + tok) * a.words32;
+#pragma unroll
+          for (int k = 0; k < C::KT; ++k) {
+            const int at = first_block(j) + 2 * k;
+            const uint32_t held = (s_bid[at] >= 0 ? 0xffffu : 0u) | (s_bid[at + 1] >= 0 ? 0xffff0000u : 0u);
+            const uint32_t keep = (tree_rows(words, a.words32, s0 * C::BN + at * kScaleRows, it.base, it.len) & held) >> (4 * hf);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (!(keep >> (8 * (i >> 2) + (i & 3)) & 1)) sc[k][i] = -INFINITY;
+          }
+        } else if (masked) {
           const int rel = lim - s0 * C::BN - first_block(j) * kScaleRows - 4 * hf;
 #pragma unroll
           for (int k = 0; k < C::KT; ++k) {
@@ -870,9 +908,9 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
     // ---- the groups' states meet -----------------------------------------------
     // The next item's first codes are fetched meanwhile, if it walks the same keys.
     const Item done = it;
-    more = get_item<D>(a, item_at(round), &it);
+    more = get_item<D, TREE>(a, item_at(round), &it);
     if (more && it.b == seg_b && it.t0 == seg_0 && it.t0 < it.t1 && it.t1 <= seg_1 && it.rec < 0 &&
-        (tile_end(a, it) + kScaleRows - 1) / kScaleRows <= seg_last && !(THIN && it.n * a.group - it.r0 <= kThinRows)) {
+        (tile_end<TREE>(a, it) + kScaleRows - 1) / kScaleRows <= seg_last && !(THIN && it.n * a.group - it.r0 <= kThinRows)) {
       start();
       primed = true;
     }
@@ -931,7 +969,21 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
         }
       }
       const int hf = ln >> 5, row = done.r0 + row32;
-      if (s_any_nan) {
+      if (TREE && s_any_nan && row < done.n * a.group) {
+        // bit (d * 2 + i) * 4 + e: the output's dim holds NaN in an attended key
+        uint64_t hit = 0;
+        const uint32_t* words = a.mask + static_cast<size_t>(done.q0 + row / a.group) * a.words32;
+#pragma unroll 1
+        for (int x = 0; x < 8 * C::DT; ++x) {
+          const int d = out_dim<D>(x >> 3, 8 * (x & 4 ? kOwn[1] : kOwn[0]) + 4 * hf + (x & 3));
+          if (s_nan[d] != kNoKey &&
+              tree_meets_nan<D>(c, words, a.words32, done.b, kvh, done.base, s_nan[d], min(done.t1 * C::BN, done.len), d))
+            hit |= 1ull << x;
+        }
+#pragma unroll
+        for (int x = 0; x < 8 * C::DT; ++x)
+          if (hit >> x & 1) o[x >> 3][4 * kOwn[x >> 2 & 1] + (x & 3)] = __uint_as_float(0x7fc00000u);
+      } else if (!TREE && s_any_nan) {
         const int tok = row / a.group;
         const int lim = max(done.len - done.n + tok + 1, 0);
 #pragma unroll
@@ -987,7 +1039,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
 // Joins the records of a tile whose keys were cut: o = sum 2^(m_i - M) o_i /
 // sum 2^(m_i - M) l_i. A workgroup takes 32 query rows and up to 128 dims; a
 // thread's values are those of the main kernel's lane.
-template <int D>
+template <int D, bool TREE>
 __global__ __launch_bounds__(256) void gqa_prefill_paged_fp8_merge_kernel(PagedFp8 c, Fp8PrefillArgs a) {
   using C = Cfg<D>;
   Item it;
@@ -996,14 +1048,14 @@ __global__ __launch_bounds__(256) void gqa_prefill_paged_fp8_merge_kernel(PagedF
     if (static_cast<int>(blockIdx.x) >= a.plan[1]) return;
     const PlanCut x = reinterpret_cast<const PlanCut*>(reinterpret_cast<const PlanItem*>(a.plan + kPlanHead) +
                                                        plan_items(a.T, a.B, a.group, a.lanes))[blockIdx.x];
-    load_request(a, x.b, &it);
+    load_request<TREE>(a, x.b, &it);
     it.r0 = x.r0;
     rec = x.rec;
     cuts = x.cuts;
   } else {
     rec = static_cast<int>(blockIdx.x) * a.splits;
     cuts = a.splits;
-    if (!get_item<D>(a, rec, &it)) return;
+    if (!get_item<D, TREE>(a, rec, &it)) return;
   }
   constexpr int G = D > 128 ? D / 128 : 1;
   const int kvh = blockIdx.y, wave = static_cast<int>(blockIdx.z) / G, g = static_cast<int>(blockIdx.z) % G;
@@ -1087,20 +1139,20 @@ size_t workspace_need(int T, int B, int Hkv, int group, int max_len, int* lanes,
   return plan_bytes(T, B, group, *lanes) + 2 * static_cast<size_t>(*lanes) * rec;
 }
 
-template <int D>
+template <int D, bool TREE = false>
 int launch(PagedFp8 c, Fp8PrefillArgs a, void* workspace, size_t workspace_bytes, hipStream_t st) {
   const size_t need = workspace_need<D>(a.T, a.B, c.Hkv, a.group, a.max_len, &a.lanes, &a.splits);
   const int tiles = static_cast<int>((static_cast<long>(a.T) * a.group + kRows - 1) / kRows);
   auto walk = [&](const PagedFp8& cache, const Fp8PrefillArgs& args) {
     // one request's last tile may be thin too, but is one of many then
-    const bool thin = a.B > 1 || static_cast<long>(a.T) * a.group <= kThinRows;
+    const bool thin = !TREE && (a.B > 1 || static_cast<long>(a.T) * a.group <= kThinRows);
     if (thin)
-      hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D, true>), dim3(args.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, cache, args);
+      hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D, !TREE, TREE>), dim3(args.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, cache, args);
     else
-      hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D, false>), dim3(args.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, cache, args);
+      hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D, false, TREE>), dim3(args.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, cache, args);
   };
   auto merge = [&](int cut_tiles) {
-    hipLaunchKernelGGL((gqa_prefill_paged_fp8_merge_kernel<D>), dim3(cut_tiles, c.Hkv, 4 * (D > 128 ? D / 128 : 1)), dim3(256), 0,
+    hipLaunchKernelGGL((gqa_prefill_paged_fp8_merge_kernel<D, TREE>), dim3(cut_tiles, c.Hkv, 4 * (D > 128 ? D / 128 : 1)), dim3(256), 0,
                        st, c, a);
   };
   if (a.B == 1) {
@@ -1128,8 +1180,8 @@ int launch(PagedFp8 c, Fp8PrefillArgs a, void* workspace, size_t workspace_bytes
     };
     // a thread a tile; few tiles: 4 waves, whose sums and barriers are shorter (us, a batch of
     // 32 with 91 tiles: 5.4 against 7.1)
-    if (a.B <= 256 && plan_items(a.T, a.B, a.group, 0) <= 256) plan(gqa_prefill_paged_fp8_plan_kernel<256>, 256);
-    else plan(gqa_prefill_paged_fp8_plan_kernel<1024>, 1024);
+    if (a.B <= 256 && plan_items(a.T, a.B, a.group, 0) <= 256) plan(gqa_prefill_paged_fp8_plan_kernel<256, TREE>, 256);
+    else plan(gqa_prefill_paged_fp8_plan_kernel<1024, TREE>, 1024);
     walk(c, a);
     merge(a.lanes);
   }
@@ -1137,6 +1189,36 @@ int launch(PagedFp8 c, Fp8PrefillArgs a, void* workspace, size_t workspace_bytes
 }
 
 }  // namespace
+
+// Wide drafted trees walk as prompts do, under their masks.
+size_t tree_as_prefill_workspace(int D, int T, int B, int Hkv, int group, int max_len) {
+  int lanes, splits;
+  switch (D) {
+    case 64: return workspace_need<64>(T, B, Hkv, group, max_len, &lanes, &splits);
+    case 128: return workspace_need<128>(T, B, Hkv, group, max_len, &lanes, &splits);
+    default: return workspace_need<256>(T, B, Hkv, group, max_len, &lanes, &splits);
+  }
+}
+
+int tree_as_prefill(int D, const PagedFp8& c, const TreeCall& t, hipStream_t st) {
+  Fp8PrefillArgs a{};
+  a.q = t.q;
+  a.q_stride = t.q_stride;
+  a.out = t.out;
+  a.query_start = t.query_start;
+  a.seq_lens = t.seq_lens;
+  a.T = t.T; a.B = t.B; a.Hq = t.Hq; a.group = t.Hq / c.Hkv;
+  a.max_len = t.max_len;
+  a.scale_log2 = kLog2e / sqrtf(static_cast<float>(D));
+  a.mask = t.mask;
+  a.words32 = t.words32;
+  switch (D) {
+    case 64: return launch<64, true>(c, a, t.workspace, t.workspace_bytes, st);
+    case 128: return launch<128, true>(c, a, t.workspace, t.workspace_bytes, st);
+    default: return launch<256, true>(c, a, t.workspace, t.workspace_bytes, st);
+  }
+}
+
 }  // namespace aila
 
 extern "C" size_t aila_hip_gqa_prefill_paged_fp8_workspace_size(int T, int B, int Hq, int Hkv, int D, int max_len) {

@@ -17,6 +17,7 @@
 #include "paged_fp8.hpp"
 
 #include <algorithm>
+#include <cstdlib>
 
 namespace aila {
 namespace {
@@ -168,19 +169,6 @@ __device__ __forceinline__ int share_begin(int w, int units, int groups) {
 // acc + the two bf16 of x.
 __device__ __forceinline__ float add_pair(uint32_t x, float acc) {
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), acc, false);
-}
-
-// The rows [row, row + 32) that a token attends, as bits: those before the draft
-// (row < base), the drafted ones by its mask words, none from len on.
-__device__ __forceinline__ uint32_t attended(const TreeArgs& a, const uint32_t* words, int row, int base, int len) {
-  const int o = row - base, i = o >> 5, sh = o & 31;
-  auto word = [&](int w) __attribute__((always_inline)) -> uint32_t {
-    return w < 0 ? ~0u : w < a.words32 ? words[w] : 0u;
-  };
-  const uint64_t both = static_cast<uint64_t>(word(i + 1)) << 32 | word(i);
-  const uint32_t keep = static_cast<uint32_t>(both >> sh);
-  const int left = len - row;
-  return left >= 32 ? keep : left > 0 ? keep & ((1u << left) - 1) : 0u;
 }
 
 __device__ __forceinline__ f32x16 mfma32(const bf16x8_t& a, const bf16x8_t& b, const f32x16& c) {
@@ -516,7 +504,7 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
         next_k(n + 1);
         const int row = row0 + (n0 + n) * rows;
         const uint32_t held = (bid(n, 0) >= 0 ? 0xffffu : 0u) | (bid(n, 1) >= 0 ? 0xffff0000u : 0u);
-        const uint32_t keep = (attended(a, words, row, s.base, end) & held) >> (4 * hf);
+        const uint32_t keep = (tree_rows(words, a.words32, row, s.base, end) & held) >> (4 * hf);
         mask_scores(sc, keep);
         mend_values<D>(col, x, keep, m32);
         make_weights<D>(p, col, sc, scales(n));
@@ -707,6 +695,12 @@ int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t wor
   return check_launch("gqa_tree_paged_fp8");
 }
 
+bool walks_as_prompt(int T, int B, int group, int D) {
+  const char* e = getenv("TREE_WALK");
+  if (e) return e[0] == '1';
+  return D == 256 && static_cast<long>(T) * group > 64L * B;
+}
+
 }  // namespace
 }  // namespace aila
 
@@ -714,6 +708,8 @@ extern "C" size_t aila_hip_gqa_tree_paged_fp8_workspace_size(int T, int B, int H
                                                              int mask_words) {
   using namespace aila;
   if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || max_len < 0 || mask_words <= 0) return 0;
+  if (D != 64 && D != 128 && D != 256) return 0;
+  if (walks_as_prompt(T, B, Hq / Hkv, D)) return tree_as_prefill_workspace(D, T, B, Hkv, Hq / Hkv, max_len);
   switch (D) {
     case 64: return workspace_need<64>(T, B, Hkv, Hq / Hkv, mask_words, max_len);
     case 128: return workspace_need<128>(T, B, Hkv, Hq / Hkv, mask_words, max_len);
@@ -761,6 +757,8 @@ extern "C" int aila_hip_gqa_tree_paged_fp8(const void* q, long q_stride, const v
   a.max_len = max_len;
   a.scale_log2 = kLog2e / sqrtf(static_cast<float>(D));
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (walks_as_prompt(T, B, Hq / Hkv, D) && (workspace ? workspace_bytes : 0) >= tree_as_prefill_workspace(D, T, B, Hkv, Hq / Hkv, max_len))
+    return tree_as_prefill(D, c, TreeCall{a.q, q_stride, a.out, a.mask, a.words32, query_start, seq_lens, T, B, Hq, max_len, workspace, workspace_bytes}, st);
   switch (D) {
     case 64: return launch<64>(c, a, mask_words, workspace, workspace_bytes, st);
     case 128: return launch<128>(c, a, mask_words, workspace, workspace_bytes, st);

@@ -322,4 +322,34 @@ __device__ __forceinline__ void strip_step(Column<D>& c, Strip<D>& s, const bf16
   }
 }
 
+// ---- drafted trees ----------------------------------------------------------
+// The rows [row, row + 32) that a token attends, as bits: those before the draft
+// (row < base), the drafted ones by its mask words, none from len on.
+__device__ __forceinline__ uint32_t tree_rows(const uint32_t* words, int words32, int row, int base, int len) {
+  const int o = row - base, i = o >> 5, sh = o & 31;
+  auto word = [&](int w) __attribute__((always_inline)) -> uint32_t {
+    return w < 0 ? ~0u : w < words32 ? words[w] : 0u;
+  };
+  const uint64_t both = static_cast<uint64_t>(word(i + 1)) << 32 | word(i);
+  const uint32_t keep = static_cast<uint32_t>(both >> sh);
+  const int left = len - row;
+  return left >= 32 ? keep : left > 0 ? keep & ((1u << left) - 1) : 0u;
+}
+
+// The tree attention's arguments, for the kernel that walks wide trees as prompts.
+struct TreeCall {
+  const bf16* q;
+  long q_stride;
+  bf16* out;
+  const uint32_t* mask;
+  int words32;
+  const int* query_start;
+  const int* seq_lens;
+  int T, B, Hq, max_len;
+  void* workspace;
+  size_t workspace_bytes;
+};
+size_t tree_as_prefill_workspace(int D, int T, int B, int Hkv, int group, int max_len);
+int tree_as_prefill(int D, const PagedFp8& c, const TreeCall& t, hipStream_t st);
+
 }  // namespace aila
