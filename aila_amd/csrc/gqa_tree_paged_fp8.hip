@@ -262,7 +262,7 @@ struct Tile {
 
 // What a strip's blocks contribute: K scales times log2(e) / sqrt(D), exponents of
 // the V scales.
-struct Scales { float ka, kb; int ea, eb; };
+struct Scales { float ka, kb, ea, eb, ia, ib; };    // and the V scales' reciprocals
 
 template <int D>
 __device__ __forceinline__ f32x16 make_scores(const Codes<D>& x, const bf16x8_t (&q)[D / 16]) {
@@ -356,15 +356,14 @@ __device__ __forceinline__ void make_weights(u32x4 (&p)[2], Tile<D>& c, const f3
   const float ref = c.m == -INFINITY ? 0.f : c.m;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const int e = s ? x.eb : x.ea;
-    const float k = s ? x.kb : x.ka, r = static_cast<float>(e) - ref;
+    const float k = s ? x.kb : x.ka, r = (s ? x.eb : x.ea) - ref;
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       p[s][i] = pack_bf16x2(fast_exp2(fmaf(sc[8 * s + 2 * i], k, r)), fast_exp2(fmaf(sc[8 * s + 2 * i + 1], k, r)));
       sum = add_pair(p[s][i], sum);
     }
-    c.l = fmaf(sum, pow2f(-e), c.l);
+    c.l = fmaf(sum, s ? x.ib : x.ia, c.l);
   }
 }
 
@@ -464,6 +463,10 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
       const int blk = (row0 + (n0 + (lane >> 1)) * rows) / kScaleRows + (lane & 1);
       const BlockRef ref = block_ref(c, b, kvh, blk, blk_end);
       const int n1 = min(ns - n0, 32);
+      // no page: all rows masked, and -inf times a scale of 0 would be NaN
+      const float my_k = (ref.bid >= 0 ? ref.ks : 1.0f) * a.scale_log2;
+      const int my_e = held_exp(ref.vs);
+      const float my_ef = static_cast<float>(my_e), my_i = pow2f(-my_e);
       Codes<D> x;
       auto bid = [&](int n, int i) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(ref.bid, (2 * n + i) & 63); };
       auto next_k = [&](int n) __attribute__((always_inline)) {
@@ -473,12 +476,13 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
         if (n < n1) load_v<D>(x, c.v_pages, bid(n, 0), bid(n, 1), m32, hf);
       };
       auto scales = [&](int n) __attribute__((always_inline)) {
-        // no page: all rows masked, and -inf times a scale of 0 would be NaN
         Scales r;
-        r.ka = (bid(n, 0) >= 0 ? readlane_f(ref.ks, 2 * n) : 1.0f) * a.scale_log2;
-        r.kb = (bid(n, 1) >= 0 ? readlane_f(ref.ks, 2 * n + 1) : 1.0f) * a.scale_log2;
-        r.ea = held_exp(readlane_f(ref.vs, 2 * n));
-        r.eb = held_exp(readlane_f(ref.vs, 2 * n + 1));
+        r.ka = readlane_f(my_k, 2 * n);
+        r.kb = readlane_f(my_k, 2 * n + 1);
+        r.ea = readlane_f(my_ef, 2 * n);
+        r.eb = readlane_f(my_ef, 2 * n + 1);
+        r.ia = readlane_f(my_i, 2 * n);
+        r.ib = readlane_f(my_i, 2 * n + 1);
         return r;
       };
       next_k(0);
