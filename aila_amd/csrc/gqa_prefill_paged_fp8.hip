@@ -71,6 +71,7 @@ struct Fp8PrefillArgs {
   float scale_log2;
   const uint32_t* mask;  // drafted trees: [T, words32] bits of the drafted rows that a token attends
   int words32;
+  int* units;            // [B + 1] key tiles of a KV head's trees before each request
 };
 
 // The list of a ragged batch's items: counts, the items in order of falling
@@ -193,24 +194,24 @@ __device__ __forceinline__ int tile_end(const Fp8PrefillArgs& a, const Item& it)
 
 // Item `index` of a KV head; false: there is none. One request: tiles with more
 // keys first, their keys in `splits` equal runs.
-template <int D, bool TREE>
+template <int D>
 __device__ __forceinline__ bool get_item(const Fp8PrefillArgs& a, int index, Item* it) {
   if (a.plan != nullptr) {
     if (index >= a.plan[0]) return false;
     const PlanItem x = reinterpret_cast<const PlanItem*>(a.plan + kPlanHead)[index];
-    load_request<TREE>(a, x.b, it);
+    load_request<false>(a, x.b, it);
     it->r0 = x.r0;
     it->t0 = x.t0;
     it->t1 = x.t1;
     it->rec = x.rec;
     return true;
   }
-  load_request<TREE>(a, 0, it);
+  load_request<false>(a, 0, it);
   const int tiles = (it->n * a.group + kRows - 1) / kRows;
   const int rank = a.splits > 1 ? index / a.splits : index, cut = index - rank * a.splits;
   if (rank >= tiles) return false;
   it->r0 = (tiles - 1 - rank) * kRows;
-  const unsigned kt = (tile_end<TREE>(a, *it) + Cfg<D>::BN - 1) / Cfg<D>::BN;
+  const unsigned kt = (tile_end<false>(a, *it) + Cfg<D>::BN - 1) / Cfg<D>::BN;
   it->t0 = 0;
   it->t1 = kt;
   it->rec = -1;
@@ -221,6 +222,105 @@ __device__ __forceinline__ bool get_item(const Fp8PrefillArgs& a, int index, Ite
     it->rec = index;
   }
   return true;
+}
+
+// Drafted trees: the key tiles of all tiles of query rows of a KV head form one
+// line, in which a tile begins with kTreeStart units for its start and end, and every
+// workgroup takes an equal piece of it. (Tiles cut into equal runs, as prompts' are,
+// leave 27 tiles of 16384 keys on 32 workgroups 1.45 times a share.) A piece that
+// covers a tile whole writes its output; the others write records, at most two a
+// workgroup: 2 w + 1 if it begins the tile, else 2 w.
+constexpr int kTreeStart = 8;
+template <int D>
+__device__ __forceinline__ int tree_tile_units(const Item& it) {
+  return kTreeStart + max((it.len + Cfg<D>::BN - 1) / Cfg<D>::BN, 1);     // an output without keys is written too
+}
+__device__ __forceinline__ int tree_tiles(const Fp8PrefillArgs& a, const Item& it) { return (it.n * a.group + kRows - 1) / kRows; }
+
+// s_pre[b] = units of the requests before b, for b <= B.
+template <int D>
+__device__ __forceinline__ void scan_tree_units(const Fp8PrefillArgs& a, int* s_pre) {
+  const int lane = threadIdx.x & 63;
+  if (threadIdx.x < 64) {
+    int sum = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      const int b = b0 + lane;
+      int n = 0;
+      if (b < a.B) {
+        Item it{};
+        load_request<true>(a, b, &it);
+        n = tree_tiles(a, it) * tree_tile_units<D>(it);
+      }
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int y = __shfl_up(n, off);
+        if (lane >= off) n += y;
+      }
+      if (b < a.B) s_pre[b + 1] = sum + n;
+      sum += __shfl(n, 63);
+    }
+    if (lane == 0) s_pre[0] = 0;
+  }
+  __syncthreads();
+}
+// The workgroup that holds unit x of a line of `units`: the largest w with w U / W < x + 1.
+__device__ __forceinline__ int tree_holder(int x, int units, int groups) {
+  return static_cast<int>((static_cast<long>(x + 1) * groups - 1) / units);
+}
+
+struct TreeLine {
+  int u, u1;          // units that are left
+  int b, pos, tile;   // the tile that holds u, and where it begins
+};
+template <int D>
+__device__ __forceinline__ bool begin_trees(const Fp8PrefillArgs& a, int* s_pre, int w, bool first, TreeLine* t) {
+  scan_tree_units<D>(a, s_pre);
+  const int units = __builtin_amdgcn_readfirstlane(s_pre[a.B]), groups = min(a.lanes, units);
+  if (first)
+    for (int i = threadIdx.x; i <= a.B; i += kThreads) a.units[i] = s_pre[i];
+  bool any = w < groups;
+  if (any) {
+    t->u = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<long>(w) * units / groups));
+    t->u1 = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<long>(w + 1) * units / groups));
+    int lo = 0, hi = a.B;      // the last request whose units begin at or before u
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_pre[mid] <= t->u) lo = mid; else hi = mid;
+    }
+    t->b = __builtin_amdgcn_readfirstlane(lo);
+    Item it{};
+    load_request<true>(a, t->b, &it);
+    const int per = tree_tile_units<D>(it), before = __builtin_amdgcn_readfirstlane(s_pre[t->b]);
+    t->tile = (t->u - before) / per;
+    t->pos = before + t->tile * per;
+  }
+  __syncthreads();    // s_pre is other things' place
+  return any;
+}
+// The next piece of the workgroup's line; false: there is none.
+template <int D>
+__device__ __forceinline__ bool next_tree(const Fp8PrefillArgs& a, int w, TreeLine* t, Item* it) {
+  while (t->u < t->u1) {
+    load_request<true>(a, t->b, it);
+    if (t->tile >= tree_tiles(a, *it)) {
+      ++t->b;
+      t->tile = 0;
+      continue;
+    }
+    const int per = tree_tile_units<D>(*it), keys = t->pos + kTreeStart;
+    const int k0 = max(t->u - keys, 0), k1 = min(t->u1 - keys, per - kTreeStart);
+    it->r0 = t->tile * kRows;
+    it->t0 = k0;
+    it->t1 = min(k1, (it->len + Cfg<D>::BN - 1) / Cfg<D>::BN);
+    it->rec = k0 == 0 && k1 == per - kTreeStart ? -1 : 2 * w + (k0 == 0 ? 1 : 0);
+    t->u = min(t->u1, t->pos + per);
+    if (t->u == t->pos + per) {
+      t->pos += per;
+      ++t->tile;
+    }
+    if (k1 > k0) return true;
+  }
+  return false;
 }
 
 // The items of a ragged batch. Each workgroup of a KV head should get the same
@@ -253,7 +353,7 @@ __device__ __forceinline__ T plan_scan(T x, T* s_wave, T* total) {
   return x + before;   // inclusive
 }
 
-template <int NT, bool TREE>
+template <int NT>
 __global__ __launch_bounds__(NT) void gqa_prefill_paged_fp8_plan_kernel(Fp8PrefillArgs a, int key_tile) {
   constexpr int kBuckets = NT;
   extern __shared__ int s_dyn_plan[];
@@ -275,7 +375,7 @@ __global__ __launch_bounds__(NT) void gqa_prefill_paged_fp8_plan_kernel(Fp8Prefi
   for (int b0 = 0; b0 < a.B; b0 += NT) {
     const int b = b0 + tid;
     Item it{};
-    if (b < a.B) load_request<TREE>(a, b, &it);
+    if (b < a.B) load_request<false>(a, b, &it);
     long all;
     const long incl = all_tiles + plan_scan<NT, long>((it.n * a.group + kRows - 1) / kRows, s_wave_l, &all);
     if (b < a.B) {
@@ -304,8 +404,8 @@ __global__ __launch_bounds__(NT) void gqa_prefill_paged_fp8_plan_kernel(Fp8Prefi
     it.n = s_n[lo];
     it.len = s_len[lo];
     it.r0 = x.r0;
-    x.kt = (tile_end<TREE>(a, it) + key_tile - 1) / key_tile;
-    x.cost = !TREE && it.n * a.group - x.r0 <= kThinRows ? x.kt : 4 * x.kt;
+    x.kt = (tile_end<false>(a, it) + key_tile - 1) / key_tile;
+    x.cost = it.n * a.group - x.r0 <= kThinRows ? x.kt : 4 * x.kt;
     return x;
   };
   Tile mine{};      // the first round's, which is all there are as a rule
@@ -592,7 +692,15 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
     return round * a.lanes + (round & 1 ? a.lanes - 1 - wl : wl);
   };
   Item it;
-  bool more = get_item<D, TREE>(a, item_at(0), &it);
+  TreeLine line{};
+  if constexpr (TREE) {
+    if (!begin_trees<D>(a, reinterpret_cast<int*>(s_dyn), wl, blockIdx.x == 0, &line)) return;
+  }
+  auto next_item = [&](int round) __attribute__((always_inline)) {
+    if constexpr (TREE) return next_tree<D>(a, wl, &line, &it);
+    else return get_item<D>(a, item_at(round), &it);
+  };
+  bool more = next_item(0);
   int seg_b = -1, seg_0 = 0, seg_1 = 0;     // the segment whose blocks are in LDS: key tiles,
   int seg_last = 0;                         // and the last block looked up (the tile may end in a later one)
   bool holes = false, primed = false;       // primed: its first DMAs are on the way
@@ -600,7 +708,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
     const int rows = it.n * a.group;
     if (THIN && rows - it.r0 <= kThinRows) {
       thin_item<D>(c, a, it, kvh, reinterpret_cast<float*>(s_dyn), &s_ml[0][0][0]);
-      more = get_item<D, TREE>(a, item_at(round), &it);
+      more = next_item(round);
       continue;
     }
     const int row = it.r0 + wave * 32 + l32;          // this lane's query row
@@ -908,7 +1016,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
     // ---- the groups' states meet -----------------------------------------------
     // The next item's first codes are fetched meanwhile, if it walks the same keys.
     const Item done = it;
-    more = get_item<D, TREE>(a, item_at(round), &it);
+    more = next_item(round);
     if (more && it.b == seg_b && it.t0 == seg_0 && it.t0 < it.t1 && it.t1 <= seg_1 && it.rec < 0 &&
         (tile_end<TREE>(a, it) + kScaleRows - 1) / kScaleRows <= seg_last && !(THIN && it.n * a.group - it.r0 <= kThinRows)) {
       start();
@@ -1044,18 +1152,31 @@ __global__ __launch_bounds__(256) void gqa_prefill_paged_fp8_merge_kernel(PagedF
   using C = Cfg<D>;
   Item it;
   int rec, cuts;
-  if (a.plan != nullptr) {
+  int rec_step = 1;     // of the records behind the second
+  if constexpr (TREE) {
+    const int per_request = static_cast<int>(gridDim.x) / a.B, b = static_cast<int>(blockIdx.x) / per_request;
+    load_request<true>(a, b, &it);
+    const int tile = static_cast<int>(blockIdx.x) - b * per_request, per = tree_tile_units<D>(it);
+    it.r0 = tile * kRows;
+    if (tile >= tree_tiles(a, it)) return;
+    const int units = a.units[a.B], groups = min(a.lanes, units), keys = a.units[b] + tile * per + kTreeStart;
+    const int w0 = tree_holder(keys, units, groups), w1 = tree_holder(keys - kTreeStart + per - 1, units, groups);
+    if (w0 == w1) return;   // one workgroup wrote the output
+    rec = 2 * w0 + 1;       // then 2 w0 + 2, 2 w0 + 4, ...
+    rec_step = 2;
+    cuts = w1 - w0 + 1;
+  } else if (a.plan != nullptr) {
     if (static_cast<int>(blockIdx.x) >= a.plan[1]) return;
     const PlanCut x = reinterpret_cast<const PlanCut*>(reinterpret_cast<const PlanItem*>(a.plan + kPlanHead) +
                                                        plan_items(a.T, a.B, a.group, a.lanes))[blockIdx.x];
-    load_request<TREE>(a, x.b, &it);
+    load_request<false>(a, x.b, &it);
     it.r0 = x.r0;
     rec = x.rec;
     cuts = x.cuts;
   } else {
     rec = static_cast<int>(blockIdx.x) * a.splits;
     cuts = a.splits;
-    if (!get_item<D, TREE>(a, rec, &it)) return;
+    if (!get_item<D>(a, rec, &it)) return;
   }
   constexpr int G = D > 128 ? D / 128 : 1;
   const int kvh = blockIdx.y, wave = static_cast<int>(blockIdx.z) / G, g = static_cast<int>(blockIdx.z) % G;
@@ -1076,7 +1197,8 @@ __global__ __launch_bounds__(256) void gqa_prefill_paged_fp8_merge_kernel(PagedF
     f32x4 v[kBatch][4];
 #pragma unroll
     for (int y = 0; y < kBatch; ++y) {
-      const size_t at = min(x0 + y, cuts - 1) * step;
+      const int x = min(x0 + y, cuts - 1);
+      const size_t at = (TREE ? max(rec_step * x - 1, 0) : x) * step;
       m[y] = x0 + y < cuts ? ml[at] : -INFINITY;
       l[y] = ml[at + 1];
 #pragma unroll
@@ -1139,20 +1261,20 @@ size_t workspace_need(int T, int B, int Hkv, int group, int max_len, int* lanes,
   return plan_bytes(T, B, group, *lanes) + 2 * static_cast<size_t>(*lanes) * rec;
 }
 
-template <int D, bool TREE = false>
+template <int D>
 int launch(PagedFp8 c, Fp8PrefillArgs a, void* workspace, size_t workspace_bytes, hipStream_t st) {
   const size_t need = workspace_need<D>(a.T, a.B, c.Hkv, a.group, a.max_len, &a.lanes, &a.splits);
   const int tiles = static_cast<int>((static_cast<long>(a.T) * a.group + kRows - 1) / kRows);
   auto walk = [&](const PagedFp8& cache, const Fp8PrefillArgs& args) {
     // one request's last tile may be thin too, but is one of many then
-    const bool thin = !TREE && (a.B > 1 || static_cast<long>(a.T) * a.group <= kThinRows);
+    const bool thin = a.B > 1 || static_cast<long>(a.T) * a.group <= kThinRows;
     if (thin)
-      hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D, !TREE, TREE>), dim3(args.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, cache, args);
+      hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D, true, false>), dim3(args.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, cache, args);
     else
-      hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D, false, TREE>), dim3(args.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, cache, args);
+      hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D, false, false>), dim3(args.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, cache, args);
   };
   auto merge = [&](int cut_tiles) {
-    hipLaunchKernelGGL((gqa_prefill_paged_fp8_merge_kernel<D, TREE>), dim3(cut_tiles, c.Hkv, 4 * (D > 128 ? D / 128 : 1)), dim3(256), 0,
+    hipLaunchKernelGGL((gqa_prefill_paged_fp8_merge_kernel<D, false>), dim3(cut_tiles, c.Hkv, 4 * (D > 128 ? D / 128 : 1)), dim3(256), 0,
                        st, c, a);
   };
   if (a.B == 1) {
@@ -1180,24 +1302,37 @@ int launch(PagedFp8 c, Fp8PrefillArgs a, void* workspace, size_t workspace_bytes
     };
     // a thread a tile; few tiles: 4 waves, whose sums and barriers are shorter (us, a batch of
     // 32 with 91 tiles: 5.4 against 7.1)
-    if (a.B <= 256 && plan_items(a.T, a.B, a.group, 0) <= 256) plan(gqa_prefill_paged_fp8_plan_kernel<256, TREE>, 256);
-    else plan(gqa_prefill_paged_fp8_plan_kernel<1024, TREE>, 1024);
+    if (a.B <= 256 && plan_items(a.T, a.B, a.group, 0) <= 256) plan(gqa_prefill_paged_fp8_plan_kernel<256>, 256);
+    else plan(gqa_prefill_paged_fp8_plan_kernel<1024>, 1024);
     walk(c, a);
     merge(a.lanes);
   }
   return check_launch("gqa_prefill_paged_fp8");
 }
 
+// ---- drafted trees: the same walk under their masks -----------------------------
+size_t tree_units_bytes(int B) { return (static_cast<size_t>(B + 1) * sizeof(int) + 255) / 256 * 256; }
+template <int D>
+size_t tree_need(int B, int Hkv) {
+  return tree_units_bytes(B) + 2 * static_cast<size_t>(std::max(1, kCus / Hkv)) * Hkv * Cfg<D>::REC * sizeof(float);
+}
+
+template <int D>
+int launch_trees(const PagedFp8& c, Fp8PrefillArgs a, void* workspace, hipStream_t st) {
+  a.lanes = std::max(1, kCus / c.Hkv);
+  a.units = static_cast<int*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + tree_units_bytes(a.B));
+  hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D, false, true>), dim3(a.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, c, a);
+  const int tiles = static_cast<int>((std::min<long>(a.T, 32L * a.words32) * a.group + kRows - 1) / kRows);     // of a request at most
+  hipLaunchKernelGGL((gqa_prefill_paged_fp8_merge_kernel<D, true>), dim3(tiles * a.B, c.Hkv, 4 * (D > 128 ? D / 128 : 1)), dim3(256), 0, st,
+                     c, a);
+  return check_launch("gqa_tree_paged_fp8");
+}
+
 }  // namespace
 
-// Wide drafted trees walk as prompts do, under their masks.
-size_t tree_as_prefill_workspace(int D, int T, int B, int Hkv, int group, int max_len) {
-  int lanes, splits;
-  switch (D) {
-    case 64: return workspace_need<64>(T, B, Hkv, group, max_len, &lanes, &splits);
-    case 128: return workspace_need<128>(T, B, Hkv, group, max_len, &lanes, &splits);
-    default: return workspace_need<256>(T, B, Hkv, group, max_len, &lanes, &splits);
-  }
+size_t tree_as_prefill_workspace(int D, int B, int Hkv) {
+  return D == 64 ? tree_need<64>(B, Hkv) : D == 128 ? tree_need<128>(B, Hkv) : tree_need<256>(B, Hkv);
 }
 
 int tree_as_prefill(int D, const PagedFp8& c, const TreeCall& t, hipStream_t st) {
@@ -1212,11 +1347,7 @@ int tree_as_prefill(int D, const PagedFp8& c, const TreeCall& t, hipStream_t st)
   a.scale_log2 = kLog2e / sqrtf(static_cast<float>(D));
   a.mask = t.mask;
   a.words32 = t.words32;
-  switch (D) {
-    case 64: return launch<64, true>(c, a, t.workspace, t.workspace_bytes, st);
-    case 128: return launch<128, true>(c, a, t.workspace, t.workspace_bytes, st);
-    default: return launch<256, true>(c, a, t.workspace, t.workspace_bytes, st);
-  }
+  return D == 64 ? launch_trees<64>(c, a, t.workspace, st) : D == 128 ? launch_trees<128>(c, a, t.workspace, st) : launch_trees<256>(c, a, t.workspace, st);
 }
 
 }  // namespace aila

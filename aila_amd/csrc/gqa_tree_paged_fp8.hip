@@ -713,7 +713,7 @@ extern "C" size_t aila_hip_gqa_tree_paged_fp8_workspace_size(int T, int B, int H
   using namespace aila;
   if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || max_len < 0 || mask_words <= 0) return 0;
   if (D != 64 && D != 128 && D != 256) return 0;
-  if (walks_as_prompt(T, B, Hq / Hkv, D)) return tree_as_prefill_workspace(D, T, B, Hkv, Hq / Hkv, max_len);
+  if (walks_as_prompt(T, B, Hq / Hkv, D)) return tree_as_prefill_workspace(D, B, Hkv);
   switch (D) {
     case 64: return workspace_need<64>(T, B, Hkv, Hq / Hkv, mask_words, max_len);
     case 128: return workspace_need<128>(T, B, Hkv, Hq / Hkv, mask_words, max_len);
@@ -761,8 +761,8 @@ extern "C" int aila_hip_gqa_tree_paged_fp8(const void* q, long q_stride, const v
   a.max_len = max_len;
   a.scale_log2 = kLog2e / sqrtf(static_cast<float>(D));
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (walks_as_prompt(T, B, Hq / Hkv, D) && (workspace ? workspace_bytes : 0) >= tree_as_prefill_workspace(D, T, B, Hkv, Hq / Hkv, max_len))
-    return tree_as_prefill(D, c, TreeCall{a.q, q_stride, a.out, a.mask, a.words32, query_start, seq_lens, T, B, Hq, max_len, workspace, workspace_bytes}, st);
+  if (walks_as_prompt(T, B, Hq / Hkv, D) && workspace != nullptr && workspace_bytes >= tree_as_prefill_workspace(D, B, Hkv))
+    return tree_as_prefill(D, c, TreeCall{a.q, q_stride, a.out, a.mask, a.words32, query_start, seq_lens, T, B, Hq, max_len, workspace}, st);
   switch (D) {
     case 64: return launch<64>(c, a, mask_words, workspace, workspace_bytes, st);
     case 128: return launch<128>(c, a, mask_words, workspace, workspace_bytes, st);

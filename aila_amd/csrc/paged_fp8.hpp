@@ -346,10 +346,9 @@ struct TreeCall {
   const int* query_start;
   const int* seq_lens;
   int T, B, Hq, max_len;
-  void* workspace;
-  size_t workspace_bytes;
+  void* workspace;      // of at least tree_as_prefill_workspace bytes
 };
-size_t tree_as_prefill_workspace(int D, int T, int B, int Hkv, int group, int max_len);
+size_t tree_as_prefill_workspace(int D, int B, int Hkv);
 int tree_as_prefill(int D, const PagedFp8& c, const TreeCall& t, hipStream_t st);
 
 }  // namespace aila
