@@ -14,10 +14,21 @@
 //     rows' dims [D/32 m, D/32 (m + 1)) and pairs the rows' bytes with v_perm.
 // Codes go from memory to registers and are converted to bf16 there (exact,
 // unscaled: the scales are powers of two and go into the softmax's exponents).
+//
+// Up to some 40 columns a request it is bound by the bytes and their latency: 32 requests
+// of 6000 rows, 8 KV heads, D = 128, 8 columns, 99 us = 4.1 TB/s; wider trees are bound by
+// the conversions (64 codes a lane and strip) and the softmax on the vector ALU, 205
+// instructions a strip and tile for 512 cycles of products, and take the other walk
+// (walks_as_prompt, below). One sequence of 612 rows with 8 drafted tokens: 9.4 us and 3.9
+// of merge, which is start-up: lengths -> shares -> blocks -> codes.
+//
+// Tried and left: strips staged by DMA in LDS (no faster: 105 against 112 us for 32
+// requests of 26 tokens after 3000 rows), lines touched some strips ahead (129), raised
+// priority of either phase or wave (same), two tiles a wave at one wave a SIMD (the compiler
+// moves all accumulators through the vector registers in every strip).
 #include "paged_fp8.hpp"
 
 #include <algorithm>
-#include <cstdlib>
 
 namespace aila {
 namespace {
@@ -575,9 +586,44 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
   }
 }
 
-// Joins the records of an item that several workgroups walked: o = sum_i 2^(m_i -
-// M) acc_i / sum_i 2^(m_i - M) l_i. A workgroup takes kMergeCols columns of a
-// request and KV head; its other threads take other records.
+// The records of column y of a request and KV head that several workgroups walked:
+// those of the workgroups w0 .. w1, none if one wrote the output.
+struct Records { const float* at; int w0, w1; };
+template <int D>
+__device__ __forceinline__ Records records_of(const PagedFp8& c, const TreeArgs& a, const Shape& s, int b, int kvh, int y, int launched) {
+  const int index = min(y / (kTile * kWaves<D>), s.full);
+  const Item it = item_at<D>(s, index + (index == s.full && s.half > 0 && y >= kTile * (s.full * kWaves<D> + s.half) ? 1 : 0));
+  const int before = a.units[b], units = a.units[a.B] * c.Hkv, groups = min(launched, units);
+  const int first = before * c.Hkv + kvh * (a.units[b + 1] - before) + it.before;
+  // workgroup w holds unit x: the largest w with w U / W < x + 1
+  return Records{a.part + static_cast<size_t>(y - kTile * it.tile0) * (D + kRecTail),
+                 static_cast<int>((static_cast<long>(first + 1) * groups - 1) / units),
+                 static_cast<int>((static_cast<long>(first + it.units) * groups - 1) / units)};
+}
+
+// A thread's running sum over records.
+struct Joined {
+  f32x4 A = {0.f, 0.f, 0.f, 0.f};
+  float M = -INFINITY, L = 0.f;
+  __device__ __forceinline__ void add(const f32x4& v, float m, float l) {
+    const float mn = fmaxf(M, m);
+    const float fo = M == -INFINITY ? 0.f : fast_exp2(M - mn), fn = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+    A = A * fo + v * fn;
+    L = L * fo + l * fn;
+    M = mn;
+  }
+};
+template <int D>
+__device__ __forceinline__ void store_joined(const TreeArgs& a, const Shape& s, int kvh, int y, int d, const Joined& x) {
+  const float inv = x.L == 0.f ? 0.f : 1.0f / x.L;
+  const int tok = y / a.group;
+  *reinterpret_cast<u32x2*>(a.out + (static_cast<size_t>(s.q0 + tok) * a.Hq + kvh * a.group + y - tok * a.group) * D + d) =
+      u32x2{pack_bf16x2(x.A[0] * inv, x.A[1] * inv), pack_bf16x2(x.A[2] * inv, x.A[3] * inv)};
+}
+
+// Joins the records: o = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i. Few
+// requests, many records each: a workgroup takes kMergeCols columns of a request and
+// KV head, its other threads other records.
 constexpr int kMergeCols = 4, kMergeThreads = 256;
 template <int D>
 __global__ __launch_bounds__(kMergeThreads) void gqa_tree_paged_fp8_merge_kernel(PagedFp8 c, TreeArgs a, int launched) {
@@ -588,55 +634,63 @@ __global__ __launch_bounds__(kMergeThreads) void gqa_tree_paged_fp8_merge_kernel
   const Shape s = shape_of<D>(a, b);
   const int cols = s.n * a.group, x0 = static_cast<int>(blockIdx.z) * kMergeCols;
   if (x0 >= cols) return;
-  const int index = min(x0 / (kTile * kWaves<D>), s.full);
-  const Item it = item_at<D>(s, index + (index == s.full && s.half > 0 && x0 >= kTile * (s.full * kWaves<D> + s.half) ? 1 : 0));
-  const int before = a.units[b], units = a.units[a.B] * c.Hkv, groups = min(launched, units);
-  const int first = before * c.Hkv + kvh * (a.units[b + 1] - before) + it.before;
-  // workgroup w holds unit x: the largest w with w U / W < x + 1
-  const int w0 = static_cast<int>((static_cast<long>(first + 1) * groups - 1) / units);
-  const int w1 = static_cast<int>((static_cast<long>(first + it.units) * groups - 1) / units);
-  if (w0 == w1) return;   // one workgroup wrote the output
   const int d = static_cast<int>(threadIdx.x) % kQuads * 4, x = static_cast<int>(threadIdx.x) / kQuads % kMergeCols;
   const int ph = static_cast<int>(threadIdx.x) / (kQuads * kMergeCols);
   const int y = min(x0 + x, cols - 1);
-  const float* at = a.part + static_cast<size_t>(y - kTile * it.tile0) * (D + kRecTail);
+  const Records r = records_of<D>(c, a, s, b, kvh, y, launched);
+  if (r.w0 == r.w1) return;
   const size_t step = static_cast<size_t>(a.rec_cols) * (D + kRecTail);
-  f32x4 A = {0.f, 0.f, 0.f, 0.f};
-  float M = -INFINITY, L = 0.f;
-  for (int w = w0 + ph; w <= w1; w += kPhases) {
-    const float* r = at + (static_cast<size_t>(w) * 2 + (w == w0 ? 1 : 0)) * step;
-    const f32x4 v = *reinterpret_cast<const f32x4*>(r + d);
-    const float m = r[D], l = r[D + 1];
-    const float mn = fmaxf(M, m);
-    const float fo = M == -INFINITY ? 0.f : fast_exp2(M - mn), fn = m == -INFINITY ? 0.f : fast_exp2(m - mn);
-    A = A * fo + v * fn;
-    L = L * fo + l * fn;
-    M = mn;
+  Joined sum;
+  for (int w = r.w0 + ph; w <= r.w1; w += kPhases) {
+    const float* p = r.at + (static_cast<size_t>(w) * 2 + (w == r.w0 ? 1 : 0)) * step;
+    sum.add(*reinterpret_cast<const f32x4*>(p + d), p[D], p[D + 1]);
   }
   if constexpr (kPhases > 1) {
-    s_a[threadIdx.x] = A;
-    s_m[threadIdx.x] = M;
-    s_l[threadIdx.x] = L;
+    s_a[threadIdx.x] = sum.A;
+    s_m[threadIdx.x] = sum.M;
+    s_l[threadIdx.x] = sum.L;
     __syncthreads();
     if (ph > 0) return;
-    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kPhases; ++i) top = fmaxf(top, s_m[threadIdx.x + i * kQuads * kMergeCols]);
-    A = f32x4{0.f, 0.f, 0.f, 0.f};
-    L = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPhases; ++i) {
+    for (int i = 1; i < kPhases; ++i) {
       const int j = threadIdx.x + i * kQuads * kMergeCols;
-      const float f = s_m[j] == -INFINITY ? 0.f : fast_exp2(s_m[j] - top);
-      A += f * s_a[j];
-      L += f * s_l[j];
+      sum.add(s_a[j], s_m[j], s_l[j]);
     }
   }
-  if (x0 + x >= cols) return;
-  const float inv = L == 0.f ? 0.f : 1.0f / L;
-  const int tok = y / a.group;
-  *reinterpret_cast<u32x2*>(a.out + (static_cast<size_t>(s.q0 + tok) * a.Hq + kvh * a.group + y - tok * a.group) * D + d) =
-      u32x2{pack_bf16x2(A[0] * inv, A[1] * inv), pack_bf16x2(A[2] * inv, A[3] * inv)};
+  if (x0 + x < cols) store_joined<D>(a, s, kvh, y, d, sum);
+}
+
+// The same for many requests, few records each: a workgroup takes as many columns
+// as it has threads for, and kBatch records at a time (past the last: the last again,
+// with weight 0).
+template <int D>
+__global__ __launch_bounds__(kMergeThreads) void gqa_tree_paged_fp8_merge_few_kernel(PagedFp8 c, TreeArgs a, int launched) {
+  constexpr int kQuads = D / 4, kColumns = kMergeThreads / kQuads, kBatch = 4;
+  const int b = blockIdx.y, kvh = blockIdx.x;
+  const Shape s = shape_of<D>(a, b);
+  const int cols = s.n * a.group, x0 = static_cast<int>(blockIdx.z) * kColumns;
+  if (x0 >= cols) return;
+  const Records r = records_of<D>(c, a, s, b, kvh, x0, launched);      // the columns are one item's
+  if (r.w0 == r.w1) return;
+  const size_t step = static_cast<size_t>(a.rec_cols) * (D + kRecTail);
+  const int d = static_cast<int>(threadIdx.x) % kQuads * 4, x = min(static_cast<int>(threadIdx.x) / kQuads, cols - 1 - x0);
+  Joined sum;
+  for (int w = r.w0; w <= r.w1; w += kBatch) {
+    f32x4 v[kBatch];
+    float m[kBatch], l[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int u = min(w + i, r.w1);
+      const float* p = r.at + x * (D + kRecTail) + (static_cast<size_t>(u) * 2 + (u == r.w0 ? 1 : 0)) * step;
+      v[i] = *reinterpret_cast<const f32x4*>(p + d);
+      m[i] = w + i <= r.w1 ? p[D] : -INFINITY;
+      l[i] = p[D + 1];
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (w + i <= r.w1) sum.add(v[i], m[i], l[i]);
+  }
+  if (static_cast<int>(threadIdx.x) / kQuads < cols - x0) store_joined<D>(a, s, kvh, x0 + x, d, sum);
 }
 
 // The most that a request may have: columns, column tiles, items of a KV head.
@@ -693,16 +747,33 @@ int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t wor
   const size_t lds = static_cast<size_t>(kWaves<D>) * kTile * (kAccStride<D> + 2) * sizeof(float) +
                      (a.part ? static_cast<size_t>(a.B + 1) * sizeof(int) : 0);
   hipLaunchKernelGGL((gqa_tree_paged_fp8_kernel<D>), dim3(groups), dim3(kThreads), lds, st, c, a);
-  if (a.part)
+  if (a.part && static_cast<long>(a.B) * c.Hkv * merges > 2048)
+    hipLaunchKernelGGL((gqa_tree_paged_fp8_merge_few_kernel<D>), dim3(c.Hkv, a.B, (m.cols * (D / 4) + kMergeThreads - 1) / kMergeThreads), dim3(kMergeThreads), 0, st, c, a,
+                       static_cast<int>(groups));
+  else if (a.part)
     hipLaunchKernelGGL((gqa_tree_paged_fp8_merge_kernel<D>), dim3(c.Hkv, a.B, merges), dim3(kMergeThreads), 0, st, c, a,
                        static_cast<int>(groups));
   return check_launch("gqa_tree_paged_fp8");
 }
 
-bool walks_as_prompt(int T, int B, int group, int D) {
-  const char* e = getenv("TREE_WALK");
-  if (e) return e[0] == '1';
-  return D == 256 && static_cast<long>(T) * group > 64L * B;
+// Wide trees walk as prompts do, 128 columns a workgroup with their codes converted
+// once in LDS (gqa_prefill_paged_fp8.hip): from some columns a request on, which the
+// host knows on average, and the more of them the fewer requests share the device.
+// us, here / as prompts, trees of up to 16, 32, 64, 128 columns (two thirds of it on
+// average where there are more than one). D = 128: 1 request of 1000 rows 13/18, 15/18,
+// 16/18, 22/21, of 8000 20/28, 22/28, 24/29, 29/30; 8 of 1000 14/20, 16/20, 27/21, 31/25,
+// of 8000 32/44, 35/43, 40/44, 54/48; 32 of 1000 27/35, 32/36, 42/40, 53/45, of 8000 101/132,
+// 104/131, 126/138, 173/147. D = 64: 1 of 8000 14/21, 15/21, 17/23, 21/24; 8 of 8000 23/35,
+// 24/35, 29/35, 39/37; 32 of 8000 58/92, 59/91, 77/95, 118/97. D = 256: 1 of 8000 37/37,
+// 41/37, 44/39, 51/41; 8 of 8000 37/45, 43/46, 53/47, 73/55; 32 of 8000 96/128, 103/128,
+// 129/129, 192/144.
+bool walks_as_prompt(int T, int B, int Hkv, int group, int words, int max_len, int D) {
+  const long columns = static_cast<long>(T) * group;
+  const long each = D == 64 ? 70 : D == 128 ? 44 : 34, more = D == 64 ? 130 : D == 128 ? 72 : 16;
+  if (columns <= each * B + more) return false;
+  // its line of key tiles and its merge's threads have to fit
+  const long tiles = (std::min<long>(T, 64L * words) * group + 127) / 128 * B;
+  return tiles * (max_len / 32 + 16) < (1L << 31) && tiles * Hkv * 8 * 256 < (1L << 32);
 }
 
 }  // namespace
@@ -713,12 +784,12 @@ extern "C" size_t aila_hip_gqa_tree_paged_fp8_workspace_size(int T, int B, int H
   using namespace aila;
   if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || max_len < 0 || mask_words <= 0) return 0;
   if (D != 64 && D != 128 && D != 256) return 0;
-  if (walks_as_prompt(T, B, Hq / Hkv, D)) return tree_as_prefill_workspace(D, B, Hkv);
+  // enough for fewer tokens too, which may take the other walk
+  const size_t wide = walks_as_prompt(T, B, Hkv, Hq / Hkv, mask_words, max_len, D) ? tree_as_prefill_workspace(D, B, Hkv) : 0;
   switch (D) {
-    case 64: return workspace_need<64>(T, B, Hkv, Hq / Hkv, mask_words, max_len);
-    case 128: return workspace_need<128>(T, B, Hkv, Hq / Hkv, mask_words, max_len);
-    case 256: return workspace_need<256>(T, B, Hkv, Hq / Hkv, mask_words, max_len);
-    default: return 0;
+    case 64: return std::max(wide, workspace_need<64>(T, B, Hkv, Hq / Hkv, mask_words, max_len));
+    case 128: return std::max(wide, workspace_need<128>(T, B, Hkv, Hq / Hkv, mask_words, max_len));
+    default: return std::max(wide, workspace_need<256>(T, B, Hkv, Hq / Hkv, mask_words, max_len));
   }
 }
 
@@ -761,7 +832,7 @@ extern "C" int aila_hip_gqa_tree_paged_fp8(const void* q, long q_stride, const v
   a.max_len = max_len;
   a.scale_log2 = kLog2e / sqrtf(static_cast<float>(D));
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (walks_as_prompt(T, B, Hq / Hkv, D) && workspace != nullptr && workspace_bytes >= tree_as_prefill_workspace(D, B, Hkv))
+  if (walks_as_prompt(T, B, Hkv, Hq / Hkv, mask_words, max_len, D) && workspace != nullptr && workspace_bytes >= tree_as_prefill_workspace(D, B, Hkv))
     return tree_as_prefill(D, c, TreeCall{a.q, q_stride, a.out, a.mask, a.words32, query_start, seq_lens, T, B, Hq, max_len, workspace}, st);
   switch (D) {
     case 64: return launch<64>(c, a, mask_words, workspace, workspace_bytes, st);

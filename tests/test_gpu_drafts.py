@@ -263,18 +263,19 @@ def test_tree_that_is_a_chain_is_the_prefill():
     assert float((a.double() - b.double()).abs().max()) <= 4 * 2.0 ** -8 * float(b.double().abs().max())
 
 
-@pytest.mark.parametrize("D,Hq,Hkv", [(64, 8, 2), (128, 4, 4), (256, 16, 2)])
-def test_masked_drafts_may_hold_anything(D, Hq, Hkv):
+@pytest.mark.parametrize("D,Hq,Hkv,n", [(64, 8, 2, 40), (128, 4, 4, 40), (256, 16, 2, 40), (64, 8, 1, 150), (128, 16, 2, 70), (256, 4, 1, 40)])
+def test_masked_drafts_may_hold_anything(D, Hq, Hkv, n):
     """NaN codes in drafted rows reach the tokens that attend them and no others; rows behind the
     last and of pages that are not there reach none; a token that attends nothing gives 0."""
     import torch
     import aila_amd as A
-    page, new, before = 16, [40, 6], [50, 0]
+    page, new, before = 16, [n, 6], [50, 0]
     q, cache, table, starts, lens, mask, seen, rows = _tree_case(D, Hq, Hkv, page, new, before, 9, extra=0.2)
     kp, vp, ks, vs = cache
-    seen[40] = []                                    # request 1 has no rows before its draft
-    seen[41] = [1]
-    mask = dref.mask_words(seen + [[]] * 3, 1).cuda()
+    seen[n] = []                                    # request 1 has no rows before its draft
+    seen[n + 1] = [1]
+    words = -(-n // 64)
+    mask = dref.mask_words(seen + [[]] * 3, words).cuda()
     t = table.cpu().numpy()
     nan_tok = 7
     row = before[0] + nan_tok
@@ -285,19 +286,19 @@ def test_masked_drafts_may_hold_anything(D, Hq, Hkv):
     kp.view(torch.uint8)[t[0, end // page], :, end % page:] = 0x7f
     table[0, 1] = -1                                 # a page that is not there
     table[0, 2] = 10**6
-    for ws in (None, torch.empty(A.gqa_tree_paged_fp8_workspace_size(q.shape[0], 2, Hq, Hkv, D, max(rows), 1), dtype=torch.uint8, device="cuda")):
+    for ws in (None, torch.empty(A.gqa_tree_paged_fp8_workspace_size(q.shape[0], 2, Hq, Hkv, D, max(rows), words), dtype=torch.uint8, device="cuda")):
         out = A.gqa_tree_paged_fp8(q, *cache, table, starts, lens, mask, max(rows), workspace=ws).double().cpu()
-        sees = torch.tensor([nan_tok in s for s in seen[:40]])
-        assert 0 < int(sees.sum()) < 40
-        want = torch.zeros((40, Hq, D), dtype=torch.bool)
+        sees = torch.tensor([nan_tok in s for s in seen[:n]])
+        assert 0 < int(sees.sum()) < n
+        want = torch.zeros((n, Hq, D), dtype=torch.bool)
         want[sees, :, 3] = True
         want[sees, :Hq // Hkv, D - 1] = True
-        assert torch.equal(out[:40].isnan(), want)
-        assert bool((out[40] == 0).all()) and bool(out[41:46].isfinite().all())
+        assert torch.equal(out[:n].isnan(), want)
+        assert bool((out[n] == 0).all()) and bool(out[n + 1:n + 6].isfinite().all())
         clean = vp.clone()
         clean.view(torch.uint8)[t[0, row // page], :, row % page] = 0
         full = A.gqa_tree_paged_fp8(q, kp, clean, ks, vs, table, starts, lens, mask, max(rows), workspace=ws)
-        assert torch.equal(full[:40].double().cpu()[~sees], out[:40][~sees])
+        assert torch.equal(full[:n].double().cpu()[~sees], out[:n][~sees])
         _tree_check(full, q, (kp, clean, ks, vs), table, new, before, seen)
         k, held = ref.gather(kp, ks, table[0].cpu(), rows[0])
         assert int((~held).sum()) == 2 * page
