@@ -5,14 +5,24 @@
 //   y = x / sqrt(mean(x^2) + eps) * w
 //   (y_d, y_{d + rot/2}) turned by p theta^(-2 d / rot), d < rot / 2
 //
-// in fp32, rounded once: q to bf16, k by the append's rule to e4m3 (the calls for
-// one step each round k to bf16 twice on its way there). An angle is a product in
+// in fp32, rounded once: q to bf16, k by the append's rule to e4m3 (the calls
+// for the single steps round k to bf16 twice on its way there). An angle is a product in
 // fp64 of whole turns, taken modulo 1 there: at position 2^20 an fp32 product is
 // off by 2^-4 radians.
 //
 // A lane holds dims 4 s .. 4 s + 3 of both halves of the rotated part (or of the
-// rest), so a pair is never apart, at two 8-byte loads instead of one of 16.
+// rest), so a pair is never apart, at two 8-byte loads instead of one of 16. The
+// cosines and sines of a workgroup's tokens are made once, in LDS (each wave its own:
+// 1800 instructions a wave instead of 500 at D = 256).
+//
+// Bound by the bytes where there are many tokens: 8191, 16 / 4 heads, D = 256, rows
+// first 54.5 us for 184 MB = 3.4 TB/s (a large copy reaches 4.77; queries alone 31 us
+// = 4.3); by launch and the chain slots -> rows -> codes where there are few: 26
+// tokens, 32 / 8, D = 128, 6.2 us. Rows and queries interleaved in one launch were
+// slower (83 us for the 8191 tokens): what stores rows takes longest, and comes last.
 #include "paged_fp8.hpp"
+
+#include <type_traits>
 
 namespace aila {
 namespace {
@@ -20,8 +30,11 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 
-struct TurnTable {
-  double f[kMaxRopePairs];     // turns a position
+// Turns a position of pair j, r^j / (2 pi) with r = theta^(-2 / rot), from powers of r
+// that stay in scalar registers.
+struct Powers {
+  double base;       // 1 / (2 pi)
+  double bit[7];     // r, r^2, ..., r^64
 };
 
 struct PrepareArgs {
@@ -32,7 +45,7 @@ struct PrepareArgs {
   uint8_t *k_pages, *v_pages;
   float *k_scale, *v_scale;
   const int* slots;
-  const int *pos_t, *pos_h, *pos_w;
+  const int *pos_t, *pos_h, *pos_w;     // the same three times: one position
   int section_h, section_w;
   const float* inv_freq;
   int T, tile, Hq, Hkv, page_size, num_slots, rot;
@@ -59,30 +72,46 @@ struct Place { int lo, hi, j; bool turns; };
 template <int D>
 __device__ __forceinline__ Place place_of(int s, int rot) {
   const int x = 4 * s, half = rot / 2;
-  return x < half ? Place{x, x + half, x, true} : Place{x + half, x + D / 2, x, false};
+  return x < half ? Place{x, x + half, x, true} : Place{x + half, x + D / 2, 0, false};
+}
+
+// (cosine, sine) of the pairs of `count` tokens from `token` on, [token][pair] in LDS:
+// each once for the workgroup, whose waves all need the same.
+__device__ __forceinline__ void fill_turns(const PrepareArgs& a, const Powers& pw, int token, int count, f32x2* s_turn) {
+  const int half = a.rot / 2;
+  for (int i = threadIdx.x; i < count * half; i += kThreads) {
+    const int t = i / half, j = i - t * half, n = j / 3, m = j - 3 * n;
+    const int* from = a.pos_t;
+    if (m == 1 && n < a.section_h) from = a.pos_h;
+    if (m == 2 && n < a.section_w) from = a.pos_w;
+    double f;
+    if (a.inv_freq != nullptr) {
+      f = static_cast<double>(a.inv_freq[j]) * 0.15915494309189535;
+    } else {
+      f = pw.base;
+#pragma unroll
+      for (int b = 0; b < 7; ++b) f *= j >> b & 1 ? pw.bit[b] : 1.0;
+    }
+    double x = static_cast<double>(from[token + t]) * f;
+    x -= __builtin_rint(x);
+    float sn, cs;
+    sincospif(2.0f * static_cast<float>(x), &sn, &cs);
+    s_turn[i] = f32x2{cs, sn};
+  }
 }
 
 struct Turn { float c[4], s[4]; };
-__device__ __forceinline__ Turn turn_of(const PrepareArgs& a, const TurnTable& tt, const Place& p, int token) {
-  Turn r;
-  const int pt = a.pos_t[token];
-  int ph = pt, pw = pt;
-  if (a.pos_h != nullptr) {
-    ph = a.pos_h[token];
-    pw = a.pos_w[token];
-  }
+__device__ __forceinline__ Turn load_turn(const f32x2* p) {      // 16-byte aligned where rot is a multiple of 8
+  Turn t;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int j = p.j + i, m = j % 3, n = j / 3;
-    int pos = pt;
-    pos = m == 1 && n < a.section_h ? ph : pos;
-    pos = m == 2 && n < a.section_w ? pw : pos;
-    const double f = a.inv_freq != nullptr ? static_cast<double>(a.inv_freq[j]) * 0.15915494309189535 : tt.f[j];
-    double t = static_cast<double>(pos) * f;
-    t -= __builtin_rint(t);
-    sincospif(2.0f * static_cast<float>(t), &r.s[i], &r.c[i]);
+  for (int i = 0; i < 2; ++i) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(p + 2 * i);
+    t.c[2 * i] = x[0];
+    t.s[2 * i] = x[1];
+    t.c[2 * i + 1] = x[2];
+    t.s[2 * i + 1] = x[3];
   }
-  return r;
+  return t;
 }
 
 __device__ __forceinline__ void load4(const bf16* p, float* f) {
@@ -122,14 +151,16 @@ __device__ __forceinline__ void norm_turn(float* x, const float* w, const Turn& 
 
 // The queries of one token.
 template <int D>
-__device__ __forceinline__ void prepare_queries(const PrepareArgs& a, const TurnTable& tt, int token) {
+__device__ __forceinline__ void prepare_queries(const PrepareArgs& a, const Powers& pw, int token, f32x2* s_turn) {
   constexpr int LR = D / 8, RI = 64 / LR;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Place p = place_of<D>(lane % LR, a.rot);
   float w[8];
   load_weights(a.q_norm, p, w);
+  fill_turns(a, pw, token, 1, s_turn);
+  __syncthreads();
   Turn t{};
-  if (p.turns) t = turn_of(a, tt, p, token);
+  if (p.turns) t = load_turn(s_turn + p.j);
   const bf16* src = a.q + static_cast<size_t>(token) * a.q_stride;
   bf16* dst = a.q_out + static_cast<size_t>(token) * a.Hq * D;
   for (int h0 = wave * RI; h0 < a.Hq; h0 += kWaves * RI) {
@@ -154,13 +185,12 @@ __device__ __forceinline__ int scale_exp_f32(int bits) {
 // Rows into the pages: as the append (a wave takes K or V of a head, the runs that
 // begin in its tile of tokens), K normalised and turned on the way.
 template <int D>
-__device__ __forceinline__ void prepare_rows(const PrepareArgs& a, const TurnTable& tt, int bx, int by) {
+__device__ __forceinline__ void prepare_rows(const PrepareArgs& a, const Powers& pw, int bx, int by, f32x2* s_turn) {
   constexpr int LR = D / 8;
   constexpr int RI = 64 / LR;
   constexpr int NI = kScaleRows / RI;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int head = by * 2 + (wave >> 1);
-  if (head >= a.Hkv) return;
   const bool isv = wave & 1;
   const bf16* src = (isv ? a.v : a.k) + static_cast<size_t>(head) * D;
   const long stride = isv ? a.v_stride : a.k_stride;
@@ -180,16 +210,26 @@ __device__ __forceinline__ void prepare_rows(const PrepareArgs& a, const TurnTab
   const int before = __shfl_up(win, 1);
   const bool begins = lane >= 1 && lane <= a.tile && win >= 0 && win < a.num_slots &&
                       !(before >= 0 && before + 1 == win && win % kScaleRows != 0);
-  unsigned long long todo = __ballot(begins);
+  unsigned long long todo = __ballot(begins);      // the same in all waves
+  if (todo == 0) return;
+  // the run that begins at lane i: its tokens' slots go on, to the block's end
+  auto run_length = [&](int i) __attribute__((always_inline)) {
+    const int slot = __builtin_amdgcn_readlane(win, i);
+    const unsigned long long off = ~(__ballot(lane >= i && lane - i < kScaleRows - slot % kScaleRows && win == slot + (lane - i)) >> i);
+    return __builtin_ctzll(off);      // 1 .. 16 - slot % 16
+  };
+  const int i1 = 63 - __builtin_clzll(todo);
+  const int first = t0 + __builtin_ctzll(todo) - 1, last = t0 + i1 - 1 + run_length(i1);      // tokens of all runs: tile + 15 at most
+  fill_turns(a, pw, first, last - first, s_turn);
+  __syncthreads();
+  if (head >= a.Hkv) return;
   while (todo) {
     const int i = __builtin_ctzll(todo);
     todo &= todo - 1;
     const int t = t0 + i - 1;
     const int slot = __builtin_amdgcn_readlane(win, i);
     const int r0 = slot % kScaleRows;
-    // the run: the tokens from i on whose slots go on, to the block's end
-    const unsigned long long off = ~(__ballot(lane >= i && lane - i < kScaleRows - r0 && win == slot + (lane - i)) >> i);
-    const int n = __builtin_ctzll(off);      // 1 .. 16 - r0
+    const int n = run_length(i);
 
     const int page = slot / a.page_size, blk = slot % a.page_size / kScaleRows;
     const size_t bid = (static_cast<size_t>(page) * a.Hkv + head) * (a.page_size / kScaleRows) + blk;
@@ -209,7 +249,7 @@ __device__ __forceinline__ void prepare_rows(const PrepareArgs& a, const TurnTab
       if (k * RI >= n) break;
       if (!isv) {
         Turn r{};
-        if (p.turns) r = turn_of(a, tt, p, t + min(k * RI + rr, n - 1));
+        if (p.turns) r = load_turn(s_turn + (t - first + min(k * RI + rr, n - 1)) * (a.rot / 2) + p.j);
         norm_turn<D>(x[k], w, r, p.turns, a.eps);
       }
 #pragma unroll
@@ -255,29 +295,25 @@ __device__ __forceinline__ void prepare_rows(const PrepareArgs& a, const TurnTab
   }
 }
 
-template <int D>
-__global__ __launch_bounds__(kThreads) void prepare_qkv_paged_fp8_kernel(PrepareArgs a, TurnTable tt) {
+enum class Part { kBoth, kRows, kQueries };
+template <int D, Part P>
+__global__ __launch_bounds__(kThreads, P == Part::kQueries ? 8 : D == 256 ? 3 : 4) void prepare_qkv_paged_fp8_kernel(PrepareArgs a, Powers pw) {
+  extern __shared__ __attribute__((aligned(16))) f32x2 s_turn[];
   const int x = blockIdx.x;
-  if (x < a.kv_groups) {
+  if (P == Part::kRows || (P == Part::kBoth && x < a.kv_groups)) {
     const int pairs = (a.Hkv + 1) / 2;
-    prepare_rows<D>(a, tt, x / pairs, x % pairs);
+    prepare_rows<D>(a, pw, x / pairs, x % pairs, s_turn);
   } else {
-    prepare_queries<D>(a, tt, x - a.kv_groups);
+    prepare_queries<D>(a, pw, P == Part::kBoth ? x - a.kv_groups : x, s_turn);
   }
 }
 
-// Turns a position of each pair: theta^(-2 j / rot) / (2 pi).
-const TurnTable& turn_table(float theta, int rot) {
-  thread_local float last_theta = 0.f;
-  thread_local int last_rot = -1;
-  thread_local TurnTable t{};
-  if (theta != last_theta || rot != last_rot) {
-    for (int j = 0; j < rot / 2; ++j)
-      t.f[j] = std::pow(static_cast<double>(theta), -2.0 * j / rot) * 0.15915494309189535;
-    last_theta = theta;
-    last_rot = rot;
-  }
-  return t;
+Powers powers_of(float theta, int rot) {
+  Powers p{};
+  const double r = -2.0 / rot;
+  p.base = 0.15915494309189535;
+  for (int i = 0; i < 7; ++i) p.bit[i] = std::pow(static_cast<double>(theta), r * (1 << i));
+  return p;
 }
 
 }  // namespace
@@ -326,20 +362,37 @@ extern "C" int aila_hip_prepare_qkv_paged_fp8(const void* q, long q_stride, long
   a.v_pages = static_cast<uint8_t*>(v_pages);
   a.k_scale = k_scale; a.v_scale = v_scale;
   a.slots = slots;
-  a.pos_t = positions; a.pos_h = pos_h; a.pos_w = pos_w;
+  a.pos_t = positions;
+  a.pos_h = pos_h != nullptr ? pos_h : positions;
+  a.pos_w = pos_w != nullptr ? pos_w : positions;
   a.section_h = section_h; a.section_w = section_w;
   a.inv_freq = inv_freq;
   a.T = T; a.tile = tile; a.Hq = Hq; a.Hkv = Hkv; a.page_size = page_size; a.num_slots = num_pages * page_size;
   a.rot = rotary_dim;
   a.kv_groups = static_cast<int>(kv_groups);
   a.eps = eps;
-  static const TurnTable none{};
-  const TurnTable& tt = rotary_dim > 0 && inv_freq == nullptr ? turn_table(theta, rotary_dim) : none;
-  auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(kv_groups + T)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a, tt);
+  const Powers pw = rotary_dim > 0 && inv_freq == nullptr ? powers_of(theta, rotary_dim) : Powers{};
+  // One launch, rows first, or two (us, one / two). 16 / 4, D = 256: T = 32 7.1 / 10.1, 1024
+  // 11.7 / 15.9, 4096 (92 MB) 26.5 / 28.9, 8191 (184 MB) 66.5 / 54.5; 32 / 8, D = 128: 4096 25.2
+  // / 27.3, 8191 59.2 / 53.6; 16 / 8, D = 128: 8191 (117 MB) 36.7 / 36.2. Where the data do not
+  // stay in the caches, queries alone run at twice the waves a SIMD.
+  constexpr long kOneLaunchBytes = 120L << 20;
+  const long moved = static_cast<long>(T) * D * (4L * Hq + 6L * Hkv);
+  const size_t lds = static_cast<size_t>(tile + kScaleRows - 1) * (rotary_dim / 2) * sizeof(f32x2);
+  auto go = [&](auto kernel, long groups, size_t bytes) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(kThreads), bytes, static_cast<hipStream_t>(stream), a, pw);
   };
-  if (D == 64) go(prepare_qkv_paged_fp8_kernel<64>);
-  else if (D == 128) go(prepare_qkv_paged_fp8_kernel<128>);
-  else go(prepare_qkv_paged_fp8_kernel<256>);
+  auto launch = [&](auto d) {
+    constexpr int kD = decltype(d)::value;
+    if (moved <= kOneLaunchBytes) {
+      go(prepare_qkv_paged_fp8_kernel<kD, Part::kBoth>, kv_groups + T, lds);
+    } else {
+      go(prepare_qkv_paged_fp8_kernel<kD, Part::kRows>, kv_groups, lds);
+      go(prepare_qkv_paged_fp8_kernel<kD, Part::kQueries>, T, (rotary_dim / 2) * sizeof(f32x2));
+    }
+  };
+  if (D == 64) launch(std::integral_constant<int, 64>{});
+  else if (D == 128) launch(std::integral_constant<int, 128>{});
+  else launch(std::integral_constant<int, 256>{});
   return check_launch(what);
 }
