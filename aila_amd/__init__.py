@@ -9,6 +9,7 @@ is missing or fails to load, every call raises.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import math
 import os
@@ -883,24 +884,42 @@ def gqa_tree_paged_fp8(q, k_pages, v_pages, k_scale, v_scale, block_table, query
 
 
 def _layer_pointers(caches, dev):
-    """(layers, shape of a cache, the four host arrays of device pointers) of one
-    cache (k_pages, v_pages, k_scale, v_scale) or a list of such."""
+    """(layers, shape of a cache, addresses of the four host arrays of device
+    pointers, what keeps them) of one cache (k_pages, v_pages, k_scale, v_scale)
+    or a list of such."""
     import torch
     if not caches:
         raise ValueError("no caches")
     if torch.is_tensor(caches[0]):
         caches = [caches]
-    shape, ptrs = None, []
-    for kp, vp, ks, vs in caches:
-        got = _pages_ok(torch, dev, kp, vp, ks, vs)
-        if got is None or (shape is not None and got[0] != shape):
-            _need_pages(kp, vp, ks, vs)
-            _same_device(dev, kp, vp, ks, vs)
-            raise ValueError(f"caches: pages {tuple(kp.shape)} beside {tuple(shape)}" if shape is not None else "bad cache tensors")
-        shape = got[0]
-        ptrs.append(got[1])
-    n = len(ptrs)
-    return n, shape, [(_P * n)(*(p[i] for p in ptrs)) for i in range(4)]
+    # a hundred tensors in a deep stack: looked at attribute by attribute, in loops of C
+    n, flat = len(caches), [t for c in caches for t in c]
+    ok = len(flat) == 4 * n and all([t is not None for t in flat])
+    if ok:
+        shape, scales = flat[0].shape, flat[2].shape
+        pages, scale = flat[0::4] + flat[1::4], flat[2::4] + flat[3::4]
+        f8, f32 = torch.float8_e4m3fn, torch.float32
+        ok = len(shape) == 4 and not shape[2] % _SCALE_ROWS and scales == (shape[0], shape[1], shape[2] // _SCALE_ROWS) \
+            and [t.shape for t in pages] == [shape] * (2 * n) and [t.shape for t in scale] == [scales] * (2 * n) \
+            and all([t.dtype is f8 for t in pages]) and all([t.dtype is f32 for t in scale]) and all([t.is_contiguous() for t in flat]) \
+            and [t.get_device() for t in flat] == [dev] * (4 * n)
+    if ok:
+        ptrs = array.array("Q", [t.data_ptr() for t in pages + scale])
+        low = 0
+        for x in ptrs[:2 * n]:
+            low |= x
+        ok = not low & 15
+    if not ok:
+        for c in caches:
+            if len(c) != 4:
+                raise ValueError("a cache is (k_pages, v_pages, k_scale, v_scale)")
+            _need_pages(*c)
+            if c[0].shape != caches[0][0].shape:
+                raise ValueError(f"caches: pages {tuple(c[0].shape)} beside {tuple(caches[0][0].shape)}")
+            _same_device(dev, *c)
+        raise ValueError("bad cache tensors")
+    at = ptrs.buffer_info()[0]
+    return n, shape, (at, at + 8 * n, at + 16 * n, at + 24 * n), ptrs
 
 
 def kv_keep_paged_fp8(caches, block_table, cached_lens, kept, kept_lens, lens=None, stream=None):
@@ -919,7 +938,7 @@ def kv_keep_paged_fp8(caches, block_table, cached_lens, kept, kept_lens, lens=No
     most = kept.shape[1]
     if lens is None:
         lens = _new_out(lambda: torch.empty(B, dtype=i32, device=block_table.device), stream)
-    n, (P, Hkv, page_size, D), ptrs = _layer_pointers(caches, dev)
+    n, (P, Hkv, page_size, D), ptrs, kept_alive = _layer_pointers(caches, dev)  # noqa: F841
     one = (B,)
     if not (block_table.dtype is i32 and cached_lens.dtype is i32 and kept.dtype is i32 and kept_lens.dtype is i32 and lens.dtype is i32
             and cached_lens.shape == kept_lens.shape == lens.shape == one and kept.shape[0] == B and block_table.is_contiguous()
@@ -941,7 +960,8 @@ def kv_keep_paged_fp8(caches, block_table, cached_lens, kept, kept_lens, lens=No
 
 def kv_pages_trim(lens, block_table, free_pages, free_count, page_size: int, stream=None):
     """Push the pages behind each request's rows (lens int32 [B]; negative: leave
-    the row alone) back onto the free stack; their table entries become -1."""
+    the row alone), up to the first entry that holds none, back onto the free
+    stack; their table entries become -1."""
     import torch
     B, max_pages = block_table.shape
     i32 = torch.int32
@@ -971,7 +991,7 @@ def kv_copy_paged_fp8(caches, block_table, src, dst, lens, max_len: int, stream=
     dev = _device_of(stream)
     B, max_pages = block_table.shape
     i32 = torch.int32
-    n, (P, Hkv, page_size, D), ptrs = _layer_pointers(caches, dev)
+    n, (P, Hkv, page_size, D), ptrs, kept_alive = _layer_pointers(caches, dev)  # noqa: F841
     pairs = src.numel()
     one = (pairs,)
     if not (block_table.dtype is i32 and src.dtype is i32 and dst.dtype is i32 and lens.dtype is i32

@@ -6,6 +6,7 @@
 #include "paged_fp8.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace aila {
 namespace {
@@ -32,94 +33,127 @@ struct KeepArgs {
   int B, most, max_pages, num_pages, Hkv, page_size;
 };
 
-// One wave: K or V of one head of one request and layer. Blocks from the one of
-// the first row that moves, in order: a row comes from behind its place (kept
+// A wave: K or V of heads of one request and layer, kHeads at a time with their loads
+// in flight; the request's lengths and places are looked up once. Blocks from the one
+// of the first row that moves, in order: a row comes from behind its place (kept
 // indices rise), so a block that has been written holds no later block's source.
 constexpr int kKeepThreads = 256;
+constexpr long kKeepGroups = 1024;
 constexpr int kNone = kMinScaleExp - 1;
-template <int D>
+template <int D, int kHeads>
 __global__ __launch_bounds__(kKeepThreads) void kv_keep_paged_fp8_kernel(Layers ly, KeepArgs a) {
   constexpr int LR = D / 16;                // lanes of a row, 16 codes each
   constexpr int RI = 64 / LR;               // rows of an instruction
   constexpr int NI = kScaleRows / RI;       // instructions of a block
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int b = blockIdx.y;
-  const int hv = static_cast<int>(blockIdx.x) * (kKeepThreads / 64) + wave;   // head, K or V
+  const int step = static_cast<int>(gridDim.x) * (kKeepThreads / 64 / 2);            // heads from a wave's to its next
+  const int head0 = static_cast<int>(blockIdx.x) * (kKeepThreads / 64 / 2) + (wave >> 1);
   const int cached = a.cached[b];
   const long max_rows = static_cast<long>(a.max_pages) * a.page_size;
   int n = min(max(a.kept_lens[b], 0), a.most);
+  const int* kept = a.kept + static_cast<size_t>(b) * a.most;
+  const int mine = lane < a.most ? kept[lane] : lane;
   if (cached < 0) n = 0;
   else n = static_cast<int>(min(static_cast<long>(n), max(max_rows - cached, 0L)));
   if (a.lens != nullptr && blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.lens[b] = cached + n;
-  if (hv >= 2 * a.Hkv || n == 0) return;
-  const int* kept = a.kept + static_cast<size_t>(b) * a.most;
   int first = n;      // rows before it stay where they are
   for (int i0 = 0; i0 < n; i0 += 64) {
     const int i = i0 + lane;
-    const unsigned long long off = __ballot(i < n && kept[i] != i);
+    const unsigned long long off = __ballot(i < n && (i0 == 0 ? mine : kept[i]) != i);
     if (off) {
       first = i0 + __builtin_ctzll(off);
       break;
     }
   }
   if (first == n) return;
-  const int head = hv >> 1, arr = 2 * blockIdx.z + (hv & 1);
+  const int arr = 2 * blockIdx.z + (wave & 1);
   uint8_t* pages = ly.pages[arr];
   float* scale = ly.scale[arr];
   const int* row_table = a.table + static_cast<size_t>(b) * a.max_pages;
   const int page_blocks = a.page_size / kScaleRows;
-  // block of a row in the pool, -1: none
+  // block of a row in the pool for head 0, -1: none
   auto block_of = [&](long row) __attribute__((always_inline)) -> int {
     if (row < 0 || row >= max_rows) return -1;
     const int r = static_cast<int>(row), p = r / a.page_size;
     const int page = row_table[p];
-    return page >= 0 && page < a.num_pages ? (page * a.Hkv + head) * page_blocks + (r - p * a.page_size) / kScaleRows : -1;
+    return page >= 0 && page < a.num_pages ? page * a.Hkv * page_blocks + (r - p * a.page_size) / kScaleRows : -1;
   };
   const int rr = lane / LR, c16 = lane % LR * 16;
   const int end = cached + n;
   for (int at = (cached + first) / kScaleRows * kScaleRows; at < end; at += kScaleRows) {
-    const int bid = block_of(at);
-    if (bid < 0) continue;
-    uint8_t* block = pages + static_cast<size_t>(bid) * (kScaleRows * D);
-    const int held = held_exp(scale[bid]);
-    u32x4 w[NI];
-    int e_from[NI];
-    bool moves[NI], stays[NI];
-    int top = kNone;
+    const int bid0 = block_of(at);
+    if (bid0 < 0) continue;
+    // where this lane's rows come from: head 0's block, byte in it
+    int from[NI], byte[NI];
+    bool moves[NI], stays[NI], any = false;
 #pragma unroll
     for (int k = 0; k < NI; ++k) {
-      const int j = k * RI + rr, row = at + j, i = row - cached;
+      const int j = k * RI + rr, i = at + j - cached;
       stays[k] = i < first;
       moves[k] = !stays[k] && i < n;
-      w[k] = u32x4{0u, 0u, 0u, 0u};
-      e_from[k] = held;
+      from[k] = bid0;
+      byte[k] = j * D + c16;
       if (moves[k]) {
-        const long src = static_cast<long>(cached) + kept[i];
-        const int sb = kept[i] < 0 ? -1 : block_of(src);
+        const int src = kept[i];
+        const int sb = src < 0 ? -1 : block_of(static_cast<long>(cached) + src);
         moves[k] = sb >= 0;
         if (sb >= 0) {
-          e_from[k] = held_exp(scale[sb]);
-          w[k] = ld16(pages + static_cast<size_t>(sb) * (kScaleRows * D) + (src % kScaleRows) * D + c16);
+          from[k] = sb;
+          byte[k] = static_cast<int>((static_cast<long>(cached) + src) % kScaleRows) * D + c16;
         }
-      } else if (stays[k]) {
-        w[k] = ld16(block + j * D + c16);
       }
-      if (moves[k] || stays[k]) top = max(top, e_from[k]);
+      any |= moves[k] || stays[k];
     }
-    const int e = wave_max(top);
-    if (e == kNone) continue;     // no row of it is in range
+    if (__ballot(any) == 0) continue;     // no row of it is in range
+    for (int h0 = head0; h0 < a.Hkv; h0 += kHeads * step) {
+      u32x4 w[kHeads][NI];
+      float s_from[kHeads][NI], s_held[kHeads];
 #pragma unroll
-    for (int k = 0; k < NI; ++k) {
-      if (moves[k] || (stays[k] && e != held)) {
-        if (e != e_from[k]) {
-          const float f = pow2f(e_from[k] - e);
+      for (int x = 0; x < kHeads; ++x) {
+        const int off = min(h0 + x * step, a.Hkv - 1) * page_blocks;     // past the last: the last again, not stored
+        s_held[x] = scale[bid0 + off];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) w[k][x] = scale_codes(w[k][x], f);
+        for (int k = 0; k < NI; ++k) {
+          s_from[x][k] = 0.f;
+          w[x][k] = u32x4{0u, 0u, 0u, 0u};
+          if (moves[k]) {
+            s_from[x][k] = scale[from[k] + off];
+            w[x][k] = ld16(pages + static_cast<size_t>(from[k] + off) * (kScaleRows * D) + byte[k]);
+          }
         }
-        *reinterpret_cast<u32x4*>(block + (k * RI + rr) * D + c16) = w[k];
+      }
+#pragma unroll
+      for (int x = 0; x < kHeads; ++x) {
+        if (h0 + x * step >= a.Hkv) break;
+        const int bid = bid0 + (h0 + x * step) * page_blocks;
+        const int held = held_exp(s_held[x]);
+        int top = kNone;
+#pragma unroll
+        for (int k = 0; k < NI; ++k)
+          if (moves[k] || stays[k]) top = max(top, stays[k] ? held : held_exp(s_from[x][k]));
+        const int e = wave_max(top);
+        uint8_t* block = pages + static_cast<size_t>(bid) * (kScaleRows * D);
+        if (e != held) {      // the rows that stay change scale too
+#pragma unroll
+          for (int k = 0; k < NI; ++k)
+            if (stays[k]) w[x][k] = ld16(block + byte[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+          if (moves[k] || (stays[k] && e != held)) {
+            const int e_from = stays[k] ? held : held_exp(s_from[x][k]);
+            if (e != e_from) {
+              const float f = pow2f(e_from - e);
+#pragma unroll
+              for (int y = 0; y < 4; ++y) w[x][k][y] = scale_codes(w[x][k][y], f);
+            }
+            *reinterpret_cast<u32x4*>(block + (k * RI + rr) * D + c16) = w[x][k];
+          }
+        }
+        if (lane == 0) scale[bid] = pow2f(e);
       }
     }
-    if (lane == 0) scale[bid] = pow2f(e);
   }
 }
 
@@ -199,20 +233,26 @@ extern "C" int aila_hip_kv_keep_paged_fp8(void* const* k_pages, void* const* v_p
                max_pages);
   AILA_REQUIRE(lens != cached_lens && lens != kept_lens, "kv_keep_paged_fp8: the lengths going out may not overwrite those coming in");
   KeepArgs a{block_table, cached_lens, kept, kept_lens, lens, B, max_kept, max_pages, num_pages, Hkv, page_size};
-  const unsigned gx = (2 * Hkv + kKeepThreads / 64 - 1) / (kKeepThreads / 64);
+  const unsigned most_gx = (Hkv + 1) / 2;      // a head a wave
   // fewer than 2^32 threads, the most of a launch
-  const long fit = ((1L << 32) - 1) / kKeepThreads / gx / B;
+  const long fit = ((1L << 32) - 1) / kKeepThreads / most_gx / B;
   AILA_REQUIRE(fit > 0, "kv_keep_paged_fp8: B=%d requests of %d heads are too many", B, Hkv);
   const int step = static_cast<int>(std::min<long>(kMaxLayers, fit));
   for (int l0 = 0; l0 < layers; l0 += step) {
     const int n = std::min(step, layers - l0);
     const Layers ly = some_layers(k_pages, v_pages, k_scale, v_scale, l0, n);
-    auto go = [&](auto kernel) {
+    const bool many = static_cast<long>(B) * n * most_gx > kKeepGroups;
+    auto go = [&](auto kernel, unsigned gx) {
       hipLaunchKernelGGL(kernel, dim3(gx, B, n), dim3(kKeepThreads), 0, static_cast<hipStream_t>(stream), ly, a);
     };
-    if (D == 64) go(kv_keep_paged_fp8_kernel<64>);
-    else if (D == 128) go(kv_keep_paged_fp8_kernel<128>);
-    else go(kv_keep_paged_fp8_kernel<256>);
+    auto launch = [&](auto d) {
+      constexpr int kD = decltype(d)::value;
+      if (many) go(kv_keep_paged_fp8_kernel<kD, 4>, (most_gx + 3) / 4);
+      else go(kv_keep_paged_fp8_kernel<kD, 1>, most_gx);
+    };
+    if (D == 64) launch(std::integral_constant<int, 64>{});
+    else if (D == 128) launch(std::integral_constant<int, 128>{});
+    else launch(std::integral_constant<int, 256>{});
     a.lens = nullptr;
   }
   return check_launch("kv_keep_paged_fp8");

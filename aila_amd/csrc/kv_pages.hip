@@ -306,8 +306,13 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_release_kernel(const in
   if (tid == 0) *free_count = min(have + sum, num_pages);
 }
 
-// Entries from lens[b] rows on go onto the stack in order of request and page.
-// As the release, but every row is looked at, from the page behind its rows.
+// Entries from lens[b] rows on, up to the first that holds no page, go onto the
+// stack in order of request and page. 16 lanes look at a row's next 16 entries, which
+// are more than a draft takes as a rule; 256 rows are looked at in one round trip, and
+// what was read is kept while the counts are summed. (A wave a row, all entries to the
+// table's end: 256 rows of up to 516 pages 26.4 us against 4.4.)
+constexpr int kTrimLanes = 16, kTrimRows = 4;                        // of a row; rows of 16 lanes
+constexpr int kTrimBatch = kPlanThreads / kTrimLanes * kTrimRows;    // rows looked at together
 __global__ __launch_bounds__(kPlanThreads) void kv_pages_trim_kernel(const int* __restrict__ lens, int* table,
                                                                      int* free_pages, int* free_count, int B,
                                                                      int max_pages, int page_size, int num_pages) {
@@ -315,7 +320,8 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_trim_kernel(const int* 
   int* s_from = s_dyn;         // [B] first entry looked at
   int* s_at = s_from + B;      // [B + 1] entries of the rows before
   __shared__ int s_wi[kPlanWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid % kTrimLanes, group = tid / kTrimLanes;
+  const int shift = tid & 63 & ~(kTrimLanes - 1);                    // this row's lanes in a ballot
   const int have = min(max(*free_count, 0), num_pages);
   for (int b = tid; b < B; b += kPlanThreads) {
     const int len = lens[b];
@@ -323,22 +329,37 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_trim_kernel(const int* 
   }
   if (tid == 0) s_at[0] = 0;
   __syncthreads();
-  int v[kRowChunk];
-  auto read = [&](const int* row, int p0) __attribute__((always_inline)) {
+  int v[kTrimRows];
+  auto entry = [&](int b, int p) __attribute__((always_inline)) {
+    return b < B && p < max_pages ? table[static_cast<size_t>(b) * max_pages + p] : -1;
+  };
+  auto row_of = [&](int b0, int r) __attribute__((always_inline)) { return b0 + r * (kPlanThreads / kTrimLanes) + group; };
+  auto look = [&](int b0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kRowChunk; ++i) {
-      const int p = p0 + 64 * i + lane;
-      v[i] = p < max_pages ? row[p] : -1;
+    for (int r = 0; r < kTrimRows; ++r) {
+      const int b = row_of(b0, r);
+      v[r] = entry(b, s_from[min(b, B - 1)] + lane);
     }
   };
-  for (int b = wave; b < B; b += kPlanWaves) {
-    int n = 0;
-    for (int p0 = s_from[b]; p0 < max_pages; p0 += 64 * kRowChunk) {
-      read(table + static_cast<size_t>(b) * max_pages, p0);
+  // entries in front of the first that holds no page, of the row's 16
+  auto held = [&](int x) __attribute__((always_inline)) {
+    const unsigned bits = static_cast<unsigned>(__ballot(x >= 0) >> shift) & ((1u << kTrimLanes) - 1);
+    return static_cast<int>(__builtin_ctz(~bits));
+  };
+  for (int b0 = 0; b0 < B; b0 += kTrimBatch) {
+    look(b0);
 #pragma unroll
-      for (int i = 0; i < kRowChunk; ++i) n += __popcll(__ballot(v[i] >= 0));
+    for (int r = 0; r < kTrimRows; ++r) {
+      const int b = row_of(b0, r);
+      int n = held(v[r]), more = n;
+      for (int p = 0; __ballot(more == kTrimLanes) != 0;) {           // a long run, of some row of the wave
+        p += kTrimLanes;
+        const int x = more == kTrimLanes ? entry(b, s_from[b] + p + lane) : -1;
+        more = held(x);
+        n += more;
+      }
+      if (b < B && lane == 0) s_at[b + 1] = n;
     }
-    if (lane == 0) s_at[b + 1] = n;
   }
   __syncthreads();
   int sum = 0;
@@ -351,21 +372,18 @@ __global__ __launch_bounds__(kPlanThreads) void kv_pages_trim_kernel(const int* 
     sum += all;
   }
   __syncthreads();
-  for (int b = wave; b < B; b += kPlanWaves) {
-    if (s_at[b + 1] == s_at[b]) continue;
-    int at = have + s_at[b];
-    int* row = table + static_cast<size_t>(b) * max_pages;
-    for (int p0 = s_from[b]; p0 < max_pages; p0 += 64 * kRowChunk) {
-      read(row, p0);
+  for (int b0 = 0; b0 < B; b0 += kTrimBatch) {
+    if (B > kTrimBatch) look(b0);
 #pragma unroll
-      for (int i = 0; i < kRowChunk; ++i) {
-        const unsigned long long held = __ballot(v[i] >= 0);
-        if (v[i] >= 0) {
-          const int j = at + __popcll(held & ((1ull << lane) - 1));
-          if (j < num_pages) free_pages[j] = v[i];
-          row[p0 + 64 * i + lane] = -1;
-        }
-        at += __popcll(held);
+    for (int r = 0; r < kTrimRows; ++r) {
+      const int b = row_of(b0, r);
+      if (b >= B) continue;
+      const int n = s_at[b + 1] - s_at[b];
+      for (int p = lane; p < n; p += kTrimLanes) {
+        const size_t at = static_cast<size_t>(b) * max_pages + s_from[b] + p;
+        const int page = p < kTrimLanes ? v[r] : table[at], j = have + s_at[b] + p;
+        if (j < num_pages) free_pages[j] = page;
+        table[at] = -1;
       }
     }
   }

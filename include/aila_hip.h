@@ -454,7 +454,7 @@ int aila_hip_gqa_prefill_paged_fp8(const void* q, long q_stride,
  *   y = x / sqrt(mean(x^2) + eps) * w, w = q_norm_w / k_norm_w [D] bf16 (NULL: 1)
  *   dims d and d + rotary_dim / 2 of y are turned by p * theta^(-2 d / rotary_dim)
  *   (inv_freq, device float[rotary_dim / 2]: by p * inv_freq[d]), d < rotary_dim / 2
- * The angle is exact to 2^-52 of itself before it is reduced, and there is one
+ * The angle is exact to 2^-49 of itself before it is reduced, and there is one
  * rounding: q to bf16, k by the rule of aila_hip_kv_append_paged_fp8, which holds
  * for the (unrounded) y here; v as there.
  *   q        head h of token t at + t * q_stride + h * q_head_stride elements
@@ -538,9 +538,10 @@ int aila_hip_kv_keep_paged_fp8(void* const* k_pages, void* const* v_pages,
                                int num_pages, int max_pages, void* stream);
 
 /* Give back the pages behind each request's rows: the entries p >= lens[b] /
- * page_size (rounded up) of row b of block_table that hold a page (>= 0) are pushed
- * onto the stack in order of request and page and become -1. lens[b] < 0: the row is
- * left alone. B <= 2048. Calls on one stack must not overlap in time. */
+ * page_size (rounded up) of row b of block_table, up to the first that holds no page
+ * (< 0; aila_hip_kv_pages_reserve leaves none in between), are pushed onto the stack
+ * in order of request and page and become -1. lens[b] < 0: the row is left alone. B
+ * <= 2048. Calls on one stack must not overlap in time. */
 int aila_hip_kv_pages_trim(const int* lens, int* block_table, int* free_pages,
                            int* free_count, int B, int max_pages, int page_size,
                            int num_pages, void* stream);

@@ -141,10 +141,12 @@ def copy(cache, table, src, dst, lens, max_len, page):
 def trim(lens, table, free, count, page):
     table, free = [list(r) for r in table], list(free)
     for b, n in enumerate(lens):
-        for p, e in enumerate(table[b]):
-            if n >= 0 and p >= -(-n // page) and e >= 0:
-                if count < len(free):
-                    free[count] = e
-                    count += 1
-                table[b][p] = -1
+        for p in range(-(-n // page) if n >= 0 else len(table[b]), len(table[b])):
+            e = table[b][p]
+            if e < 0:
+                break
+            if count < len(free):
+                free[count] = e
+                count += 1
+            table[b][p] = -1
     return table, free, count
