@@ -53,7 +53,7 @@ struct TreeArgs {
   const int* seq_lens;
   int T, B, Hq, group;
   int max_len;
-  int chunks;                          // most items of a request and KV head
+  int chunks;                          // without a split: workgroups of a request and KV head
   int rec_cols;                        // columns of a record
   float scale_log2;
 };
@@ -403,10 +403,11 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m32 = lane & 31, hf = lane >> 5;
 
-  int u, u1;
+  int u, u1, index = 0;
   if (a.part == nullptr) {
-    u = blockIdx.x;       // (request, KV head, item) here
+    u = blockIdx.x;       // (request, KV head, first item) here
     u1 = u + 1;
+    index = u % a.chunks;
   } else {
     scan_units<D>(a, s_pre);
     const int units = s_pre[a.B] * c.Hkv, groups = min(static_cast<int>(gridDim.x), units);
@@ -422,15 +423,14 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
     Shape s;
     Item it;
     if (a.part == nullptr) {
-      b = u / (c.Hkv * a.chunks);
-      const int hi = u % (c.Hkv * a.chunks);
-      kvh = hi / a.chunks;
+      kvh = u / a.chunks % c.Hkv;
+      b = u / a.chunks / c.Hkv;
       s = shape_of<D>(a, b);
-      if (hi % a.chunks >= item_count(s)) return;
-      it = item_at<D>(s, hi % a.chunks);
+      if (index >= item_count(s)) return;
+      it = item_at<D>(s, index);
+      index += a.chunks;
       i0 = 0;
       i1 = it.units;
-      u = u1;
     } else {
       b = __builtin_amdgcn_readfirstlane(find_request(s_pre, a.B, u / c.Hkv));
       s = shape_of<D>(a, b);
@@ -723,10 +723,24 @@ size_t workspace_need(int T, int B, int Hkv, int group, int words, int max_len) 
   return units_bytes(B) + std::max(2L, split_groups<D>(B, Hkv, m, max_len)) * record_bytes<D>(m);
 }
 
+// Whether a request and KV head is one workgroup's, for all keys: up to a length that
+// grows with the CUs they fill. us in a graph, whole / split, trees of up to 4 tokens,
+// lengths between half the bound and all of it. D = 128, 8 KV heads of 4: 1 request of 500
+// rows 10.6 / 12.7, 1000 13.0 / 13.1, 2000 17.8 / 13.9; 4 of 1000 13.2 / 13.4, 2000 18.0 /
+// 15.3; 16 of 2000 19.6 / 25.0, 4000 29.3 / 30.6; 32 of 2000 25.0 / 34.2, 4000 51.9 / 58.9. D
+// = 64: 1 of 1000 10.2 / 11.1, 2000 13.6 / 11.6; 32 of 4000 24.6 / 31.5. D = 256, 4 heads: 1 of
+// 500 15.7 / 15.6, 1000 21.8 / 17.0; 16 of 1000 22.8 / 24.8, 2000 34.9 / 29.6; 32 of 1000 23.5 /
+// 29.3, 2000 35.9 / 34.5.
+bool walks_whole(int B, int Hkv, int max_len, int D) {
+  const long items = static_cast<long>(B) * Hkv;
+  return max_len <= (D == 256 ? std::min(2048L, 450 + 10 * items) : std::min(4096L, 900 + 16 * items));
+}
+
 template <int D>
 int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t workspace_bytes, hipStream_t st) {
   const Most m = most_of<D>(a.T, words, a.group);
-  a.chunks = m.items;
+  // a workgroup for each item that a request of average size has
+  a.chunks = static_cast<int>(std::min<long>(m.items, (static_cast<long>(a.T) * a.group + 32L * kWaves<D> * a.B - 1) / (32L * kWaves<D> * a.B)));
   a.rec_cols = m.rec_cols;
   constexpr int kThreads = 64 * kWaves<D>;
   const long items = static_cast<long>(a.B) * c.Hkv * m.items;
@@ -734,15 +748,17 @@ int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t wor
                "gqa_tree_paged_fp8: B=%d requests of up to %ld query rows and %d keys are too many", a.B, m.cols, a.max_len);
   const long merges = (m.cols + kMergeCols - 1) / kMergeCols;
   AILA_REQUIRE(merges <= 65535, "gqa_tree_paged_fp8: %ld query rows of a KV head are too many", m.cols);
-  long groups = items;
+  long groups = static_cast<long>(a.B) * c.Hkv * a.chunks;
   if (workspace != nullptr) {
     const size_t rec = record_bytes<D>(m);
     if (workspace_bytes < units_bytes(a.B) + 2 * rec)
       return set_error(AILA_HIP_EWORKSPACE, "gqa_tree_paged_fp8: workspace %zu bytes, %zu are the least", workspace_bytes,
                        units_bytes(a.B) + 2 * rec);
-    groups = std::min<long>(split_groups<D>(a.B, c.Hkv, m, a.max_len), static_cast<long>((workspace_bytes - units_bytes(a.B)) / rec));
-    a.units = static_cast<int*>(workspace);
-    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + units_bytes(a.B));
+    if (!walks_whole(a.B, c.Hkv, a.max_len, D)) {
+      groups = std::min<long>(split_groups<D>(a.B, c.Hkv, m, a.max_len), static_cast<long>((workspace_bytes - units_bytes(a.B)) / rec));
+      a.units = static_cast<int*>(workspace);
+      a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + units_bytes(a.B));
+    }
   }
   const size_t lds = static_cast<size_t>(kWaves<D>) * kTile * (kAccStride<D> + 2) * sizeof(float) +
                      (a.part ? static_cast<size_t>(a.B + 1) * sizeof(int) : 0);
@@ -759,18 +775,22 @@ int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t wor
 // Wide trees walk as prompts do, 128 columns a workgroup with their codes converted
 // once in LDS (gqa_prefill_paged_fp8.hip): from some columns a request on, which the
 // host knows on average, and the more of them the fewer requests share the device.
-// us, here / as prompts, trees of up to 16, 32, 64, 128 columns (two thirds of it on
-// average where there are more than one). D = 128: 1 request of 1000 rows 13/18, 15/18,
-// 16/18, 22/21, of 8000 20/28, 22/28, 24/29, 29/30; 8 of 1000 14/20, 16/20, 27/21, 31/25,
-// of 8000 32/44, 35/43, 40/44, 54/48; 32 of 1000 27/35, 32/36, 42/40, 53/45, of 8000 101/132,
-// 104/131, 126/138, 173/147. D = 64: 1 of 8000 14/21, 15/21, 17/23, 21/24; 8 of 8000 23/35,
-// 24/35, 29/35, 39/37; 32 of 8000 58/92, 59/91, 77/95, 118/97. D = 256: 1 of 8000 37/37,
-// 41/37, 44/39, 51/41; 8 of 8000 37/45, 43/46, 53/47, 73/55; 32 of 8000 96/128, 103/128,
+// us, here split / as prompts, trees of up to 16, 32, 64, 128 columns (two thirds of it
+// on average where there are more than one), 8000 rows. D = 128: 1 request 20/28, 22/28,
+// 24/29, 29/30; 8 32/44, 35/43, 40/44, 54/48; 32 101/132, 104/131, 126/138, 173/147. D = 64:
+// 1 14/21, 15/21, 17/23, 21/24; 8 23/35, 24/35, 29/35, 39/37; 32 58/92, 59/91, 77/95, 118/97.
+// D = 256: 1 37/37, 41/37, 44/39, 51/41; 8 37/45, 43/46, 53/47, 73/55; 32 96/128, 103/128,
 // 129/129, 192/144.
+// But not if requests that fill the device are short for their columns: each is one
+// workgroup's here then. us, here whole / as prompts, of up to 500, 1000, 2000, 4000 rows.
+// D = 128, 8 heads: 16 requests of up to 128 columns 23/27, 33/34, 51/40, 88/52; 32 25/40,
+// 36/47, 55/60, 100/85; 32 of up to 256 columns 41/52, 61/64, 98/83, 178/132. D = 64: 32 of
+// 256 29/39, 44/49, 72/63, 126/90. D = 256, 4 heads: 32 of 64 30/35, 41/41, 64/54, 121/80.
 bool walks_as_prompt(int T, int B, int Hkv, int group, int words, int max_len, int D) {
   const long columns = static_cast<long>(T) * group;
   const long each = D == 64 ? 70 : D == 128 ? 44 : 34, more = D == 64 ? 130 : D == 128 ? 72 : 16;
   if (columns <= each * B + more) return false;
+  if (static_cast<double>(max_len) * columns <= (D == 64 ? 800.0 : D == 128 ? 700.0 : 250.0) * B * B * Hkv) return false;
   // its line of key tiles and its merge's threads have to fit
   const long tiles = (std::min<long>(T, 64L * words) * group + 127) / 128 * B;
   return tiles * (max_len / 32 + 16) < (1L << 31) && tiles * Hkv * 8 * 256 < (1L << 32);

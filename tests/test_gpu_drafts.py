@@ -251,6 +251,45 @@ def test_tree_over_long_contexts(D, Hq, Hkv, page, new, before):
         _tree_check(outs[-1], q, cache, table, new, before, seen, pick={0, 1, 4, 25, 40})
 
 
+@pytest.mark.parametrize("D,Hq,Hkv,page,new,before", [
+    (128, 16, 8, 16, [12, 3, 0, 20], [3000, 5000, 10, 2500]),                     # a split with several requests
+    (64, 32, 8, 64, [9], [4000]), (256, 16, 4, 32, [6], [3000]), (128, 5, 1, 16, [7], [1500]),
+    (128, 16, 8, 32, [90] + [1] * 7, [5000, 30] + [700 * i for i in range(1, 7)]),   # one wide tree among single tokens: several items
+    (256, 16, 4, 64, [70] + [1] * 15, [2500, 0] + [150 * i for i in range(1, 15)]),  # the same, and the merge of many requests
+    (64, 64, 2, 16, [3, 4], [9000, 2])])
+def test_tree_split_over_workgroups(D, Hq, Hkv, page, new, before):
+    """Few columns after long contexts: the items' line, both merges, any workspace; twice the same bits."""
+    import torch
+    import aila_amd as A
+    q, cache, table, starts, lens, mask, seen, rows = _tree_case(D, Hq, Hkv, page, new, before, 7)
+    size = A.gqa_tree_paged_fp8_workspace_size(q.shape[0], len(new), Hq, Hkv, D, max(rows), mask.shape[1])
+    whole = A.gqa_tree_paged_fp8(q, *cache, table, starts, lens, mask, max(rows))
+    _tree_check(whole, q, cache, table, new, before, seen, pick={0, 2, 11, 40})
+    for n in (size, size // 2, size // 5):
+        ws = torch.full((n,), 0xff, dtype=torch.uint8, device="cuda")        # NaN records where none is written
+        a = A.gqa_tree_paged_fp8(q, *cache, table, starts, lens, mask, max(rows), workspace=ws)
+        _tree_check(a, q, cache, table, new, before, seen, pick={0, 2, 11, 40})
+        b = A.gqa_tree_paged_fp8(q, *cache, table, starts, lens, mask, max(rows), workspace=ws)
+        assert torch.equal(a[:sum(new)], b[:sum(new)])
+
+
+@pytest.mark.parametrize("B,D,Hq,Hkv,most,long", [(1300, 128, 4, 2, 3, 40), (4096, 64, 2, 2, 2, 20), (600, 256, 8, 1, 9, 300), (700, 128, 16, 1, 12, 30)])
+def test_trees_of_many_requests(B, D, Hq, Hkv, most, long):
+    import torch
+    import aila_amd as A
+    rng = np.random.default_rng(B)
+    new, before = rng.integers(0, most + 1, B).tolist(), rng.integers(0, long, B).tolist()
+    q, cache, table, starts, lens, mask, seen, rows = _tree_case(D, Hq, Hkv, 16, new, before, 3)
+    ws = torch.empty(A.gqa_tree_paged_fp8_workspace_size(q.shape[0], B, Hq, Hkv, D, max(rows), 1), dtype=torch.uint8, device="cuda")
+    out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+    A.gqa_tree_paged_fp8(q, *cache, table, starts, lens, mask, max(rows), out=out, workspace=ws)
+    assert bool(out.isfinite().all()) and bool((out[sum(new):] == 7.0).all())
+    at = np.concatenate([[0], np.cumsum(new)])
+    for b in rng.choice(B, 40, replace=False):
+        a, z = int(at[b]), int(at[b + 1])
+        _tree_check(out[a:z], q[a:z], cache, table[b:b + 1], [new[b]], [before[b]], seen[a:z])
+
+
 def test_tree_that_is_a_chain_is_the_prefill():
     import torch
     import aila_amd as A
