@@ -88,6 +88,42 @@ void attention_prefill_paged_fp8(Context& ctx, Tensor& q, Tensor& k_pages, Tenso
                                  Tensor& v_scale, Tensor& block_table, Tensor& query_start, Tensor& seq_lens,
                                  Tensor& output, int num_heads, int max_len, Tensor* workspace = nullptr);
 
+// A speculative step is reserve (new_lens: the drafts), then per layer prepare and
+// attention_tree, then once for all layers kv_keep and kv_pages_trim.
+//
+// Per-head norm and rotation of q [T, Hq * q_head_stride] (0: D; 2 D for packed
+// q|gate rows) into q_out [T, Hq*D], and of new_k [T, Hkv*D], which goes into the
+// cache with new_v. q_norm, k_norm [D] bf16 or null; positions [T], or [3, T] with
+// section_h and section_w (interleaved mRoPE); rotary_dim 0: no rotation.
+void prepare_qkv_paged_fp8(Context& ctx, Tensor& q, Tensor& new_k, Tensor& new_v, Tensor& k_pages, Tensor& v_pages,
+                           Tensor& k_scale, Tensor& v_scale, Tensor& slots, Tensor& positions, Tensor* q_norm,
+                           Tensor* k_norm, Tensor& q_out, int num_heads, int rotary_dim, float theta, float eps,
+                           int q_head_stride = 0, int section_h = 0, int section_w = 0, Tensor* inv_freq = nullptr);
+
+// attention_prefill_paged_fp8 of drafted trees: tree_mask [T, 2 * mask_words] s32,
+// the halves of 64-bit words, lower first.
+void attention_tree_paged_fp8(Context& ctx, Tensor& q, Tensor& k_pages, Tensor& v_pages, Tensor& k_scale,
+                              Tensor& v_scale, Tensor& block_table, Tensor& query_start, Tensor& seq_lens,
+                              Tensor& tree_mask, Tensor& output, int num_heads, int max_len, Tensor* workspace = nullptr);
+
+// One layer's 8-bit pages, for the operators that take all layers at once.
+struct PagedLayerFp8 {
+  Tensor *k_pages, *v_pages, *k_scale, *v_scale;
+};
+
+// Rows cached_lens[b] + kept[b, i] become rows cached_lens[b] + i in every layer;
+// kept [B, max_kept], kept_lens/lens [B].
+void kv_keep_paged_fp8(Context& ctx, const std::vector<PagedLayerFp8>& layers, Tensor& block_table, Tensor& cached_lens,
+                       Tensor& kept, Tensor& kept_lens, Tensor& lens);
+
+// Gives the pages behind lens [B] rows back.
+void kv_pages_trim(Context& ctx, Tensor& lens, Tensor& block_table, Tensor& free_pages, Tensor& free_count, int page_size);
+
+// Rows [0, lens[i]) of request src[i] to the pages of request dst[i] in every layer;
+// src/dst/lens [n].
+void kv_copy_paged_fp8(Context& ctx, const std::vector<PagedLayerFp8>& layers, Tensor& block_table, Tensor& src,
+                       Tensor& dst, Tensor& lens, int max_len);
+
 // Causal prefill over the current chunk (Ops.hpp:271-282). q [S, Hq*D],
 // k/v [S, Hkv*D]; output [S, Hq*D]. scores_buf is accepted and unused (no
 // [H, S, S] score matrix is materialised).

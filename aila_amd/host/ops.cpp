@@ -245,6 +245,135 @@ void attention_prefill_paged_fp8(Context& ctx, Tensor& q, Tensor& k_pages, Tenso
         "attention_prefill_paged_fp8");
 }
 
+void prepare_qkv_paged_fp8(Context& ctx, Tensor& q, Tensor& new_k, Tensor& new_v, Tensor& k_pages, Tensor& v_pages,
+                           Tensor& k_scale, Tensor& v_scale, Tensor& slots, Tensor& positions, Tensor* q_norm,
+                           Tensor* k_norm, Tensor& q_out, int num_heads, int rotary_dim, float theta, float eps,
+                           int q_head_stride, int section_h, int section_w, Tensor* inv_freq) {
+  const PagesFp8 p = pages_fp8(k_pages, v_pages, k_scale, v_scale, "prepare_qkv_paged_fp8");
+  const int64_t step = q_head_stride ? q_head_stride : p.D, q_row = num_heads * step, row = int64_t{p.Hkv} * p.D;
+  const int T = rows_of(q, q_row, "prepare_qkv_paged_fp8 q");
+  if (rows_of(new_k, row, "prepare_qkv_paged_fp8 new_k") != T || rows_of(new_v, row, "prepare_qkv_paged_fp8 new_v") != T ||
+      rows_of(q_out, int64_t{num_heads} * p.D, "prepare_qkv_paged_fp8 q_out") != T)
+    throw std::runtime_error("prepare_qkv_paged_fp8: q, new_k, new_v and q_out differ in rows");
+  for (Tensor* w : {q_norm, k_norm})
+    if (w && w->valid() && rows_of(*w, 1, "prepare_qkv_paged_fp8 norm") != p.D)
+      throw std::runtime_error("prepare_qkv_paged_fp8: q_norm and k_norm must be [D]");
+  const bool freqs = inv_freq && inv_freq->valid();
+  if (freqs) {
+    need_dtype(*inv_freq, DType::f32, "prepare_qkv_paged_fp8 inv_freq");
+    if (inv_freq->numel() < rotary_dim / 2) throw std::runtime_error("prepare_qkv_paged_fp8 inv_freq: too few elements");
+  }
+  const int* pos = nullptr;
+  bool streams = false;
+  if (rotary_dim != 0) {
+    streams = positions.ndim() == 2;
+    pos = s32(positions, "prepare_qkv_paged_fp8 positions", streams ? 3 * int64_t{T} : T);
+    if (streams && (positions.shape(0) != 3 || positions.shape(1) != T))
+      throw std::runtime_error("prepare_qkv_paged_fp8 positions: must be [T] or [3, T]");
+  }
+  check(aila_hip_prepare_qkv_paged_fp8(
+            q.data(), q_row, step, new_k.data(), row, new_v.data(), row, q_out.data(),
+            q_norm && q_norm->valid() ? q_norm->data() : nullptr, k_norm && k_norm->valid() ? k_norm->data() : nullptr,
+            k_pages.data(), v_pages.data(), k_scale.data_as<float>(), v_scale.data_as<float>(),
+            s32(slots, "prepare_qkv_paged_fp8 slots", T), pos, streams ? pos + T : nullptr, streams ? pos + 2 * int64_t{T} : nullptr,
+            streams ? section_h : 0, streams ? section_w : 0, T, num_heads, p.Hkv, p.D, p.page_size, p.num_pages, rotary_dim, theta,
+            freqs ? inv_freq->data_as<float>() : nullptr, eps, ctx.stream()),
+        "prepare_qkv_paged_fp8");
+}
+
+void attention_tree_paged_fp8(Context& ctx, Tensor& q, Tensor& k_pages, Tensor& v_pages, Tensor& k_scale,
+                              Tensor& v_scale, Tensor& block_table, Tensor& query_start, Tensor& seq_lens,
+                              Tensor& tree_mask, Tensor& output, int num_heads, int max_len, Tensor* workspace) {
+  const PagesFp8 p = pages_fp8(k_pages, v_pages, k_scale, v_scale, "attention_tree_paged_fp8");
+  const int T = rows_of(q, int64_t{num_heads} * p.D, "attention_tree_paged_fp8 q");
+  if (rows_of(output, int64_t{num_heads} * p.D, "attention_tree_paged_fp8 output") != T)
+    throw std::runtime_error("attention_tree_paged_fp8: q and output differ in rows");
+  need_dtype(block_table, DType::s32, "attention_tree_paged_fp8 block_table");
+  if (block_table.ndim() != 2) throw std::runtime_error("attention_tree_paged_fp8 block_table: must be [B, max_pages]");
+  need_dtype(tree_mask, DType::s32, "attention_tree_paged_fp8 tree_mask");
+  if (tree_mask.ndim() != 2 || tree_mask.shape(0) != T || tree_mask.shape(1) % 2)
+    throw std::runtime_error("attention_tree_paged_fp8 tree_mask: must be [T, 2 * mask_words]");
+  const int B = static_cast<int>(block_table.shape(0));
+  const bool ws = workspace && workspace->valid();
+  check(aila_hip_gqa_tree_paged_fp8(q.data(), static_cast<long>(num_heads) * p.D, k_pages.data(), v_pages.data(), p.k_scale,
+                                    p.v_scale, output.data(), ws ? workspace->data() : nullptr, ws ? workspace->size_bytes() : 0,
+                                    T, B, num_heads, p.Hkv, p.D, p.page_size, p.num_pages, block_table.data_as<int>(),
+                                    static_cast<int>(block_table.shape(1)), max_len,
+                                    s32(query_start, "attention_tree_paged_fp8 query_start", B + 1),
+                                    s32(seq_lens, "attention_tree_paged_fp8 seq_lens", B), tree_mask.data(),
+                                    static_cast<int>(tree_mask.shape(1) / 2), ctx.stream()),
+        "attention_tree_paged_fp8");
+}
+
+namespace {
+
+// The layers' pointers, every layer checked to have the first one's sizes.
+struct LayersFp8 {
+  PagesFp8 p;
+  std::vector<void*> k, v;
+  std::vector<float*> ks, vs;
+};
+LayersFp8 layers_fp8(const std::vector<PagedLayerFp8>& layers, const char* what) {
+  LayersFp8 out{};
+  for (const auto& l : layers) {
+    if (!l.k_pages || !l.v_pages || !l.k_scale || !l.v_scale) throw std::runtime_error(std::string(what) + ": a layer lacks a tensor");
+    const PagesFp8 p = pages_fp8(*l.k_pages, *l.v_pages, *l.k_scale, *l.v_scale, what);
+    if (l.k_pages->shape() != layers[0].k_pages->shape()) throw std::runtime_error(std::string(what) + ": layers differ in shape");
+    out.p = p;
+    out.k.push_back(l.k_pages->data());
+    out.v.push_back(l.v_pages->data());
+    out.ks.push_back(l.k_scale->data_as<float>());
+    out.vs.push_back(l.v_scale->data_as<float>());
+  }
+  if (layers.empty()) throw std::runtime_error(std::string(what) + ": no layers");
+  return out;
+}
+
+}  // namespace
+
+void kv_keep_paged_fp8(Context& ctx, const std::vector<PagedLayerFp8>& layers, Tensor& block_table, Tensor& cached_lens,
+                       Tensor& kept, Tensor& kept_lens, Tensor& lens) {
+  const LayersFp8 l = layers_fp8(layers, "kv_keep_paged_fp8");
+  need_dtype(block_table, DType::s32, "kv_keep_paged_fp8 block_table");
+  need_dtype(kept, DType::s32, "kv_keep_paged_fp8 kept");
+  if (block_table.ndim() != 2 || kept.ndim() != 2 || kept.shape(0) != block_table.shape(0))
+    throw std::runtime_error("kv_keep_paged_fp8: block_table must be [B, max_pages], kept [B, max_kept]");
+  const int B = static_cast<int>(block_table.shape(0));
+  s32(lens, "kv_keep_paged_fp8 lens", B);
+  check(aila_hip_kv_keep_paged_fp8(l.k.data(), l.v.data(), l.ks.data(), l.vs.data(), static_cast<int>(layers.size()),
+                                   block_table.data_as<int>(), s32(cached_lens, "kv_keep_paged_fp8 cached_lens", B),
+                                   kept.data_as<int>(), s32(kept_lens, "kv_keep_paged_fp8 kept_lens", B), lens.data_as<int>(), B,
+                                   static_cast<int>(kept.shape(1)), l.p.Hkv, l.p.D, l.p.page_size, l.p.num_pages,
+                                   static_cast<int>(block_table.shape(1)), ctx.stream()),
+        "kv_keep_paged_fp8");
+}
+
+void kv_pages_trim(Context& ctx, Tensor& lens, Tensor& block_table, Tensor& free_pages, Tensor& free_count, int page_size) {
+  need_dtype(block_table, DType::s32, "kv_pages_trim block_table");
+  if (block_table.ndim() != 2) throw std::runtime_error("kv_pages_trim block_table: must be [B, max_pages]");
+  const int B = static_cast<int>(block_table.shape(0));
+  s32(free_pages, "kv_pages_trim free_pages", 1);
+  s32(free_count, "kv_pages_trim free_count", 1);
+  check(aila_hip_kv_pages_trim(s32(lens, "kv_pages_trim lens", B), block_table.data_as<int>(), free_pages.data_as<int>(),
+                               free_count.data_as<int>(), B, static_cast<int>(block_table.shape(1)), page_size,
+                               static_cast<int>(free_pages.numel()), ctx.stream()),
+        "kv_pages_trim");
+}
+
+void kv_copy_paged_fp8(Context& ctx, const std::vector<PagedLayerFp8>& layers, Tensor& block_table, Tensor& src,
+                       Tensor& dst, Tensor& lens, int max_len) {
+  const LayersFp8 l = layers_fp8(layers, "kv_copy_paged_fp8");
+  need_dtype(block_table, DType::s32, "kv_copy_paged_fp8 block_table");
+  if (block_table.ndim() != 2) throw std::runtime_error("kv_copy_paged_fp8 block_table: must be [B, max_pages]");
+  const int n = static_cast<int>(src.numel());
+  check(aila_hip_kv_copy_paged_fp8(l.k.data(), l.v.data(), l.ks.data(), l.vs.data(), static_cast<int>(layers.size()),
+                                   block_table.data_as<int>(), s32(src, "kv_copy_paged_fp8 src", n),
+                                   s32(dst, "kv_copy_paged_fp8 dst", n), s32(lens, "kv_copy_paged_fp8 lens", n), n, max_len,
+                                   static_cast<int>(block_table.shape(0)), l.p.Hkv, l.p.D, l.p.page_size, l.p.num_pages,
+                                   static_cast<int>(block_table.shape(1)), ctx.stream()),
+        "kv_copy_paged_fp8");
+}
+
 void attention_prefill(Context& ctx, Tensor& q, Tensor& k, Tensor& v, Tensor& output,
                        Tensor& scores_buf, int seq_len, int num_heads, int num_kv_heads,
                        int head_dim) {
