@@ -340,12 +340,21 @@ extern "C" int aila_hip_prepare_qkv_paged_fp8(const void* q, long q_stride, long
   AILA_REQUIRE(q_head_stride >= D && q_head_stride % 8 == 0 && q_stride % 8 == 0 && q_stride >= (Hq - 1) * q_head_stride + D,
                "%s: query strides %ld (token) and %ld (head) must be multiples of 8 and hold %d heads of %d", what, q_stride,
                q_head_stride, Hq, D);
+  AILA_REQUIRE(q_out != q || ((Hq == 1 || q_head_stride == D) && (T == 1 || q_stride == static_cast<long>(Hq) * D)),
+               "%s: q_out may be q where its heads and tokens follow each other", what);
   AILA_REQUIRE(k_stride >= static_cast<long>(Hkv) * D && k_stride % 8 == 0 && v_stride >= static_cast<long>(Hkv) * D && v_stride % 8 == 0,
                "%s: token strides %ld (k) and %ld (v) must be multiples of 8 and hold Hkv * D = %ld values", what, k_stride, v_stride,
                static_cast<long>(Hkv) * D);
   const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
                         reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(q_norm_w) | reinterpret_cast<uintptr_t>(k_norm_w);
   AILA_REQUIRE(all % 16 == 0, "%s: q, k, v, q_out and the weights must be 16-byte aligned", what);
+  // A wave takes the runs that begin in its tile one after the other. us, tiles of 1, 4, 8
+  // and 16 tokens, a run a token / prompts of T / 4, 32 / 8 heads, D = 128: T = 256
+  // 7.7/7.2, 8.5/7.8, 12.4/8.0, 20.9/8.9; 512 11.6/10.4, 10.0/7.6, 13.0/8.3, 21.1/8.3; 1024
+  // 21.7/16.7, 15.9/11.2, 16.4/9.8, 23.9/10.7; 2048 39.8/28.0, 27.2/17.0, 24.9/14.4,
+  // 27.4/13.9; 4096 74.2/49.5, 48.2/34.6, 44.6/28.2, 43.3/22.6. 16 / 4, D = 256: 256 6.5/8.8,
+  // 9.4/10.3, 14.1/10.5, 24.1/12.3; 1024 18.2/20.2, 14.1/11.6, 16.9/11.9, 27.2/13.6; 4096
+  // 60.3/64.9, 43.5/35.6, 40.3/29.7, 39.6/25.1.
   const int tile = T <= 256 ? 1 : T <= 1024 ? 4 : T <= 2048 ? 8 : kScaleRows;
   // fewer than 2^32 threads, the most of a launch
   const long kv_groups = (static_cast<long>(T) + tile - 1) / tile * ((Hkv + 1) / 2);

@@ -459,7 +459,8 @@ int aila_hip_gqa_prefill_paged_fp8(const void* q, long q_stride,
  * for the (unrounded) y here; v as there.
  *   q        head h of token t at + t * q_stride + h * q_head_stride elements
  *            (multiples of 8: the queries of a packed q|gate row have head stride
- *            2 D); q_out [T, Hq, D] (may be q, where that is [T, Hq, D])
+ *            2 D); q_out [T, Hq, D] (may be q, where that is [T, Hq, D]; it may not
+ *            overlap k, v or q otherwise)
  *   k, v     [Hkv, D] of token t at + t * k_stride, t * v_stride elements
  *   slots    int[T], as aila_hip_kv_append_paged_fp8; -1: k and v are skipped
  *   positions  p of each token, int[T] (NULL where rotary_dim is 0). With pos_h and
@@ -496,7 +497,7 @@ int aila_hip_prepare_qkv_paged_fp8(const void* q, long q_stride,
  * aila_hip_gqa_prefill_paged_fp8.
  * The workspace holds the records of the items whose keys are split: workspace_size
  * bytes let as many workgroups work as the device holds, a smaller workspace fewer
- * (2 records at least, else AILA_HIP_EWORKSPACE), and NULL none but one for each
+ * (2 records at least, else AILA_HIP_EWORKSPACE), and NULL at most one for each
  * request, KV head and 256 query rows (D = 256: 128). Calls that may overlap in time
  * need workspaces of their own. */
 size_t aila_hip_gqa_tree_paged_fp8_workspace_size(int T, int B, int Hq, int Hkv,
@@ -520,15 +521,16 @@ int aila_hip_gqa_tree_paged_fp8(const void* q, long q_stride,
  *   cached_lens[b]  rows before the draft; negative: the request is absent
  *   kept        int[B, max_kept], each request's drafted tokens that stay, rising
  *               (entries past kept_lens[b] are not read as rows). max_kept <= 65536.
+ *   kept_lens[b]  0 for a request that reserve refused: it has no drafted rows
  *   lens[B]     out: cached_lens[b] + kept_lens[b] (of at most max_kept, and within
- *               the table); cached_lens[b] where that is negative. May not be the
- *               array of cached_lens or kept_lens.
- * Rows up to the first that moves stay untouched. A block of 16 rows that rows move
- * into gets the largest of the scales that its rows come from: its own for rows
+ *               the table); cached_lens[b] where that is negative. May not overlap
+ *               the other arrays.
+ * Blocks of 16 rows before the first row that moves stay untouched. A block that rows
+ * move into gets the largest of the scales that its rows come from: its own for rows
  * before the first moved one, the source's for each moved row. Codes move as they
  * are, or times the power of two between the scales: exact but for underflow. Rows
- * behind lens[b] are not valid any more. A row whose index or page is out of range is
- * left as it was. */
+ * behind lens[b] are not valid any more. A row whose index or page is out of range
+ * keeps its codes. Pages are one cache's only: the same twice is refused. */
 int aila_hip_kv_keep_paged_fp8(void* const* k_pages, void* const* v_pages,
                                float* const* k_scale, float* const* v_scale,
                                int layers, const int* block_table,

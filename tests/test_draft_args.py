@@ -83,6 +83,26 @@ def test_every_layer_is_checked():
     assert rc == -1
 
 
+@pytest.mark.parametrize("bad", [dict(lens=P16 + 4), dict(lens=P16 + 56), dict(counts=P16 + 136), dict(cached=P16 + 124), dict(table=P16 + 48)])
+def test_keep_lengths_over_what_comes_in(bad):
+    """kept is 15 ints from P16 on, the table 24, the lengths going out 3 from P16 + 128 on."""
+    rc, msg = _keep(**bad)
+    assert rc == -1 and "comes in" in msg, (rc, msg)
+
+
+def test_keep_of_the_same_pages_twice():
+    for k, v in (((P16, P16 + 4096), (P16 + 64, P16)), ((P16, P16), (P16 + 64, P16 + 128)), ((P16, P16 + 64), (P16 + 128, P16 + 128)), ((P16,), (P16,))):
+        a = [_arr(*k), _arr(*v), _arr(*[P16] * len(k)), _arr(*[P16] * len(k))]
+        rc = aila_amd.lib().aila_hip_kv_keep_paged_fp8(*a, len(k), P16, P16, P16, P16 + 128, P16 + 256, 3, 5, 2, 128, 16, 10, 8, None)
+        assert rc == -1 and b"twice" in aila_amd.lib().aila_hip_last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(qs=1024), dict(qh=256, qs=1024), dict(qh=256, qs=1024, T=1)])
+def test_prepare_of_strided_queries_in_place(bad):
+    rc, msg = _rc("prepare_qkv_paged_fp8", PREPARE, **bad)
+    assert rc == -1 and "q_out may be q" in msg, (rc, msg)
+
+
 def test_a_copy_of_no_rows_does_nothing():
     assert _copy(max_len=0)[0] == 0
 
