@@ -1147,7 +1147,9 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
 // Joins the records of a tile whose keys were cut: o = sum 2^(m_i - M) o_i /
 // sum 2^(m_i - M) l_i. A workgroup takes 32 query rows and up to 128 dims; a
 // thread's values are those of the main kernel's lane.
-template <int D, bool TREE>
+// kPhases: as many threads share a value's records and meet in LDS, each workgroup with
+// 1 / kPhases of the dims.
+template <int D, bool TREE, int kPhases>
 __global__ __launch_bounds__(256) void gqa_prefill_paged_fp8_merge_kernel(PagedFp8 c, Fp8PrefillArgs a) {
   using C = Cfg<D>;
   Item it;
@@ -1178,12 +1180,14 @@ __global__ __launch_bounds__(256) void gqa_prefill_paged_fp8_merge_kernel(PagedF
     cuts = a.splits;
     if (!get_item<D>(a, rec, &it)) return;
   }
-  constexpr int G = D > 128 ? D / 128 : 1;
-  const int kvh = blockIdx.y, wave = static_cast<int>(blockIdx.z) / G, g = static_cast<int>(blockIdx.z) % G;
-  const int lane = threadIdx.x & 63, i = threadIdx.x >> 6, l32 = lane & 31, hf = lane >> 5;
-  if (D == 64 && i > 1) return;
+  constexpr int G = D > 128 ? D / 128 : 1, kWide = 256 / kPhases;      // threads of a phase
+  const int z = static_cast<int>(blockIdx.z) / kPhases, part = static_cast<int>(blockIdx.z) % kPhases;
+  const int kvh = blockIdx.y, wave = z / G, g = z % G, ph = static_cast<int>(threadIdx.x) / kWide;
+  const int x = static_cast<int>(threadIdx.x) % kWide;
+  const int lane = threadIdx.x & 63, i = part * (4 / kPhases) + (x >> 6), l32 = lane & 31, hf = lane >> 5;
   const int row = it.r0 + wave * 32 + l32;
-  if (row >= it.n * a.group) return;
+  const bool mine = !(D == 64 && i > 1) && row < it.n * a.group;
+  if (kPhases == 1 && !mine) return;
   const size_t step = static_cast<size_t>(c.Hkv) * C::REC;
   const float* r0 = a.part + (static_cast<size_t>(rec) * c.Hkv + kvh) * C::REC;
   const float* ml = r0 + kRows * D + (wave * 32 + l32) * 2;
@@ -1192,7 +1196,7 @@ __global__ __launch_bounds__(256) void gqa_prefill_paged_fp8_merge_kernel(PagedF
   constexpr int kBatch = 4;
   float M = -INFINITY, L = 0.f;
   f32x4 o[4] = {};
-  for (int x0 = 0; x0 < cuts; x0 += kBatch) {
+  for (int x0 = ph * kBatch; x0 < cuts && mine; x0 += kPhases * kBatch) {
     float m[kBatch], l[kBatch];
     f32x4 v[kBatch][4];
 #pragma unroll
@@ -1223,6 +1227,32 @@ __global__ __launch_bounds__(256) void gqa_prefill_paged_fp8_merge_kernel(PagedF
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += f * v[y][e];
       }
+    }
+  }
+  if constexpr (kPhases > 1) {
+    __shared__ f32x4 s_o[kPhases - 1][4][kWide];
+    __shared__ float s_ml[kPhases - 1][2][kWide];
+    if (ph > 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s_o[ph - 1][e][x] = o[e];
+      s_ml[ph - 1][0][x] = M;
+      s_ml[ph - 1][1][x] = L;
+    }
+    __syncthreads();
+    if (ph > 0 || !mine) return;
+    const float own = M;
+#pragma unroll
+    for (int y = 0; y < kPhases - 1; ++y) M = fmaxf(M, s_ml[y][0][x]);
+    const float f0 = own == -INFINITY ? 0.f : fast_exp2(own - M);
+    L *= f0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= f0;
+#pragma unroll
+    for (int y = 0; y < kPhases - 1; ++y) {
+      const float m = s_ml[y][0][x], f = m == -INFINITY ? 0.f : fast_exp2(m - M);
+      L += f * s_ml[y][1][x];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += f * s_o[y][e][x];
     }
   }
   const float inv = L == 0.f ? 0.f : 1.0f / L;
@@ -1274,7 +1304,7 @@ int launch(PagedFp8 c, Fp8PrefillArgs a, void* workspace, size_t workspace_bytes
       hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D, false, false>), dim3(args.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, cache, args);
   };
   auto merge = [&](int cut_tiles) {
-    hipLaunchKernelGGL((gqa_prefill_paged_fp8_merge_kernel<D, false>), dim3(cut_tiles, c.Hkv, 4 * (D > 128 ? D / 128 : 1)), dim3(256), 0,
+    hipLaunchKernelGGL((gqa_prefill_paged_fp8_merge_kernel<D, false, 1>), dim3(cut_tiles, c.Hkv, 4 * (D > 128 ? D / 128 : 1)), dim3(256), 0,
                        st, c, a);
   };
   if (a.B == 1) {
@@ -1317,6 +1347,13 @@ size_t tree_need(int B, int Hkv) {
   return tree_units_bytes(B) + 2 * static_cast<size_t>(std::max(1, kCus / Hkv)) * Hkv * Cfg<D>::REC * sizeof(float);
 }
 
+// Few tiles in many pieces: the merge's threads share a value's records and spread over
+// more CUs, from so many records a tile on. us, the whole call with 1 / 4 phases, 8000
+// rows. 16 / 4, D = 256: 64 records 39.9/28.5, 32 38.4/34.8, 16 43.5/42.4, 9 53.4/53.0; 32 /
+// 8, D = 128: 32 30.9/25.5, 16 30.7/28.7, 8 37.8/37.4; D = 64: 16 24.7/22.8, 8 29.5/29.3. The
+// merge alone with 2 (32 requests, 40 / 8, D = 128) 10.5/20.6: most of its workgroups
+// find no tile.
+constexpr int kMergePhases = 4, kMergeCuts = 8;
 template <int D>
 int launch_trees(const PagedFp8& c, Fp8PrefillArgs a, void* workspace, hipStream_t st) {
   a.lanes = std::max(1, kCus / c.Hkv);
@@ -1324,8 +1361,12 @@ int launch_trees(const PagedFp8& c, Fp8PrefillArgs a, void* workspace, hipStream
   a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + tree_units_bytes(a.B));
   hipLaunchKernelGGL((gqa_prefill_paged_fp8_kernel<D, false, true>), dim3(a.lanes * c.Hkv), dim3(kThreads), Cfg<D>::LDS, st, c, a);
   const int tiles = static_cast<int>((std::min<long>(a.T, 32L * a.words32) * a.group + kRows - 1) / kRows);     // of a request at most
-  hipLaunchKernelGGL((gqa_prefill_paged_fp8_merge_kernel<D, true>), dim3(tiles * a.B, c.Hkv, 4 * (D > 128 ? D / 128 : 1)), dim3(256), 0, st,
-                     c, a);
+  const long all = (static_cast<long>(a.T) * a.group + kRows - 1) / kRows;      // tiles of a KV head, about
+  const int parts = 4 * (D > 128 ? D / 128 : 1);
+  if (a.lanes >= kMergeCuts * all)
+    hipLaunchKernelGGL((gqa_prefill_paged_fp8_merge_kernel<D, true, kMergePhases>), dim3(tiles * a.B, c.Hkv, parts * kMergePhases), dim3(256), 0, st, c, a);
+  else
+    hipLaunchKernelGGL((gqa_prefill_paged_fp8_merge_kernel<D, true, 1>), dim3(tiles * a.B, c.Hkv, parts), dim3(256), 0, st, c, a);
   return check_launch("gqa_tree_paged_fp8");
 }
 

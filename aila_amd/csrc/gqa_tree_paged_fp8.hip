@@ -622,50 +622,58 @@ __device__ __forceinline__ void store_joined(const TreeArgs& a, const Shape& s, 
 }
 
 // Joins the records: o = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i. Few
-// requests, many records each: a workgroup takes kMergeCols columns of a request and
-// KV head, its other threads other records.
-constexpr int kMergeCols = 4, kMergeThreads = 256;
+// columns, many records each: a workgroup takes one column of a request and KV head,
+// its threads other records, kBatch at a time (past the last: the last again, with
+// weight 0).
+constexpr int kMergeThreads = 256, kBatch = 4;
+template <int D>
+__device__ __forceinline__ void join_batch(Joined* sum, const float* at, const Records& r, int w, int stride, size_t step, int d) {
+  f32x4 v[kBatch];
+  float m[kBatch], l[kBatch];
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    const int u = min(w + i * stride, r.w1);
+    const float* p = at + (static_cast<size_t>(u) * 2 + (u == r.w0 ? 1 : 0)) * step;
+    v[i] = *reinterpret_cast<const f32x4*>(p + d);
+    m[i] = p[D];
+    l[i] = p[D + 1];
+  }
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i)
+    if (w + i * stride <= r.w1) sum->add(v[i], m[i], l[i]);
+}
 template <int D>
 __global__ __launch_bounds__(kMergeThreads) void gqa_tree_paged_fp8_merge_kernel(PagedFp8 c, TreeArgs a, int launched) {
-  constexpr int kQuads = D / 4, kPhases = kMergeThreads / (kMergeCols * kQuads);
+  constexpr int kQuads = D / 4, kPhases = kMergeThreads / kQuads;
   __shared__ f32x4 s_a[kMergeThreads];
   __shared__ float s_m[kMergeThreads], s_l[kMergeThreads];
-  const int b = blockIdx.y, kvh = blockIdx.x;
+  const int b = blockIdx.y, kvh = blockIdx.x, y = blockIdx.z;
   const Shape s = shape_of<D>(a, b);
-  const int cols = s.n * a.group, x0 = static_cast<int>(blockIdx.z) * kMergeCols;
-  if (x0 >= cols) return;
-  const int d = static_cast<int>(threadIdx.x) % kQuads * 4, x = static_cast<int>(threadIdx.x) / kQuads % kMergeCols;
-  const int ph = static_cast<int>(threadIdx.x) / (kQuads * kMergeCols);
-  const int y = min(x0 + x, cols - 1);
+  if (y >= s.n * a.group) return;
+  const int d = static_cast<int>(threadIdx.x) % kQuads * 4, ph = static_cast<int>(threadIdx.x) / kQuads;
   const Records r = records_of<D>(c, a, s, b, kvh, y, launched);
   if (r.w0 == r.w1) return;
   const size_t step = static_cast<size_t>(a.rec_cols) * (D + kRecTail);
   Joined sum;
-  for (int w = r.w0 + ph; w <= r.w1; w += kPhases) {
-    const float* p = r.at + (static_cast<size_t>(w) * 2 + (w == r.w0 ? 1 : 0)) * step;
-    sum.add(*reinterpret_cast<const f32x4*>(p + d), p[D], p[D + 1]);
-  }
-  if constexpr (kPhases > 1) {
-    s_a[threadIdx.x] = sum.A;
-    s_m[threadIdx.x] = sum.M;
-    s_l[threadIdx.x] = sum.L;
-    __syncthreads();
-    if (ph > 0) return;
+  for (int w = r.w0 + ph; w <= r.w1; w += kBatch * kPhases) join_batch<D>(&sum, r.at, r, w, kPhases, step, d);
+  s_a[threadIdx.x] = sum.A;
+  s_m[threadIdx.x] = sum.M;
+  s_l[threadIdx.x] = sum.L;
+  __syncthreads();
+  if (ph > 0) return;
 #pragma unroll
-    for (int i = 1; i < kPhases; ++i) {
-      const int j = threadIdx.x + i * kQuads * kMergeCols;
-      sum.add(s_a[j], s_m[j], s_l[j]);
-    }
+  for (int i = 1; i < kPhases; ++i) {
+    const int j = threadIdx.x + i * kQuads;
+    sum.add(s_a[j], s_m[j], s_l[j]);
   }
-  if (x0 + x < cols) store_joined<D>(a, s, kvh, y, d, sum);
+  store_joined<D>(a, s, kvh, y, d, sum);
 }
 
-// The same for many requests, few records each: a workgroup takes as many columns
-// as it has threads for, and kBatch records at a time (past the last: the last again,
-// with weight 0).
+// The same for many columns, few records each: a workgroup takes as many columns as it
+// has threads for.
 template <int D>
 __global__ __launch_bounds__(kMergeThreads) void gqa_tree_paged_fp8_merge_few_kernel(PagedFp8 c, TreeArgs a, int launched) {
-  constexpr int kQuads = D / 4, kColumns = kMergeThreads / kQuads, kBatch = 4;
+  constexpr int kQuads = D / 4, kColumns = kMergeThreads / kQuads;
   const int b = blockIdx.y, kvh = blockIdx.x;
   const Shape s = shape_of<D>(a, b);
   const int cols = s.n * a.group, x0 = static_cast<int>(blockIdx.z) * kColumns;
@@ -675,21 +683,7 @@ __global__ __launch_bounds__(kMergeThreads) void gqa_tree_paged_fp8_merge_few_ke
   const size_t step = static_cast<size_t>(a.rec_cols) * (D + kRecTail);
   const int d = static_cast<int>(threadIdx.x) % kQuads * 4, x = min(static_cast<int>(threadIdx.x) / kQuads, cols - 1 - x0);
   Joined sum;
-  for (int w = r.w0; w <= r.w1; w += kBatch) {
-    f32x4 v[kBatch];
-    float m[kBatch], l[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int u = min(w + i, r.w1);
-      const float* p = r.at + x * (D + kRecTail) + (static_cast<size_t>(u) * 2 + (u == r.w0 ? 1 : 0)) * step;
-      v[i] = *reinterpret_cast<const f32x4*>(p + d);
-      m[i] = w + i <= r.w1 ? p[D] : -INFINITY;
-      l[i] = p[D + 1];
-    }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-      if (w + i <= r.w1) sum.add(v[i], m[i], l[i]);
-  }
+  for (int w = r.w0; w <= r.w1; w += kBatch) join_batch<D>(&sum, r.at + x * (D + kRecTail), r, w, 1, step, d);
   if (static_cast<int>(threadIdx.x) / kQuads < cols - x0) store_joined<D>(a, s, kvh, x0 + x, d, sum);
 }
 
@@ -724,17 +718,31 @@ size_t workspace_need(int T, int B, int Hkv, int group, int words, int max_len) 
 }
 
 // Whether a request and KV head is one workgroup's, for all keys: up to a length that
-// grows with the CUs they fill. us in a graph, whole / split, trees of up to 4 tokens,
-// lengths between half the bound and all of it. D = 128, 8 KV heads of 4: 1 request of 500
-// rows 10.6 / 12.7, 1000 13.0 / 13.1, 2000 17.8 / 13.9; 4 of 1000 13.2 / 13.4, 2000 18.0 /
-// 15.3; 16 of 2000 19.6 / 25.0, 4000 29.3 / 30.6; 32 of 2000 25.0 / 34.2, 4000 51.9 / 58.9. D
-// = 64: 1 of 1000 10.2 / 11.1, 2000 13.6 / 11.6; 32 of 4000 24.6 / 31.5. D = 256, 4 heads: 1 of
-// 500 15.7 / 15.6, 1000 21.8 / 17.0; 16 of 1000 22.8 / 24.8, 2000 34.9 / 29.6; 32 of 1000 23.5 /
-// 29.3, 2000 35.9 / 34.5.
-bool walks_whole(int B, int Hkv, int max_len, int D) {
-  const long items = static_cast<long>(B) * Hkv;
-  return max_len <= (D == 256 ? std::min(2048L, 450 + 10 * items) : std::min(4096L, 900 + 16 * items));
+// grows with the CUs they fill, and is shared by the tiles of a request (of average
+// size), since a workgroup's waves that have no tile take other keys. us in a graph, whole
+// / split, lengths between half the bound and all of it, trees of up to 4 tokens (16: in
+// parentheses), G = 4. D = 128, 8 KV heads: 1 request of 600 rows 11.0/12.9 (16.6/15.5), 1000
+// 13.0/13.2 (20.0/15.8), 2000 17.8/13.3 (28.9/17.6); 4 of 1000 13.2/13.5 (20.2/18.9), 1500
+// 15.4/14.0 (24.6/27.5); 8 of 1500 16.5/22.2 (25.5/27.4), 3000 23.7/24.7 (39.7/30.1); 16 of
+// 2000 19.7/25.4 (31.0/33.1), 3000 24.3/28.1 (40.3/36.4). D = 64: 1 of 1000 10.3/12.0
+// (14.4/13.3), 2000 13.6/12.1 (21.4/13.9); 8 of 2000 13.7/17.4 (21.6/20.8). D = 256, 4 heads:
+// 1 of 200 13.0/14.5 (20.7/18.9), 400 15.9/14.5 (25.3/19.7); 8 of 400 16.1/15.1 (25.6/24.8),
+// 800 20.0/16.5 (33.8/33.8); 16 of 800 21.4/25.0 (35.5/39.5), 2000 34.5/29.8 (62.5/43.0).
+bool walks_whole(long columns, int B, int Hkv, int max_len, int D) {
+  const long items = static_cast<long>(B) * Hkv, tiles = (columns + 32L * B - 1) / (32L * B);
+  const long most = D == 256 ? 300 + items * items / 5 : (D == 128 ? 1000 : 1500) + items * items * 3 / 10;
+  return max_len <= (D == 256 ? 2048 : 4096) && max_len * std::min<long>(tiles, D == 256 ? 4 : 8) <= most;
 }
+
+// Records of a column, where requests share evenly, from which a workgroup joins one
+// column's. us, the whole call, columns by columns / each, 8000 rows (30000: in
+// parentheses), a request's columns. 1 request, D = 256, 4 heads: 4 27.3/17.2 (34.3/24.2), 64
+// 37.7/27.5 (47.9/37.5); 2: 52 in all 37.9/33.2 (49.3/44.0); 8: 332 52.9/52.5, 676
+// 74.6/73.5; 32: 128 92.7/96.0, 616 103.6/113.9. D = 128, 8 heads: 1 request, 4 19.6/14.3
+// (27.4/21.8), 128 30.2/25.7; 4: 92 30.7/29.8, 192 34.5/35.0, 388 43.4/45.9; 8: 36
+// 30.4/29.8, 160 35.1/37.8; 32: 128 97.6/108.7. D = 64: 1: 4 16.9/12.4, 128 24.8/20.0; 4: 92
+// 22.2/21.8, 192 25.5/26.6; 32: 128 57.8/69.4.
+constexpr int kEachRecords = 8;
 
 template <int D>
 int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t workspace_bytes, hipStream_t st) {
@@ -746,15 +754,15 @@ int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t wor
   const long items = static_cast<long>(a.B) * c.Hkv * m.items;
   AILA_REQUIRE(items * most_units(a.max_len) < (1L << 31) && items * kThreads < (1L << 32),
                "gqa_tree_paged_fp8: B=%d requests of up to %ld query rows and %d keys are too many", a.B, m.cols, a.max_len);
-  const long merges = (m.cols + kMergeCols - 1) / kMergeCols;
-  AILA_REQUIRE(merges <= 65535, "gqa_tree_paged_fp8: %ld query rows of a KV head are too many", m.cols);
+  const long few = (m.cols * (D / 4) + kMergeThreads - 1) / kMergeThreads;
+  AILA_REQUIRE(few <= 65535, "gqa_tree_paged_fp8: %ld query rows of a KV head are too many", m.cols);
   long groups = static_cast<long>(a.B) * c.Hkv * a.chunks;
   if (workspace != nullptr) {
     const size_t rec = record_bytes<D>(m);
     if (workspace_bytes < units_bytes(a.B) + 2 * rec)
       return set_error(AILA_HIP_EWORKSPACE, "gqa_tree_paged_fp8: workspace %zu bytes, %zu are the least", workspace_bytes,
                        units_bytes(a.B) + 2 * rec);
-    if (!walks_whole(a.B, c.Hkv, a.max_len, D)) {
+    if (!walks_whole(static_cast<long>(a.T) * a.group, a.B, c.Hkv, a.max_len, D)) {
       groups = std::min<long>(split_groups<D>(a.B, c.Hkv, m, a.max_len), static_cast<long>((workspace_bytes - units_bytes(a.B)) / rec));
       a.units = static_cast<int*>(workspace);
       a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + units_bytes(a.B));
@@ -763,11 +771,13 @@ int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t wor
   const size_t lds = static_cast<size_t>(kWaves<D>) * kTile * (kAccStride<D> + 2) * sizeof(float) +
                      (a.part ? static_cast<size_t>(a.B + 1) * sizeof(int) : 0);
   hipLaunchKernelGGL((gqa_tree_paged_fp8_kernel<D>), dim3(groups), dim3(kThreads), lds, st, c, a);
-  if (a.part && static_cast<long>(a.B) * c.Hkv * merges > 2048)
-    hipLaunchKernelGGL((gqa_tree_paged_fp8_merge_few_kernel<D>), dim3(c.Hkv, a.B, (m.cols * (D / 4) + kMergeThreads - 1) / kMergeThreads), dim3(kMergeThreads), 0, st, c, a,
+  const long all = static_cast<long>(a.T) * a.group * c.Hkv;      // columns
+  const bool each = kEachRecords * a.B * c.Hkv <= kCus && all <= (D == 256 ? 4096 : 1024);
+  if (a.part && each)
+    hipLaunchKernelGGL((gqa_tree_paged_fp8_merge_kernel<D>), dim3(c.Hkv, a.B, m.cols), dim3(kMergeThreads), 0, st, c, a,
                        static_cast<int>(groups));
   else if (a.part)
-    hipLaunchKernelGGL((gqa_tree_paged_fp8_merge_kernel<D>), dim3(c.Hkv, a.B, merges), dim3(kMergeThreads), 0, st, c, a,
+    hipLaunchKernelGGL((gqa_tree_paged_fp8_merge_few_kernel<D>), dim3(c.Hkv, a.B, few), dim3(kMergeThreads), 0, st, c, a,
                        static_cast<int>(groups));
   return check_launch("gqa_tree_paged_fp8");
 }

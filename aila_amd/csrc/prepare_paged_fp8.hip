@@ -76,27 +76,30 @@ __device__ __forceinline__ Place place_of(int s, int rot) {
 }
 
 // (cosine, sine) of the pairs of `count` tokens from `token` on, [token][pair] in LDS:
-// each once for the workgroup, whose waves all need the same.
+// each once for the workgroup, whose waves all need the same. A thread keeps to a pair.
 __device__ __forceinline__ void fill_turns(const PrepareArgs& a, const Powers& pw, int token, int count, f32x2* s_turn) {
   const int half = a.rot / 2;
-  for (int i = threadIdx.x; i < count * half; i += kThreads) {
-    const int t = i / half, j = i - t * half, n = j / 3, m = j - 3 * n;
-    const int* from = a.pos_t;
-    if (m == 1 && n < a.section_h) from = a.pos_h;
-    if (m == 2 && n < a.section_w) from = a.pos_w;
-    double f;
-    if (a.inv_freq != nullptr) {
-      f = static_cast<double>(a.inv_freq[j]) * 0.15915494309189535;
-    } else {
-      f = pw.base;
+  if (half == 0) return;
+  const int first = static_cast<int>(threadIdx.x) / half, j = static_cast<int>(threadIdx.x) - first * half, step = kThreads / half;
+  if (first >= step) return;
+  const int n = j / 3, m = j - 3 * n;
+  const int* from = a.pos_t;
+  if (m == 1 && n < a.section_h) from = a.pos_h;
+  if (m == 2 && n < a.section_w) from = a.pos_w;
+  double f;
+  if (a.inv_freq != nullptr) {
+    f = static_cast<double>(a.inv_freq[j]) * 0.15915494309189535;
+  } else {
+    f = pw.base;
 #pragma unroll
-      for (int b = 0; b < 7; ++b) f *= j >> b & 1 ? pw.bit[b] : 1.0;
-    }
+    for (int b = 0; b < 7; ++b) f *= j >> b & 1 ? pw.bit[b] : 1.0;
+  }
+  for (int t = first; t < count; t += step) {
     double x = static_cast<double>(from[token + t]) * f;
     x -= __builtin_rint(x);
     float sn, cs;
     sincospif(2.0f * static_cast<float>(x), &sn, &cs);
-    s_turn[i] = f32x2{cs, sn};
+    s_turn[t * half + j] = f32x2{cs, sn};
   }
 }
 
@@ -114,8 +117,8 @@ __device__ __forceinline__ Turn load_turn(const f32x2* p) {      // 16-byte alig
   return t;
 }
 
-__device__ __forceinline__ void load4(const bf16* p, float* f) {
-  const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+__device__ __forceinline__ u32x2 load4(const bf16* p) { return *reinterpret_cast<const u32x2*>(p); }
+__device__ __forceinline__ void widen4(const u32x2& w, float* f) {
   f[0] = __uint_as_float(w[0] << 16);
   f[1] = __uint_as_float(w[0] & 0xffff0000u);
   f[2] = __uint_as_float(w[1] << 16);
@@ -125,8 +128,8 @@ __device__ __forceinline__ void load_weights(const bf16* w, const Place& p, floa
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = 1.0f;
   if (w != nullptr) {
-    load4(w + p.lo, f);
-    load4(w + p.hi, f + 4);
+    widen4(load4(w + p.lo), f);
+    widen4(load4(w + p.hi), f + 4);
   }
 }
 
@@ -157,19 +160,27 @@ __device__ __forceinline__ void prepare_queries(const PrepareArgs& a, const Powe
   const Place p = place_of<D>(lane % LR, a.rot);
   float w[8];
   load_weights(a.q_norm, p, w);
+  const bf16* src = a.q + static_cast<size_t>(token) * a.q_stride;
+  bf16* dst = a.q_out + static_cast<size_t>(token) * a.Hq * D;
+  u32x2 lo, hi;      // of the next head, on their way while the turns are made
+  auto fetch = [&](int h0) __attribute__((always_inline)) {
+    const bf16* row = src + min(h0 + lane / LR, a.Hq - 1) * a.q_head_stride;
+    lo = load4(row + p.lo);
+    hi = load4(row + p.hi);
+  };
+  fetch(wave * RI);
   fill_turns(a, pw, token, 1, s_turn);
   __syncthreads();
   Turn t{};
   if (p.turns) t = load_turn(s_turn + p.j);
-  const bf16* src = a.q + static_cast<size_t>(token) * a.q_stride;
-  bf16* dst = a.q_out + static_cast<size_t>(token) * a.Hq * D;
   for (int h0 = wave * RI; h0 < a.Hq; h0 += kWaves * RI) {
-    const int h = min(h0 + lane / LR, a.Hq - 1);
+    const int h = h0 + lane / LR;
     float x[8];
-    load4(src + h * a.q_head_stride + p.lo, x);
-    load4(src + h * a.q_head_stride + p.hi, x + 4);
+    widen4(lo, x);
+    widen4(hi, x + 4);
+    if (h0 + kWaves * RI < a.Hq) fetch(h0 + kWaves * RI);
     norm_turn<D>(x, w, t, p.turns, a.eps);
-    if (h0 + lane / LR < a.Hq) {
+    if (h < a.Hq) {
       *reinterpret_cast<u32x2*>(dst + h * D + p.lo) = u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
       *reinterpret_cast<u32x2*>(dst + h * D + p.hi) = u32x2{pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
     }
@@ -218,6 +229,25 @@ __device__ __forceinline__ void prepare_rows(const PrepareArgs& a, const Powers&
     const unsigned long long off = ~(__ballot(lane >= i && lane - i < kScaleRows - slot % kScaleRows && win == slot + (lane - i)) >> i);
     return __builtin_ctzll(off);      // 1 .. 16 - slot % 16
   };
+  auto block_of = [&](int slot) __attribute__((always_inline)) {
+    const int page = slot / a.page_size, blk = slot % a.page_size / kScaleRows;
+    return (static_cast<size_t>(page) * a.Hkv + head) * (a.page_size / kScaleRows) + blk;
+  };
+  // a run's rows, the first's on their way while the turns are made
+  u32x2 lo[NI], hi[NI];
+  float old = 0.f;     // its block's scale
+  auto fetch = [&]() __attribute__((always_inline)) {
+    const int i = __builtin_ctzll(todo), n = run_length(i);
+    const bf16* from = src + static_cast<size_t>(t0 + i - 1) * stride;
+    old = scale[block_of(__builtin_amdgcn_readlane(win, i))];
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+      const bf16* row = from + min(k * RI + rr, n - 1) * stride;      // past the last: its copy
+      lo[k] = load4(row + p.lo);
+      hi[k] = load4(row + p.hi);
+    }
+  };
+  if (head < a.Hkv) fetch();
   const int i1 = 63 - __builtin_clzll(todo);
   const int first = t0 + __builtin_ctzll(todo) - 1, last = t0 + i1 - 1 + run_length(i1);      // tokens of all runs: tile + 15 at most
   fill_turns(a, pw, first, last - first, s_turn);
@@ -231,18 +261,15 @@ __device__ __forceinline__ void prepare_rows(const PrepareArgs& a, const Powers&
     const int r0 = slot % kScaleRows;
     const int n = run_length(i);
 
-    const int page = slot / a.page_size, blk = slot % a.page_size / kScaleRows;
-    const size_t bid = (static_cast<size_t>(page) * a.Hkv + head) * (a.page_size / kScaleRows) + blk;
+    const size_t bid = block_of(slot);
     uint8_t* block = pages + bid * (kScaleRows * D);
-    const int held = held_exp(scale[bid]);
+    const int held = held_exp(old);
     float x[NI][8];
     int top = 0;
 #pragma unroll
     for (int k = 0; k < NI; ++k) {
-      const int j = min(k * RI + rr, n - 1);      // past the last: its copy
-      const bf16* row = src + static_cast<size_t>(t + j) * stride;
-      load4(row + p.lo, x[k]);
-      load4(row + p.hi, x[k] + 4);
+      widen4(lo[k], x[k]);
+      widen4(hi[k], x[k] + 4);
     }
 #pragma unroll
     for (int k = 0; k < NI; ++k) {
@@ -292,6 +319,7 @@ __device__ __forceinline__ void prepare_rows(const PrepareArgs& a, const Powers&
       }
     }
     if (lane == 0) scale[bid] = pow2f(e);
+    if (todo) fetch();     // behind the stores: it may be the same block's next run
   }
 }
 
