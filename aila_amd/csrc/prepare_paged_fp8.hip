@@ -16,10 +16,13 @@
 // 1800 instructions a wave instead of 500 at D = 256).
 //
 // Bound by the bytes where there are many tokens: 8191, 16 / 4 heads, D = 256, rows
-// first 54.5 us for 184 MB = 3.4 TB/s (a large copy reaches 4.77; queries alone 31 us
-// = 4.3); by launch and the chain slots -> rows -> codes where there are few: 26
-// tokens, 32 / 8, D = 128, 6.2 us. Rows and queries interleaved in one launch were
-// slower (83 us for the 8191 tokens): what stores rows takes longest, and comes last.
+// first 54.2 us for 184 MB = 3.4 TB/s (a large copy reaches 4.9; queries alone 32 us
+// = 4.2; without the rotation 47 us in all, since a workgroup's turns are 1 to 2
+// thousand sines and cosines); by launch and the chain slots -> rows -> codes where
+// there are few: 26 tokens, 32 / 8, D = 128, 5.9 us. The rows, or a wave's first head,
+// are on their way while the turns are made (26 tokens 6.3 -> 5.9 us, 4096 of 32 / 8, D =
+// 128, 25.2 -> 23.9). Rows and queries interleaved in one launch were slower (83 us for
+// the 8191 tokens): what stores rows takes longest, and comes last.
 #include "paged_fp8.hpp"
 
 #include <type_traits>
@@ -409,10 +412,11 @@ extern "C" int aila_hip_prepare_qkv_paged_fp8(const void* q, long q_stride, long
   a.kv_groups = static_cast<int>(kv_groups);
   a.eps = eps;
   const Powers pw = rotary_dim > 0 && inv_freq == nullptr ? powers_of(theta, rotary_dim) : Powers{};
-  // One launch, rows first, or two (us, one / two). 16 / 4, D = 256: T = 32 7.1 / 10.1, 1024
-  // 11.7 / 15.9, 4096 (92 MB) 26.5 / 28.9, 8191 (184 MB) 66.5 / 54.5; 32 / 8, D = 128: 4096 25.2
-  // / 27.3, 8191 59.2 / 53.6; 16 / 8, D = 128: 8191 (117 MB) 36.7 / 36.2. Where the data do not
-  // stay in the caches, queries alone run at twice the waves a SIMD.
+  // One launch, rows first, or two (us, one / two). 16 / 4, D = 256: T = 32 7.0 / 10.0, 1024
+  // 11.8 / 16.1, 4096 (92 MB) 24.6 / 28.0, 6000 (135 MB) 42.9 / 37.7, 8191 (184 MB) 62.3 / 54.2;
+  // 32 / 8, D = 128: 4096 23.9 / 26.2, 6000 37.8 / 37.5, 8191 53.5 / 50.6; 16 / 8, D = 128: 8191
+  // (117 MB) 34.3 / 34.5. Where the data do not stay in the caches, queries alone run at
+  // twice the waves a SIMD.
   constexpr long kOneLaunchBytes = 120L << 20;
   const long moved = static_cast<long>(T) * D * (4L * Hq + 6L * Hkv);
   const size_t lds = static_cast<size_t>(tile + kScaleRows - 1) * (rotary_dim / 2) * sizeof(f32x2);
