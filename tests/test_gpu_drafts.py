@@ -273,6 +273,26 @@ def test_tree_split_over_workgroups(D, Hq, Hkv, page, new, before):
         assert torch.equal(a[:sum(new)], b[:sum(new)])
 
 
+@pytest.mark.parametrize("D,Hq,Hkv,page,new,before", [
+    (128, 32, 8, 64, [33], [7000]), (256, 16, 4, 16, [120, 120, 60], [3000, 1000, 2000]), (64, 32, 8, 32, [100, 100, 60], [4000, 100, 900]),   # wide: few tiles, many
+    (64, 32, 8, 16, [3] * 6, [5000 - 700 * i for i in range(6)]), (256, 16, 4, 32, [64], [16000]), (64, 8, 2, 64, [1], [60000]),             # narrow: few columns, many
+    (128, 16, 8, 16, [64, 0, 1], [9000, 7, 0]), (256, 8, 8, 64, [2, 2], [12000, 0])])
+def test_tree_joins(D, Hq, Hkv, page, new, before):
+    """Joins of few and of many records of both walks, over records that hold NaN where none is written; masks that leave nothing; twice the same bits."""
+    import torch
+    import aila_amd as A
+    q, cache, table, starts, lens, mask, seen, rows = _tree_case(D, Hq, Hkv, page, new, before, 13)
+    mask[sum(new) - 1] = 0          # the last token attends no drafted row, and nothing at all where none is before them
+    seen[sum(new) - 1] = []
+    size = A.gqa_tree_paged_fp8_workspace_size(q.shape[0], len(new), Hq, Hkv, D, max(rows), mask.shape[1])
+    ws = torch.full((size,), 0xff, dtype=torch.uint8, device="cuda")
+    outs = [torch.full((q.shape[0], Hq, D), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for out in outs:
+        A.gqa_tree_paged_fp8(q, *cache, table, starts, lens, mask, max(rows), out=out, workspace=ws)
+    assert torch.equal(*outs) and bool((outs[0][sum(new):] == 7.0).all())
+    _tree_check(outs[0], q, cache, table, new, before, seen, pick={0, 1, 31, 32, 63, 64, 99})
+
+
 @pytest.mark.parametrize("B,D,Hq,Hkv,most,long", [(1300, 128, 4, 2, 3, 40), (4096, 64, 2, 2, 2, 20), (600, 256, 8, 1, 9, 300), (700, 128, 16, 1, 12, 30)])
 def test_trees_of_many_requests(B, D, Hq, Hkv, most, long):
     import torch
