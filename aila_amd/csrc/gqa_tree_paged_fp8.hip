@@ -786,10 +786,10 @@ int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t wor
 // once in LDS (gqa_prefill_paged_fp8.hip): from some columns a request on, which the
 // host knows on average, and the more of them the fewer requests share the device.
 // us, here split / as prompts, trees of up to 16, 32, 64, 128 columns (two thirds of it
-// on average where there are more than one), 8000 rows. D = 128: 1 request 20/28, 22/28,
-// 24/29, 29/30; 8 32/44, 35/43, 40/44, 54/48; 32 101/132, 104/131, 126/138, 173/147. D = 64:
-// 1 14/21, 15/21, 17/23, 21/24; 8 23/35, 24/35, 29/35, 39/37; 32 58/92, 59/91, 77/95, 118/97.
-// D = 256: 1 37/37, 41/37, 44/39, 51/41; 8 37/45, 43/46, 53/47, 73/55; 32 96/128, 103/128,
+// on average where there are more than one), 8000 rows. D = 128: 1 request 16/23, 18/23,
+// 21/24, 26/26; 8 32/44, 35/43, 40/44, 54/48; 32 101/132, 104/131, 126/138, 173/147. D = 64:
+// 1 13/18, 14/18, 17/19, 20/20; 8 23/35, 24/35, 29/35, 39/37; 32 58/92, 59/91, 77/95, 118/97.
+// D = 256: 1 20/27, 24/28, 28/29, 36/32; 8 37/45, 43/46, 53/47, 73/55; 32 96/128, 103/128,
 // 129/129, 192/144.
 // But not if requests that fill the device are short for their columns: each is one
 // workgroup's here then. us, here whole / as prompts, of up to 500, 1000, 2000, 4000 rows.
