@@ -29,6 +29,7 @@
 #include "paged_fp8.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace aila {
 namespace {
@@ -81,9 +82,11 @@ __device__ __forceinline__ int item_units(int tiles, int len) {
 template <int D>
 __device__ __forceinline__ Shape shape_of(const TreeArgs& a, int b) {
   Shape s;
-  s.q0 = min(max(a.query_start[b], 0), a.T);
-  s.n = max(min(max(a.query_start[b + 1], 0), a.T) - s.q0, 0);
-  s.len = min(max(a.seq_lens[b], 0), a.max_len);
+  const int begin = a.query_start[b], end = a.query_start[b + 1], len = a.seq_lens[b];
+  __builtin_amdgcn_sched_barrier(0);      // one round trip
+  s.q0 = min(max(begin, 0), a.T);
+  s.n = max(min(max(end, 0), a.T) - s.q0, 0);
+  s.len = min(max(len, 0), a.max_len);
   s.base = s.len - s.n;
   s.n = min(s.n, 32 * a.words32);   // those behind have no mask
   const int all = (s.n * a.group + kTile - 1) / kTile;
@@ -472,12 +475,16 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
     for (int n0 = 0; n0 < ns; n0 += 32) {
       // lane l holds block l % 2 of strip n0 + l / 2
       const int blk = (row0 + (n0 + (lane >> 1)) * rows) / kScaleRows + (lane & 1);
-      const BlockRef ref = block_ref(c, b, kvh, blk, blk_end);
+      // without branches, at whose ends the loads would be waited for
+      BlockRef ref;
+      {
+        const int at = min(blk, blk_end - 1), p = at / c.page_blocks;
+        const int page = c.table[static_cast<size_t>(b) * c.max_pages + p];
+        ref.bid = blk < blk_end && page >= 0 && page < c.num_pages ? (page * c.Hkv + kvh) * c.page_blocks + at - p * c.page_blocks : -1;
+        ref.ks = c.k_scale[max(ref.bid, 0)];
+        ref.vs = c.v_scale[max(ref.bid, 0)];
+      }
       const int n1 = min(ns - n0, 32);
-      // no page: all rows masked, and -inf times a scale of 0 would be NaN
-      const float my_k = (ref.bid >= 0 ? ref.ks : 1.0f) * a.scale_log2;
-      const int my_e = held_exp(ref.vs);
-      const float my_ef = static_cast<float>(my_e), my_i = pow2f(-my_e);
       Codes<D> x;
       auto bid = [&](int n, int i) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(ref.bid, (2 * n + i) & 63); };
       auto next_k = [&](int n) __attribute__((always_inline)) {
@@ -486,6 +493,13 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
       auto next_v = [&](int n) __attribute__((always_inline)) {
         if (n < n1) load_v<D>(x, c.v_pages, bid(n, 0), bid(n, 1), m32, hf);
       };
+      next_k(0);
+      next_v(0);
+      __builtin_amdgcn_sched_barrier(0);      // the codes do not wait for the scales
+      // no page: all rows masked, and -inf times a scale of 0 would be NaN
+      const float my_k = (ref.bid >= 0 ? ref.ks : 1.0f) * a.scale_log2;
+      const int my_e = held_exp(ref.vs);
+      const float my_ef = static_cast<float>(my_e), my_i = pow2f(-my_e);
       auto scales = [&](int n) __attribute__((always_inline)) {
         Scales r;
         r.ka = readlane_f(my_k, 2 * n);
@@ -496,8 +510,6 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
         r.ib = readlane_f(my_i, 2 * n + 1);
         return r;
       };
-      next_k(0);
-      next_v(0);
       // the strips whose rows all columns attend, then the others
       const bool hole = __ballot(blk < blk_end && ref.bid < 0) != 0;
       const int plain = hole ? 0 : min(n1, max(0, open - row0 - n0 * rows + rows - 32) / rows);
@@ -515,11 +527,11 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
         __builtin_amdgcn_sched_barrier(0);
       }
       for (; n < n1; ++n) {
-        f32x16 sc = make_scores<D>(x, q);
-        next_k(n + 1);
         const int row = row0 + (n0 + n) * rows;
         const uint32_t held = (bid(n, 0) >= 0 ? 0xffffu : 0u) | (bid(n, 1) >= 0 ? 0xffff0000u : 0u);
         const uint32_t keep = (tree_rows(words, a.words32, row, s.base, end) & held) >> (4 * hf);
+        f32x16 sc = make_scores<D>(x, q);
+        next_k(n + 1);
         mask_scores(sc, keep);
         mend_values<D>(col, x, keep, m32);
         make_weights<D>(p, col, sc, scales(n));
@@ -529,6 +541,8 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
     }
 
     // ---- the waves' results meet ------------------------------------------
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));      // places in LDS are made here, not held over the strips
     __syncthreads();   // the item before has been read
     {
       const float l = half_sum(col.l);
@@ -554,35 +568,49 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
     const bool whole = i0 == 0 && i1 == it.units;
     float* rec = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (i0 == 0 ? 1 : 0)) * a.rec_cols * (D + kRecTail);
     const int here = min(kTile * it.tiles, cols - kTile * it.tile0);      // columns of the item
-    const int parts = kWaves<D> >> lg;
-    for (int idx = threadIdx.x; idx < here * (D / 4); idx += kThreads) {
-      const int x = idx / (D / 4), d = idx % (D / 4) * 4;
-      const int slot0 = x;                      // wave x / kTile
-      const int step = lanes * kTile;           // the same column, other keys
-      float M = -INFINITY, L = 0.f;
-      for (int i = 0; i < parts; ++i) M = fmaxf(M, s_ml[(slot0 + i * step) * 2]);
-      f32x4 A = {0.f, 0.f, 0.f, 0.f};
-      for (int i = 0; i < parts; ++i) {
-        const int slot = slot0 + i * step;
-        const float mw = s_ml[slot * 2];
-        const float f = mw == -INFINITY ? 0.f : fast_exp2(mw - M);
-        A += f * *reinterpret_cast<const f32x4*>(s_acc + slot * kStride + d);
-        L += f * s_ml[slot * 2 + 1];
-      }
-      if (whole) {
-        const int y = kTile * it.tile0 + x, tok = y / a.group;
-        const float inv = L == 0.f ? 0.f : 1.0f / L;
-        *reinterpret_cast<u32x2*>(a.out + (static_cast<size_t>(s.q0 + tok) * a.Hq + kvh * a.group + y - tok * a.group) * D + d) =
-            u32x2{pack_bf16x2(A[0] * inv, A[1] * inv), pack_bf16x2(A[2] * inv, A[3] * inv)};
-      } else {
-        float* r = rec + x * (D + kRecTail);
-        *reinterpret_cast<f32x4*>(r + d) = A;
-        if (d == 0) {
-          r[D] = M;
-          r[D + 1] = L;
+    // a column's results are those of waves x / kTile + i * lanes; the loads of all go out
+    // together (one after the other they took 3 us of 14, D = 256, 32 columns)
+    auto join = [&](auto parts) __attribute__((always_inline)) {
+      constexpr int N = decltype(parts)::value;
+      for (int idx = tid; idx < here * (D / 4); idx += kThreads) {
+        const int x = idx / (D / 4), d = idx % (D / 4) * 4;
+        f32x2 ml[N];
+        f32x4 v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int slot = x + i * lanes * kTile;
+          ml[i] = *reinterpret_cast<const f32x2*>(s_ml + slot * 2);
+          v[i] = *reinterpret_cast<const f32x4*>(s_acc + slot * kStride + d);
+        }
+        float M = ml[0][0], L = 0.f;
+#pragma unroll
+        for (int i = 1; i < N; ++i) M = fmaxf(M, ml[i][0]);
+        f32x4 A = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float f = ml[i][0] == -INFINITY ? 0.f : fast_exp2(ml[i][0] - M);
+          A += f * v[i];
+          L += f * ml[i][1];
+        }
+        if (whole) {
+          const int y = kTile * it.tile0 + x, tok = y / a.group;
+          const float inv = L == 0.f ? 0.f : 1.0f / L;
+          *reinterpret_cast<u32x2*>(a.out + (static_cast<size_t>(s.q0 + tok) * a.Hq + kvh * a.group + y - tok * a.group) * D + d) =
+              u32x2{pack_bf16x2(A[0] * inv, A[1] * inv), pack_bf16x2(A[2] * inv, A[3] * inv)};
+        } else {
+          float* r = rec + x * (D + kRecTail);
+          *reinterpret_cast<f32x4*>(r + d) = A;
+          if (d == 0) {
+            r[D] = M;
+            r[D + 1] = L;
+          }
         }
       }
-    }
+    };
+    if (lg == 0) join(std::integral_constant<int, kWaves<D>>{});
+    else if (lg == 1) join(std::integral_constant<int, kWaves<D> / 2>{});
+    else if (lg == 2) join(std::integral_constant<int, kWaves<D> / 4>{});
+    else join(std::integral_constant<int, 1>{});
   }
 }
 
