@@ -569,7 +569,7 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
     float* rec = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (i0 == 0 ? 1 : 0)) * a.rec_cols * (D + kRecTail);
     const int here = min(kTile * it.tiles, cols - kTile * it.tile0);      // columns of the item
     // a column's results are those of waves x / kTile + i * lanes; the loads of all go out
-    // together (one after the other they took 3 us of 14, D = 256, 32 columns)
+    // together (one after the other they took 2.6 us of 14.4, D = 256, 32 columns)
     auto join = [&](auto parts) __attribute__((always_inline)) {
       constexpr int N = decltype(parts)::value;
       for (int idx = tid; idx < here * (D / 4); idx += kThreads) {
@@ -749,13 +749,13 @@ size_t workspace_need(int T, int B, int Hkv, int group, int words, int max_len) 
 // grows with the CUs they fill, and is shared by the tiles of a request (of average
 // size), since a workgroup's waves that have no tile take other keys. us in a graph, whole
 // / split, lengths between half the bound and all of it, trees of up to 4 tokens (16: in
-// parentheses), G = 4. D = 128, 8 KV heads: 1 request of 600 rows 11.0/12.9 (16.6/15.5), 1000
-// 13.0/13.2 (20.0/15.8), 2000 17.8/13.3 (28.9/17.6); 4 of 1000 13.2/13.5 (20.2/18.9), 1500
-// 15.4/14.0 (24.6/27.5); 8 of 1500 16.5/22.2 (25.5/27.4), 3000 23.7/24.7 (39.7/30.1); 16 of
-// 2000 19.7/25.4 (31.0/33.1), 3000 24.3/28.1 (40.3/36.4). D = 64: 1 of 1000 10.3/12.0
-// (14.4/13.3), 2000 13.6/12.1 (21.4/13.9); 8 of 2000 13.7/17.4 (21.6/20.8). D = 256, 4 heads:
-// 1 of 200 13.0/14.5 (20.7/18.9), 400 15.9/14.5 (25.3/19.7); 8 of 400 16.1/15.1 (25.6/24.8),
-// 800 20.0/16.5 (33.8/33.8); 16 of 800 21.4/25.0 (35.5/39.5), 2000 34.5/29.8 (62.5/43.0).
+// parentheses), G = 4. D = 128, 8 KV heads: 1 request of 600 rows 10.3/12.2 (15.3/14.1), 1000
+// 12.3/12.5 (18.7/14.4), 2000 17.0/12.5 (27.8/15.8); 4 of 1000 12.5/12.8 (19.0/17.0), 1500
+// 14.7/13.1 (23.5/23.7); 8 of 1500 15.6/19.8 (24.3/23.8), 3000 23.0/22.5 (38.4/26.5); 16 of
+// 2000 18.8/23.0 (30.1/29.6), 3000 23.4/25.6 (39.4/32.8). D = 64: 1 of 1000 9.5/11.4
+// (14.0/12.7), 2000 13.2/11.6 (21.1/13.4); 8 of 2000 13.4/16.3 (21.4/18.9). D = 256, 4 heads:
+// 1 of 200 11.8/13.1 (18.1/16.0), 400 14.7/13.2 (22.8/16.7); 8 of 400 15.0/13.8 (23.1/21.7),
+// 800 19.2/15.0 (31.7/28.7); 16 of 800 20.2/22.1 (32.9/33.1), 2000 33.7/26.7 (60.5/36.8).
 bool walks_whole(long columns, int B, int Hkv, int max_len, int D) {
   const long items = static_cast<long>(B) * Hkv, tiles = (columns + 32L * B - 1) / (32L * B);
   const long most = D == 256 ? 300 + items * items / 5 : (D == 128 ? 1000 : 1500) + items * items * 3 / 10;
@@ -764,12 +764,12 @@ bool walks_whole(long columns, int B, int Hkv, int max_len, int D) {
 
 // Records of a column, where requests share evenly, from which a workgroup joins one
 // column's. us, the whole call, columns by columns / each, 8000 rows (30000: in
-// parentheses), a request's columns. 1 request, D = 256, 4 heads: 4 27.3/17.2 (34.3/24.2), 64
-// 37.7/27.5 (47.9/37.5); 2: 52 in all 37.9/33.2 (49.3/44.0); 8: 332 52.9/52.5, 676
-// 74.6/73.5; 32: 128 92.7/96.0, 616 103.6/113.9. D = 128, 8 heads: 1 request, 4 19.6/14.3
-// (27.4/21.8), 128 30.2/25.7; 4: 92 30.7/29.8, 192 34.5/35.0, 388 43.4/45.9; 8: 36
-// 30.4/29.8, 160 35.1/37.8; 32: 128 97.6/108.7. D = 64: 1: 4 16.9/12.4, 128 24.8/20.0; 4: 92
-// 22.2/21.8, 192 25.5/26.6; 32: 128 57.8/69.4.
+// parentheses), all columns of a KV head. 1 request, D = 256, 4 heads: 4 26.2/16.7
+// (33.8/23.8), 64 35.1/24.8 (45.0/34.9); 2: 52 33.4/27.7 (44.4/38.2); 8: 332 48.1/46.8, 676
+// 68.8/67.9; 32: 128 91.8/94.6, 272 95.1/104.4. D = 128, 8 heads: 1: 4 18.4/13.2 (26.3/21.2),
+// 128 28.7/24.3 (44.1/39.1); 4: 92 27.2/26.5, 192 31.3/32.1, 388 40.8/43.0; 8: 36 28.7/27.8,
+// 160 31.8/34.3; 32: 128 92.6/104.5. D = 64: 1: 4 16.3/11.9, 128 23.9/19.3; 4: 92 20.8/20.2,
+// 192 23.9/24.9; 32: 128 56.7/68.2.
 constexpr int kEachRecords = 8;
 
 template <int D>
@@ -814,19 +814,21 @@ int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t wor
 // once in LDS (gqa_prefill_paged_fp8.hip): from some columns a request on, which the
 // host knows on average, and the more of them the fewer requests share the device.
 // us, here split / as prompts, trees of up to 16, 32, 64, 128 columns (two thirds of it
-// on average where there are more than one), 8000 rows. D = 128: 1 request 16/23, 18/23,
-// 21/24, 26/26; 8 32/44, 35/43, 40/44, 54/48; 32 101/132, 104/131, 126/138, 173/147. D = 64:
-// 1 13/18, 14/18, 17/19, 20/20; 8 23/35, 24/35, 29/35, 39/37; 32 58/92, 59/91, 77/95, 118/97.
-// D = 256: 1 20/27, 24/28, 28/29, 36/32; 8 37/45, 43/46, 53/47, 73/55; 32 96/128, 103/128,
-// 129/129, 192/144.
+// on average where there are more than one), 8000 rows. D = 128: 1 request 14/23, 16/23,
+// 19/24, 25/26; 2 19/24, 22/24, 27/25, 35/29; 4 24/32, 27/32, 31/35, 41/38; 8 30/44, 32/44,
+// 37/47, 53/50; 32 97/138, 100/133, 123/136, 173/149. D = 64: 1 12/18, 13/18, 16/19, 19/20; 2
+// 16/19, 18/19, 21/20, 26/22; 8 23/35, 23/35, 28/36, 39/38; 32 57/101, 58/95, 77/97,
+// 119/100. D = 256: 1 19/27, 21/27, 25/29, 33/32; 2 24/28, 28/28, 35/30, 45/36; 4 28/32,
+// 32/33, 37/36, 53/43; 8 33/44, 36/45, 48/49, 70/56; 32 95/129, 100/133, 128/132, 188/144.
+// (One request of D = 256, whose records are joined a column each, keeps to itself longer.)
 // But not if requests that fill the device are short for their columns: each is one
 // workgroup's here then. us, here whole / as prompts, of up to 500, 1000, 2000, 4000 rows.
-// D = 128, 8 heads: 16 requests of up to 128 columns 23/27, 33/34, 51/40, 88/52; 32 25/40,
-// 36/47, 55/60, 100/85; 32 of up to 256 columns 41/52, 61/64, 98/83, 178/132. D = 64: 32 of
-// 256 29/39, 44/49, 72/63, 126/90. D = 256, 4 heads: 32 of 64 30/35, 41/41, 64/54, 121/80.
+// D = 128, 8 heads: 16 requests of up to 128 columns 22/27, 31/34, 50/40, 85/53; 32 23/40,
+// 33/46, 52/60, 101/90; 32 of up to 256 columns 39/51, 58/64, 96/85, 175/137. D = 64: 32 of
+// 256 28/38, 43/48, 72/62, 127/92. D = 256, 4 heads: 32 of 64 27/35, 38/41, 61/54, 120/84.
 bool walks_as_prompt(int T, int B, int Hkv, int group, int words, int max_len, int D) {
   const long columns = static_cast<long>(T) * group;
-  const long each = D == 64 ? 70 : D == 128 ? 44 : 34, more = D == 64 ? 130 : D == 128 ? 72 : 16;
+  const long each = D == 64 ? 62 : D == 128 ? 54 : 40, more = D == 64 ? 80 : D == 128 ? 60 : B == 1 ? 70 : 10;
   if (columns <= each * B + more) return false;
   if (static_cast<double>(max_len) * columns <= (D == 64 ? 800.0 : D == 128 ? 700.0 : 250.0) * B * B * Hkv) return false;
   // its line of key tiles and its merge's threads have to fit
