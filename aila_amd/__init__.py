@@ -11,7 +11,10 @@ from __future__ import annotations
 
 import array
 import ctypes
+import functools
+import itertools
 import math
+import operator
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -883,6 +886,9 @@ def gqa_tree_paged_fp8(q, k_pages, v_pages, k_scale, v_scale, block_table, query
     return out
 
 
+_SHAPE, _DTYPE = operator.attrgetter("shape"), operator.attrgetter("dtype")
+
+
 def _layer_pointers(caches, dev):
     """(layers, shape of a cache, addresses of the four host arrays of device
     pointers, what keeps them) of one cache (k_pages, v_pages, k_scale, v_scale)
@@ -893,22 +899,18 @@ def _layer_pointers(caches, dev):
     if torch.is_tensor(caches[0]):
         caches = [caches]
     # a hundred tensors in a deep stack: looked at attribute by attribute, in loops of C
-    n, flat = len(caches), [t for c in caches for t in c]
+    n, flat = len(caches), list(itertools.chain.from_iterable(caches))
     ok = len(flat) == 4 * n and all([t is not None for t in flat])
     if ok:
-        shape, scales = flat[0].shape, flat[2].shape
+        kind, shape, scales = type(flat[0]), flat[0].shape, flat[2].shape
         pages, scale = flat[0::4] + flat[1::4], flat[2::4] + flat[3::4]
-        f8, f32 = torch.float8_e4m3fn, torch.float32
-        ok = len(shape) == 4 and not shape[2] % _SCALE_ROWS and scales == (shape[0], shape[1], shape[2] // _SCALE_ROWS) \
-            and [t.shape for t in pages] == [shape] * (2 * n) and [t.shape for t in scale] == [scales] * (2 * n) \
-            and all([t.dtype is f8 for t in pages]) and all([t.dtype is f32 for t in scale]) and all([t.is_contiguous() for t in flat]) \
-            and [t.get_device() for t in flat] == [dev] * (4 * n)
+        ok = all(map(kind.is_contiguous, flat)) and list(map(kind.get_device, flat)).count(dev) == 4 * n \
+            and len(shape) == 4 and not shape[2] % _SCALE_ROWS and scales == (shape[0], shape[1], shape[2] // _SCALE_ROWS) \
+            and list(map(_SHAPE, pages)).count(shape) == list(map(_SHAPE, scale)).count(scales) == 2 * n \
+            and list(map(_DTYPE, pages)).count(torch.float8_e4m3fn) == list(map(_DTYPE, scale)).count(torch.float32) == 2 * n
     if ok:
-        ptrs = array.array("Q", [t.data_ptr() for t in pages + scale])
-        low = 0
-        for x in ptrs[:2 * n]:
-            low |= x
-        ok = not low & 15
+        ptrs = array.array("Q", list(map(kind.data_ptr, pages + scale)))
+        ok = not functools.reduce(operator.or_, ptrs[:2 * n]) & 15
     if not ok:
         for c in caches:
             if len(c) != 4:

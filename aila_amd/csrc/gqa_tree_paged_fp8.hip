@@ -19,7 +19,7 @@
 // of 6000 rows, 8 KV heads, D = 128, 8 columns, 99 us = 4.1 TB/s; wider trees are bound by
 // the conversions (64 codes a lane and strip) and the softmax on the vector ALU, 205
 // instructions a strip and tile for 512 cycles of products, and take the other walk
-// (walks_as_prompt, below). One sequence of 612 rows with 8 drafted tokens: 10 us in one
+// (walks_as_prompt, below). One sequence of 612 rows with 8 drafted tokens: 9.9 us in one
 // launch, which is start-up and three strips in a row: lengths -> blocks -> codes.
 //
 // Tried and left: strips staged by DMA in LDS (no faster: 105 against 112 us for 32
