@@ -770,6 +770,7 @@ bool walks_whole(long columns, int B, int Hkv, int max_len, int D) {
 // 128 28.7/24.3 (44.1/39.1); 4: 92 27.2/26.5, 192 31.3/32.1, 388 40.8/43.0; 8: 36 28.7/27.8,
 // 160 31.8/34.3; 32: 128 92.6/104.5. D = 64: 1: 4 16.3/11.9, 128 23.9/19.3; 4: 92 20.8/20.2,
 // 192 23.9/24.9; 32: 128 56.7/68.2.
+// Up to 1024 columns of all heads, D = 256 (a quarter of the phases, so less to meet) 4096.
 constexpr int kEachRecords = 8;
 
 template <int D>
