@@ -951,8 +951,12 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
       if (!reuse) {
         for (int i = threadIdx.x; i < fill; i += kThreads) {
           const int bid = s_bid[i];
-          s_ks[i] = bid >= 0 ? c.k_scale[bid] : 0.f;
-          s_vs[i] = bid >= 0 ? c.v_scale[bid] : 0.f;
+          // TREE: a block that no token attends may hold any scale
+          auto scale = [&](const float* s) __attribute__((always_inline)) {
+            return TREE ? fminf(fmaxf(s[bid], kMinScale), kMaxScale) : s[bid];
+          };
+          s_ks[i] = bid >= 0 ? scale(c.k_scale) : 0.f;
+          s_vs[i] = bid >= 0 ? scale(c.v_scale) : 0.f;
         }
       }
       primed = false;

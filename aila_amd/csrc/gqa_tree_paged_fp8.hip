@@ -496,8 +496,9 @@ __global__ __launch_bounds__(64 * kWaves<D>, 1) void gqa_tree_paged_fp8_kernel(P
       next_k(0);
       next_v(0);
       __builtin_amdgcn_sched_barrier(0);      // the codes do not wait for the scales
-      // no page: all rows masked, and -inf times a scale of 0 would be NaN
-      const float my_k = (ref.bid >= 0 ? ref.ks : 1.0f) * a.scale_log2;
+      // within its range, which leaves a scale as it is: a block that no token attends may
+      // hold any (NaN too), and -inf times 0 or NaN would not mask its rows
+      const float my_k = fminf(fmaxf(ref.ks, kMinScale), kMaxScale) * a.scale_log2;
       const int my_e = held_exp(ref.vs);
       const float my_ef = static_cast<float>(my_e), my_i = pow2f(-my_e);
       auto scales = [&](int n) __attribute__((always_inline)) {

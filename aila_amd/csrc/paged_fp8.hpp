@@ -18,6 +18,7 @@ constexpr int kScaleRows = 16;
 // Exponents of a scale: the smallest e with amax <= 448 * 2^e, bounded so that
 // 448 * 2^e stays finite and the smallest code times it stays a normal bf16.
 constexpr int kMinScaleExp = -100, kMaxScaleExp = 119;
+constexpr float kMinScale = 0x1p-100f, kMaxScale = 0x1p119f;
 constexpr float kE4m3Max = 448.0f;
 
 // 2^e in fp32; 0 below its normal range.

@@ -490,8 +490,9 @@ int aila_hip_prepare_qkv_paged_fp8(const void* q, long q_stride,
  *              64. A token attends itself only if its own bit is set. mask_words <=
  *              64. A request's tokens from the (64 * mask_words)-th on have no mask
  *              and are not computed.
- * Tokens from query_start[B] on are not touched. The softmax weights are rounded to
- * bf16 (2^-8 of each at most) before they meet V. Sums are held in fp32, of weights
+ * Tokens from query_start[B] on are not touched. Rows that a token does not attend may
+ * hold anything, and so may the scale of a block of which no token attends a row. The
+ * softmax weights are rounded to bf16 (2^-8 of each at most) before they meet V. Sums are held in fp32, of weights
  * of up to 2^8: the largest value that a block of V can hold (448 times its scale)
  * times the rows attended has to stay below 2^120. Other arguments as
  * aila_hip_gqa_prefill_paged_fp8.
