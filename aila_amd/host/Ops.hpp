@@ -94,11 +94,12 @@ void attention_prefill_paged_fp8(Context& ctx, Tensor& q, Tensor& k_pages, Tenso
 // Per-head norm and rotation of q [T, Hq * q_head_stride] (0: D; 2 D for packed
 // q|gate rows) into q_out [T, Hq*D], and of new_k [T, Hkv*D], which goes into the
 // cache with new_v. q_norm, k_norm [D] bf16 or null; positions [T], or [3, T] with
-// section_h and section_w (interleaved mRoPE); rotary_dim 0: no rotation.
+// section_h and section_w (interleaved mRoPE; both have to be given then); rotary_dim
+// 0: no rotation.
 void prepare_qkv_paged_fp8(Context& ctx, Tensor& q, Tensor& new_k, Tensor& new_v, Tensor& k_pages, Tensor& v_pages,
                            Tensor& k_scale, Tensor& v_scale, Tensor& slots, Tensor& positions, Tensor* q_norm,
                            Tensor* k_norm, Tensor& q_out, int num_heads, int rotary_dim, float theta, float eps,
-                           int q_head_stride = 0, int section_h = 0, int section_w = 0, Tensor* inv_freq = nullptr);
+                           int q_head_stride = 0, int section_h = -1, int section_w = -1, Tensor* inv_freq = nullptr);
 
 // attention_prefill_paged_fp8 of drafted trees: tree_mask [T, 2 * mask_words] s32,
 // the halves of 64-bit words, lower first.

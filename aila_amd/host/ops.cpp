@@ -270,6 +270,8 @@ void prepare_qkv_paged_fp8(Context& ctx, Tensor& q, Tensor& new_k, Tensor& new_v
     pos = s32(positions, "prepare_qkv_paged_fp8 positions", streams ? 3 * int64_t{T} : T);
     if (streams && (positions.shape(0) != 3 || positions.shape(1) != T))
       throw std::runtime_error("prepare_qkv_paged_fp8 positions: must be [T] or [3, T]");
+    if (streams && (section_h < 0 || section_w < 0))
+      throw std::runtime_error("prepare_qkv_paged_fp8: positions [3, T] need section_h and section_w");
   }
   check(aila_hip_prepare_qkv_paged_fp8(
             q.data(), q_row, step, new_k.data(), row, new_v.data(), row, q_out.data(),
