@@ -339,6 +339,13 @@ __global__ __launch_bounds__(kThreads, P == Part::kQueries ? 8 : D == 256 ? 3 : 
   }
 }
 
+// Whether [o, o + n) meets one of `count` runs of w elements from x on, `step` (>= w) apart.
+bool meets(const bf16* o, long n, const bf16* x, long count, long step, long w) {
+  const intptr_t at = (reinterpret_cast<intptr_t>(o) - reinterpret_cast<intptr_t>(x)) / static_cast<intptr_t>(sizeof(bf16));
+  const long i = at < w ? 0 : (at - w) / step + 1;      // the first run that ends behind o
+  return i < count && i * step < at + n;
+}
+
 Powers powers_of(float theta, int rot) {
   Powers p{};
   const double r = -2.0 / rot;
@@ -390,6 +397,18 @@ extern "C" int aila_hip_prepare_qkv_paged_fp8(const void* q, long q_stride, long
   // fewer than 2^32 threads, the most of a launch
   const long kv_groups = (static_cast<long>(T) + tile - 1) / tile * ((Hkv + 1) / 2);
   AILA_REQUIRE(T > 0 && T <= (1 << 30) && (kv_groups + T) * kThreads < (1L << 32), "%s: T=%d tokens are none or too many for one call", what, T);
+  {
+    const bf16 *o = static_cast<const bf16*>(q_out), *x = static_cast<const bf16*>(q);
+    const long n = static_cast<long>(T) * Hq * D, span = (Hq - 1) * q_head_stride + D, row = static_cast<long>(Hkv) * D;
+    bool over = meets(o, n, static_cast<const bf16*>(k), T, k_stride, row) || meets(o, n, static_cast<const bf16*>(v), T, v_stride, row);
+    if (o != x) {
+      // the first token that ends behind q_out's begin may have it between two heads; the next one may not
+      const long at = (reinterpret_cast<intptr_t>(o) - reinterpret_cast<intptr_t>(x)) / static_cast<long>(sizeof(bf16));
+      const long i = at < span ? 0 : (at - span) / q_stride + 1;
+      over |= (i < T && meets(o, n, x + i * q_stride, Hq, q_head_stride, D)) || (i + 1 < T && (i + 1) * q_stride < at + n);
+    }
+    AILA_REQUIRE(!over, "%s: q_out overlaps q, k or v", what);
+  }
   PrepareArgs a{};
   a.q = static_cast<const bf16*>(q);
   a.k = static_cast<const bf16*>(k);

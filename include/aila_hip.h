@@ -459,8 +459,8 @@ int aila_hip_gqa_prefill_paged_fp8(const void* q, long q_stride,
  * for the (unrounded) y here; v as there.
  *   q        head h of token t at + t * q_stride + h * q_head_stride elements
  *            (multiples of 8: the queries of a packed q|gate row have head stride
- *            2 D); q_out [T, Hq, D] (may be q, where that is [T, Hq, D]; it may not
- *            overlap k, v or q otherwise)
+ *            2 D); q_out [T, Hq, D] (may be q, where that is [T, Hq, D]; it is refused
+ *            where it overlaps k, v or q otherwise)
  *   k, v     [Hkv, D] of token t at + t * k_stride, t * v_stride elements
  *   slots    int[T], as aila_hip_kv_append_paged_fp8; -1: k and v are skipped
  *   positions  p of each token, int[T] (NULL where rotary_dim is 0). With pos_h and
