@@ -78,6 +78,27 @@ __device__ __forceinline__ Place place_of(int s, int rot) {
   return x < half ? Place{x, x + half, x, true} : Place{x + half, x + D / 2, 0, false};
 }
 
+// (cosine, sine) of x turns, |x| <= 1/2, each rounded once: Taylor's series within an eighth
+// of a turn, in fp64 (the first terms left out are below 2^-32 of them). The fp32 functions
+// of the angle in fp32 are off by up to 2^-22, which shows in codes next to a border.
+__device__ __forceinline__ f32x2 turn_of(double x) {
+  const double k = __builtin_rint(4.0 * x);
+  const double a = (x - 0.25 * k) * 6.283185307179586, z = a * a;
+  double s = -1.0 / 39916800, c = -1.0 / 3628800;
+  s = fma(s, z, 1.0 / 362880);
+  c = fma(c, z, 1.0 / 40320);
+  s = fma(s, z, -1.0 / 5040);
+  c = fma(c, z, -1.0 / 720);
+  s = fma(s, z, 1.0 / 120);
+  c = fma(c, z, 1.0 / 24);
+  s = fma(s, z, -1.0 / 6);
+  c = fma(c, z, -0.5);
+  const float sn = static_cast<float>(fma(a * z, s, a)), cs = static_cast<float>(fma(z, c, 1.0));
+  const int q = static_cast<int>(k) & 3;      // quarter turns
+  const float u = q & 1 ? sn : cs, v = q & 1 ? cs : sn;
+  return f32x2{q == 1 || q == 2 ? -u : u, q >= 2 ? -v : v};
+}
+
 // (cosine, sine) of the pairs of `count` tokens from `token` on, [token][pair] in LDS:
 // each once for the workgroup, whose waves all need the same. A thread keeps to a pair.
 __device__ __forceinline__ void fill_turns(const PrepareArgs& a, const Powers& pw, int token, int count, f32x2* s_turn) {
@@ -99,10 +120,7 @@ __device__ __forceinline__ void fill_turns(const PrepareArgs& a, const Powers& p
   }
   for (int t = first; t < count; t += step) {
     double x = static_cast<double>(from[token + t]) * f;
-    x -= __builtin_rint(x);
-    float sn, cs;
-    sincospif(2.0f * static_cast<float>(x), &sn, &cs);
-    s_turn[t * half + j] = f32x2{cs, sn};
+    s_turn[t * half + j] = turn_of(x - __builtin_rint(x));
   }
 }
 
@@ -142,9 +160,12 @@ __device__ __forceinline__ void norm_turn(float* x, const float* w, const Turn& 
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-  const float r = 1.0f / sqrtf(row_sum<D / 8>(ss) * (1.0f / D) + eps);
+  // x / root, rounded once: the reciprocal in two parts (the second of an infinite root,
+  // which makes finite x 0, from the largest finite one)
+  const float root = sqrtf(row_sum<D / 8>(ss) * (1.0f / D) + eps), r = 1.0f / root;
+  const float rest = r * fmaf(-fminf(root, 0x1.fffffep127f), r, 1.0f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+  for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], r, x[i] * rest) * w[i];
   if (turns) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -454,8 +454,9 @@ int aila_hip_gqa_prefill_paged_fp8(const void* q, long q_stride,
  *   y = x / sqrt(mean(x^2) + eps) * w, w = q_norm_w / k_norm_w [D] bf16 (NULL: 1)
  *   dims d and d + rotary_dim / 2 of y are turned by p * theta^(-2 d / rotary_dim)
  *   (inv_freq, device float[rotary_dim / 2]: by p * inv_freq[d]), d < rotary_dim / 2
- * The angle is exact to 2^-49 of itself before it is reduced, and there is one
- * rounding: q to bf16, k by the rule of aila_hip_kv_append_paged_fp8, which holds
+ * The angle is exact to 2^-49 of itself before it is reduced; quotient, cosine and
+ * sine are each rounded to fp32 once (a head's sum of squares has to stay below 2^128).
+ * There is one rounding to fewer bits: q to bf16, k by the rule of aila_hip_kv_append_paged_fp8, which holds
  * for the (unrounded) y here; v as there.
  *   q        head h of token t at + t * q_stride + h * q_head_stride elements
  *            (multiples of 8: the queries of a packed q|gate row have head stride

@@ -58,3 +58,75 @@ def test_blocks_that_nobody_attends_may_have_any_scale(D, Hq, Hkv, wide):
             ks[p, :, blk], vs[p, :, blk] = k_bad, v_bad
         out = A.gqa_tree_paged_fp8(q, kp, vp, ks, vs, table, starts, lens, mask, max(rows), workspace=ws)
         assert torch.equal(out[:63], want), (k_bad, v_bad)
+
+
+# ------------------------------------------------------------- prepare's roundings ----
+def test_prepare_divides_as_the_definition():
+    """Rows of +-s, whose root is s: x / root is +-1, and times a weight it is a tie between two codes. A
+    product with the rounded reciprocal falls short of it for these s."""
+    import torch
+    import aila_amd as A
+    s = [x for x in range(1, 257) if np.float32(x) * (np.float32(1) / np.float32(x)) != 1]
+    assert len(s) > 10
+    for D in (64, 128, 256):
+        page, H = 16, 2
+        P = -(-len(s) // page)
+        sign = 1 - 2 * torch.randint(0, 2, (len(s), H, D), generator=torch.Generator().manual_seed(D)).double()
+        k = (torch.tensor(s).double()[:, None, None] * sign).to(torch.bfloat16).cuda()
+        w = (1 + (2 * (torch.arange(D) % 8) + 1) / 16).double()
+        cache = A.paged_fp8_cache(P, H, page, D)
+        q = A.prepare_qkv_paged_fp8(k, k, k, *cache, torch.arange(len(s), dtype=torch.int32, device="cuda"), None, q_norm=w.to(torch.bfloat16).cuda(),
+                                    k_norm=w.to(torch.bfloat16).cuda(), rotary_dim=0, eps=0.0)
+        y = (sign * w).numpy()
+        assert np.array_equal(q.double().cpu().numpy(), y)
+        got = ref.Cache(cache[0], cache[2])
+        e = ref.scale_exp(float(np.abs(y).max()))
+        assert np.all(got.scale.reshape(P, H)[:len(s) // page] == 2.0 ** e)
+        rows = got.val.transpose(0, 2, 1, 3).reshape(P * page, H, D)[:len(s)]
+        assert np.array_equal(rows, ref.e4m3(y * 2.0 ** -e)), D
+
+
+def test_prepare_turns_as_the_definition():
+    """Rows of ones turned by angles at which cos - sin or sin + cos comes closest to a border between two
+    codes, but no closer than cosine, sine and their sum, each rounded to fp32, can cross: half a unit of
+    each, and what the angle (2^20 radians in fp64) and the series leave, 2e-9."""
+    import torch
+    import aila_amd as A
+    D, theta = 128, 1e6
+    f = theta ** (-2.0 * np.arange(D // 2) / D)
+
+    def values(pos, freq, m):
+        """y, and the distance to the next border less what the roundings may take."""
+        a = pos * freq
+        c, s = m.cos(a), m.sin(a)
+        out = []
+        for y in (c - s, s + c):
+            v = y.abs() if m is torch else np.abs(y)
+            half = [m.exp2(m.floor(m.log2(x)) - 24) for x in (c.abs(), s.abs(), v)] if m is torch else [
+                np.exp2(np.floor(np.log2(x)) - 24) for x in (np.abs(c), np.abs(s), v)]
+            unit = m.exp2(m.floor(m.log2(v * 256)) - 3) / 256
+            part = v / unit
+            slack = half[0] + half[1] + half[2] + 2e-9
+            out.append((y, (part - m.floor(part) - 0.5) * unit, slack))
+        return out
+
+    hits = []
+    for j in range(0, D // 2):
+        pos = torch.arange(1, 1 << 20, dtype=torch.float64, device="cuda")
+        for which, (y, d, slack) in enumerate(values(pos, float(f[j]), torch)):
+            near = ((d.abs() > slack * 1.01) & (d.abs() < slack * 1.35) & (y.abs() > 2.0 ** -6)).nonzero().view(-1)
+            hits += [(int(pos[i]), j, which) for i in near.tolist()]
+    hits = [h for h in hits if (lambda x: abs(x[1]) > x[2])(values(float(h[0]), f[h[1]], np)[h[2]])]
+    assert len(hits) > 60
+    n = len(hits)
+    page, P = 16, -(-n // 16)
+    cache = A.paged_fp8_cache(P, 1, page, D)
+    one = torch.ones((n, 1, D), dtype=torch.bfloat16, device="cuda")
+    pos = torch.tensor([h[0] for h in hits], dtype=torch.int32, device="cuda")
+    A.prepare_qkv_paged_fp8(one, one, one, *cache, torch.arange(n, dtype=torch.int32, device="cuda"), pos, theta=theta, eps=0.0)
+    got = ref.Cache(cache[0], cache[2])
+    assert np.all(got.scale == 2.0 ** -8)
+    rows = got.val.transpose(0, 2, 1, 3).reshape(P * page, D)
+    wrong = [(p, j, which) for i, (p, j, which) in enumerate(hits)
+             if rows[i, j + which * (D // 2)] != ref.e4m3(np.float64(values(float(p), f[j], np)[which][0] * 256))]
+    assert not wrong, (len(wrong), n, wrong[:5])
