@@ -699,21 +699,22 @@ __global__ __launch_bounds__(kMergeThreads) void gqa_tree_paged_fp8_merge_kernel
 }
 
 // The same for many columns, few records each: a workgroup takes as many columns as it
-// has threads for.
+// has threads for, and then those gridDim.z times as many further on.
 template <int D>
 __global__ __launch_bounds__(kMergeThreads) void gqa_tree_paged_fp8_merge_few_kernel(PagedFp8 c, TreeArgs a, int launched) {
   constexpr int kQuads = D / 4, kColumns = kMergeThreads / kQuads;
   const int b = blockIdx.y, kvh = blockIdx.x;
   const Shape s = shape_of<D>(a, b);
-  const int cols = s.n * a.group, x0 = static_cast<int>(blockIdx.z) * kColumns;
-  if (x0 >= cols) return;
-  const Records r = records_of<D>(c, a, s, b, kvh, x0, launched);      // the columns are one item's
-  if (r.w0 == r.w1) return;
+  const int cols = s.n * a.group, d = static_cast<int>(threadIdx.x) % kQuads * 4, mine = static_cast<int>(threadIdx.x) / kQuads;
   const size_t step = static_cast<size_t>(a.rec_cols) * (D + kRecTail);
-  const int d = static_cast<int>(threadIdx.x) % kQuads * 4, x = min(static_cast<int>(threadIdx.x) / kQuads, cols - 1 - x0);
-  Joined sum;
-  for (int w = r.w0; w <= r.w1; w += kBatch) join_batch<D>(&sum, r.at + x * (D + kRecTail), r, w, 1, step, d);
-  if (static_cast<int>(threadIdx.x) / kQuads < cols - x0) store_joined<D>(a, s, kvh, x0 + x, d, sum);
+  for (int x0 = static_cast<int>(blockIdx.z) * kColumns; x0 < cols; x0 += static_cast<int>(gridDim.z) * kColumns) {
+    const Records r = records_of<D>(c, a, s, b, kvh, x0, launched);      // the columns are one item's
+    if (r.w0 == r.w1) continue;
+    const int x = min(mine, cols - 1 - x0);
+    Joined sum;
+    for (int w = r.w0; w <= r.w1; w += kBatch) join_batch<D>(&sum, r.at + x * (D + kRecTail), r, w, 1, step, d);
+    if (mine < cols - x0) store_joined<D>(a, s, kvh, x0 + x, d, sum);
+  }
 }
 
 // The most that a request may have: columns, column tiles, items of a KV head.
@@ -784,8 +785,10 @@ int launch(const PagedFp8& c, TreeArgs a, int words, void* workspace, size_t wor
   const long items = static_cast<long>(a.B) * c.Hkv * m.items;
   AILA_REQUIRE(items * most_units(a.max_len) < (1L << 31) && items * kThreads < (1L << 32),
                "gqa_tree_paged_fp8: B=%d requests of up to %ld query rows and %d keys are too many", a.B, m.cols, a.max_len);
-  const long few = (m.cols * (D / 4) + kMergeThreads - 1) / kMergeThreads;
-  AILA_REQUIRE(few <= 65535, "gqa_tree_paged_fp8: %ld query rows of a KV head are too many", m.cols);
+  const long joins = (m.cols * (D / 4) + kMergeThreads - 1) / kMergeThreads;      // workgroups of a request and KV head
+  AILA_REQUIRE(joins <= 65535, "gqa_tree_paged_fp8: %ld query rows of a KV head are too many", m.cols);
+  // fewer than 2^32 threads, the most of a launch
+  const long few = std::min(joins, ((1L << 32) - 1) / kMergeThreads / (static_cast<long>(a.B) * c.Hkv));
   long groups = static_cast<long>(a.B) * c.Hkv * a.chunks;
   if (workspace != nullptr) {
     const size_t rec = record_bytes<D>(m);

@@ -130,3 +130,26 @@ def test_prepare_turns_as_the_definition():
     wrong = [(p, j, which) for i, (p, j, which) in enumerate(hits)
              if rows[i, j + which * (D // 2)] != ref.e4m3(np.float64(values(float(p), f[j], np)[which][0] * 256))]
     assert not wrong, (len(wrong), n, wrong[:5])
+
+
+# -------------------------------------------------------------------------- trees ----
+def test_tree_merge_of_more_columns_than_a_launch_has_threads():
+    """4096 requests of whom one may have 16384 query rows a KV head: a thread for each would be 2^33."""
+    import torch
+    import aila_amd as A
+    B, D, Hq, Hkv, page, words = 4096, 64, 32, 8, 16, 64
+    rng = np.random.default_rng(2)
+    new, before = rng.integers(0, 3, B).tolist(), rng.integers(0, 20, B).tolist()
+    new[7], before[7], new[B - 1], before[B - 1] = 300, 900, 70, 8100
+    q, cache, table, starts, lens, mask, seen, rows = _tree_case(D, Hq, Hkv, page, new, before, 3, words=words)
+    max_len = table.shape[1] * page                    # above 4096: not a workgroup for each request
+    assert max_len > 4096 and q.shape[0] > 4096 and B * Hkv * 4 * 64 * words * D // 4 >= 1 << 32
+    ws = _workspace(q, cache, new, max_len, mask)
+    out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+    A.gqa_tree_paged_fp8(q, *cache, table, starts, lens, mask, max_len, out=out, workspace=ws)
+    assert not _walked_as_prompt(ws, new, rows, Hq // Hkv, D, words)
+    assert bool(out.isfinite().all()) and bool((out[sum(new):] == 7.0).all())
+    at = np.concatenate([[0], np.cumsum(new)])
+    for b in [7, B - 1] + rng.choice(B, 20, replace=False).tolist():
+        a, z = int(at[b]), int(at[b + 1])
+        _tree_check(out[a:z], q[a:z], cache, table[b:b + 1], [new[b]], [before[b]], seen[a:z], pick={0, 1, 63, 64, 255, 299}, words=words)
