@@ -33,8 +33,8 @@ struct KeepArgs {
   int B, most, max_pages, num_pages, Hkv, page_size;
 };
 
-// A wave: K or V of heads of one request and layer, kHeads at a time with their loads
-// in flight; the request's lengths and places are looked up once. Blocks from the one
+// A wave: K or V of kHeads heads of one request and layer, their loads in flight
+// together; the request's lengths and places are looked up once. Blocks from the one
 // of the first row that moves, in order: a row comes from behind its place (kept
 // indices rise), so a block that has been written holds no later block's source.
 //
@@ -42,9 +42,13 @@ struct KeepArgs {
 // layers of 4 heads, D = 256, 19 moved rows, 4.9 us; 64 requests, 32 layers of 8 heads, D
 // = 128, 160 moved rows (21 MB read and written, in runs of 128 bytes) 26 us.
 constexpr int kKeepThreads = 256;
-// Workgroups with one head a wave from which a wave takes four: the 64 requests above
-// 26.1 us against 30.2 with one, the 8 (128 workgroups) 4.9 with one.
-constexpr long kKeepGroups = 1024;
+// Workgroups with one head a wave above which a wave takes four. us in a graph, one / four, drafts of
+// 26 tokens (60: in parentheses). D = 64, 8 heads: 512 workgroups 5.7/6.7, 1024 6.9/6.7 (7.1/6.7), 2048
+// 8.7/7.3 (8.8/7.3), 4096 12.0/9.0, 8192 19.0/12.3. D = 128, 8 heads: 512 5.8/8.4, 1024 7.1/8.5
+// (7.2/8.4), 2048 9.3/9.3 (9.4/9.2), 3072 11.7/10.3, 8192 21.0/18.8 (22.4/19.6). D = 256 takes one:
+// 4 heads, 1024 7.9/8.3, 2048 10.7/10.4, 4096 15.6/17.2 (16.6/18.9); 16 heads, 2048 10.6/10.8, 4096
+// 14.4/14.3 (15.2/14.3), 8192 23.4/25.3, 16384 40.7/38.4 (42.6/42.8).
+template <int D> constexpr long kKeepGroups = D == 64 ? 1000 : 2000;
 constexpr int kNone = kMinScaleExp - 1;
 template <int D, int kHeads>
 __global__ __launch_bounds__(kKeepThreads) void kv_keep_paged_fp8_kernel(Layers ly, KeepArgs a) {
@@ -54,7 +58,7 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_paged_fp8_kernel(Layers 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int b = blockIdx.y;
   const int step = static_cast<int>(gridDim.x) * (kKeepThreads / 64 / 2);            // heads from a wave's to its next
-  const int head0 = static_cast<int>(blockIdx.x) * (kKeepThreads / 64 / 2) + (wave >> 1);
+  const int head0 = static_cast<int>(blockIdx.x) * (kKeepThreads / 64 / 2) + (wave >> 1);      // kHeads * step reach the last
   const int cached = a.cached[b];
   const long max_rows = static_cast<long>(a.max_pages) * a.page_size;
   int n = min(max(a.kept_lens[b], 0), a.most);
@@ -72,7 +76,7 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_paged_fp8_kernel(Layers 
       break;
     }
   }
-  if (first == n) return;
+  if (first == n || head0 >= a.Hkv) return;
   const int arr = 2 * blockIdx.z + (wave & 1);
   uint8_t* pages = ly.pages[arr];
   float* scale = ly.scale[arr];
@@ -112,53 +116,51 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_paged_fp8_kernel(Layers 
       any |= moves[k] || stays[k];
     }
     if (__ballot(any) == 0) continue;     // no row of it is in range
-    for (int h0 = head0; h0 < a.Hkv; h0 += kHeads * step) {
-      u32x4 w[kHeads][NI];
-      float s_from[kHeads][NI], s_held[kHeads];
+    u32x4 w[kHeads][NI];
+    float s_from[kHeads][NI], s_held[kHeads];
 #pragma unroll
-      for (int x = 0; x < kHeads; ++x) {
-        const int off = min(h0 + x * step, a.Hkv - 1) * page_blocks;     // past the last: the last again, not stored
-        s_held[x] = scale[bid0 + off];
+    for (int x = 0; x < kHeads; ++x) {
+      const int off = min(head0 + x * step, a.Hkv - 1) * page_blocks;     // past the last: the last again, not stored
+      s_held[x] = scale[bid0 + off];
 #pragma unroll
-        for (int k = 0; k < NI; ++k) {
-          s_from[x][k] = 0.f;
-          w[x][k] = u32x4{0u, 0u, 0u, 0u};
-          if (moves[k]) {
-            s_from[x][k] = scale[from[k] + off];
-            w[x][k] = ld16(pages + static_cast<size_t>(from[k] + off) * (kScaleRows * D) + byte[k]);
-          }
+      for (int k = 0; k < NI; ++k) {
+        s_from[x][k] = 0.f;
+        w[x][k] = u32x4{0u, 0u, 0u, 0u};
+        if (moves[k]) {
+          s_from[x][k] = scale[from[k] + off];
+          w[x][k] = ld16(pages + static_cast<size_t>(from[k] + off) * (kScaleRows * D) + byte[k]);
         }
       }
+    }
 #pragma unroll
-      for (int x = 0; x < kHeads; ++x) {
-        if (h0 + x * step >= a.Hkv) break;
-        const int bid = bid0 + (h0 + x * step) * page_blocks;
-        const int held = held_exp(s_held[x]);
-        int top = kNone;
+    for (int x = 0; x < kHeads; ++x) {
+      if (head0 + x * step >= a.Hkv) break;
+      const int bid = bid0 + (head0 + x * step) * page_blocks;
+      const int held = held_exp(s_held[x]);
+      int top = kNone;
+#pragma unroll
+      for (int k = 0; k < NI; ++k)
+        if (moves[k] || stays[k]) top = max(top, stays[k] ? held : held_exp(s_from[x][k]));
+      const int e = wave_max(top);
+      uint8_t* block = pages + static_cast<size_t>(bid) * (kScaleRows * D);
+      if (e != held) {      // the rows that stay change scale too
 #pragma unroll
         for (int k = 0; k < NI; ++k)
-          if (moves[k] || stays[k]) top = max(top, stays[k] ? held : held_exp(s_from[x][k]));
-        const int e = wave_max(top);
-        uint8_t* block = pages + static_cast<size_t>(bid) * (kScaleRows * D);
-        if (e != held) {      // the rows that stay change scale too
-#pragma unroll
-          for (int k = 0; k < NI; ++k)
-            if (stays[k]) w[x][k] = ld16(block + byte[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < NI; ++k) {
-          if (moves[k] || (stays[k] && e != held)) {
-            const int e_from = stays[k] ? held : held_exp(s_from[x][k]);
-            if (e != e_from) {
-              const float f = pow2f(e_from - e);
-#pragma unroll
-              for (int y = 0; y < 4; ++y) w[x][k][y] = scale_codes(w[x][k][y], f);
-            }
-            *reinterpret_cast<u32x4*>(block + (k * RI + rr) * D + c16) = w[x][k];
-          }
-        }
-        if (lane == 0) scale[bid] = pow2f(e);
+          if (stays[k]) w[x][k] = ld16(block + byte[k]);
       }
+#pragma unroll
+      for (int k = 0; k < NI; ++k) {
+        if (moves[k] || (stays[k] && e != held)) {
+          const int e_from = stays[k] ? held : held_exp(s_from[x][k]);
+          if (e != e_from) {
+            const float f = pow2f(e_from - e);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) w[x][k][y] = scale_codes(w[x][k][y], f);
+          }
+          *reinterpret_cast<u32x4*>(block + (k * RI + rr) * D + c16) = w[x][k];
+        }
+      }
+      if (lane == 0) scale[bid] = pow2f(e);
     }
   }
 }
@@ -260,14 +262,15 @@ extern "C" int aila_hip_kv_keep_paged_fp8(void* const* k_pages, void* const* v_p
   for (int l0 = 0; l0 < layers; l0 += step) {
     const int n = std::min(step, layers - l0);
     const Layers ly = some_layers(k_pages, v_pages, k_scale, v_scale, l0, n);
-    const bool many = static_cast<long>(B) * n * most_gx > kKeepGroups;
     auto go = [&](auto kernel, unsigned gx) {
       hipLaunchKernelGGL(kernel, dim3(gx, B, n), dim3(kKeepThreads), 0, static_cast<hipStream_t>(stream), ly, a);
     };
     auto launch = [&](auto d) {
       constexpr int kD = decltype(d)::value;
-      if (many) go(kv_keep_paged_fp8_kernel<kD, 4>, (most_gx + 3) / 4);
-      else go(kv_keep_paged_fp8_kernel<kD, 1>, most_gx);
+      if constexpr (kD != 256) {
+        if (static_cast<long>(B) * n * most_gx > kKeepGroups<kD>) return go(kv_keep_paged_fp8_kernel<kD, 4>, (most_gx + 3) / 4);
+      }
+      go(kv_keep_paged_fp8_kernel<kD, 1>, most_gx);
     };
     if (D == 64) launch(std::integral_constant<int, 64>{});
     else if (D == 128) launch(std::integral_constant<int, 128>{});

@@ -382,13 +382,13 @@ def test_tree_of_nan_keys_and_queries(D, Hq, Hkv, wide):
 
 
 # --------------------------------------------------------------------------- keep ----
-@pytest.mark.parametrize("D,H,page,B,layers", [(64, 13, 16, 40, 5), (128, 11, 32, 40, 6), (256, 9, 16, 50, 5), (128, 1, 16, 300, 4), (256, 16, 64, 20, 8)])
+@pytest.mark.parametrize("D,H,page,B,layers", [(64, 13, 16, 40, 5), (128, 11, 32, 40, 10), (256, 9, 16, 50, 5), (128, 1, 16, 300, 8), (256, 16, 64, 20, 8)])
 def test_keep_of_many_is_that_of_each_layer(D, H, page, B, layers):
-    """Many requests and layers, where a wave takes four heads (the last of them doubled where the heads are
-    no multiple), against a call for each layer, where it takes one."""
+    """Many requests and layers, where a wave of D = 64 or 128 takes four heads (the last of them doubled where
+    the heads are no multiple), against a call for each layer, where it takes one."""
     import torch
     import aila_amd as A
-    assert B * layers * (-(-H // 2)) > 1024 >= B * (-(-H // 2))
+    assert B * layers * (-(-H // 2)) > (2000 if D == 128 else 1000) >= B * (-(-H // 2))
     rng = np.random.default_rng(D + H)
     cached, new = rng.integers(0, 70, B).tolist(), rng.integers(1, 60, B).tolist()
     cached[3], new[4] = -1, 1
