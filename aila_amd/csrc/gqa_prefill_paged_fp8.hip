@@ -109,31 +109,12 @@ struct Cfg {
   static constexpr int REC = kRows * (D + 2);     // floats of a record: {o[rows][D], {m, l}[rows]}
 };
 
-__device__ __forceinline__ f32x16 mfma32(const bf16x8_t& a, const bf16x8_t& b, const f32x16& c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-
-// Max over lanes l and l ^ 32.
-__device__ __forceinline__ float half_max(float x) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-}
-__device__ __forceinline__ float half_sum(float x) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
-}
-
 // x, as a value the compiler cannot follow: what is made of it inside a loop is
 // made there again, a few instructions, and not kept in registers (or spilled)
 // over all loops around it.
 __device__ __forceinline__ int here(int x) {
   asm volatile("" : "+v"(x));
   return x;
-}
-
-// acc + the two bf16 of x.
-__device__ __forceinline__ float add_pair(uint32_t x, float acc) {
-  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), acc, false);
 }
 
 __device__ __forceinline__ void pin(u32x4& x) { asm volatile("" : "+v"(x)); }

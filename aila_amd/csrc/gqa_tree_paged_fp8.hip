@@ -180,25 +180,6 @@ __device__ __forceinline__ int share_begin(int w, int units, int groups) {
   return __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<long>(w) * units / groups));
 }
 
-// acc + the two bf16 of x.
-__device__ __forceinline__ float add_pair(uint32_t x, float acc) {
-  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), acc, false);
-}
-
-__device__ __forceinline__ f32x16 mfma32(const bf16x8_t& a, const bf16x8_t& b, const f32x16& c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-
-// Max / sum over lanes l and l ^ 32.
-__device__ __forceinline__ float half_max(float x) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-}
-__device__ __forceinline__ float half_sum(float x) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
-}
-
 // Codes of a strip's K and V, one strip's registers each: the next strip's K goes
 // out when this one's scores are made, its V when this one's products are. A block
 // without a page is read as block 0: all its rows are masked.
