@@ -907,8 +907,9 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_prefill_paged_fp8_kernel(Page
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] = fast_exp2(fmaf(sc[k][i], a.scale_log2, nm));
           // P is rounded to bf16 once (half a step, 2^-8 of each weight, at random): its
-          // sum of two, as the decode takes, would double this product. The sum is
-          // taken of the rounded weights, in fp32, so that they add up to 1.
+          // sum of two, as the decode takes, would double this product, and trees of 120
+          // tokens took 246 us with it, 196 without. The sum is taken of the rounded
+          // weights, in fp32, so that they add up to 1.
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             p[k][0][i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);

@@ -38,9 +38,13 @@ struct KeepArgs {
 // of the first row that moves, in order: a row comes from behind its place (kept
 // indices rise), so a block that has been written holds no later block's source.
 //
-// Bound by the chain lengths -> kept -> table -> scales and codes -> rows: 8 requests, 8
-// layers of 4 heads, D = 256, 19 moved rows, 4.9 us; 64 requests, 32 layers of 8 heads, D
-// = 128, 160 moved rows (21 MB read and written, in runs of 128 bytes) 26 us.
+// A few requests are bound by the chain lengths -> kept -> table -> scales and codes -> rows:
+// 8 requests, 8 layers of 4 heads, D = 256, 19 moved rows, 4.8 us. Of many, 64 requests, 32
+// layers of 8 heads, D = 128, 160 moved rows a layer (21 MB read and written, in runs of 128
+// bytes; 4.3 us at a copy's rate), every wave of K or V of a layer goes through that chain
+// for itself, and has nothing in flight behind its one batch: 19.6 us in a graph, 26 with the
+// cache's rows not in the L2s; waves wait for 71% of their time, the vector ALU (places and
+// scales) is busy for 39%.
 constexpr int kKeepThreads = 256;
 // Workgroups with one head a wave above which a wave takes four. us in a graph, one / four, drafts of
 // 26 tokens (60: in parentheses). D = 64, 8 heads: 512 workgroups 5.7/6.7, 1024 6.9/6.7 (7.1/6.7), 2048

@@ -12,17 +12,18 @@
 //
 // A lane holds dims 4 s .. 4 s + 3 of both halves of the rotated part (or of the
 // rest), so a pair is never apart, at two 8-byte loads instead of one of 16. The
-// cosines and sines of a workgroup's tokens are made once, in LDS (each wave its own:
-// 1800 instructions a wave instead of 500 at D = 256).
+// cosines and sines of a workgroup's tokens are made once, in LDS, for all its waves.
 //
-// Bound by the bytes where there are many tokens: 8191, 16 / 4 heads, D = 256, rows
-// first 54.2 us for 184 MB = 3.4 TB/s (a large copy reaches 4.9; queries alone 32 us
-// = 4.2; without the rotation 47 us in all, since a workgroup's turns are 1 to 2
-// thousand sines and cosines); by launch and the chain slots -> rows -> codes where
-// there are few: 26 tokens, 32 / 8, D = 128, 5.9 us. The rows, or a wave's first head,
-// are on their way while the turns are made (26 tokens 6.3 -> 5.9 us, 4096 of 32 / 8, D =
-// 128, 25.2 -> 23.9). Rows and queries interleaved in one launch were slower (83 us for
-// the 8191 tokens): what stores rows takes longest, and comes last.
+// Many tokens, 8191 of 16 / 4 heads, D = 256 (184 MB): 54.3 us where tokens follow each
+// other, 58.8 with gates between the queries, where a large copy takes 38. Queries alone 30
+// us for 135 MB = 4.5 TB/s, their vector ALU busy for 84% of it. Rows 25 to 30 us for 50 MB:
+// a wave holds a whole block, so a CU has 10 of them, which wait for 45% of their time with
+// the vector ALU busy for 56%; loads, arithmetic and stores of a wave's one run follow each
+// other. (The append alone takes 14; without the rotation 7 us go.) Few tokens are bound
+// by launch and the chain slots -> rows -> codes: 26 tokens, 32 / 8, D = 128, 5.9 us. The rows,
+// or a wave's first head, are on their way while the turns are made (26 tokens 6.3 -> 5.9 us,
+// 4096 of 32 / 8, D = 128, 25.2 -> 23.9). Rows and queries interleaved in one launch were
+// slower (83 us for the 8191 tokens): what stores rows takes longest, and comes last.
 #include "paged_fp8.hpp"
 
 #include <type_traits>
@@ -409,11 +410,11 @@ extern "C" int aila_hip_prepare_qkv_paged_fp8(const void* q, long q_stride, long
   AILA_REQUIRE(all % 16 == 0, "%s: q, k, v, q_out and the weights must be 16-byte aligned", what);
   // A wave takes the runs that begin in its tile one after the other. us, tiles of 1, 4, 8
   // and 16 tokens, a run a token / prompts of T / 4, 32 / 8 heads, D = 128: T = 256
-  // 7.7/7.2, 8.5/7.8, 12.4/8.0, 20.9/8.9; 512 11.6/10.4, 10.0/7.6, 13.0/8.3, 21.1/8.3; 1024
-  // 21.7/16.7, 15.9/11.2, 16.4/9.8, 23.9/10.7; 2048 39.8/28.0, 27.2/17.0, 24.9/14.4,
-  // 27.4/13.9; 4096 74.2/49.5, 48.2/34.6, 44.6/28.2, 43.3/22.6. 16 / 4, D = 256: 256 6.5/8.8,
-  // 9.4/10.3, 14.1/10.5, 24.1/12.3; 1024 18.2/20.2, 14.1/11.6, 16.9/11.9, 27.2/13.6; 4096
-  // 60.3/64.9, 43.5/35.6, 40.3/29.7, 39.6/25.1.
+  // 8.0/7.5, 9.1/7.9, 13.6/8.0, 22.8/8.8; 512 12.6/10.7, 10.8/7.9, 14.2/8.4, 23.3/8.3; 1024
+  // 23.0/16.3, 17.0/11.1, 18.0/9.7, 25.9/10.7; 2048 41.1/27.4, 29.0/16.7, 26.8/14.5,
+  // 29.6/13.7; 4096 77.3/48.6, 52.4/33.7, 48.2/27.5, 46.2/22.3. 16 / 4, D = 256: 256 7.1/9.0,
+  // 10.2/10.6, 15.6/10.6, 26.6/12.3; 1024 19.0/20.3, 14.8/11.9, 17.9/12.1, 29.1/13.9; 4096
+  // 60.9/64.2, 45.0/35.7, 41.4/29.2, 40.3/24.2.
   const int tile = T <= 256 ? 1 : T <= 1024 ? 4 : T <= 2048 ? 8 : kScaleRows;
   // fewer than 2^32 threads, the most of a launch
   const long kv_groups = (static_cast<long>(T) + tile - 1) / tile * ((Hkv + 1) / 2);
@@ -452,10 +453,10 @@ extern "C" int aila_hip_prepare_qkv_paged_fp8(const void* q, long q_stride, long
   a.kv_groups = static_cast<int>(kv_groups);
   a.eps = eps;
   const Powers pw = rotary_dim > 0 && inv_freq == nullptr ? powers_of(theta, rotary_dim) : Powers{};
-  // One launch, rows first, or two (us, one / two). 16 / 4, D = 256: T = 32 7.0 / 10.0, 1024
-  // 11.8 / 16.1, 4096 (92 MB) 24.6 / 28.0, 6000 (135 MB) 42.9 / 37.7, 8191 (184 MB) 62.3 / 54.2;
-  // 32 / 8, D = 128: 4096 23.9 / 26.2, 6000 37.8 / 37.5, 8191 53.5 / 50.6; 16 / 8, D = 128: 8191
-  // (117 MB) 34.3 / 34.5. Where the data do not stay in the caches, queries alone run at
+  // One launch, rows first, or two (us, one / two). 16 / 4, D = 256: T = 32 7.0 / 10.1, 1024
+  // 12.0 / 16.4, 4096 (92 MB) 24.9 / 28.6, 6000 (135 MB) 43.3 / 38.4, 8191 (184 MB) 63.4 / 54.3;
+  // 32 / 8, D = 128: 4096 24.4 / 26.7, 6000 38.2 / 38.0, 8191 55.2 / 50.8; 16 / 8, D = 128: 8191
+  // (117 MB) 34.0 / 34.6. Where the data do not stay in the caches, queries alone run at
   // twice the waves a SIMD.
   constexpr long kOneLaunchBytes = 120L << 20;
   const long moved = static_cast<long>(T) * D * (4L * Hq + 6L * Hkv);
