@@ -493,10 +493,10 @@ int aila_hip_prepare_qkv_paged_fp8(const void* q, long q_stride,
  *              and are not computed.
  * Tokens from query_start[B] on are not touched. Rows that a token does not attend may
  * hold anything, and so may the scale of a block of which no token attends a row. The
- * softmax weights are rounded to bf16 (2^-8 of each at most) before they meet V. Sums
- * are held in fp32, of weights of up to 2^8: the largest value that a block of V can
- * hold (448 times its scale) times the rows attended has to stay below 2^120. Other
- * arguments as aila_hip_gqa_prefill_paged_fp8.
+ * softmax weights are rounded to bf16 (2^-8 of each at most) before they meet V and are
+ * summed up. Sums are held in fp32, of weights of up to 2^8: the largest value that a
+ * block of V can hold (448 times its scale) times the rows attended has to stay below
+ * 2^120. Other arguments as aila_hip_gqa_prefill_paged_fp8.
  * The workspace holds the records of the items whose keys are split: workspace_size
  * bytes let as many workgroups work as the device holds, a smaller workspace fewer
  * (2 records at least, else AILA_HIP_EWORKSPACE), and NULL at most one for each
