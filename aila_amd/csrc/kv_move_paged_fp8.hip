@@ -49,7 +49,7 @@ constexpr int kKeepThreads = 256;
 // Workgroups with one head a wave above which a wave takes four. us in a graph, one / four, drafts of
 // 26 tokens (60: in parentheses). D = 64, 8 heads: 512 workgroups 5.7/6.7, 1024 6.9/6.7 (7.1/6.7), 2048
 // 8.7/7.3 (8.8/7.3), 4096 12.0/9.0, 8192 19.0/12.3. D = 128, 8 heads: 512 5.8/8.4, 1024 7.1/8.5
-// (7.2/8.4), 2048 9.3/9.3 (9.4/9.2), 3072 11.7/10.3, 8192 21.0/18.8 (22.4/19.6). D = 256 takes one:
+// (7.2/8.4), 2048 9.3/9.3 (9.4/9.2), 4096 12.5/11.5, 8192 21.0/18.8 (22.4/19.6). D = 256 takes one:
 // 4 heads, 1024 7.9/8.3, 2048 10.7/10.4, 4096 15.6/17.2 (16.6/18.9); 16 heads, 2048 10.6/10.8, 4096
 // 14.4/14.3 (15.2/14.3), 8192 23.4/25.3, 16384 40.7/38.4 (42.6/42.8).
 template <int D> constexpr long kKeepGroups = D == 64 ? 1000 : 2000;
