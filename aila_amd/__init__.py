@@ -789,8 +789,8 @@ def prepare_qkv_paged_fp8(q, k, v, k_pages, v_pages, k_scale, v_scale, slots, po
     of 8, 0: none) turned at positions int32 [T], or [3,T]: the t, h and w
     streams of interleaved mRoPE with ``sections`` (t, h, w); k and v quantised
     into the rows ``slots`` (int32 [T], -1: skip) as kv_append_paged_fp8 does
-    -> q_out [T,Hq,D] bf16 (may be q itself, if contiguous). inv_freq: float32
-    [rotary_dim/2] in place of theta^(-2d/rotary_dim)."""
+    -> q_out [T,Hq,D] bf16 (may be q itself, if contiguous; refused where it
+    overlaps q, k or v otherwise). inv_freq: float32 [rotary_dim/2] in place of theta^(-2d/rotary_dim)."""
     import torch
     dev = _device_of(stream)
     T, Hq, D = q.shape
